@@ -48,7 +48,8 @@ const char *pn_status_string(int status);
 /* Message of the last failing call on this host thread ("" if none). */
 const char *pn_last_error(void);
 /* Device-side status word of the current device: a kernel that abandons a
- * bounded wait records PN_ERR_TIMEOUT there.  Synchronises the device.  When
+ * bounded wait records PN_ERR_TIMEOUT there, one that meets a block-table entry
+ * outside its cache PN_ERR_ARG.  Synchronises the device.  When
  * reset != 0 the word is cleared after reading. */
 int pn_device_status(int reset, int *status_out);
 
@@ -263,6 +264,95 @@ int pn_linear_i8_epi(const int8_t *xq, int64_t xq_pitch, const float *s_x, const
  * 100-101,127).  In place (y == x) when the dtypes match. */
 int pn_layer_norm(const void *x, int x_dtype, int64_t M, int64_t C, const float *weight, const float *bias,
                   float eps, void *y, int y_dtype, void *stream);
+
+/* Root-mean-square norm over the last dimension with the residual's addition
+ * (no reference counterpart; beside pn_layer_norm and pn_quant_act_i8):
+ *   h = x + residual, rounded to x's type          (residual, h: both or none)
+ *   y[m, :] = (h[m, :] * rstd) * weight,  rstd = 1 / sqrt(mean(h^2) + eps)
+ * The sum runs in fp64 and rstd is rounded to fp32 once; the two products are
+ * fp32.  x, residual, h: (M, C) PN_BF16 or PN_F32, contiguous; h may be x or
+ * residual itself.  weight: NULL or C values, PN_F32 or PN_BF16.
+ * pn_rms_norm writes y (PN_BF16 or PN_F32) rounded once.  pn_rms_norm_i8
+ * writes what pn_quant_act_i8 makes of that y in fp32 (xq with pitch
+ * pn_act_i8_pitch(C), s_x, rowsum), ready for pn_linear_i8; a row that holds
+ * an inf or NaN gets s_x = NaN and codes 0. */
+int pn_rms_norm(const void *x, int x_dtype, const void *residual, int64_t M, int64_t C, const void *weight, int w_dtype,
+                double eps, void *h, void *y, int y_dtype, void *stream);
+int pn_rms_norm_i8(const void *x, int x_dtype, const void *residual, int64_t M, int64_t C, const void *weight,
+                   int w_dtype, double eps, void *h, int8_t *xq, int64_t xq_pitch, float *s_x, int32_t *rowsum,
+                   void *stream);
+
+/* ---- a paged cache of keys and values in 4 bits, and attention over it (no
+ *      reference counterpart; its GPT recomputes the whole prefix) ----------
+ *
+ * cache: (n_pages, kv_heads, 2, pn_kv4_block_bytes(page, head_dim)) bytes, keys
+ * at index 0 of the third axis and values at 1, 16-byte aligned.  A block is
+ * page * head_dim / 2 bytes of 4-bit codes, then page pairs of bf16 (s, z); code
+ * c stands for s * c + z.  Keys: token by token, dim d in the low (d even) or
+ * high half of byte d / 2.  Values: tokens 2i and 2i + 1 share head_dim bytes;
+ * 32-bit word j of these holds dims 4j .. 4j+3 of token 2i in its low half and
+ * of token 2i + 1 in its high half, four bits per dim, the first dim lowest.
+ * z is the vector's minimum rounded down to bf16, s = (max - z) / 15 rounded up
+ * to bf16, c = clamp(rint((x - z) / s), 0, 15) in fp32; a vector that holds an
+ * inf or NaN reads back as NaN.  head_dim: 64 or 128.  page: a multiple of 16.
+ *
+ * block_table: (B, table_w) int32, rows table_ld apart: entry i of sequence b is
+ * the page of its positions [i * page, (i + 1) * page).  seq_lens: (B) int32, the
+ * sequences' lengths WITH the rows of this call, taken as at most table_w * page
+ * (at most 2^30).  The T rows of a call are the newest positions of their sequences: T / B rows
+ * each, or rows [cu_q[b], cu_q[b + 1]) with cu_q (B + 1) int32.  Rows behind
+ * cu_q[B] are not touched.  Entries used that are no page of the cache are
+ * skipped (nothing is stored; their tokens read as zeros and are not attended
+ * to) and recorded as PN_ERR_ARG in the device status word.
+ * Strides are in elements: of a sequence, a row and a head (the first is not
+ * used with cu_q); the last dimension is contiguous. */
+int64_t pn_kv4_block_bytes(int64_t page, int64_t head_dim);
+
+/* Quantise and store the rows' keys and values (PN_BF16 or PN_F32).  A row at
+ * a negative position (more rows than the sequence is long) is dropped. */
+int pn_kv4_append(const void *k, int64_t k_sb, int64_t k_sl, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sl,
+                  int64_t v_sh, int kv_dtype, void *cache, int64_t n_pages, int64_t kv_heads, int64_t page,
+                  int64_t head_dim, const int32_t *block_table, int64_t table_ld, int64_t table_w,
+                  const int32_t *seq_lens, const int32_t *cu_q, int64_t B, int64_t T, void *stream);
+
+/* Read the rows' keys and values back: k, v (T, kv_heads, head_dim) of kv_dtype,
+ * contiguous, 16-byte aligned; zeros at negative positions. */
+int pn_kv4_gather(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
+                  const int32_t *block_table, int64_t table_ld, int64_t table_w, const int32_t *seq_lens,
+                  const int32_t *cu_q, int64_t B, int64_t T, void *k, void *v, int kv_dtype, void *stream);
+
+/* Causal attention: row i of sequence b (of L_b rows) sees the cached positions
+ * up to seq_lens[b] - L_b + i, its own included (store the rows' keys and values
+ * first).  out (T, q_heads, head_dim) of q's type (PN_BF16 or PN_F32),
+ * contiguous, 16-byte aligned; zeros for a row that sees nothing.  Query head
+ * h reads kv head h / (q_heads / kv_heads).  The logits are scale * q . k.
+ * Queries enter the products as fp16 relative to the row's largest (bf16 ones
+ * exactly), weights as fp16; sums and the softmax are fp32.
+ * Workspace: pn_kv4_attention_workspace_size bytes, 256-byte aligned, no
+ * initialisation needed; calls that may overlap need one each. */
+size_t pn_kv4_attention_workspace_size(int64_t B, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
+int pn_kv4_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
+                     const void *cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
+                     const int32_t *block_table, int64_t table_ld, int64_t table_w, const int32_t *seq_lens,
+                     const int32_t *cu_q, int64_t B, int64_t T, float scale, void *out, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* One token per row of logits ((rows, vocab) PN_BF16 or PN_F32, rows ld elements
+ * apart, vocab <= 2^18) from a uniform number u[row] in [0, 1):
+ *   w_i = exp((x_i - max) / T); keep the top_k largest logits (ties: lowest
+ *   index first; <= 0: all), of them those with w_i >= min_p, of them the
+ *   smallest prefix in that order whose sum reaches top_p of the sum of all
+ *   left (top_p >= 1: all; never less than one token); the token is the first index whose running sum of
+ *   the kept w exceeds u * their sum.
+ * T <= 0 takes the first largest logit.  A NaN logit counts as -inf; a row with
+ * nothing above -inf gives -1; logits of +inf share all the weight.  Each
+ * setting is a device array of one value per row, or, where its pointer is
+ * NULL, the value after it.  Weights are 45-bit fractions of the largest (one
+ * below 2^-46 of it counts as zero); their sums are exact.  No reference
+ * counterpart. */
+int pn_sample_tokens(const void *logits, int x_dtype, int64_t rows, int64_t vocab, int64_t ld, const float *u,
+                     const float *temperature, float temperature0, const int32_t *top_k, int32_t top_k0,
+                     const float *top_p, float top_p0, const float *min_p, float min_p0, int64_t *tokens, void *stream);
 
 /* Number of SMs of the current device (used to size launches and shards). */
 int pn_device_sm_count(int *count_out);

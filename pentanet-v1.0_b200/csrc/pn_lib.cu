@@ -16,3 +16,7 @@
 #include "pn_peer.cu"
 #include "pn_i8w.cu"
 #include "pn_ternary2.cu"
+#include "pn_rms.cu"
+#include "pn_kv4.cu"
+#include "pn_kv4_attn.cu"
+#include "pn_sample.cu"

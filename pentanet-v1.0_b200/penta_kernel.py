@@ -354,6 +354,120 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     return y.reshape(x.shape)
 
 
+_FLOATS = {torch.float32: _nat.PN_F32, torch.bfloat16: _nat.PN_BF16}
+
+
+def _rms_args(x, weight, residual, what):
+    """(x, residual, h, weight, rows, C) of the RMS norms, ready for the C ABI."""
+    assert x.is_cuda and x.dtype in _FLOATS, f"{what} takes a bfloat16 or float32 CUDA tensor"
+    assert x.dim() >= 1 and x.shape[-1] > 0, f"{what}: the last dimension is empty"
+    C = x.shape[-1]
+    x = x.contiguous()
+    r = h = w = None
+    if residual is not None:
+        assert residual.dtype == x.dtype, f"{what}: the residual has the type of x"
+        assert residual.device == x.device and residual.shape == x.shape, f"{what}: the residual has the shape of x"
+        r = residual.contiguous()
+        h = torch.empty_like(x)
+    if weight is not None:
+        w = weight.detach()
+        assert w.dtype in _FLOATS and w.device == x.device and w.numel() == C, f"{what}: weight is ({C},) on x's device"
+        w = w.contiguous()
+    return x, r, h, w, x.numel() // C, C
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+             residual: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16):
+    """Root-mean-square norm over the last dimension: (h / sqrt(mean(h^2) + eps))
+    * weight in fp32 (the sum in fp64), rounded once to out_dtype.
+
+    Without a residual h is x and y is returned; with one (x's shape and type)
+    h = x + residual rounded to x's type, and (y, h) is returned: h is the
+    residual stream of the next block.  x: (..., C) bf16/fp32 CUDA; weight: (C,)
+    bf16/fp32 or None.  Not in the reference; beside layer_norm."""
+    assert out_dtype in _FLOATS
+    xc, r, h, w, M, C = _rms_args(x, weight, residual, "rms_norm")
+    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+    with _nat.device_of(x):
+        _nat.check(_nat.load().pn_rms_norm(xc.data_ptr(), _FLOATS[x.dtype], _nat.ptr(r), M, C, _nat.ptr(w),
+                                           _FLOATS[w.dtype] if w is not None else _nat.PN_F32, eps, _nat.ptr(h),
+                                           y.data_ptr(), _FLOATS[out_dtype], _nat.stream_of(x)), "rms_norm")
+    return y if h is None else (y, h)
+
+
+def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6,
+                residual: torch.Tensor | None = None):
+    """rms_norm with its output quantised per token for penta_linear_i8_prequant:
+    (xq, s_x, rowsum), with a residual (xq, s_x, rowsum, h).  The values are those
+    of quantize_activations_i8(rms_norm(x, ..., out_dtype=torch.float32)), in one
+    pass over x; xq is (M, pitch) int8 zero-padded past C.  A row that holds an
+    inf or NaN gets s_x = NaN.  Not in the reference."""
+    xc, r, h, w, M, C = _rms_args(x, weight, residual, "rms_norm_i8")
+    pitch = (C + 31) // 32 * 32  # pn_act_i8_pitch
+    xq = torch.empty(M, pitch, dtype=torch.int8, device=x.device)
+    s_x = torch.empty(M, dtype=torch.float32, device=x.device)
+    rowsum = torch.empty(M, dtype=torch.int32, device=x.device)
+    with _nat.device_of(x):
+        _nat.check(_nat.load().pn_rms_norm_i8(xc.data_ptr(), _FLOATS[x.dtype], _nat.ptr(r), M, C, _nat.ptr(w),
+                                              _FLOATS[w.dtype] if w is not None else _nat.PN_F32, eps, _nat.ptr(h),
+                                              xq.data_ptr(), pitch, s_x.data_ptr(), rowsum.data_ptr(),
+                                              _nat.stream_of(x)), "rms_norm_i8")
+    return (xq, s_x, rowsum) if h is None else (xq, s_x, rowsum, h)
+
+
+# ── Sampling ─────────────────────────────────────────────────────────────────
+
+_MAX_VOCAB = 1 << 18
+
+
+def _setting(v, rows, dtype, device, what):
+    """A sampling setting as (tensor or None, number)."""
+    if isinstance(v, torch.Tensor):
+        assert v.dtype == dtype and v.device == device and v.shape == (rows,), \
+            f"sample_tokens: {what} is a number or a ({rows},) {dtype} tensor on the logits' device"
+        return v.contiguous(), 0
+    return None, v
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0
+                  ) -> torch.Tensor:
+    """One token per row of logits (B, V), bf16/fp32 CUDA, from uniform numbers u
+    (B,) float32 in [0, 1); returns (B,) int64.
+
+    With w = exp((x - max) / temperature): the top_k largest logits are kept
+    (ties: lowest index first; 0 keeps all), of them those with w >= min_p, of
+    them the smallest prefix in that order whose sum reaches top_p of the sum of
+    all left (at least one); the token is the first index whose running sum of kept w exceeds
+    u times their sum.  The same inputs always give the same token.
+
+    temperature (0 takes the first largest logit), top_p and min_p are numbers or
+    (B,) float32 tensors, top_k a number or a (B,) int32 tensor.  NaN logits are
+    never drawn; a row with nothing above -inf gives -1.  V is at most 2^18.
+    Not in the reference."""
+    assert logits.dim() == 2 and logits.dtype in _FLOATS, "logits must be a (B, V) bfloat16 or float32 tensor"
+    _require_cuda(logits, "sample_tokens")
+    B, V = logits.shape
+    assert 0 < V <= _MAX_VOCAB, f"the vocabulary must hold 1 to {_MAX_VOCAB} tokens, got {V}"
+    assert u.dtype == torch.float32 and u.device == logits.device and u.shape == (B,), \
+        f"u must be a ({B},) float32 tensor on the logits' device"
+    dev = logits.device
+    t, t0 = _setting(temperature, B, torch.float32, dev, "temperature")
+    k, k0 = _setting(top_k, B, torch.int32, dev, "top_k")
+    p, p0 = _setting(top_p, B, torch.float32, dev, "top_p")
+    m, m0 = _setting(min_p, B, torch.float32, dev, "min_p")
+    assert t0 >= 0 and k0 >= 0 and 0 <= p0 and 0 <= m0 <= 1, "settings out of range"
+    if logits.stride(1) != 1 or logits.stride(0) < V:
+        logits = logits.contiguous()
+    u = u.contiguous()
+    out = torch.empty(B, dtype=torch.int64, device=dev)
+    with _nat.device_of(logits):
+        _nat.check(_nat.load().pn_sample_tokens(logits.data_ptr(), _FLOATS[logits.dtype], B, V, max(logits.stride(0), V),
+                                                u.data_ptr(), _nat.ptr(t), t0, _nat.ptr(k), min(int(k0), 0x7fffffff),
+                                                _nat.ptr(p), p0, _nat.ptr(m), m0, out.data_ptr(),
+                                                _nat.stream_of(logits)), "sample_tokens")
+    return out
+
+
 # ── int8 activation path ─────────────────────────────────────────────────────
 
 def quantize_activations_i8(x: torch.Tensor):

@@ -33,6 +33,8 @@ EXPORTS = (
     "pn_linear_bf16_peers", "pn_peer_barrier", "pn_peer_barrier_wait", "pn_set_gemv_max_tokens",
     "pn_set_limb_max_tokens", "pn_matmul_i8w",
     "pn_words_2bit", "pn_quantize_pack_2bit", "pn_unpack_2bit", "pn_linear_bf16_2bit",
+    "pn_rms_norm", "pn_rms_norm_i8", "pn_kv4_block_bytes", "pn_kv4_append", "pn_kv4_gather",
+    "pn_kv4_attention_workspace_size", "pn_kv4_attention", "pn_sample_tokens",
 )
 
 _lib = None
@@ -57,6 +59,7 @@ def load() -> ctypes.CDLL:
                           f"or `make -C {HERE}`")
     L = ctypes.CDLL(path)
     P, I, I64, F, SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+    D = ctypes.c_double
     sig = {
         "pn_abi_version": (I, []),
         "pn_status_string": (ctypes.c_char_p, [I]),
@@ -94,6 +97,16 @@ def load() -> ctypes.CDLL:
         "pn_quantize_pack_2bit": (I, [P, I, I64, I64, P, P, P]),
         "pn_unpack_2bit": (I, [P, I64, I64, I64, P, P]),
         "pn_linear_bf16_2bit": (I, [P, I64, I64, P, I64, I64, F, P, P, I, P]),
+        "pn_rms_norm": (I, [P, I, P, I64, I64, P, I, D, P, P, I, P]),
+        "pn_rms_norm_i8": (I, [P, I, P, I64, I64, P, I, D, P, P, I64, P, P, P]),
+        "pn_kv4_block_bytes": (I64, [I64, I64]),
+        "pn_kv4_append": (I, [P, I64, I64, I64, P, I64, I64, I64, I, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64,
+                              P]),
+        "pn_kv4_gather": (I, [P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, P, I, P]),
+        "pn_kv4_attention_workspace_size": (SZ, [I64, I64, I64, I64, I64]),
+        "pn_kv4_attention": (I, [P, I64, I64, I64, I, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, F, P, P,
+                                 SZ, P]),
+        "pn_sample_tokens": (I, [P, I, I64, I64, I64, P, P, F, P, ctypes.c_int32, P, F, P, F, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -125,6 +138,25 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+class _SameDevice:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_same_device = _SameDevice()
+
+
+def device_of(t: torch.Tensor):
+    """Context in which t's device is the current one (free where it already is)."""
+    return _same_device if t.device.index == _get_device() else torch.cuda.device(t.device)
 
 
 @functools.lru_cache(maxsize=4096)
