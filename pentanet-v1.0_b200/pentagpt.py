@@ -21,6 +21,12 @@ throughput measurement; a trained reference model converts with
 `pentanet_layer.convert_to_fast_inference`, which packs the same layers.
 Forward without targets returns the logits of the last position only, as the
 reference does (train_pentagpt.py:129-134).
+
+`generate` continues prompts token by token.  Keys and values of past tokens are
+kept in 4 bits (penta_cache), so a step computes the new tokens only:
+`forward(idx, cache=...)` appends a chunk's keys and values and attends over the
+cache, for prompts, for prompts in pieces and for single tokens alike; each
+token is drawn by penta_kernel.sample_tokens.
 """
 from __future__ import annotations
 
@@ -33,9 +39,11 @@ import torch.nn.functional as F
 
 try:
     from .pentanet_layer import PentaLinearFast
+    from . import penta_cache as pc
     from . import penta_kernel as pk
 except ImportError:
     from pentanet_layer import PentaLinearFast
+    import penta_cache as pc
     import penta_kernel as pk
 
 
@@ -68,15 +76,20 @@ class _Block(nn.Module):
         self.c_fc = _packed(weights["c_fc"], act_quant)
         self.mlp_proj = _packed(weights["mlp_proj"], act_quant)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, layer: torch.Tensor | None = None, cache: "PentaGPTCache | None" = None
+                ) -> torch.Tensor:
         B, T, C = x.shape
         h = pk.layer_norm(x, self.ln_1.weight, self.ln_1.bias, self.ln_1.eps)
         q, k, v = self.c_attn(h).split(C, dim=2)
-        q = q.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
-        k = k.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
-        v = v.view(B, T, self.n_head, C // self.n_head).transpose(1, 2)
-        y = F.scaled_dot_product_attention(q, k, v, is_causal=True)
-        y = y.transpose(1, 2).contiguous().view(B, T, C)
+        q = q.view(B, T, self.n_head, C // self.n_head)
+        k = k.view(B, T, self.n_head, C // self.n_head)
+        v = v.view(B, T, self.n_head, C // self.n_head)
+        if cache is None:
+            y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
+            y = y.transpose(1, 2).contiguous().view(B, T, C)
+        else:
+            pc.kv4_append(k, v, layer, cache.block_table, cache.seq_lens)
+            y = pc.kv4_attention(q, layer, cache.block_table, cache.seq_lens).view(B, T, C)
         if B * T <= FUSE_MAX_TOKENS:
             x = self.attn_proj(y, residual=x)  # x + attn(ln_1(x)), train_pentagpt.py:100
             h = pk.layer_norm(x, self.ln_2.weight, self.ln_2.bias, self.ln_2.eps)
@@ -84,6 +97,26 @@ class _Block(nn.Module):
         x = x + self.attn_proj(y)
         h = pk.layer_norm(x, self.ln_2.weight, self.ln_2.bias, self.ln_2.eps)
         return x + self.mlp_proj(F.gelu(self.c_fc(h)))
+
+
+class PentaGPTCache:
+    """The past tokens of a batch: a 4-bit cache per layer (penta_cache), their
+    pages and the sequences' lengths.  The pages are handed out up front;
+    seq_lens lives on the GPU, so a captured step goes on where it stands."""
+
+    def __init__(self, cfg: PentaGPTConfig, batch: int, device, max_tokens: int | None = None, page_size: int = 64):
+        self.capacity = cfg.block_size if max_tokens is None else max_tokens
+        pages = -(-self.capacity // page_size)
+        self.layers = [pc.kv4_cache(batch * pages, cfg.n_head, cfg.n_embd // cfg.n_head, page_size, device)
+                       for _ in range(cfg.n_layer)]
+        self.block_table = torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages)
+        self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.length = 0  # what the host knows: tokens appended so far
+
+    def reset(self) -> None:
+        """Forget all tokens (their pages are written over)."""
+        self.seq_lens.zero_()
+        self.length = 0
 
 
 class PentaGPTFast(nn.Module):
@@ -124,15 +157,50 @@ class PentaGPTFast(nn.Module):
     def n_packed_params(self) -> int:
         return sum(m.packed_w.shape[0] * m.K_orig for m in self.modules() if isinstance(m, PentaLinearFast))
 
+    def new_cache(self, batch: int, max_tokens: int | None = None, page_size: int = 64) -> PentaGPTCache:
+        """An empty cache for `batch` sequences of up to max_tokens (block_size)."""
+        return PentaGPTCache(self.cfg, batch, self.wte.weight.device, max_tokens, page_size)
+
     @torch.no_grad()
-    def forward(self, idx: torch.Tensor, all_logits: bool = False) -> torch.Tensor:
+    def forward(self, idx: torch.Tensor, all_logits: bool = False, cache: PentaGPTCache | None = None) -> torch.Tensor:
+        """Logits of the last position (all with all_logits).  With a cache, idx
+        holds the tokens that follow those in it; their keys and values are added
+        and attention runs over the cache."""
         B, T = idx.shape
-        assert T <= self.cfg.block_size
-        pos = torch.arange(T, device=idx.device)
+        if cache is None:
+            assert T <= self.cfg.block_size
+            pos = torch.arange(T, device=idx.device)
+        else:
+            assert B == cache.seq_lens.shape[0], f"{B} sequences, the cache holds {cache.seq_lens.shape[0]}"
+            assert cache.length + T <= min(cache.capacity, self.cfg.block_size), "the cache is full"
+            # (a captured step replayed past the block stays at its last position)
+            pos = (cache.seq_lens[:, None] + torch.arange(T, device=idx.device)).clamp(max=self.cfg.block_size - 1)
+            cache.seq_lens += T
+            cache.length += T
         x = (self.wte(idx) + self.wpe(pos)).to(torch.bfloat16)
-        for block in self.h:
-            x = block(x)
+        for i, block in enumerate(self.h):
+            x = block(x) if cache is None else block(x, cache.layers[i], cache)
         if not all_logits:
-            x = x[:, [-1], :]  # LayerNorm is per position: normalise only what the lm_head reads
+            x = x[:, -1:, :]  # LayerNorm is per position: normalise only what the lm_head reads
         x = pk.layer_norm(x, self.ln_f.weight, self.ln_f.bias, self.ln_f.eps)
         return self.lm_head(x)
+
+    @torch.no_grad()
+    def generate(self, idx: torch.Tensor, max_new_tokens: int, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                 generator: torch.Generator | None = None, cache: PentaGPTCache | None = None) -> torch.Tensor:
+        """idx (B, T) with max_new_tokens sampled tokens behind it: (B, T +
+        max_new_tokens).  The settings are those of penta_kernel.sample_tokens
+        (temperature=0: the most likely token), its uniform numbers come from
+        `generator`.  With a cache from an earlier call, idx holds what follows
+        the tokens in it (the last token returned is not in it yet)."""
+        B, T = idx.shape
+        assert T >= 1 and max_new_tokens >= 0
+        cache = cache if cache is not None else self.new_cache(B, min(T + max_new_tokens, self.cfg.block_size))
+        assert cache.length + T + max(max_new_tokens - 1, 0) <= min(cache.capacity, self.cfg.block_size), \
+            f"{cache.length} + {T} + {max_new_tokens} tokens do not fit the model's block or the cache"
+        out = [idx]
+        u = torch.rand(max_new_tokens, B, device=idx.device, generator=generator)
+        for i in range(max_new_tokens):
+            logits = self(out[-1].clamp(min=0), cache=cache)  # -1: a row of NaN logits has no token
+            out.append(pk.sample_tokens(logits[:, 0], u[i], temperature, top_k, top_p, min_p)[:, None])
+        return torch.cat(out, dim=1)

@@ -153,3 +153,94 @@ def test_pentagpt_fast_matches_reference(cuda_device, name):
     got = model(idx.to(cuda_device))[:, 0].float().cpu()
     assert _rel(got, ref32) <= 3 * _rel(refbf, ref32), (_rel(got, ref32), _rel(refbf, ref32))
     assert (got - ref32).abs().max() <= 3 * (refbf - ref32).abs().max()
+
+
+def _cached_forward_f64(model, idx):
+    """The network with keys and values rounded to their 4-bit form, attention in float64."""
+    import kv4_oracle
+    cfg = model.cfg
+    B, T = idx.shape
+    C, H = cfg.n_embd, cfg.n_head
+    x = (model.wte(idx) + model.wpe(torch.arange(T, device=idx.device))).to(torch.bfloat16)
+    for blk in model.h:
+        h = pk.layer_norm(x, blk.ln_1.weight, blk.ln_1.bias, blk.ln_1.eps)
+        q, k, v = (t.view(B, T, H, C // H) for t in blk.c_attn(h).split(C, dim=2))
+        y = torch.stack([kv4_oracle.attention(q[b], k[b], v[b])[0] for b in range(B)])
+        x = x + blk.attn_proj(y.to(torch.bfloat16).to(idx.device).view(B, T, C))
+        h = pk.layer_norm(x, blk.ln_2.weight, blk.ln_2.bias, blk.ln_2.eps)
+        x = x + blk.mlp_proj(F.gelu(blk.c_fc(h)))
+    return model.lm_head(pk.layer_norm(x, model.ln_f.weight, model.ln_f.bias, model.ln_f.eps))
+
+
+@pytest.mark.parametrize("act_quant", [None, "int8"])
+def test_cached_forward(cuda_device, act_quant):
+    """A prompt at once, in pieces, and token by token over the 4-bit cache, against
+    the same network with attention from the definition."""
+    cfg = PentaGPTConfig(n_layer=2, n_head=2, n_embd=128, block_size=160, vocab_size=700)
+    model = PentaGPTFast.random(cfg, seed=3, device=cuda_device, act_quant=act_quant)
+    idx = torch.randint(0, cfg.vocab_size, (3, 83), generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    want = _cached_forward_f64(model, idx).float()
+    tol = 2e-2 * want.abs().max().item() + 1e-3  # as the dense comparison above: bf16 through the whole network
+    for cuts in ([83], [40, 43], [70] + [1] * 13, [64, 3, 16]):
+        cache = model.new_cache(3, page_size=32)
+        got = torch.cat([model(p, all_logits=True, cache=cache) for p in idx.split(cuts, dim=1)], 1).float()
+        assert cache.seq_lens.tolist() == [83] * 3 and cache.length == 83
+        assert (got - want).abs().max().item() <= tol, cuts
+    cache.reset()
+    assert (model(idx, cache=cache).float()[:, 0] - want[:, -1]).abs().max().item() <= tol
+
+
+def test_generate(cuda_device):
+    cfg = PentaGPTConfig(n_layer=2, n_head=2, n_embd=128, block_size=96, vocab_size=700)
+    model = PentaGPTFast.random(cfg, seed=3, device=cuda_device)
+    idx = torch.randint(0, cfg.vocab_size, (4, 20), generator=torch.Generator().manual_seed(5)).to(cuda_device)
+    kw = dict(temperature=0.8, top_k=40, top_p=0.95, min_p=0.01)
+    rng = lambda: torch.Generator(device=cuda_device).manual_seed(9)
+    out = model.generate(idx, 30, generator=rng(), **kw)
+    assert out.shape == (4, 50) and torch.equal(out[:, :20], idx) and 0 <= out.min() and out.max() < cfg.vocab_size
+    assert torch.equal(out, model.generate(idx, 30, generator=rng(), **kw))
+    # the steps by hand
+    cache, u, step = model.new_cache(4, 50), torch.rand(30, 4, device=cuda_device, generator=rng()), idx
+    for i in range(30):
+        step = pk.sample_tokens(model(step, cache=cache)[:, 0], u[i], **kw)[:, None]
+        assert torch.equal(step, out[:, 20 + i:21 + i])
+    # greedy: the largest logit; and going on with the cache of an earlier call
+    greedy = model.generate(idx, 12, temperature=0.0)
+    cache = model.new_cache(4)
+    first = model.generate(idx, 5, temperature=0.0, cache=cache)
+    assert torch.equal(model.generate(first[:, -1:], 7, temperature=0.0, cache=cache)[:, 1:], greedy[:, 25:])
+    assert model.generate(idx, 0).shape == (4, 20)
+    with pytest.raises(AssertionError, match="do not fit"):
+        model.generate(idx, 78)
+    assert model.generate(idx, 77).shape == (4, 97)  # the last token is never fed back
+
+
+def test_captured_decode_step(cuda_device):
+    """One decode step (append, attention, products, sampling) captured once and
+    replayed: the lengths on the GPU carry it on."""
+    cfg = PentaGPTConfig(n_layer=2, n_head=2, n_embd=128, block_size=96, vocab_size=700)
+    model = PentaGPTFast.random(cfg, seed=3, device=cuda_device)
+    idx = torch.randint(0, cfg.vocab_size, (2, 15), generator=torch.Generator().manual_seed(5)).to(cuda_device)
+    want = model.generate(idx, 20, temperature=0.0)
+    cache = model.new_cache(2)
+    tok, u = model.generate(idx, 2, temperature=0.0, cache=cache)[:, -1:].clone(), torch.zeros(2, device=cuda_device)
+    got = [tok.clone()]
+    keep = cache.seq_lens.clone()
+
+    def step():
+        tok.copy_(pk.sample_tokens(model(tok, cache=cache)[:, 0], u, temperature=0.0)[:, None])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    cache.seq_lens.copy_(keep)
+    tok.copy_(got[0])
+    for _ in range(18):
+        graph.replay()
+        got.append(tok.clone())
+    assert torch.equal(torch.cat(got, 1), want[:, 16:])
