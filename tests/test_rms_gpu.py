@@ -120,6 +120,18 @@ def test_zero_rows_and_rows_that_are_not_finite(cuda_device, C, dtype):
     assert torch.isfinite(y[0]).all() and torch.isfinite(y[5]).all()
 
 
+@pytest.mark.parametrize("C", [512, 1001])
+def test_tiny_values(cuda_device, C):
+    """Rows whose scale is a subnormal number, or rounds to zero."""
+    x, _, _ = _inputs(6, C, torch.float32, 2, cuda_device)
+    w = torch.full((C,), 1e-38, device=cuda_device)
+    for k, size in enumerate((1.0, 1e-3, 1e-5, 1e-6, 3e-7, 1e-8)):
+        y = pk.rms_norm(x, w * size, 1e-6, out_dtype=torch.float32)
+        xq, s, total = pk.rms_norm_i8(x, w * size, 1e-6)
+        want = pk.quantize_activations_i8(y)
+        assert torch.equal(xq, want[0]) and torch.equal(s, want[1]) and torch.equal(total, want[2]), size
+
+
 def test_residual_stream_in_place(cuda_device):
     """The C ABI may write the stream over x or over the residual."""
     for dtype, C in ((torch.bfloat16, 1024), (torch.float32, 1001), (torch.bfloat16, 40000)):
