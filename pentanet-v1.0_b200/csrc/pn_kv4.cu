@@ -113,43 +113,113 @@ __device__ __forceinline__ void kv4_load8(const T* p, bool vec, float (&v)[8]) {
     }
 }
 
+// Where a row lives, looked up once per row and block.
+struct Kv4Row {
+    int64_t src[2];  // first element of its keys and values in the inputs
+    int64_t page;    // page of the cache; -1: none; -2: behind the last sequence
+    int tok;         // its place in the page
+};
+constexpr int kKv4Threads = 256;
+constexpr int kKv4MaxRows = 8;  // rows per block
+
+// A block's vectors are numbered row by row, a row's keys before its values; a
+// thread steps from one to the next without a division.
+struct Kv4Step {
+    int per_row;  // 2 * kv heads
+    int dr, dh;   // 256 / lanes per vector, as whole rows and the rest
+};
+struct Kv4At {
+    int r, hv;  // row in the block; head, or Hk + head
+    __device__ __forceinline__ Kv4At(const Kv4Step& s, int vec) : r(vec / s.per_row), hv(vec - r * s.per_row) {}
+    __device__ __forceinline__ void next(const Kv4Step& s) {
+        r += s.dr;
+        hv += s.dh;
+        if (hv >= s.per_row) {
+            hv -= s.per_row;
+            ++r;
+        }
+    }
+};
+
+__device__ __forceinline__ void kv4_rows_of_block(const Kv4Seq& s, int64_t row0, int n, const int64_t* sb, const int64_t* sl,
+                                                  Kv4Row* rows) {
+    if ((int)threadIdx.x < n) {
+        Kv4Row r;
+        const int64_t row = row0 + threadIdx.x;
+        int64_t b, i;
+        r.page = -2;
+        r.tok = 0;
+        if (kv4_find(s, row, b, i)) {
+            int64_t first, count;
+            kv4_rows(s, b, first, count);
+            const int pos = (int)(kv4_len(s, b) - count + i);
+            r.page = -1;
+            if (pos >= 0) {
+                r.page = kv4_page(s, b, pos);
+                r.tok = pos % s.page;
+            }
+            if (sb)
+                for (int kv = 0; kv < 2; ++kv) r.src[kv] = s.cu ? row * sl[kv] : b * sb[kv] + i * sl[kv];
+        }
+        rows[threadIdx.x] = r;
+    }
+    __syncthreads();
+}
+
 struct Kv4AppendArgs {
     Kv4Seq s;
-    const void* x[2];           // keys, values
+    const void* x[2];             // keys, values
     int64_t sb[2], sl[2], sh[2];  // their strides in elements: sequence, row, head
-    int vec;                    // 16-byte loads allowed
+    int vec;                      // 16-byte loads allowed
+    int rows;                     // per block
+    Kv4Step step;
     uint8_t* cache;
 };
 
-constexpr int kKv4Threads = 256;
-
-// D / 8 lanes per vector, eight dims each.
-template <typename T, int D>
-__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4AppendArgs a) {
-    asm volatile("griddepcontrol.launch_dependents;");
-    constexpr int VT = D / 8;
-    const int64_t vec = ((int64_t)blockIdx.x * kKv4Threads + threadIdx.x) / VT;
-    const int l = threadIdx.x % VT;
-    const int kv = (int)(vec & 1);
-    const int64_t rh = vec >> 1;
-    const int64_t row = rh / a.s.Hk;
-    const int head = (int)(rh - row * a.s.Hk);
-    int64_t b = 0, i = 0;
-    bool live = row < a.s.T && kv4_find(a.s, row, b, i);
-    int64_t page = -1;
-    int pos = -1;
-    float v[8];
+// Eight codes of a vector as nibbles: c_j = rint((v_j - z) / s), IEEE division,
+// ties to even.  With bf16 inputs quotients that are exact half-integers are
+// common (about one in 10^2), so the borders are decided exactly, without a
+// division: h is the quotient in half steps, e = d - h * s / 2 is exact (h * s has
+// 13 bits and cancels the head of d), and h / 2 + e / s, rounded to an integer,
+// goes the way that the sign of e says, or to even where e is 0.  (s has 8 bits, so
+// a quotient that is no half-integer lies at least ulp(d) / s away from one: more
+// than half an ulp of the quotient, neither the rounding of h / 2 + e / s nor that
+// of the IEEE quotient reaches the border.)  s >= (max - z) / 15 keeps c within
+// 0 .. 15.
+__device__ __forceinline__ uint32_t kv4_codes8(const float (&v)[8], float s, float z) {
+    float rs;  // within an ulp
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(rs) : "f"(s));
+    const float2 up = make_float2(kRoundMagic, kRoundMagic), down = make_float2(-kRoundMagic, -kRoundMagic);
+    float2 q[4];
+    if (rs >= 0x1p-125f && rs <= 0x1p125f) {
+        const float2 z2 = make_float2(-z, -z), rs1 = make_float2(rs, rs), rs2 = make_float2(2.0f * rs, 2.0f * rs);
+        const float2 half_s = make_float2(-0.5f * s, -0.5f * s), half = make_float2(0.5f, 0.5f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    if (live) {
-        int64_t first, n;
-        kv4_rows(a.s, b, first, n);
-        pos = (int)(kv4_len(a.s, b) - n + i);
-        if (pos >= 0) page = kv4_page(a.s, b, pos);
-        const T* x = static_cast<const T*>(a.x[kv]) + (a.s.cu ? row * a.sl[kv] : b * a.sb[kv] + i * a.sl[kv]) +
-                     head * a.sh[kv] + l * 8;
-        kv4_load8(x, a.vec, v);
+        for (int j = 0; j < 4; ++j) {
+            const float2 d = add2(make_float2(v[j], v[j + 4]), z2);
+            const float2 h = add2(fma2(d, rs2, up), down);
+            const float2 e = fma2(h, half_s, d);
+            q[j] = add2(add2(fma2(e, rs1, mul2(h, half)), up), down);
+        }
+    } else {  // 1/s or its neighbours are no normal numbers
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            q[j].x = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[j], z), s)), 0.0f), 15.0f);
+            q[j].y = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[j + 4], z), s)), 0.0f), 15.0f);
+        }
     }
+    // q0 + 16 (q1 + 16 (q2 + 16 q3)): exact below 2^16, and the integer is in the low bits of a sum with 2^23
+    const float2 sixteen = make_float2(16.0f, 16.0f);
+    const float2 w = add2(fma2(fma2(fma2(q[3], sixteen, q[2]), sixteen, q[1]), sixteen, q[0]),
+                          make_float2(8388608.0f, 8388608.0f));
+    return __byte_perm(__float_as_uint(w.x), __float_as_uint(w.y), 0x5410);
+}
+
+// The range of VT lanes' values, a NaN among them kept: (min, max).
+template <int VT>
+__device__ __forceinline__ float2 kv4_range(const Raw8<float>& x) {
+    float v[8];
+    x.get(v);
     float lo = v[0], hi = v[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) {
@@ -161,34 +231,88 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4Append
         lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    if (page < 0) return;
-    float z = floor_bf16(lo);
-    float s = ceil_bf16_pos(__fdiv_rn(__fsub_rn(hi, z), 15.0f));
-    if (!(s < INFINITY) || !(fabsf(z) < INFINITY)) {  // an inf or NaN in the vector: all of it reads back as NaN
-        s = 0.0f;
-        z = __int_as_float(0x7fc00000);
-    }
-    uint32_t w = 0;
-    if (s > 0.0f) {
+    return make_float2(lo, hi);
+}
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// bf16: (min, -max) share a register, one shuffle and one minimum per step.
+template <int VT>
+__device__ __forceinline__ float2 kv4_range(const Raw8<__nv_bfloat16>& x) {
+    constexpr uint32_t kNeg = 0x80008000u;
+    const uint4 u = x.u;
+    const uint32_t lo = min2_nan(min2_nan(u.x, u.y), min2_nan(u.z, u.w));
+    const uint32_t hi = min2_nan(min2_nan(u.x ^ kNeg, u.y ^ kNeg), min2_nan(u.z ^ kNeg, u.w ^ kNeg));
+    uint32_t r = min2_nan(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float q = rintf(__fdiv_rn(__fsub_rn(v[j], z), s));
-            w |= (uint32_t)fminf(fmaxf(q, 0.0f), 15.0f) << (4 * j);
-        }
-    }
-    const int tok = pos % a.s.page;
+    for (int o = VT / 2; o > 0; o >>= 1) r = min2_nan(r, __shfl_xor_sync(0xffffffffu, r, o));
+    return make_float2(__uint_as_float(r << 16), __uint_as_float((r & 0xFFFF0000u) ^ 0x80000000u));
+}
+
+// D / 8 lanes per vector, eight dims each; a block takes a few rows with all
+// their heads, the next vector's values in flight while one is stored.  One read
+// of the inputs; what bounds it beside the bytes is the instructions per eight
+// values (the range's shuffles, scale and codes).
+template <typename T, int D>
+__global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4AppendArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    constexpr int VT = D / 8, kVecs = kKv4Threads / VT;
+    __shared__ Kv4Row rows[kKv4MaxRows];
+    const int64_t row0 = (int64_t)blockIdx.x * a.rows;
+    const int n_rows = (int)min((int64_t)a.rows, a.s.T - row0);
+    kv4_rows_of_block(a.s, row0, n_rows, a.sb, a.sl, rows);
+    const int l = threadIdx.x % VT;
     const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
-    uint8_t* blk = a.cache + ((page * a.s.Hk + head) * 2 + kv) * block;
-    if (kv == 0) {
-        *reinterpret_cast<uint32_t*>(blk + tok * (D / 2) + l * 4) = w;
-    } else {
-        uint8_t* p = blk + (tok >> 1) * D + l * 8 + (tok & 1) * 2;
-        *reinterpret_cast<uint16_t*>(p) = (uint16_t)w;
-        *reinterpret_cast<uint16_t*>(p + 4) = (uint16_t)(w >> 16);
+
+    Kv4At at(a.step, threadIdx.x / VT);
+    auto load = [&](Raw8<T>& x) {
+        x.zero();
+        if (at.r >= n_rows || rows[at.r].page < 0) return;
+        const bool kv = at.hv >= a.s.Hk;
+        const T* p = static_cast<const T*>(kv ? a.x[1] : a.x[0]) + rows[at.r].src[kv] + l * 8 +
+                     (kv ? (at.hv - a.s.Hk) * a.sh[1] : at.hv * a.sh[0]);
+        if (a.vec) {
+            x.load(p);
+        } else {
+            float v[8];
+            kv4_load8(p, false, v);
+            x.set(v);
+        }
+    };
+    Raw8<T> x;
+    load(x);
+    for (int base = 0; base < n_rows * a.step.per_row; base += kVecs) {
+        const Raw8<T> now = x;
+        const Kv4At was = at;
+        at.next(a.step);
+        load(x);
+        const float2 range = kv4_range<VT>(now);
+        if (was.r >= n_rows || rows[was.r].page < 0) continue;
+        const int kv = was.hv >= a.s.Hk ? 1 : 0;
+        float z = floor_bf16(range.x);
+        float s = ceil_bf16_pos(__fdiv_rn(__fsub_rn(range.y, z), 15.0f));
+        if (!(s < INFINITY) || !(fabsf(z) < INFINITY)) {  // an inf or NaN in the vector: all of it reads back as NaN
+            s = 0.0f;
+            z = __int_as_float(0x7fc00000);
+        }
+        float v[8];
+        now.get(v);
+        const uint32_t w = s > 0.0f ? kv4_codes8(v, s, z) : 0;
+        const int tok = rows[was.r].tok;
+        uint8_t* blk = a.cache + (rows[was.r].page * a.step.per_row + (kv ? 2 * (was.hv - a.s.Hk) + 1 : 2 * was.hv)) * block;
+        if (kv == 0) {
+            *reinterpret_cast<uint32_t*>(blk + tok * (D / 2) + l * 4) = w;
+        } else {
+            uint8_t* p = blk + (tok >> 1) * D + l * 8 + (tok & 1) * 2;
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)w;
+            *reinterpret_cast<uint16_t*>(p + 4) = (uint16_t)(w >> 16);
+        }
+        if (l == 0)
+            *reinterpret_cast<uint32_t*>(blk + (int64_t)a.s.page * (D / 2) + tok * 4) =
+                (__float_as_uint(s) >> 16) | (__float_as_uint(z) & 0xFFFF0000u);
     }
-    if (l == 0)
-        *reinterpret_cast<uint32_t*>(blk + (int64_t)a.s.page * (D / 2) + tok * 4) =
-            (__float_as_uint(s) >> 16) | (__float_as_uint(z) & 0xFFFF0000u);
 }
 
 struct Kv4GatherArgs {
@@ -196,58 +320,82 @@ struct Kv4GatherArgs {
     const uint8_t* cache;
     void* y[2];
     int y_f32;
+    int rows;  // per block
+    Kv4Step step;
 };
 
 template <int D>
 __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4GatherArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
     constexpr int VT = D / 8;
-    const int64_t vec = ((int64_t)blockIdx.x * kKv4Threads + threadIdx.x) / VT;
+    __shared__ Kv4Row rows[kKv4MaxRows];
+    const int64_t row0 = (int64_t)blockIdx.x * a.rows;
+    const int n_rows = (int)min((int64_t)a.rows, a.s.T - row0);
+    kv4_rows_of_block(a.s, row0, n_rows, nullptr, nullptr, rows);
     const int l = threadIdx.x % VT;
-    const int kv = (int)(vec & 1);
-    const int64_t rh = vec >> 1;
-    const int64_t row = rh / a.s.Hk;
-    const int head = (int)(rh - row * a.s.Hk);
-    int64_t b, i;
-    if (row >= a.s.T || !kv4_find(a.s, row, b, i)) return;
-    int64_t first, n;
-    kv4_rows(a.s, b, first, n);
-    const int pos = (int)(kv4_len(a.s, b) - n + i);
-    const int64_t page = pos >= 0 ? kv4_page(a.s, b, pos) : -1;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    if (page >= 0) {
-        const int tok = pos % a.s.page;
-        const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
-        const uint8_t* blk = a.cache + ((page * a.s.Hk + head) * 2 + kv) * block;
-        const uint32_t pair = *reinterpret_cast<const uint32_t*>(blk + (int64_t)a.s.page * (D / 2) + tok * 4);
-        uint32_t w;
-        if (kv == 0) {
+    const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
+    Kv4At at(a.step, threadIdx.x / VT);
+    uint32_t w = 0, pair = 0;  // the next vector's codes and (scale, zero)
+    auto load = [&]() {
+        w = pair = 0;  // stands for zeros
+        if (at.r >= n_rows || rows[at.r].page < 0) return;
+        const bool kv = at.hv >= a.s.Hk;
+        const int tok = rows[at.r].tok;
+        const uint8_t* blk = a.cache + (rows[at.r].page * a.step.per_row + (kv ? 2 * (at.hv - a.s.Hk) + 1 : 2 * at.hv)) * block;
+        pair = *reinterpret_cast<const uint32_t*>(blk + (int64_t)a.s.page * (D / 2) + tok * 4);
+        if (!kv) {
             w = *reinterpret_cast<const uint32_t*>(blk + tok * (D / 2) + l * 4);
         } else {
-            const uint8_t* p = blk + (tok >> 1) * D + l * 8 + (tok & 1) * 2;
-            w = *reinterpret_cast<const uint16_t*>(p) | (uint32_t) * reinterpret_cast<const uint16_t*>(p + 4) << 16;
+            const uint2 two = *reinterpret_cast<const uint2*>(blk + (tok >> 1) * D + l * 8);
+            w = __byte_perm(two.x, two.y, tok & 1 ? 0x7632 : 0x5410);
         }
-        const float s = __uint_as_float(pair << 16), z = __uint_as_float(pair & 0xFFFF0000u);
+    };
+    load();
+    while (at.r < n_rows) {
+        const uint32_t now_w = w, now_pair = pair;
+        const Kv4At was = at;
+        at.next(a.step);
+        load();
+        if (rows[was.r].page == -2) continue;
+        const bool kv = was.hv >= a.s.Hk;
+        const float s = __uint_as_float(now_pair << 16), z = __uint_as_float(now_pair & 0xFFFF0000u);
+        // masked into the low bits of 2^23 a code reads as 2^23 + 16^j c; s * c is exact (12 bits), so one rounding
+        float v[8];
+        const float2 z2 = make_float2(z, z), down = make_float2(-8388608.0f, -8388608.0f);
+        float sj = s;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fmaf(s, (float)(w >> (4 * j) & 15u), z);  // s * c is exact: one rounding
-    }
-    const int64_t at = (row * a.s.Hk + head) * D + l * 8;
-    void* out = kv ? a.y[1] : a.y[0];
-    if (a.y_f32) {
-        float4* y = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-        y[0] = make_float4(v[0], v[1], v[2], v[3]);
-        y[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        uint32_t u[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
-            u[k] = *reinterpret_cast<const uint32_t*>(&h);
+        for (int j = 0; j < 4; ++j) {
+            const float2 c = make_float2(__uint_as_float((now_w & (15u << (4 * j))) | 0x4B000000u),
+                                         __uint_as_float(((now_w >> 16) & (15u << (4 * j))) | 0x4B000000u));
+            const float2 y = fma2(add2(c, down), make_float2(sj, sj), z2);
+            v[j] = y.x, v[j + 4] = y.y;
+            sj *= 0.0625f;
         }
-        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(out) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+        const int64_t to = ((row0 + was.r) * a.s.Hk + was.hv - (kv ? a.s.Hk : 0)) * D + l * 8;
+        void* out = kv ? a.y[1] : a.y[0];
+        if (a.y_f32) {
+            Raw8<float> o;
+            o.set(v);
+            o.store(static_cast<float*>(out) + to);
+        } else {
+            Raw8<__nv_bfloat16> o;
+            o.set(v);
+            o.store(static_cast<__nv_bfloat16*>(out) + to);
+        }
     }
+}
+
+// Rows per block: as many as leave eight blocks to an SM (each looks its rows up
+// first), one where there are few.
+static int kv4_block_rows(int64_t T) {
+    const int64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    int r = 1;
+    while (r < kKv4MaxRows && T / (2 * r) >= 8 * sms) r *= 2;
+    return r;
+}
+static Kv4Step kv4_step(int Hk, int64_t D) {
+    const int vecs = kKv4Threads / (int)(D / 8), per_row = 2 * Hk;
+    return {per_row, vecs / per_row, vecs % per_row};
 }
 
 }  // namespace pn
@@ -301,9 +449,9 @@ int pn_kv4_append(const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh, const
         return aligned(a.x[i], 16) && a.sb[i] % n == 0 && a.sl[i] % n == 0 && a.sh[i] % n == 0;
     };
     a.vec = whole(0) && whole(1);
-    const int64_t blocks = (T * kv_heads * 2 * (head_dim / 8) + pn::kKv4Threads - 1) / pn::kKv4Threads;
-    if (blocks > 0x7fffffff) return fail(PN_ERR_SHAPE, "pn_kv4_append: too many rows");
-    const unsigned g = (unsigned)blocks;
+    a.rows = pn::kv4_block_rows(T);
+    a.step = pn::kv4_step((int)kv_heads, head_dim);
+    const unsigned g = (unsigned)((T + a.rows - 1) / a.rows);
     const cudaStream_t s = (cudaStream_t)stream;
     if (kv_dtype == PN_F32) {
         if (head_dim == 64) pn::kv4_append_kernel<float, 64><<<g, pn::kKv4Threads, 0, s>>>(a);
@@ -333,11 +481,12 @@ int pn_kv4_gather(const void* cache, int64_t n_pages, int64_t kv_heads, int64_t 
     a.y[0] = k;
     a.y[1] = v;
     a.y_f32 = kv_dtype == PN_F32;
-    const int64_t blocks = (T * kv_heads * 2 * (head_dim / 8) + pn::kKv4Threads - 1) / pn::kKv4Threads;
-    if (blocks > 0x7fffffff) return fail(PN_ERR_SHAPE, "pn_kv4_gather: too many rows");
+    a.rows = pn::kv4_block_rows(T);
+    a.step = pn::kv4_step((int)kv_heads, head_dim);
+    const unsigned g = (unsigned)((T + a.rows - 1) / a.rows);
     const cudaStream_t s = (cudaStream_t)stream;
-    if (head_dim == 64) pn::kv4_gather_kernel<64><<<(unsigned)blocks, pn::kKv4Threads, 0, s>>>(a);
-    else pn::kv4_gather_kernel<128><<<(unsigned)blocks, pn::kKv4Threads, 0, s>>>(a);
+    if (head_dim == 64) pn::kv4_gather_kernel<64><<<g, pn::kKv4Threads, 0, s>>>(a);
+    else pn::kv4_gather_kernel<128><<<g, pn::kKv4Threads, 0, s>>>(a);
     const cudaError_t err = cudaGetLastError();
     return err == cudaSuccess ? ok() : cuda_fail(err, "pn_kv4_gather");
 }
