@@ -19,18 +19,19 @@
 // Shape of the decode kernel.  Keys are the 16-row operand of m16n8k16 (16
 // tokens), the query rows of one kv head (group x new tokens) its 8 columns,
 // so one product serves a whole group and wastes no more than 8 - rows
-// columns.  Each warp streams 16-token pieces of its own, with its own running
-// maximum, total and output in registers: no block-wide step inside the loop;
-// the four warps of a block are joined in shared memory at the end of a
-// segment.  The pieces come through a ring of cp.async copies private to the
-// warp.
+// columns.  Each warp streams runs of 32 tokens of its own (two 16-token pieces,
+// whose products are interleaved), with its own running maximum, total and
+// output in registers: no block-wide step inside the loop; the four warps of a
+// block are joined in shared memory at the end of a segment.  The pieces come
+// through a ring of cp.async copies private to the warp.
 //
-// Work split.  The units (64 tokens of one row tile, kv head and sequence) of
+// Work split.  The units (128 tokens of one row tile, kv head and sequence) of
 // the whole call are laid end to end and every block takes an equal run of
 // them, so ragged batches and single long sequences alike fill the SMs without
 // the host knowing any length.  A block's run may start or end inside a row
-// tile: such partial results go to the workspace and a second kernel joins
-// them in a fixed order, so results do not depend on timing.
+// tile: such partial results go to the workspace, with a note by the block that
+// holds the tile's last unit, and a second kernel joins them in a fixed order,
+// so results do not depend on timing.
 #include <cuda_fp16.h>
 
 #include "pn_common.cuh"
@@ -38,20 +39,32 @@
 
 namespace pn {
 
+// What the joining kernel needs to know of a row tile whose last unit a block
+// holds and whose first unit another one does.
+struct Kv4Join {
+    int rows;        // query rows of the tile; 0: nothing to join
+    int first;       // the block with the tile's first unit ..
+    int first_slot;  // .. and which of its two partial results that is
+    int G;
+    int64_t row0;    // first row of the tile's sequence
+    int64_t r0;      // first query row of the tile
+    int64_t head;
+};
+
 struct Kv4AttnArgs {
     Kv4Seq s;
     const void* q;
     int q_f32, q_vec;
     int64_t q_sb, q_sl, q_sh;
     const uint8_t* cache;
-    int G;            // query heads per kv head
-    float scale_log2; // softmax scale * log2(e)
-    void* out;        // (T, Hk * G, D), q's type
-    int64_t* prefix;  // workspace: units before each sequence (B + 1)
-    float* part;      // workspace: partial results of two segments per block
+    int G;             // query heads per kv head
+    float scale_log2;  // softmax scale * log2(e)
+    void* out;         // (T, Hk * G, D), q's type
+    Kv4Join* notes;    // workspace: one per block
+    float* part;       // workspace: partial results of two segments per block
 };
 
-constexpr int kAttnTokens = 64;  // tokens of a unit
+constexpr int kAttnTokens = 128;  // tokens of a unit: 32 per warp
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 
@@ -70,14 +83,14 @@ __device__ __forceinline__ void cp_wait() {
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
@@ -89,54 +102,123 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 
 // Row tiles of RT query rows and the units of sequence b (every row tile is
 // walked over all of the sequence's tokens; what a tile may not see is skipped
-// when it is met).
-__device__ __forceinline__ int64_t attn_units(const Kv4AttnArgs& a, int64_t b, int rt_rows, int& nt) {
+// when it is met).  The host has checked that all units together fit 31 bits.
+__device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, uint32_t rt_rows, uint32_t& nt) {
     int64_t first, n;
     kv4_rows(a.s, b, first, n);
     nt = max((kv4_len(a.s, b) + kAttnTokens - 1) / kAttnTokens, 1);
-    return (n * a.G + rt_rows - 1) / rt_rows * nt * a.s.Hk;
+    return ((uint32_t)n * a.G + rt_rows - 1) / rt_rows * nt * a.s.Hk;
 }
 
-// Units before sequence b for every b, and the sequence that holds `want`:
-// all threads of the block; block 0 leaves the sums for the joining kernel.
-__device__ __forceinline__ int64_t attn_plan(const Kv4AttnArgs& a, int rt_rows, int64_t* sh_sum, int64_t& total) {
-    // thread t takes sequences [t * per, (t + 1) * per)
-    const int64_t per = (a.s.B + kAttnThreads - 1) / kAttnThreads;
-    const int64_t b0 = min(threadIdx.x * per, a.s.B), b1 = min(b0 + per, a.s.B);
-    int64_t sum = 0;
-    int nt;
-    for (int64_t b = b0; b < b1; ++b) sum += attn_units(a, b, rt_rows, nt);
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int64_t inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-    }
-    if (lane == 31) sh_sum[w] = inc;
-    __syncthreads();
-    int64_t before = inc - sum;
-    total = 0;
-#pragma unroll
-    for (int i = 0; i < kAttnWarps; ++i) {
-        if (i < w) before += sh_sum[i];
-        total += sh_sum[i];
-    }
-    if (blockIdx.x == 0) {
-        int64_t at = before;
-        for (int64_t b = b0; b < b1; ++b) {
-            a.prefix[b] = at;
-            at += attn_units(a, b, rt_rows, nt);
-        }
-        if (threadIdx.x == 0) a.prefix[a.s.B] = total;
-    }
-    return before;
-}
-
-// Block c's first unit.
-__device__ __forceinline__ int64_t attn_begin(int64_t total, int64_t blocks, int64_t c) {
+// The units of the call, and this block's run [begin, end): all threads of the
+// block.  seq, in_seq: the sequence that holds `begin` and the unit's place in it.
+struct AttnRun {
+    uint32_t total, begin, end, seq, in_seq;
+};
+__device__ __forceinline__ uint32_t attn_begin(uint32_t total, uint32_t blocks, uint32_t c) {
     return total / blocks * c + min(c, total % blocks);
 }
+__device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a, uint32_t rt_rows) {
+    __shared__ uint32_t sums[kAttnWarps], start[2];
+    // thread t takes sequences [t * per, (t + 1) * per)
+    const uint32_t B = (uint32_t)a.s.B, per = (B + kAttnThreads - 1) / kAttnThreads;
+    const uint32_t b0 = min(threadIdx.x * per, B), b1 = min(b0 + per, B);
+    uint32_t sum = 0, nt;
+    for (uint32_t b = b0; b < b1; ++b) sum += attn_units(a, b, rt_rows, nt);
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    uint32_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) sums[w] = inc;
+    __syncthreads();
+    uint32_t at = inc - sum;
+    AttnRun run;
+    run.total = 0;
+#pragma unroll
+    for (int i = 0; i < kAttnWarps; ++i) {
+        if (i < w) at += sums[i];
+        run.total += sums[i];
+    }
+    run.begin = attn_begin(run.total, gridDim.x, blockIdx.x);
+    run.end = attn_begin(run.total, gridDim.x, blockIdx.x + 1);
+    if (run.begin >= at && run.begin < at + sum) {
+        uint32_t b = b0;
+        for (; b < b1; ++b) {
+            const uint32_t n = attn_units(a, b, rt_rows, nt);
+            if (run.begin < at + n) break;
+            at += n;
+        }
+        start[0] = b;
+        start[1] = run.begin - at;
+    }
+    __syncthreads();
+    run.seq = start[0];
+    run.in_seq = start[1];
+    return run;
+}
+
+// One segment: a run of units of one row tile.
+struct AttnSeg {
+    uint32_t b, nt, t0, t1;  // sequence; token tiles of it, and the segment's [t0, t1)
+    int head, rows;          // kv head; query rows in the tile
+    int64_t row0, r0;        // first row of the sequence; first query row of the tile
+    int pos0;                // query row r sees positions up to pos0 + r / G
+    int kv_end;              // tokens that the tile's last row sees
+    int lim_min;             // the last position that its first row sees
+
+    // Advances `in_seq` to its sequence first.
+    __device__ __forceinline__ AttnSeg(const Kv4AttnArgs& a, uint32_t rt_rows, uint32_t& seq, uint32_t& in_seq,
+                                       uint32_t left) {
+        uint32_t n = attn_units(a, seq, rt_rows, nt);
+        while (in_seq >= n) {  // past the sequence (or one without rows)
+            in_seq -= n;
+            ++seq;
+            n = attn_units(a, seq, rt_rows, nt);
+        }
+        b = seq;
+        // a row tile's units are consecutive: (head, row tile, token tile)
+        int64_t n_rows;
+        kv4_rows(a.s, b, row0, n_rows);
+        const uint32_t q_rows = (uint32_t)n_rows * a.G, n_rt = (q_rows + rt_rows - 1) / rt_rows;
+        const uint32_t tile = in_seq / nt;
+        head = (int)(tile / n_rt);
+        r0 = (tile - head * n_rt) * rt_rows;
+        rows = (int)min(rt_rows, q_rows - (uint32_t)r0);
+        t0 = in_seq - tile * nt;
+        t1 = min(nt, t0 + left);
+        pos0 = kv4_len(a.s, b) - (int)n_rows;
+        kv_end = max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0);
+        lim_min = pos0 + (int)((uint32_t)r0 / a.G);
+    }
+    // Where query row r of the tile (r < rows) lies in q, in elements.
+    __device__ __forceinline__ int64_t query(const Kv4AttnArgs& a, int r) const {
+        const uint32_t rr = (uint32_t)r0 + r, i = rr / a.G;
+        return (a.s.cu ? (row0 + i) * a.q_sl : b * a.q_sb + i * a.q_sl) + (head * a.G + (rr - i * a.G)) * a.q_sh;
+    }
+};
+
+// Looks up the pages of a sequence, 32 pieces of 16 tokens at a time: lane l
+// holds where piece (base + l)'s keys begin.
+struct AttnPages {
+    uint64_t addr;  // the page block of the keys; 0: not there
+    int off;        // the piece's first token in its page
+
+    __device__ __forceinline__ void look_up(const Kv4AttnArgs& a, uint32_t b, int head, int64_t block, int tok, bool want) {
+        addr = 0;
+        off = 0;
+        if (!want) return;
+        const uint32_t i = (uint32_t)tok / (uint32_t)a.s.page;
+        const int p = __ldg(a.s.table + b * a.s.table_ld + i);
+        off = tok - (int)i * a.s.page;
+        if (p >= 0 && p < a.s.n_pages)
+            addr = (uint64_t)(a.cache + ((int64_t)p * a.s.Hk + head) * 2 * block);
+        else
+            record_status(PN_ERR_ARG);
+    }
+};
 
 __device__ __forceinline__ void store_out(const Kv4AttnArgs& a, int64_t at, const float4& y, float inv) {
     if (a.q_f32) {
@@ -204,14 +286,15 @@ template <int D, int NT>
 struct AttnCfg {
     static constexpr int W = D / 32;             // words per thread and token
     static constexpr int kRows = 8 * NT;         // query rows of a row tile
-    static constexpr int kStages = 4;
+    static constexpr int kStages = NT == 4 ? 8 : 6;
     static constexpr int kCodes = 16 * (D / 2);  // bytes of one 16-token piece of keys or values
     static constexpr int kStage = 2 * kCodes + 128;
-    static constexpr int kRing = kAttnWarps * kStages * kStage;
-    static constexpr int kPitch = D + 8;         // floats per row of the join buffer
-    static constexpr int kJoin = kAttnWarps * kRows * kPitch * 4;
-    static constexpr int kSmem = kRing + kJoin + kAttnWarps * kRows * 8;
+    static constexpr int kRing = kStages * kStage;  // per warp
+    static constexpr int kSmem = kAttnWarps * kRing;
+    static constexpr int kPitch = D + 8;         // floats per row of the join buffer (over the warp's own ring)
     static constexpr int kPart = kRows * (D + 2);  // floats of one partial result
+    static constexpr int kBlocks = NT <= 2 ? 3 : 2;  // per SM
+    static_assert(kRows * kPitch * 4 <= kRing, "the join buffer lies over the ring");
 };
 
 // Byte position of 16-byte chunk j of token pair p inside a piece's values:
@@ -222,279 +305,251 @@ __device__ __forceinline__ int v_chunk(int p, int j) {
     return D == 128 ? p * 128 + ((j + 2 * p) & 7) * 16 : p * 64 + ((j + (p & 2)) & 3) * 16;
 }
 
+// W words of a row of codes.
+template <int W>
+__device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[W]) {
+    if constexpr (W == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+    } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
+    }
+}
+__device__ __forceinline__ float pair_lo(uint32_t p) { return __uint_as_float(p << 16); }
+__device__ __forceinline__ float pair_hi(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
+
 template <int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) kv4_decode_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_decode_kernel(const Kv4AttnArgs a) {
     using C = AttnCfg<D, NT>;
     constexpr int W = C::W, RT = C::kRows, ST = C::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t sh_sum[kAttnWarps];
-    __shared__ int64_t sh_start[2];
+    __shared__ float join_ml[kAttnWarps * RT * 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int g = lane >> 2, t = lane & 3;
-    uint8_t* ring = smem + warp * ST * C::kStage;
+    uint8_t* ring = smem + warp * C::kRing;
     const uint32_t ring_u = smem_u32(ring);
-    float* join = reinterpret_cast<float*>(smem + C::kRing);
-    float* join_ml = reinterpret_cast<float*>(smem + C::kRing + C::kJoin);
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    int64_t total;
-    const int64_t before = attn_plan(a, RT, sh_sum, total);
-    const int64_t begin = attn_begin(total, gridDim.x, blockIdx.x), end = attn_begin(total, gridDim.x, blockIdx.x + 1);
-    if (begin >= end) return;
-    {   // the sequence that holds unit `begin`
-        const int64_t per = (a.s.B + kAttnThreads - 1) / kAttnThreads;
-        const int64_t b0 = min(tid * per, a.s.B), b1 = min(b0 + per, a.s.B);
-        int64_t at = before;
-        int nt;
-        for (int64_t b = b0; b < b1; ++b) {
-            const int64_t n = attn_units(a, b, RT, nt);
-            if (begin >= at && begin < at + n) {
-                sh_start[0] = b;
-                sh_start[1] = begin - at;
-            }
-            at += n;
-        }
-        __syncthreads();
-    }
-    int64_t b = sh_start[0], in_seq = sh_start[1], unit = begin;
+    AttnRun run = attn_plan(a, RT);
+    if (tid == 0) a.notes[blockIdx.x].rows = 0;
     const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
+    // a lane's part of a piece: 16-byte chunks of codes, and of the pairs (lanes 0-3 keys, 4-7 values)
+    const uint32_t pair_off = (uint32_t)a.s.page * (D / 2) + (lane & 3) * 16 + (lane & 4 ? (uint32_t)block : 0u);
+    // (a second chunk of a lane lies four pairs on: the same rotation, 512 bytes further)
+    const uint32_t dst_k = ring_u + lane * 16, dst_v = ring_u + C::kCodes + v_chunk<D>(lane / (D / 16), lane % (D / 16)),
+                   dst_p = ring_u + 2 * C::kCodes + lane * 16;
 
-    while (unit < end) {
-        int nt;
-        while (in_seq >= attn_units(a, b, RT, nt)) {  // past the sequence (or one without rows)
-            in_seq -= attn_units(a, b, RT, nt);
-            ++b;
-        }
-        // a row tile's units are consecutive: (head, row tile, token tile)
-        int64_t row0, n_rows;
-        kv4_rows(a.s, b, row0, n_rows);
-        const int len = kv4_len(a.s, b);
-        const int64_t q_rows = n_rows * a.G, n_rt = (q_rows + RT - 1) / RT;
-        const int64_t tile_id = in_seq / nt;
-        const int head = (int)(tile_id / n_rt);
-        const int64_t r0 = (tile_id - head * n_rt) * RT;  // first query row of the tile
-        const int rows = (int)min((int64_t)RT, q_rows - r0);
-        const int t0 = (int)(in_seq - tile_id * nt);
-        const int t1 = (int)min((int64_t)nt, t0 + (end - unit));
-        // positions: row r sees tokens up to len - n_rows + r / G
-        const int64_t pos0 = len - n_rows;
-        const int kv_end = (int)max(pos0 + (r0 + rows - 1) / a.G + 1, (int64_t)0);  // seen by the tile's last row
-        const int lim_min = (int)(pos0 + r0 / a.G);                                  // ... by its first
-        const int used = min(t1, (kv_end + kAttnTokens - 1) / kAttnTokens);           // tiles behind it are skipped
+    uint32_t seq = run.seq, in_seq = run.in_seq;
+    for (uint32_t unit = run.begin; unit < run.end;) {
+        const AttnSeg sg(a, RT, seq, in_seq, run.end - unit);
+
+        // ---- the warp's runs: tokens [128 * tile + 32 * warp, + 32), two pieces each
+        const int used = min((int)sg.t1, (sg.kv_end + kAttnTokens - 1) / kAttnTokens);  // tiles behind it are skipped
+        const int count = used - (int)sg.t0;
+        const int tok_base = (int)sg.t0 * kAttnTokens + warp * 32;
+        AttnPages pages;
+        uint32_t dead = 0;  // ring of flags: the piece is not there
+        auto issue = [&](int i, uint32_t slot) {  // run i; slot: its first stage's offset in the ring
+            if ((i & 15) == 0) {  // lane 2 k + j looks up piece j of run i + k
+                const int k = i + (lane >> 1), tok = tok_base + k * kAttnTokens + (lane & 1) * 16;
+                pages.look_up(a, sg.b, sg.head, block, tok, k < count && tok < sg.kv_end);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int from = 2 * (i & 15) + j;
+                const uint64_t addr = __shfl_sync(0xffffffffu, pages.addr, from);
+                const uint32_t off = __shfl_sync(0xffffffffu, pages.off, from);
+                const uint32_t bit = 1u << from;
+                if (addr) {
+                    dead &= ~bit;
+                    const uint8_t* kc = reinterpret_cast<const uint8_t*>(addr) + (off * (D / 2) + lane * 16);
+                    const uint8_t* vc = kc + block;
+                    const uint32_t st = slot + j * C::kStage;
+#pragma unroll
+                    for (int c = 0; c < C::kCodes / 512; ++c) {
+                        cp_async16(dst_k + st + c * 512, kc + c * 512);
+                        cp_async16(dst_v + st + c * 512, vc + c * 512);
+                    }
+                    if (lane < 8) cp_async16(dst_p + st, reinterpret_cast<const uint8_t*>(addr) + (pair_off + off * 4));
+                } else {
+                    dead |= bit;
+                }
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < ST / 2 - 1; ++i) issue(i, 2 * i * C::kStage);
 
         // ---- queries
         uint32_t qb[NT][D / 8];
-        float ca[NT][2], cb[NT][2];
+        float2 ca[NT], cb[NT];
         int lim[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int64_t r = r0 + n * 8 + g;
             const char* row = nullptr;
-            if (n * 8 + g < rows) {
-                const int64_t i = r / a.G, at = (a.s.cu ? (row0 + i) * a.q_sl : b * a.q_sb + i * a.q_sl) +
-                                                (head * a.G + r % a.G) * a.q_sh;
-                row = static_cast<const char*>(a.q) + at * (a.q_f32 ? 4 : 2);
-            }
+            if (n * 8 + g < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, n * 8 + g) * (a.q_f32 ? 4 : 2);
             float fa, fb;
             load_query<D>(a, row, t, qb[n], fa, fb);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                ca[n][k] = __shfl_sync(0xffffffffu, fa, (2 * t + k) * 4);
-                cb[n][k] = __shfl_sync(0xffffffffu, fb, (2 * t + k) * 4);
+                const float va = __shfl_sync(0xffffffffu, fa, (2 * t + k) * 4), vb = __shfl_sync(0xffffffffu, fb, (2 * t + k) * 4);
+                if (k == 0)
+                    ca[n].x = va, cb[n].x = vb;
+                else
+                    ca[n].y = va, cb[n].y = vb;
                 const int rl = n * 8 + 2 * t + k;
-                lim[n][k] = rl < rows ? (int)(pos0 + (r0 + rl) / a.G) : kv_end - 1;
+                lim[n][k] = rl < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + rl) / a.G) : sg.kv_end - 1;
             }
         }
 
-        // ---- the warp's pieces: tokens [64 * tile + 16 * warp, + 16)
-        const int count = used - t0;
-        uint32_t bad = 0;  // ring of flags: the piece is not there
-        int page_id = 0, page_off = 0;
-        auto issue = [&](int i) {
-            if ((i & 31) == 0) {  // lane l looks up piece i + l
-                const int tok = (t0 + i + lane) * kAttnTokens + warp * 16;
-                page_id = -1;
-                if (i + lane < count && tok < kv_end) {
-                    const int p = __ldg(a.s.table + b * a.s.table_ld + tok / a.s.page);
-                    page_off = tok % a.s.page;
-                    if (p >= 0 && p < a.s.n_pages)
-                        page_id = p;
-                    else
-                        record_status(PN_ERR_ARG);
-                }
-            }
-            const int p = __shfl_sync(0xffffffffu, page_id, i & 31), off = __shfl_sync(0xffffffffu, page_off, i & 31);
-            const uint32_t bit = 1u << (i & 31);
-            if (i < count && p >= 0) {
-                bad &= ~bit;
-                const uint8_t* kb = a.cache + ((int64_t)p * a.s.Hk + head) * 2 * block;
-                const uint8_t* vb = kb + block;
-                const uint32_t dst = ring_u + (i % ST) * C::kStage;
-#pragma unroll
-                for (int c = lane; c < C::kCodes / 16; c += 32) {
-                    cp_async16(dst + c * 16, kb + off * (D / 2) + c * 16);
-                    cp_async16(dst + C::kCodes + v_chunk<D>(c / (D / 16), c % (D / 16)), vb + off * (D / 2) + c * 16);
-                }
-                if (lane < 8)
-                    cp_async16(dst + 2 * C::kCodes + lane * 16,
-                               (lane < 4 ? kb : vb) + (int64_t)a.s.page * (D / 2) + off * 4 + (lane & 3) * 16);
-            } else {
-                bad |= bit;
-            }
-            cp_commit();
-        };
-
-        float m[NT][2], l[NT][2], zs[NT][2], o[NT][D / 16][4];
+        float o[NT][D / 16][4];
+        float2 neg_m[NT], l[NT], zs[NT];  // minus the running maximum; totals of p and of p z (this lane's tokens)
         float S = 0.0f, inv_S = 0.0f;  // power of two not below the largest value scale seen, and its inverse
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) m[n][k] = -INFINITY, l[n][k] = 0.0f, zs[n][k] = 0.0f;
+            neg_m[n] = make_float2(INFINITY, INFINITY), l[n] = zs[n] = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[n][j][k] = 0.0f;
         }
+
+        // The two pieces of run i.  kMask: some token of them is not seen by some row.
+        auto pieces = [&](int i, uint32_t slot, auto mask) {
+            constexpr bool kMask = decltype(mask)::value;
+            const uint8_t* st[2] = {ring + slot, ring + slot + C::kStage};
+            // ---- logits: 16 tokens x 8 rows per piece and n
+            float acc[2][NT][4];
+            uint32_t vp[2][2], ka[2][W], kb[2][W];
 #pragma unroll
-        for (int i = 0; i < ST - 1; ++i) issue(i);
-        for (int i = 0; i < count; ++i) {
-            issue(i + ST - 1);
-            cp_wait<ST - 1>();
-            __syncwarp();
-            const int tok0 = (t0 + i) * kAttnTokens + warp * 16;
-            if (!(bad >> (i & 31) & 1u)) {
-                const uint8_t* st = ring + (i % ST) * C::kStage;
-                // ---- logits: 16 tokens x 8 rows per n
-                float acc[NT][4];
+            for (int j = 0; j < 2; ++j) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) acc[n][k] = 0.0f;
-                uint32_t ka[W], kb[W];
-                if constexpr (W == 4) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(st + g * (D / 2) + t * 16);
-                    const uint4 v = *reinterpret_cast<const uint4*>(st + (g + 8) * (D / 2) + t * 16);
-                    ka[0] = u.x, ka[1] = u.y, ka[2] = u.z, ka[3] = u.w;
-                    kb[0] = v.x, kb[1] = v.y, kb[2] = v.z, kb[3] = v.w;
-                } else {
-                    const uint2 u = *reinterpret_cast<const uint2*>(st + g * (D / 2) + t * 8);
-                    const uint2 v = *reinterpret_cast<const uint2*>(st + (g + 8) * (D / 2) + t * 8);
-                    ka[0] = u.x, ka[1] = u.y, kb[0] = v.x, kb[1] = v.y;
-                }
+                    for (int k = 0; k < 4; ++k) acc[j][n][k] = 0.0f;
+                lds_words<W>(st[j] + g * (D / 2) + t * 4 * W, ka[j]);
+                lds_words<W>(st[j] + (g + 8) * (D / 2) + t * 4 * W, kb[j]);
+            }
+            // the two pieces' products in turn: each is a chain over the dims
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
+            for (int w = 0; w < W; ++w)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t u = h ? ka[w] >> 8 : ka[w], v = h ? kb[w] >> 8 : kb[w];
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t u = h ? ka[j][w] >> 8 : ka[j][w], v = h ? kb[j][w] >> 8 : kb[j][w];
                         const uint32_t a0 = u & 0x000F000Fu, a1 = v & 0x000F000Fu, a2 = u & 0x00F000F0u, a3 = v & 0x00F000F0u;
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
-                            mma_f16(acc[n], a0, a1, a2, a3, qb[n][w * 4 + h * 2], qb[n][w * 4 + h * 2 + 1]);
+                            mma_f16(acc[j][n], a0, a1, a2, a3, qb[n][w * 4 + h * 2], qb[n][w * 4 + h * 2 + 1]);
                     }
-                }
-                uint32_t kp[2], vp[2];
+            float top = -INFINITY, vtop = 0.0f, rel[2][NT][4];  // rel: logit - m
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int tok0 = tok_base + i * kAttnTokens + j * 16;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    kp[k] = *reinterpret_cast<const uint32_t*>(st + 2 * C::kCodes + (g + 8 * k) * 4);
-                    vp[k] = *reinterpret_cast<const uint32_t*>(st + 2 * C::kCodes + 64 + (g + 8 * k) * 4);
-                    if (tok0 + g + 8 * k >= kv_end) vp[k] = 0;  // whatever lies behind the sequence
-                }
-                bool grow = false;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float ks = __uint_as_float(kp[k] << 16), kz = __uint_as_float(kp[k] & 0xFFFF0000u);
-                    grow |= __uint_as_float(vp[k] << 16) > S;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            float& x = acc[n][2 * k + j];
-                            x = fmaf(ks, x * ca[n][j], kz * cb[n][j]);
-                        }
-                }
-                if (tok0 + 15 > lim_min) {
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (tok0 + g + 8 * (k >> 1) > lim[n][k & 1]) acc[n][k] = -INFINITY;
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) grow |= acc[n][k] > m[n][k & 1] + 8.0f;
-                // The maximum need not be exact: a weight may exceed 1 by up to 2^8
-                // before the sums are rescaled (fp16 holds 2^15), so most pieces
-                // skip this.
-                if (__any_sync(0xffffffffu, grow)) {
-                    float vs = fmaxf(__uint_as_float(vp[0] << 16), __uint_as_float(vp[1] << 16));
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) vs = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, d));
-                    float fs = 1.0f;
-                    if (vs > S) {
-                        // next power of two, kept where the inverse and 2^24 times it are normal numbers
-                        const int e = min(max((int)(__float_as_uint(vs) >> 23) - 126, -100), 102);
-                        const float was = S;
-                        S = pow2i(e);
-                        inv_S = pow2i(-e);
-                        fs = was * inv_S;
-                    }
+                    const uint32_t kp = *reinterpret_cast<const uint32_t*>(st[j] + 2 * C::kCodes + (g + 8 * k) * 4);
+                    vp[j][k] = *reinterpret_cast<const uint32_t*>(st[j] + 2 * C::kCodes + 64 + (g + 8 * k) * 4);
+                    const bool none = kMask && ((dead >> (2 * (i & 15) + j) & 1u) || tok0 + g + 8 * k >= sg.kv_end);
+                    if (kMask && none) vp[j][k] = 0;  // whatever lies behind the sequence
+                    const float2 ks = make_float2(pair_lo(kp), pair_lo(kp)), kz = make_float2(pair_hi(kp), pair_hi(kp));
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float f[2];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            float x = fmaxf(acc[n][k], acc[n][2 + k]);
-#pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                            const float mn = fmaxf(m[n][k], x);
-                            f[k] = mn == m[n][k] ? 1.0f : ex2f(m[n][k] - mn);
-                            m[n][k] = mn;
-                            l[n][k] *= f[k];
-                            zs[n][k] *= f[k];
-                            f[k] *= fs;
+                        float2 x = make_float2(acc[j][n][2 * k], acc[j][n][2 * k + 1]);
+                        x = fma2(ks, mul2(x, ca[n]), mul2(kz, cb[n]));
+                        if constexpr (kMask) {
+                            if (none || tok0 + g + 8 * k > lim[n][0]) x.x = -INFINITY;
+                            if (none || tok0 + g + 8 * k > lim[n][1]) x.y = -INFINITY;
                         }
-#pragma unroll
-                        for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) o[n][j][k] *= f[k & 1];
+                        acc[j][n][2 * k] = x.x, acc[j][n][2 * k + 1] = x.y;
+                        x = add2(x, neg_m[n]);
+                        rel[j][n][2 * k] = x.x, rel[j][n][2 * k + 1] = x.y;
+                        top = fmaxf(top, fmaxf(x.x, x.y));
                     }
+                    vtop = fmaxf(vtop, pair_lo(vp[j][k]));
                 }
-                // ---- weights
-                uint32_t pb[NT][2];
-                const float vn[2] = {__uint_as_float(vp[0] << 16) * inv_S, __uint_as_float(vp[1] << 16) * inv_S};
-                const float vz[2] = {__uint_as_float(vp[0] & 0xFFFF0000u), __uint_as_float(vp[1] & 0xFFFF0000u)};
+            }
+            // The maximum need not be exact: a weight may exceed 1 by up to 2^8
+            // before the sums are rescaled (fp16 holds 2^15), so most pieces
+            // skip this.  (The first one does not: m is -inf there.)
+            if (__any_sync(0xffffffffu, top > 8.0f || vtop > S)) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
+                float fs = 1.0f;
+                if (vtop > S) {
+                    // next power of two, kept where the inverse and 2^24 times it are normal numbers
+                    const int e = min(max((int)(__float_as_uint(vtop) >> 23) - 126, -100), 102);
+                    const float was = S;
+                    S = pow2i(e);
+                    inv_S = pow2i(-e);
+                    fs = was * inv_S;
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float wgt[4];
+                    float f[2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        // a token that a row does not see adds nothing, whatever its pair holds
-                        const bool none = acc[n][k] == -INFINITY;
-                        const float p = none ? 0.0f : ex2f(acc[n][k] - m[n][k & 1]);
-                        l[n][k & 1] += p;
-                        zs[n][k & 1] += none ? 0.0f : p * vz[k >> 1];
-                        wgt[k] = none ? 0.0f : p * vn[k >> 1];
+                    for (int k = 0; k < 2; ++k) {
+                        float x = fmaxf(fmaxf(acc[0][n][k], acc[0][n][2 + k]), fmaxf(acc[1][n][k], acc[1][n][2 + k]));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        const float was = k ? neg_m[n].y : neg_m[n].x, now = fminf(was, -x);
+                        f[k] = now == was ? 1.0f : ex2f(now - was);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) rel[j][n][2 * c + k] = acc[j][n][2 * c + k] + now;
+                        if (k == 0)
+                            neg_m[n].x = now;
+                        else
+                            neg_m[n].y = now;
                     }
-                    pb[n][0] = movmatrix_t(pack_f16(wgt[0], wgt[1]));
-                    pb[n][1] = movmatrix_t(pack_f16(wgt[2], wgt[3]));
-                }
-                // ---- output: dims x rows
-                uint32_t va[W], vb[W];
-                const uint8_t* sv = st + C::kCodes;
-                if constexpr (W == 4) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(sv + v_chunk<D>(t, g));
-                    const uint4 v = *reinterpret_cast<const uint4*>(sv + v_chunk<D>(t + 4, g));
-                    va[0] = u.x, va[1] = u.y, va[2] = u.z, va[3] = u.w;
-                    vb[0] = v.x, vb[1] = v.y, vb[2] = v.z, vb[3] = v.w;
-                } else {
-                    const uint2 u = *reinterpret_cast<const uint2*>(sv + v_chunk<D>(t, g >> 1) + (g & 1) * 8);
-                    const uint2 v = *reinterpret_cast<const uint2*>(sv + v_chunk<D>(t + 4, g >> 1) + (g & 1) * 8);
-                    va[0] = u.x, va[1] = u.y, vb[0] = v.x, vb[1] = v.y;
-                }
+                    l[n] = mul2(l[n], make_float2(f[0], f[1]));
+                    zs[n] = mul2(zs[n], make_float2(f[0], f[1]));
+                    f[0] *= fs, f[1] *= fs;
 #pragma unroll
-                for (int w = 0; w < W; ++w) {
+                    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[n][j][k] *= f[k & 1];
+                }
+            }
+            // ---- weights, then dims x rows of the output
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint32_t pb[NT][2];
+                const float vn[2] = {pair_lo(vp[j][0]) * inv_S, pair_lo(vp[j][1]) * inv_S};
+                const float vz[2] = {pair_hi(vp[j][0]), pair_hi(vp[j][1])};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint32_t wgt[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float2 p = make_float2(ex2f(rel[j][n][2 * k]), ex2f(rel[j][n][2 * k + 1]));
+                        float2 pz = p, pv = p;
+                        if constexpr (kMask) {  // a token that a row does not see adds nothing, whatever its pair holds
+                            const bool n0 = acc[j][n][2 * k] == -INFINITY, n1 = acc[j][n][2 * k + 1] == -INFINITY;
+                            p.x = n0 ? 0.0f : p.x, p.y = n1 ? 0.0f : p.y;
+                            pz = make_float2(n0 ? 0.0f : p.x * vz[k], n1 ? 0.0f : p.y * vz[k]);
+                            pv = make_float2(n0 ? 0.0f : p.x * vn[k], n1 ? 0.0f : p.y * vn[k]);
+                            zs[n] = add2(zs[n], pz);
+                        } else {
+                            zs[n] = fma2(p, make_float2(vz[k], vz[k]), zs[n]);
+                            pv = mul2(p, make_float2(vn[k], vn[k]));
+                        }
+                        l[n] = add2(l[n], p);
+                        wgt[k] = pack_f16(pv.x, pv.y);
+                    }
+                    pb[n][0] = movmatrix_t(wgt[0]);
+                    pb[n][1] = movmatrix_t(wgt[1]);
+                }
+                uint32_t va[W], vb[W];
+                const uint8_t* sv = st[j] + C::kCodes;
+                lds_words<W>(sv + (W == 4 ? v_chunk<D>(t, g) : v_chunk<D>(t, g >> 1) + (g & 1) * 8), va);
+                lds_words<W>(sv + (W == 4 ? v_chunk<D>(t + 4, g) : v_chunk<D>(t + 4, g >> 1) + (g & 1) * 8), vb);
+#pragma unroll
+                for (int w = 0; w < W; ++w)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t u = h ? va[w] >> 8 : va[w], v = h ? vb[w] >> 8 : vb[w];
@@ -502,37 +557,53 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) k
 #pragma unroll
                         for (int n = 0; n < NT; ++n) mma_f16(o[n][w * 2 + h], a0, a1, a2, a3, pb[n][0], pb[n][1]);
                     }
-                }
             }
-            __syncwarp();  // every lane has read the stage before it is filled again
+        };
+        uint32_t slot = 0, fill = (ST - 2) * C::kStage;  // stages of runs i and i + ST / 2 - 1
+        for (int i = 0; i < count; ++i) {
+            issue(i + ST / 2 - 1, fill);
+            cp_wait<ST / 2 - 1>();
+            __syncwarp();
+            const bool mask = (dead >> (2 * (i & 15)) & 3u) || tok_base + i * kAttnTokens + 31 > sg.lim_min;
+            if (mask)
+                pieces(i, slot, std::true_type{});
+            else
+                pieces(i, slot, std::false_type{});
+            __syncwarp();  // every lane has read the stages before they are filled again
+            fill = slot;
+            slot = slot == (ST - 2) * C::kStage ? 0 : slot + 2 * C::kStage;
         }
 
         // ---- join the four warps
-        const float up = S * 16777216.0f;  // the codes' 2^-24 and the weights' scale
+        float* mine = reinterpret_cast<float*>(ring);  // nothing is in flight
+        const float up = S * 16777216.0f;              // the codes' 2^-24 and the weights' scale
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+                l[n].x += __shfl_xor_sync(0xffffffffu, l[n].x, d);
+                l[n].y += __shfl_xor_sync(0xffffffffu, l[n].y, d);
+                zs[n].x += __shfl_xor_sync(0xffffffffu, zs[n].x, d);
+                zs[n].y += __shfl_xor_sync(0xffffffffu, zs[n].y, d);
+            }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) {
-                    l[n][k] += __shfl_xor_sync(0xffffffffu, l[n][k], d);
-                    zs[n][k] += __shfl_xor_sync(0xffffffffu, zs[n][k], d);
-                }
                 const int r = n * 8 + 2 * t + k;
-                float* dst = join + (warp * RT + r) * C::kPitch;
+                const float z = k ? zs[n].y : zs[n].x;
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
-                    *reinterpret_cast<float2*>(dst + 4 * (g * W + j / 2) + 2 * (j & 1)) =
-                        make_float2(fmaf(o[n][j][k], up, zs[n][k]), fmaf(o[n][j][2 + k], up * 0.0625f, zs[n][k]));
+                    *reinterpret_cast<float2*>(mine + r * C::kPitch + 4 * (g * W + j / 2) + 2 * (j & 1)) =
+                        make_float2(fmaf(o[n][j][k], up, z), fmaf(o[n][j][2 + k], up * 0.0625f, z));
                 if (g == 0) {
-                    join_ml[(warp * RT + r) * 2] = m[n][k];
-                    join_ml[(warp * RT + r) * 2 + 1] = l[n][k];
+                    join_ml[(warp * RT + r) * 2] = k ? -neg_m[n].y : -neg_m[n].x;
+                    join_ml[(warp * RT + r) * 2 + 1] = k ? l[n].y : l[n].x;
                 }
             }
+        }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == nt;
-        float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == begin ? 0 : 1)) * C::kPart;
-        for (int idx = tid; idx < rows * (D / 4); idx += kAttnThreads) {
+        const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
+        float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
+        for (int idx = tid; idx < sg.rows * (D / 4); idx += kAttnThreads) {
             const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
             float mx = -INFINITY;
 #pragma unroll
@@ -545,76 +616,103 @@ __global__ void __launch_bounds__(kAttnThreads, NT == 1 ? 4 : NT == 2 ? 3 : 2) k
                 if (mw == -INFINITY && lw == 0.0f) continue;  // the warp saw nothing
                 const float f = ex2f(mw - mx);
                 sum = fmaf(f, lw, sum);
-                const float4 u = *reinterpret_cast<const float4*>(join + (w * RT + r) * C::kPitch + d);
+                const float4 u = *reinterpret_cast<const float4*>(smem + w * C::kRing + (r * C::kPitch + d) * 4);
                 y.x = fmaf(f, u.x, y.x), y.y = fmaf(f, u.y, y.y), y.z = fmaf(f, u.z, y.z), y.w = fmaf(f, u.w, y.w);
             }
             if (whole) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                const int64_t rr = r0 + r;
-                store_out(a, ((row0 + rr / a.G) * a.s.Hk * a.G + head * a.G + rr % a.G) * D + d, y, inv);
+                const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
+                store_out(a, (((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G) * D + d, y, inv);
             } else {
                 *reinterpret_cast<float4*>(part + r * D + d) = y;
                 if (d == 0) part[RT * D + r * 2] = mx, part[RT * D + r * 2 + 1] = sum;
             }
         }
+        if (tid == 0 && sg.t0 > 0 && sg.t1 == sg.nt) {  // the tile ends here and began in an earlier block
+            // the block that holds the tile's first unit: the first `rem` blocks hold one more
+            const uint32_t u0 = unit - sg.t0, each = run.total / gridDim.x, rem = run.total % gridDim.x;
+            const uint32_t c0 = u0 < (each + 1) * rem ? u0 / (each + 1) : rem + (u0 - (each + 1) * rem) / each;
+            a.notes[blockIdx.x] = {sg.rows, (int)c0, attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0, a.G,
+                                   sg.row0, sg.r0, sg.head};
+        }
         __syncthreads();
-        unit += t1 - t0;
-        in_seq += t1 - t0;
+        unit += sg.t1 - sg.t0;
+        in_seq += sg.t1 - sg.t0;
     }
 }
 
-// Joins the partial results of row tiles that several blocks share: a warp per
-// query row and head.
+// Joins the partial results of a row tile that several blocks share: block c of
+// this grid those of the tile that ends in block c of the other, gridDim.y blocks
+// sharing its rows.  The warps of a block are shared out over its rows; those of
+// one row take its partial results in turn, then meet in shared memory.
+constexpr int kJoinWarps = 8;  // at most
 template <int D>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const Kv4AttnArgs a, int rt_rows, int64_t blocks) {
+__global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4AttnArgs a, int rt_rows) {
+    constexpr int E = D / 32;  // dims per lane
+    __shared__ float sh[kJoinWarps][D + 2];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31;
-    const int Hq = a.s.Hk * a.G;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int64_t row = id / Hq;
-    const int hq = (int)(id - row * Hq);
-    int64_t b, i;
-    if (row >= a.s.T || !kv4_find(a.s, row, b, i)) return;
-    int64_t row0, n_rows;
-    kv4_rows(a.s, b, row0, n_rows);
-    const int head = hq / a.G;
-    const int64_t rr = i * a.G + hq % a.G, n_rt = (n_rows * a.G + rt_rows - 1) / rt_rows;
-    const int nt = max((kv4_len(a.s, b) + kAttnTokens - 1) / kAttnTokens, 1);
-    const int64_t total = __ldcg(a.prefix + a.s.B);
-    const int64_t u0 = __ldcg(a.prefix + b) + (head * n_rt + rr / rt_rows) * nt;
-    // the block that holds unit u: the first `rem` blocks hold one more
-    const int64_t each = total / blocks, rem = total % blocks;
-    auto owner = [&](int64_t u) { return u < (each + 1) * rem ? u / (each + 1) : rem + (u - (each + 1) * rem) / each; };
-    const int64_t c0 = owner(u0), c1 = owner(u0 + nt - 1);
-    if (c0 == c1) return;
-    const int r = (int)(rr % rt_rows);
+    const int c1 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Kv4Join j = a.notes[c1];
+    const int share = (rt_rows + gridDim.y - 1) / gridDim.y, from = blockIdx.y * share, to = min(from + share, j.rows);
+    if (from >= to) return;
+    const int warps = blockDim.x >> 5;
+    int per_row = warps;  // of them per row
+    while (per_row > 1 && warps / per_row < to - from && per_row > c1 - j.first) per_row /= 2;
+    const int at_once = warps / per_row, part = warp % per_row;
     const int64_t size = (int64_t)rt_rows * (D + 2);
-    auto slot = [&](int64_t c) { return a.part + (c * 2 + (attn_begin(total, blocks, c) < u0 ? 1 : 0)) * size; };
-    float mx = -INFINITY;
-    for (int64_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(slot(c) + rt_rows * D + r * 2));
+    for (int base = from; base < to; base += at_once) {
+        const int r = base + warp / per_row;
+        float mx = -INFINITY, sum = 0.0f, y[E];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    constexpr int E = D / 32;
-    float y[E], sum = 0.0f;
+        for (int e = 0; e < E; ++e) y[e] = 0.0f;
+        if (r < to) {
+#pragma unroll 8
+            for (int c = j.first + part; c <= c1; c += per_row) {
+                const float* p = a.part + ((int64_t)c * 2 + (c == j.first ? j.first_slot : 0)) * size;
+                const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + rt_rows * D + r * 2));
+                float u[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = 0.0f;
-    for (int64_t c = c0; c <= c1; ++c) {
-        const float* p = slot(c);
-        const float mc = __ldcg(p + rt_rows * D + r * 2), lc = __ldcg(p + rt_rows * D + r * 2 + 1);
-        if (mc == -INFINITY && lc == 0.0f) continue;
-        const float f = ex2f(mc - mx);
-        sum = fmaf(f, lc, sum);
+                for (int e = 0; e < E; ++e) u[e] = __ldcg(p + r * D + e * 32 + lane);
+                if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+                const float mn = fmaxf(mx, ml.x), f = mx == mn ? 1.0f : ex2f(mx - mn), k = ex2f(ml.x - mn);
+                mx = mn;
+                sum = fmaf(k, ml.y, sum * f);
 #pragma unroll
-        for (int e = 0; e < E; ++e) y[e] = fmaf(f, __ldcg(p + r * D + lane * E + e), y[e]);
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t at = (row * Hq + hq) * D + lane * E;
+                for (int e = 0; e < E; ++e) y[e] = fmaf(k, u[e], y[e] * f);
+            }
+        }
+        if (per_row > 1) {
+            __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        if (a.q_f32)
-            static_cast<float*>(a.out)[at + e] = y[e] * inv;
-        else
-            static_cast<__nv_bfloat16*>(a.out)[at + e] = __float2bfloat16_rn(y[e] * inv);
+            for (int e = 0; e < E; ++e) sh[warp][e * 32 + lane] = y[e];
+            if (lane == 0) sh[warp][D] = mx, sh[warp][D + 1] = sum;
+            __syncthreads();
+            if (part != 0) continue;
+            float top = mx;
+            for (int w = 1; w < per_row; ++w) top = fmaxf(top, sh[warp + w][D]);
+            sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = 0.0f;
+            for (int w = 0; w < per_row; ++w) {
+                const float mw = sh[warp + w][D], lw = sh[warp + w][D + 1];
+                if (mw == -INFINITY && lw == 0.0f) continue;
+                const float f = ex2f(mw - top);
+                sum = fmaf(f, lw, sum);
+#pragma unroll
+                for (int e = 0; e < E; ++e) y[e] = fmaf(f, sh[warp + w][e * 32 + lane], y[e]);
+            }
+        }
+        if (r >= to) continue;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const uint32_t rr = (uint32_t)j.r0 + r, i = rr / j.G;
+        const int64_t at = (((j.row0 + i) * a.s.Hk + j.head) * j.G + rr - i * j.G) * D + lane;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (a.q_f32)
+                static_cast<float*>(a.out)[at + e * 32] = y[e] * inv;
+            else
+                static_cast<__nv_bfloat16*>(a.out)[at + e * 32] = __float2bfloat16_rn(y[e] * inv);
+        }
     }
 }
 
@@ -625,13 +723,13 @@ static int attn_nt(int64_t B, int64_t T, int64_t G) {
 }
 static int attn_blocks(int nt) {  // blocks that the device holds at once
     const int sms = device_sm_count();
-    return (sms > 0 ? sms : 148) * (nt == 1 ? 4 : nt == 2 ? 3 : 2);
+    return (sms > 0 ? sms : 148) * (nt <= 2 ? 3 : 2);  // AttnCfg::kBlocks
 }
-static size_t attn_prefix_bytes(int64_t B) { return ((size_t)(B + 1) * 8 + 255) / 256 * 256; }
+static size_t attn_notes_bytes(int blocks) { return ((size_t)blocks * sizeof(Kv4Join) + 255) / 256 * 256; }
 static size_t attn_workspace(int64_t B, int64_t T, int64_t G, int64_t D) {
     if (B == 0 || T == 0) return 0;
-    const int nt = attn_nt(B, T, G);
-    return attn_prefix_bytes(B) + (size_t)attn_blocks(nt) * 2 * (8 * nt) * (D + 2) * 4;
+    const int nt = attn_nt(B, T, G), blocks = attn_blocks(nt);
+    return attn_notes_bytes(blocks) + (size_t)blocks * 2 * (8 * nt) * (D + 2) * 4;
 }
 
 template <int D, int NT>
@@ -659,10 +757,16 @@ static cudaError_t launch_attn(const Kv4AttnArgs& a, cudaStream_t s) {
     cfg.numAttrs = 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NT>, a);
     if (e != cudaSuccess) return e;
-    cfg.gridDim = dim3((unsigned)((a.s.T * a.s.Hk * a.G + 3) / 4));
-    cfg.blockDim = dim3(128);
+    // Few tiles have many partial results each: more blocks and warps per tile.
+    // Many tiles: fewer, most blocks find nothing to join.  (8 tiles of 55
+    // partial results: 41 us with 8 x 8 warps, 47 us with 4 x 4; 256 tiles of 2:
+    // 52 us and 47 us.)
+    const int64_t tiles = (a.s.B + a.s.T * a.G / C::kRows) * a.s.Hk;
+    const bool few = tiles * 8 <= blocks;
+    cfg.gridDim = dim3((unsigned)blocks, few ? 8 : 4);
+    cfg.blockDim = dim3(few ? kJoinWarps * 32 : kJoinWarps * 16);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, a, C::kRows, (int64_t)blocks);
+    return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, a, (int)C::kRows);
 }
 
 }  // namespace pn
@@ -690,7 +794,10 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     if (T > 0 && B > 0 && (!q || !out)) return fail(PN_ERR_ARG, "pn_kv4_attention: null pointer");
     const size_t e = q_dtype == PN_F32 ? 4 : 2;
     if (!aligned(q, e) || !aligned(out, 16)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: misaligned pointer");
-    if ((T * q_heads + 3) / 4 > 0x7fffffff) return fail(PN_ERR_SHAPE, "pn_kv4_attention: too many rows");
+    // an upper bound on the units that the kernels count in 31 bits
+    if (B > 0 && ((double)T * (q_heads / kv_heads) / 8 + B) * kv_heads * ((double)table_w * page / pn::kAttnTokens + 1) > 2e9)
+        return fail(PN_ERR_SHAPE, "pn_kv4_attention: %lld rows over tables of %lld tokens are too much for one call",
+                    (long long)T, (long long)(table_w * page));
     if (int st = check_device()) return st;
     if (T == 0 || B == 0) return ok();
     const size_t need = pn::attn_workspace(B, T, q_heads / kv_heads, head_dim);
@@ -705,10 +812,10 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     a.G = (int)(q_heads / kv_heads);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.out = out;
-    a.prefix = static_cast<int64_t*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_prefix_bytes(B));
-    const cudaStream_t s = (cudaStream_t)stream;
     const int nt = pn::attn_nt(B, T, a.G);
+    a.notes = static_cast<pn::Kv4Join*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_notes_bytes(pn::attn_blocks(nt)));
+    const cudaStream_t s = (cudaStream_t)stream;
     cudaError_t err;
     if (head_dim == 64)
         err = nt == 1 ? pn::launch_attn<64, 1>(a, s) : nt == 2 ? pn::launch_attn<64, 2>(a, s) : pn::launch_attn<64, 4>(a, s);
