@@ -17,15 +17,21 @@
 // shared memory (read from memory once).  Few rows: as many blocks as there are,
 // for latency; many: as few as hold the row, two rows' blocks to an SM.
 //
-// No sort.  Logits within 2^-12 of the largest weight are the candidates: a few
-// hundred in a model's distribution.  They are brought to the first block,
-// which finds the k-th largest and the border of top-p by a histogram over 2048
-// buckets of (max - x) / T (64 to a unit; beyond 32 units a weight is zero) and
-// then among the few logits of one bucket.  Where the candidates do not reach
-// the border, or do not fit (flat distributions, large k), every block
-// histograms its run instead, and the border's bucket is searched by bisection on
-// the logits' ordered bit patterns: on a list of them or, where one bucket holds
-// too many (all logits nearly alike), over the runs themselves.
+// No sort.  The candidates, a few hundred in a model's distribution, are for top-k
+// the logits not below the k-th largest of some block's per-thread maxima (there
+// are k such at least), for top-p alone those within 2^-12 of the largest weight.
+// They are brought to the first block, which finds the k-th largest and the border
+// of top-p by a histogram over (max - x) / T, 32 buckets to an octave of weight, and
+// then among the few logits of one bucket.  Where the candidates do not reach the
+// border, or do not fit (flat distributions, k above 256), the histogram is taken
+// over the blocks' runs instead, and the border's bucket is searched by bisection on
+// the logits' ordered bit patterns: on a list of them or, where one bucket holds too
+// many (all logits nearly alike), over the runs themselves.
+//
+// What bounds it: large batches the weights, about thirty instructions each (six of
+// them fp64; the split into table index and rest runs in fp32), and the histogram's
+// atomics where it covers whole runs; small ones the chain of short steps, each
+// behind a barrier of the cluster (1 to 2 us).
 #include <cooperative_groups.h>
 
 #include "pn_common.cuh"
@@ -53,29 +59,61 @@ struct SampleArgs {
 constexpr int kSmpThreads = 512;
 constexpr int kSmpWarps = kSmpThreads / 32;
 constexpr int kSmpBuckets = 2048;
+constexpr int kSmpUnits = 46 * 256;  // (max - x) / T in 1/256 octaves from which a weight is zero; eight units to a bucket
 constexpr int kSmpList = 4096;
 constexpr int kSmpBlocks = 8;  // of a cluster, at most
 constexpr int64_t kSmpMaxVocab = 1 << 18;
 constexpr double kSmpOne = 35184372088832.0;  // 2^45
-constexpr float kSmpCut = 8.3f * 64.0f;       // candidates lie before this bucket: 12 ln 2 units
+constexpr float kSmpCut = 12 * 256;           // top-p's candidates lie within 12 octaves of the largest weight
+constexpr int kSmpKMost = kSmpThreads / 2;    // top-k of at most so many takes its candidates by the threads' maxima
+
+// One row's rule.  A logit is kept when it lies above `key`, or equals it and is
+// among the first `ties` such in index order, and its weight is not zero.
+struct SampleRow {
+    float max;
+    float per;       // 256 log2(e) / T
+    double c;        // the same in fp64
+    uint64_t floor;  // min-p as a weight (at least 1)
+    bool flat;       // all weights are zero or one: T <= 0, or a maximum of +inf
+    float key;
+    uint32_t ties;
+
+    // (max - x) / T in 1/256 octaves, monotone; kSmpUnits and more: no weight.  (The
+    // products that are NaN belong to the maximum itself: 0 * inf, inf - inf.)
+    __device__ __forceinline__ float place(float x) const { return fmaxf((max - x) * per, 0.0f); }
+    __device__ __forceinline__ int bucket(float x) const { return (int)fminf(place(x), (float)kSmpUnits) >> 3; }
+    static constexpr int kNone = kSmpUnits >> 3;  // the bucket of logits without weight
+};
+
+struct SampleFound {
+    float key;
+    uint32_t ties;
+    uint32_t ok;  // the candidates sufficed
+};
 
 struct SampleShared {
-    double table[64];  // 2^(j / 64 + 45)
+    double table[256];  // 2^(45 - j / 256)
     uint32_t lo[kSmpBuckets], hi[kSmpBuckets];  // 64-bit sums in two halves (shared memory adds 32 bits natively)
     float list[kSmpList];
+    SampleRow row;
     uint64_t red[kSmpWarps];
     uint32_t redc[kSmpWarps];
     float redf[kSmpWarps];
-    // one entry per block of the cluster, written by that block
-    uint64_t of_sum[2][kSmpBlocks];
-    uint64_t of_cand[kSmpBlocks];
-    uint32_t of_n[kSmpBlocks];
-    float of_max[kSmpBlocks];
-    // the first block's findings
-    uint64_t sum, before, total;
-    uint32_t bucket, ties;
-    float key;
-    uint32_t n;  // entries of list
+    // read by the other blocks of the cluster between two of its barriers
+    float max, kth;
+    uint32_t n;  // logits pushed to list (those past kSmpList are not held)
+    uint64_t sum;
+    uint64_t part[2];
+    uint64_t kept;
+    uint32_t kept_ties;
+    // written by the first block
+    SampleFound found[3];
+    uint64_t total[2], before[2];
+    uint32_t bucket[2];
+    // within the block
+    uint64_t b_sum, b_before;
+    uint32_t b_bucket;
+    float b_key;
     float few[32];
     uint32_t n_few;
 };
@@ -106,37 +144,43 @@ __device__ __forceinline__ uint64_t block_sum(SampleShared& s, uint64_t v) {
     return v;
 }
 
-// One row's rule.  A logit is kept when it lies above `key`, or equals it and is
-// among the first `ties` such in index order, and its weight is not zero.
-struct SampleRow {
-    const double* table;
-    float max;
-    double c;       // 64 log2(e) / T
-    float per;      // buckets per unit of max - x
-    uint64_t floor; // min-p as a weight (at least 1)
-    float key;
-    uint32_t ties;
+// 2^45 exp((x - max) / T) + 2^52 rounded to a whole number, as its bit pattern, for a
+// logit of weight at `place`: the weight is what exceeds kSmpBase.  With (x - max) / T =
+// (f - n) / 256 octaves, n = rint(place): 2^(45 - n / 256) from the table and the exponent,
+// 2^(f / 256) from its series (|f| <= 0.51, so the fourth term is below 2^-42 of the sum).
+constexpr uint64_t kSmpBase = 0x4330000000000000ull;
+__device__ __forceinline__ uint64_t smp_weight52(const double* table, float x, float place, double max, double c) {
+    constexpr double a1 = 0.0027076061740622863, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3;  // ln 2 / 256
+    const float m = place + 12582912.0f;  // 1.5 * 2^23: the low bits are n
+    const int n = __float_as_int(m) & 0x3FFFFF;
+    const double f = fma((double)x - max, c, (double)(m - 12582912.0f));
+    const double p = fma(f, fma(f, fma(f, a3, a2), a1), 1.0);
+    const double t = table[n & 255];
+    return (uint64_t)__double_as_longlong(fma(__hiloint2double(__double2hiint(t) - ((n >> 8) << 20), __double2loint(t)), p, 4503599627370496.0));
+}
 
-    __device__ __forceinline__ float place(float x) const { return (max - x) * per; }  // NaN: a NaN logit, or greedy
-    __device__ __forceinline__ int bucket(float x) const {  // monotone; kSmpBuckets: no weight
-        return x == max ? 0 : (int)fminf(place(x), (float)kSmpBuckets);
+// The weights of N logits, those without one as 0.
+template <int N>
+__device__ __forceinline__ void smp_weights(const SampleShared& s, const float (&v)[N], uint64_t (&w)[N]) {
+    const SampleRow& r = s.row;
+    const double max = (double)r.max, c = r.c;
+    const float mx = r.max, per = r.per;
+    const bool flat = r.flat;
+    const uint64_t floor = r.floor;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float at = fmaxf((mx - v[i]) * per, 0.0f);
+        const bool in = at < (float)kSmpUnits;
+        const uint64_t q = flat ? (uint64_t)kSmpOne : smp_weight52(s.table, in ? v[i] : mx, in ? at : 0.0f, max, c) - kSmpBase;
+        w[i] = in && q >= floor ? q : 0;
     }
-    // round(2^45 exp((x - max) / T)), 0 below the floor; for x in a bucket.  With
-    // s = 64 log2(e) (x - max) / T = n + f: 2^(n / 64) from the table, 2^(f / 64) from its
-    // series (|f| <= 1/2, so the fifth term is below 2^-44 of the sum).
-    __device__ __forceinline__ uint64_t weight(float x) const {
-        if (x == max) return (uint64_t)kSmpOne;
-        constexpr double kShift = 6755399441055744.0;  // 1.5 * 2^52
-        constexpr double a1 = 0.010830424696249145, a2 = a1 * a1 / 2, a3 = a2 * a1 / 3, a4 = a3 * a1 / 4;  // ln 2 / 64
-        const double d = ((double)x - (double)max) * c, r = d + kShift, f = d - (r - kShift);
-        const int n = __double2loint(r);
-        const double p = fma(f, fma(f, fma(f, fma(f, a4, a3), a2), a1), 1.0);
-        double t = table[n & 63];
-        t = __hiloint2double(__double2hiint(t) + ((n >> 6) << 20), __double2loint(t));
-        const uint64_t w = (uint64_t)__double_as_longlong(fma(t, p, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
-        return w >= floor ? w : 0;
-    }
-};
+}
+// The weight of a logit of weight, 0 below the floor.
+__device__ __noinline__ uint64_t smp_weight(const SampleShared& s, float x) {
+    if (s.row.flat) return (uint64_t)kSmpOne;
+    const uint64_t w = smp_weight52(s.table, x, s.row.place(x), (double)s.row.max, s.row.c) - kSmpBase;
+    return w >= s.row.floor ? w : 0;
+}
 
 // 16 bytes of logits as fp32.
 template <typename T>
@@ -151,7 +195,10 @@ struct SmpChunk<float> {
     static __device__ __forceinline__ float max(const uint4& u) {
         return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
     }
-    static __device__ __forceinline__ void drop(uint4& u, int i) { (&u.x)[i] = kNone; }
+    static __device__ __forceinline__ uint32_t no_nan(uint32_t w) {
+        return __float_as_uint(fmaxf(__uint_as_float(w), -INFINITY));
+    }
+    static __device__ __forceinline__ void set_none(uint8_t* p) { *reinterpret_cast<uint32_t*>(p) = kNone; }
 };
 template <>
 struct SmpChunk<__nv_bfloat16> {
@@ -174,10 +221,8 @@ struct SmpChunk<__nv_bfloat16> {
         const uint32_t m = max2(max2(u.x, u.y), max2(u.z, u.w));
         return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
     }
-    static __device__ __forceinline__ void drop(uint4& u, int i) {
-        uint32_t& w = (&u.x)[i >> 1];
-        w = i & 1 ? (w & 0xFFFFu) | 0xFF800000u : (w & 0xFFFF0000u) | 0xFF80u;
-    }
+    static __device__ __forceinline__ uint32_t no_nan(uint32_t w) { return max2(w, kNone); }
+    static __device__ __forceinline__ void set_none(uint8_t* p) { *reinterpret_cast<uint16_t*>(p) = 0xFF80; }
 };
 
 __device__ __forceinline__ void hist_clear(SampleShared& s) {
@@ -191,7 +236,7 @@ __device__ __forceinline__ void hist_add(SampleShared& s, int b, uint64_t w) {
 }
 
 // The bucket in which the running sum reaches `need` (the first with inclusive sum
-// >= need) and the sum before it, in s.bucket and s.before.  All buckets together
+// >= need) and the sum before it, in s.b_bucket and s.b_before.  All buckets together
 // hold at least `need`.
 template <typename F>
 __device__ __forceinline__ void find_bucket(SampleShared& s, F&& value, uint64_t need) {
@@ -214,73 +259,104 @@ __device__ __forceinline__ void find_bucket(SampleShared& s, F&& value, uint64_t
 #pragma unroll
     for (int i = 0; i < per; ++i) {
         if (before < need && before + v[i] >= need) {
-            s.bucket = tid * per + i;
-            s.before = before;
+            s.b_bucket = tid * per + i;
+            s.b_before = before;
         }
         before += v[i];
     }
     __syncthreads();
 }
 
-// Of the listed logits in `bucket`: the smallest key v (not below r.key) for which
-// the sum of value(x) over x > v is below `need`; that sum goes to s.sum.
-template <typename F>
-__device__ __forceinline__ float list_border(SampleShared& s, const SampleRow& r, int n, int bucket, uint64_t need, F&& value) {
-    const int tid = threadIdx.x;
-    if (tid == 0) s.n_few = 0;
-    __syncthreads();
-    for (int i = tid; i < n; i += kSmpThreads) {
-        const float v = s.list[i];
-        if (r.bucket(v) == bucket && value(v) != 0) {
-            const uint32_t at = atomicAdd(&s.n_few, 1);
-            if (at < 32) s.few[at] = v;
-        }
-    }
-    __syncthreads();
-    const int few = (int)s.n_few;
-    if (few <= 32) {
-        // the border is the largest listed key with sum over x >= key of at least need, or r.key
-        if (tid < 32) {
-            const float mine = tid < few ? s.few[tid] : -INFINITY;
-            const uint64_t w = tid < few ? value(mine) : 0;
-            uint64_t above = 0, with = 0;
-            for (int i = 0; i < few; ++i) {
-                const float v = __shfl_sync(0xffffffffu, mine, i);
-                const uint64_t q = __shfl_sync(0xffffffffu, w, i);
-                if (v > mine) above += q;
-                if (v >= mine) with += q;
-            }
-            const bool is = tid < few && above < need && with >= need;
-            const uint32_t b = __ballot_sync(0xffffffffu, is);
-            const uint64_t all = warp_sum_u64(w);
-            if (b ? tid == __ffs(b) - 1 : tid == 0) {
-                s.key = b ? mine : r.key;
-                s.sum = b ? above : all;
-            }
-        }
+// What is summed: the number of logits, or their weights, above the row's present key.
+__device__ __forceinline__ uint64_t smp_value(const SampleShared& s, float x, bool weights) {
+    return x <= s.row.key ? 0 : weights ? smp_weight(s, x) : 1;
+}
+
+// Of the n listed logits in `bucket`: the smallest key v (not below the present one)
+// for which the sum of values over x > v is below `need`; that sum goes to s.b_sum.
+// While more than a warp's logits are in question, a histogram over their ordered
+// bit patterns leaves those of one of 2048 equal parts of their range.
+__device__ __noinline__ float list_border(SampleShared& s, int n, int bucket, uint64_t need, bool weights) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const SampleRow& r = s.row;
+    auto value = [&](float v) { return smp_value(s, v, weights); };
+    uint32_t from = 0, to = 0xffffffffu;  // the patterns in question
+    uint64_t done = 0;                    // sum of the values above them
+#pragma unroll 1
+    while (true) {
+        uint32_t least = 0xffffffffu, most = 0, count = 0;
         __syncthreads();
-        return s.key;
-    }
-    uint32_t lo = order_bits(r.key), hi = order_bits(r.max);  // the answer is in [lo, hi]
-    uint64_t above = 0;
-    while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        uint64_t sum = 0;
+        if (tid == 0) s.n_few = 0;
+        __syncthreads();
         for (int i = tid; i < n; i += kSmpThreads) {
             const float v = s.list[i];
-            if (order_bits(v) > mid && r.bucket(v) == bucket) sum += value(v);
+            const uint32_t o = order_bits(v);
+            if (v > r.key && r.bucket(v) == bucket && o >= from && o <= to) {
+                least = min(least, o), most = max(most, o);
+                ++count;
+                const uint32_t at = atomicAdd(&s.n_few, 1);
+                if (at < 32) s.few[at] = v;
+            }
         }
-        sum = block_sum(s, sum);
-        if (sum < need) {
-            hi = mid;
-            above = sum;
-        } else {
-            lo = mid + 1;
+        least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) s.redc[warp] = least, s.red[warp] = most;
+        __syncthreads();
+        least = __reduce_min_sync(0xffffffffu, s.redc[tid % kSmpWarps]);
+        most = __reduce_max_sync(0xffffffffu, (uint32_t)s.red[tid % kSmpWarps]);
+        const int few = (int)s.n_few;
+        if (few <= 32) {
+            // the border is the largest of them with sum over x >= key of at least need, or the present key
+            if (tid < 32) {
+                const float mine = tid < few ? s.few[tid] : -INFINITY;
+                const uint64_t w = tid < few ? value(mine) : 0;
+                uint64_t above = 0, with = 0;
+                for (int i = 0; i < few; ++i) {
+                    const float v = __shfl_sync(0xffffffffu, mine, i);
+                    const uint64_t q = __shfl_sync(0xffffffffu, w, i);
+                    if (v > mine) above += q;
+                    if (v >= mine) with += q;
+                }
+                const bool is = tid < few && above < need && with >= need;
+                const uint32_t b = __ballot_sync(0xffffffffu, is);
+                const uint64_t all = warp_sum_u64(w);
+                if (b ? tid == __ffs(b) - 1 : tid == 0) {
+                    s.b_key = b ? mine : r.key;
+                    s.b_sum = done + (b ? above : all);
+                }
+            }
+            __syncthreads();
+            return s.b_key;
         }
+        if (least == most) {  // one key, many times
+            const uint64_t all = block_sum(s, value(from_order(least)) * count);
+            if (tid == 0) s.b_sum = all >= need ? done : done + all;
+            __syncthreads();
+            return all >= need ? from_order(least) : r.key;
+        }
+        const int shift = max(32 - __clz(most - least) - 11, 0);
+        hist_clear(s);
+        uint64_t all = 0;
+        for (int i = tid; i < n; i += kSmpThreads) {
+            const float v = s.list[i];
+            const uint32_t o = order_bits(v);
+            if (v > r.key && r.bucket(v) == bucket && o >= least && o <= most) {
+                const uint64_t w = value(v);
+                if (w) hist_add(s, (int)((most - o) >> shift), w);
+                all += w;
+            }
+        }
+        all = block_sum(s, all);
+        if (all < need) {  // the border is the present key
+            if (tid == 0) s.b_sum = done + all;
+            __syncthreads();
+            return r.key;
+        }
+        find_bucket(s, [&](int b) { return (uint64_t)s.hi[b] << 32 | s.lo[b]; }, need);
+        const uint32_t b = s.b_bucket;
+        done += s.b_before, need -= s.b_before;
+        to = most - (b << shift);
+        from = to - least >= (1u << shift) ? to - (1u << shift) + 1 : least;
     }
-    if (tid == 0) s.sum = above;
-    __syncthreads();
-    return from_order(lo);
 }
 
 template <typename T>
@@ -300,7 +376,17 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
         else
             __syncthreads();
     };
-    // s.*entry of every block of the cluster, for this block's value (block-uniform)
+    // another block's entry of s
+    auto of = [&](auto* entry, int i) { return *cluster.map_shared_rank(entry, i); };
+    // after a barrier: the sum of the blocks' entries
+    auto total_of = [&](auto* entry) {
+        auto v = of(entry, lane < blocks ? lane : 0);
+        if (lane >= blocks) v = 0;
+#pragma unroll
+        for (int o = kSmpBlocks / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return __shfl_sync(0xffffffffu, v, 0);
+    };
+    // writes the first block's value to every block's entry
     auto tell = [&](auto* entry, auto value) {
         if (tid < blocks) *cluster.map_shared_rank(entry, tid) = value;
     };
@@ -312,6 +398,14 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
     const int chunks = (a.V + shift + K::N - 1) / K::N;
     const int chunk0 = (rank * kSmpWarps + warp) * a.steps * 32 + lane;  // index order: block, warp, step, lane
     uint4* mine = raw + warp * a.steps * 32 + lane;
+    const float temp = a.t ? __ldg(a.t + row) : a.t0, top_p = a.p ? __ldg(a.p + row) : a.p0,
+                min_p = a.m ? __ldg(a.m + row) : a.m0;
+    int k = a.k ? __ldg(a.k + row) : a.k0;
+    const double ud = fmin(fmax((double)__ldg(a.u + row), 0.0), 1.0);
+    // T <= 0 (and NaN) takes the first largest logit
+    const bool greedy = !(temp > 0.0f);
+    if (greedy) k = 1;
+    const bool by_k = k > 0 && k < a.V, by_p = top_p < 1.0f && !greedy;
     float mx = -INFINITY;
 #pragma unroll 4
     for (int j = 0; j < a.steps; ++j) {
@@ -319,352 +413,382 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
         uint4 u = make_uint4(K::kNone, K::kNone, K::kNone, K::kNone);
         if (c < chunks) {
             u = __ldg(src + c);
-            if (c == 0 || c == chunks - 1) {  // what lies beside the row in its first and last chunk
-                for (int i = 0; i < K::N; ++i) {
-                    const int at = c * K::N - shift + i;
-                    if (at < 0 || at >= a.V) K::drop(u, i);
-                }
-            }
+            u.x = K::no_nan(u.x), u.y = K::no_nan(u.y), u.z = K::no_nan(u.z), u.w = K::no_nan(u.w);
         }
         mine[j * 32] = u;
+        if (c == 0 || c == chunks - 1) {  // what lies beside the row in its first and last chunk
+#pragma unroll 1
+            for (int i = 0; i < K::N; ++i) {
+                const int at = c * K::N - shift + i;
+                if (at < 0 || at >= a.V) K::set_none(reinterpret_cast<uint8_t*>(mine + j * 32) + i * sizeof(T));
+            }
+            u = mine[j * 32];
+        }
         mx = fmaxf(mx, K::max(u));
     }
-    if (tid < 64) s.table[tid] = exp2((double)tid / 64.0) * kSmpOne;
+    if (tid < 256) s.table[tid] = exp2(45.0 - (double)tid / 256.0);
     if (tid == 0) s.n = 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float own = mx;
+    auto warp_max = [](float v, int lanes) {
+        for (int o = lanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    };
+    mx = warp_max(mx, 32);
     if (lane == 0) s.redf[warp] = mx;
     __syncthreads();
-    mx = s.redf[tid % kSmpWarps];
-#pragma unroll
-    for (int o = kSmpWarps / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = warp_max(s.redf[tid % kSmpWarps], kSmpWarps);
+    float kth = -INFINITY;  // not above the k-th largest logit
+    if (by_k && k <= kSmpKMost && mx > -INFINITY) {
+        uint32_t lo = order_bits(-INFINITY), hi = order_bits(mx);  // k threads or more are not below lo
+        if (k == 1) lo = hi;
+        // the 14 bits below the first in which the border can differ settle it well enough
+        const uint32_t from = order_bits(own);
+        const float least = mx - 64.0f * fabsf(mx) - 64.0f;
+        if (__syncthreads_count(own >= least) >= k) lo = max(lo, order_bits(least));
+#pragma unroll 1
+        for (int i = 0; i < 16 && lo < hi; ++i) {
+            const uint32_t mid = lo + (hi - lo + 1) / 2;
+            if (__syncthreads_count(from >= mid) >= k)
+                lo = mid;
+            else
+                hi = mid - 1;
+        }
+        kth = from_order(lo);
+    }
     if (blocks > 1) {
-        cluster.sync();  // every block runs before its shared memory is written from outside
-        tell(&s.of_max[rank], mx);
+        if (tid == 0) s.max = mx, s.kth = kth;
         cluster.sync();
-        for (int i = 0; i < blocks; ++i) mx = fmaxf(mx, s.of_max[i]);
+        const int i = lane < blocks ? lane : 0;
+        mx = of(&s.max, i), kth = of(&s.kth, i);
+        mx = __shfl_sync(0xffffffffu, warp_max(mx, kSmpBlocks), 0);
+        kth = __shfl_sync(0xffffffffu, warp_max(kth, kSmpBlocks), 0);
     }
-    if (mx == -INFINITY) {  // nothing to draw from
-        if (rank == 0 && tid == 0) a.out[row] = -1;
-        return;
+    SampleRow& r = s.row;
+    if (tid == 0) {
+        r.max = mx;
+        r.per = greedy ? INFINITY : fmaxf(369.32993f / temp, 1.2e-38f);
+        r.c = greedy ? 0.0 : 369.32993046757463 / (double)temp;
+        r.floor = min_p > 0.0f ? max((uint64_t)__double2ull_ru(fmin((double)min_p, 1.0) * kSmpOne), (uint64_t)1) : 1;
+        r.flat = greedy || mx == INFINITY;
+        r.key = -INFINITY;
+        r.ties = 0;
     }
-
-    const float temp = a.t ? __ldg(a.t + row) : a.t0, top_p = a.p ? __ldg(a.p + row) : a.p0,
-                min_p = a.m ? __ldg(a.m + row) : a.m0;
-    int k = a.k ? __ldg(a.k + row) : a.k0;
-    SampleRow r;
-    r.table = s.table;
-    r.max = mx;
-    // T <= 0 (and NaN) takes the first largest logit
-    const bool greedy = !(temp > 0.0f);
-    r.c = greedy ? 0.0 : 92.332482616893657 / (double)temp;
-    r.per = greedy ? INFINITY : 64.0f / temp;
-    r.floor = min_p > 0.0f ? max((uint64_t)__double2ull_ru(fmin((double)min_p, 1.0) * kSmpOne), (uint64_t)1) : 1;
-    r.key = -INFINITY;
-    r.ties = 0;
-    if (greedy) k = 1;
-    const bool by_k = k > 0 && k < a.V, by_p = top_p < 1.0f && !greedy;
+    __syncthreads();
     const double p = fmax((double)top_p, 0.0);
     // kept while the sum before an element is < top_p * total: need = ceil(top_p * total), at least 1
     auto share = [&](uint64_t total) { return max((uint64_t)ceil(p * (double)total), (uint64_t)1); };
-    auto one = [](float) { return (uint64_t)1; };
 
-    // Every element of the block's run that may have weight: f(x).
+    // Every logit of the thread's part of the run: f(x).
     auto each = [&](auto&& f) {
 #pragma unroll 1
         for (int j = 0; j < a.steps; ++j) {
-            const uint4 u = mine[j * 32];
-            float v[K::N];
-            K::get(u, v);
-#pragma unroll
-            for (int i = 0; i < K::N; ++i) f(v[i]);
+            const T* e = reinterpret_cast<const T*>(mine + j * 32);
+#pragma unroll 1
+            for (int i = 0; i < K::N; ++i) f((float)e[i]);
         }
     };
     auto push = [&](float v) {
         const uint32_t at = atomicAdd(&s.n, 1);
         if (at < kSmpList) s.list[at] = v;
     };
-    // The blocks' lists, joined in the first block's: how many; more than
-    // kSmpList: they do not fit, and nothing is joined.
-    auto join_lists = [&]() {
-        __syncthreads();
-        const uint32_t n = s.n;
-        tell(&s.of_n[rank], n);
-        sync();
-        uint32_t at = 0, all = 0;
-        for (int i = 0; i < blocks; ++i) {
-            if (i < rank) at += s.of_n[i];
-            all += s.of_n[i];
-        }
+    // After a barrier: all blocks' lists into the first block's (they fit).  The first block.
+    auto pull_lists = [&]() {
         if (blocks > 1) {
-            if (rank > 0 && all <= kSmpList) {
-                float* to = cluster.map_shared_rank(s.list, 0) + at;
-                for (uint32_t i = tid; i < n; i += kSmpThreads) to[i] = s.list[i];
-            }
-            cluster.sync();
+            const uint32_t n = of(&s.n, lane < blocks ? lane : 0);
+            const int from = 1 + warp % (blocks - 1);  // a warp or more per block
+            const uint32_t at = __reduce_add_sync(0xffffffffu, lane < from ? n : 0), count = __shfl_sync(0xffffffffu, n, from);
+            const float* list = cluster.map_shared_rank(s.list, from);
+            const int warps = (kSmpWarps - from) / (blocks - 1) + 1;
+            for (uint32_t e = warp / (blocks - 1) * 32 + lane; e < count; e += warps * 32) s.list[at + e] = list[e];
         }
-        return all;
+        __syncthreads();
     };
     // The first block's findings, for all.
-    auto publish = [&](float key, uint32_t ties) {
+    auto publish = [&](int slot, float key, uint32_t ties, uint32_t ok) {
         __syncthreads();
-        if (rank == 0) {
-            tell(&s.key, key);
-            tell(&s.ties, ties);
-        }
+        if (rank == 0) tell(&s.found[slot], SampleFound{key, ties, ok});
         sync();
-        r.key = s.key;
-        r.ties = s.ties;
-        sync();
+        if (tid == 0) r.key = s.found[slot].key, r.ties = s.found[slot].ties;
+        __syncthreads();
+        return s.found[slot].ok != 0;
     };
-
-    // The border by a histogram over the runs: sets r.key and r.ties so that value
-    // (of logits above the present r.key; that border's own ties weigh tie_value
-    // together) is kept up to need(total).  All blocks.
-    auto dense = [&](auto&& value, uint64_t tie_value, auto&& need_of) {
-        hist_clear(s);
-        each([&](float v) {
-            const int b = r.bucket(v);
-            if (b < kSmpBuckets && v > r.key) {
-                const uint64_t w = value(v);
-                if (w) hist_add(s, b, w);
-            }
-        });
-        if (rank == 0 && tid == 0 && tie_value) hist_add(s, r.bucket(r.key), tie_value);
-        sync();
-        if (rank == 0) {
-            uint64_t sum = 0;
-            for (int b = tid * 4; b < kSmpBuckets; b += kSmpThreads * 4) {
-                uint64_t w[4] = {};
-                for (int i = 0; i < blocks; ++i) {
-                    const uint4 l = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.lo, i) + b);
-                    const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.hi, i) + b);
-                    w[0] += (uint64_t)h.x << 32 | l.x, w[1] += (uint64_t)h.y << 32 | l.y;
-                    w[2] += (uint64_t)h.z << 32 | l.z, w[3] += (uint64_t)h.w << 32 | l.w;
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s.lo[b + i] = (uint32_t)w[i], s.hi[b + i] = (uint32_t)(w[i] >> 32);
-                    sum += w[i];
-                }
-            }
-            const uint64_t total = block_sum(s, sum), need = need_of(total);
-            if (need < total) find_bucket(s, [&](int b) { return (uint64_t)s.hi[b] << 32 | s.lo[b]; }, need);
-            const uint64_t before = s.before;
-            const uint32_t bucket = s.bucket;
-            __syncthreads();
-            tell(&s.total, total);
-            if (need < total) {
-                tell(&s.bucket, bucket);
-                tell(&s.before, before);
-            }
-        }
-        if (tid == 0) s.n = 0;
-        sync();
-        const uint64_t total = s.total, need = need_of(total);
-        if (need >= total) {
-            sync();
-            return;
-        }
-        const int bucket = (int)s.bucket;
-        const uint64_t left = need - s.before;
-        each([&](float v) {
-            if (r.bucket(v) == bucket && v > r.key && value(v) != 0) push(v);
-        });
-        const uint32_t n = join_lists();
-        float key;
-        uint64_t above;
-        if (n <= kSmpList) {
-            key = r.key, above = 0;
-            if (rank == 0) {
-                key = list_border(s, r, (int)n, bucket, left, value);
-                above = s.sum;
-            }
-        } else {  // over the runs: all blocks see the same sums and take the same steps
-            uint32_t lo = order_bits(r.key), hi = order_bits(r.max);
-            above = 0;
-            for (int step = 0; lo < hi; step ^= 1) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                uint64_t sum = 0;
-                each([&](float v) {
-                    if (order_bits(v) > mid && r.bucket(v) == bucket) sum += value(v);
-                });
-                sum = block_sum(s, sum);
-                tell(&s.of_sum[step][rank], sum);
-                sync();
-                sum = 0;
-                for (int i = 0; i < blocks; ++i) sum += s.of_sum[step][i];
-                if (sum < left) {
-                    hi = mid;
-                    above = sum;
-                } else {
-                    lo = mid + 1;
-                }
-            }
-            key = from_order(lo);
-        }
-        const uint64_t w = value(key), rest = left - above;
+    // How many of a border's ties are kept when `rest` is still missing above it.
+    auto ties_for = [&](float key, uint64_t rest, bool weights) {
+        const uint64_t w = weights ? smp_weight(s, key) : 1;
         uint32_t ties = w ? (uint32_t)min((rest + w - 1) / w, (uint64_t)0xffffffffu) : 0;
-        if (key == r.key) ties = min(ties, r.ties);  // at the earlier border, whose ties come last
-        publish(key, ties);
+        if (key == r.key) ties = min(ties, r.ties);  // at the earlier border, whose own ties come last
+        return ties;
     };
 
     // ---- top-k and top-p
-    if (by_k || by_p) {
-        const bool all_weights = by_p && !by_k;  // top-p of the whole row: its sum is needed
-        uint64_t sum = 0, cand = 0;
-        if (all_weights) {
-            each([&](float v) {
-                const float at = r.place(v);
-                if (at < (float)kSmpBuckets || v == r.max) {
-                    const uint64_t w = r.weight(v);
-                    sum += w;
-                    if (w && (at < kSmpCut || v == r.max)) {
-                        cand += w;
-                        push(v);
-                    }
+    if ((by_k || by_p) && mx > -INFINITY) {
+        uint64_t sum = 0;
+        const bool try_list = !by_k || k <= kSmpKMost;
+        bool done = false;
+        if (try_list) {
+            uint64_t part = 0;
+            const float cut = by_k ? (float)kSmpUnits : kSmpCut;
+#pragma unroll 1
+            for (int j = 0; j < a.steps; ++j) {
+                const uint4 u = mine[j * 32];
+                const float top = K::max(u), top_at = r.place(top);
+                if (!(top >= kth && top_at < (float)kSmpUnits)) continue;
+                float v[K::N];
+                K::get(u, v);
+                if (!by_k) {  // top-p of the whole row: its sum is needed
+                    uint64_t w[K::N];
+                    smp_weights(s, v, w);
+#pragma unroll
+                    for (int i = 0; i < K::N; ++i) part += w[i];
+                    if (top_at >= kSmpCut) continue;
                 }
-            });
-            sum = block_sum(s, sum);
-            cand = block_sum(s, cand);
-        } else {
+#pragma unroll
+                for (int i = 0; i < K::N; ++i)
+                    if (v[i] >= kth && r.place(v[i]) < cut) push(v[i]);
+            }
+            if (!by_k) {
+                sum = block_sum(s, part);
+                if (tid == 0) s.sum = sum;
+            }
+            sync();
+            const uint32_t n = total_of(&s.n);
+            if (!by_k) sum = total_of(&s.sum);
+            if (n <= kSmpList) {  // the first block looks for the borders among the candidates
+                bool ok = true;
+                if (rank == 0) {
+                    pull_lists();
+                    if (by_k && n > (uint32_t)k) {  // (fewer: all with any weight are candidates, and are kept)
+                        hist_clear(s);
+                        for (int i = tid; i < (int)n; i += kSmpThreads) atomicAdd(&s.lo[r.bucket(s.list[i])], 1u);
+                        __syncthreads();
+                        find_bucket(s, [&](int b) { return (uint64_t)s.lo[b]; }, (uint64_t)k);
+                        const uint64_t left = k - s.b_before;
+                        const float key = list_border(s, (int)n, (int)s.b_bucket, left, false);
+                        if (tid == 0) r.key = key, r.ties = (uint32_t)(left - s.b_sum);
+                    } else if (by_k && n == (uint32_t)k) {  // all candidates, and nothing below them
+                        float low = INFINITY;
+                        for (int i = tid; i < (int)n; i += kSmpThreads) low = fminf(low, s.list[i]);
+                        low = -warp_max(-low, 32);
+                        if (lane == 0) s.redf[warp] = low;
+                        __syncthreads();
+                        low = -warp_max(-s.redf[tid % kSmpWarps], kSmpWarps);
+                        uint64_t same = 0;
+                        for (int i = tid; i < (int)n; i += kSmpThreads) same += s.list[i] == low;
+                        same = block_sum(s, same);
+                        if (tid == 0) r.key = low, r.ties = (uint32_t)same;
+                    }
+                    __syncthreads();
+                    if (by_p) {
+                        uint64_t listed = 0;
+                        for (int i = tid; i < (int)n; i += kSmpThreads) listed += smp_value(s, s.list[i], true);
+                        if (tid == 0 && r.ties) listed += smp_weight(s, r.key) * r.ties;
+                        listed = block_sum(s, listed);
+                        if (by_k) sum = listed;
+                        const uint64_t need = share(sum);
+                        ok = listed >= need;
+                        if (ok && need < sum) {
+                            hist_clear(s);
+                            for (int i = tid; i < (int)n; i += kSmpThreads) {
+                                const uint64_t w = smp_value(s, s.list[i], true);
+                                if (w) hist_add(s, r.bucket(s.list[i]), w);
+                            }
+                            if (tid == 0 && r.ties) {
+                                const uint64_t w = smp_weight(s, r.key) * r.ties;
+                                if (w) hist_add(s, r.bucket(r.key), w);
+                            }
+                            __syncthreads();
+                            find_bucket(s, [&](int b) { return (uint64_t)s.hi[b] << 32 | s.lo[b]; }, need);
+                            const uint64_t left = need - s.b_before;
+                            const float key = list_border(s, (int)n, (int)s.b_bucket, left, true);
+                            const uint32_t ties = ties_for(key, left - s.b_sum, true);
+                            __syncthreads();
+                            if (tid == 0) r.key = key, r.ties = ties;
+                        }
+                    }
+                    __syncthreads();
+                }
+                done = publish(0, r.key, r.ties, ok);
+            }
+        }
+        // By a histogram over the runs, first for top-k, then for top-p: all blocks.
+#pragma unroll 1
+        for (int pass = 0; pass < 2 && !done; ++pass) {
+            const bool weights = pass == 1;
+            if (!(weights ? by_p : by_k)) continue;
+            hist_clear(s);
 #pragma unroll 1
             for (int j = 0; j < a.steps; ++j) {
                 const uint4 u = mine[j * 32];
                 const float top = K::max(u);
-                if (r.place(top) < kSmpCut || top == r.max) {
-                    float v[K::N];
-                    K::get(u, v);
+                if (!(top > r.key && r.place(top) < (float)kSmpUnits)) continue;
+                float v[K::N];
+                K::get(u, v);
+                if (weights) {
+                    uint64_t w[K::N];
+                    smp_weights(s, v, w);
 #pragma unroll
                     for (int i = 0; i < K::N; ++i)
-                        if (r.place(v[i]) < kSmpCut || v[i] == r.max) push(v[i]);
+                        if (v[i] > r.key && w[i]) hist_add(s, r.bucket(v[i]), w[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < K::N; ++i) {
+                        const int b = r.bucket(v[i]);
+                        if (v[i] > r.key && b < SampleRow::kNone) atomicAdd(&s.lo[b], 1u);
+                    }
                 }
             }
-        }
-        tell(&s.of_sum[0][rank], sum);
-        tell(&s.of_cand[rank], cand);
-        const uint32_t n = join_lists();
-        sum = cand = 0;
-        for (int i = 0; i < blocks; ++i) sum += s.of_sum[0][i], cand += s.of_cand[i];
-        bool done_k = !by_k, done_p = !by_p;
-        if (n <= kSmpList && (by_k ? n >= (uint32_t)k : cand >= share(sum))) {
-            // the borders are among the candidates: the first block finds them
-            float key = r.key;
-            uint32_t ties = 0;
+            if (rank == 0 && tid == 0 && r.ties) {  // (top-p behind top-k) the earlier border's own ties
+                const uint64_t w = smp_weight(s, r.key) * r.ties;
+                if (w) hist_add(s, r.bucket(r.key), w);
+            }
+            sync();
+            auto need_of = [&](uint64_t total) { return weights ? share(total) : min((uint64_t)k, total); };
             if (rank == 0) {
-                if (by_k) {
-                    hist_clear(s);
-                    for (int i = tid; i < (int)n; i += kSmpThreads) atomicAdd(&s.lo[r.bucket(s.list[i])], 1u);
-                    __syncthreads();
-                    find_bucket(s, [&](int b) { return (uint64_t)s.lo[b]; }, (uint64_t)k);
-                    const uint64_t left = k - s.before;
-                    key = list_border(s, r, (int)n, (int)s.bucket, left, one);
-                    ties = (uint32_t)(left - s.sum);
-                    r.key = key, r.ties = ties;
-                }
-                if (by_p) {
-                    auto value = [&](float v) { return v > r.key ? r.weight(v) : (uint64_t)0; };
-                    hist_clear(s);
-                    uint64_t listed = 0;
-                    for (int i = tid; i < (int)n; i += kSmpThreads) {
-                        const float v = s.list[i];
-                        const uint64_t w = value(v);
-                        if (w) hist_add(s, r.bucket(v), w);
-                        listed += w;
+                uint64_t all = 0;
+                for (int b = tid * 4; b < kSmpBuckets; b += kSmpThreads * 4) {
+                    uint64_t w[4] = {};
+                    for (int i = 0; i < blocks; ++i) {
+                        const uint4 l = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.lo, i) + b);
+                        const uint4 h = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(s.hi, i) + b);
+                        w[0] += (uint64_t)h.x << 32 | l.x, w[1] += (uint64_t)h.y << 32 | l.y;
+                        w[2] += (uint64_t)h.z << 32 | l.z, w[3] += (uint64_t)h.w << 32 | l.w;
                     }
-                    if (tid == 0 && r.ties) {
-                        const uint64_t w = r.weight(r.key) * r.ties;
-                        if (w) hist_add(s, r.bucket(r.key), w);
-                        listed += w;
-                    }
-                    if (by_k) sum = block_sum(s, listed);
-                    __syncthreads();
-                    const uint64_t need = share(sum);
-                    if (need < sum) {
-                        find_bucket(s, [&](int b) { return (uint64_t)s.hi[b] << 32 | s.lo[b]; }, need);
-                        const uint64_t left = need - s.before;
-                        key = list_border(s, r, (int)n, (int)s.bucket, left, value);
-                        const uint64_t rest = left - s.sum, w = r.weight(key);
-                        ties = w ? (uint32_t)min((rest + w - 1) / w, (uint64_t)0xffffffffu) : 0;
-                        if (key == r.key) ties = min(ties, r.ties);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s.lo[b + i] = (uint32_t)w[i], s.hi[b + i] = (uint32_t)(w[i] >> 32);
+                        all += w[i];
                     }
                 }
-                __syncthreads();
+                all = block_sum(s, all);
+                const uint64_t need = need_of(all);
+                if (need < all) {
+                    find_bucket(s, [&](int b) { return (uint64_t)s.hi[b] << 32 | s.lo[b]; }, need);
+                    tell(&s.bucket[pass], s.b_bucket);
+                    tell(&s.before[pass], s.b_before);
+                }
+                tell(&s.total[pass], all);
             }
-            publish(key, ties);
-            done_k = done_p = true;
-        }
-        if (!done_k)  // (no cut where there are not more than k logits with weight)
-            dense(one, 0, [&](uint64_t total) { return min((uint64_t)k, total); });
-        if (!done_p) {
-            const float key = r.key;
-            dense([&](float v) { return r.weight(v); }, r.ties ? r.weight(key) * r.ties : 0, share);
+            if (tid == 0) s.n = 0;
+            sync();
+            const uint64_t total = s.total[pass], need = need_of(total);
+            if (need >= total) continue;  // no cut
+            const int bucket = (int)s.bucket[pass];
+            const uint64_t left = need - s.before[pass];
+#pragma unroll 1
+            for (int j = 0; j < a.steps; ++j) {
+                const uint4 u = mine[j * 32];
+                if (r.bucket(K::max(u)) > bucket) continue;
+                float v[K::N];
+                K::get(u, v);
+#pragma unroll
+                for (int i = 0; i < K::N; ++i)
+                    if (v[i] > r.key && r.bucket(v[i]) == bucket) push(v[i]);
+            }
+            sync();
+            const uint32_t n = total_of(&s.n);
+            float key = r.key;
+            uint64_t above = 0;
+            if (n <= kSmpList) {
+                if (rank == 0) {
+                    pull_lists();
+                    key = list_border(s, (int)n, bucket, left, weights);
+                    above = s.b_sum;
+                }
+            } else {  // over the runs: all blocks see the same sums and take the same steps
+                uint32_t lo = order_bits(r.key), hi = order_bits(r.max);
+#pragma unroll 1
+                for (int step = 0; lo < hi; step ^= 1) {
+                    const uint32_t mid = lo + (hi - lo) / 2;
+                    uint64_t part = 0;
+                    each([&](float v) {
+                        if (order_bits(v) > mid && r.bucket(v) == bucket) part += smp_value(s, v, weights);
+                    });
+                    part = block_sum(s, part);
+                    if (tid == 0) s.part[step] = part;
+                    sync();
+                    part = total_of(&s.part[step]);
+                    if (part < left) {
+                        hi = mid;
+                        above = part;
+                    } else {
+                        lo = mid + 1;
+                    }
+                }
+                key = from_order(lo);
+            }
+            publish(1 + pass, key, ties_for(key, left - above, weights), 1);
         }
     }
 
     // ---- draw
+    const float key = r.key;
+    const uint32_t key_ties = r.ties;
     uint64_t sum = 0;
     uint32_t ties = 0;
 #pragma unroll 1
     for (int j = 0; j < a.steps; ++j) {
         const uint4 u = mine[j * 32];
-        if (K::max(u) >= r.key) {
-            float v[K::N];
-            K::get(u, v);
+        const float top = K::max(u);
+        if (top < key || !(r.place(top) < (float)kSmpUnits)) continue;
+        float v[K::N];
+        uint64_t w[K::N];
+        K::get(u, v);
+        smp_weights(s, v, w);
 #pragma unroll
-            for (int i = 0; i < K::N; ++i) {
-                if (v[i] > r.key && (r.place(v[i]) < (float)kSmpBuckets || v[i] == r.max)) sum += r.weight(v[i]);
-                if (r.ties && v[i] == r.key) ++ties;
-            }
+        for (int i = 0; i < K::N; ++i) {
+            sum += v[i] > key ? w[i] : 0;
+            ties += key_ties && v[i] == key ? 1 : 0;
         }
     }
     sum = warp_sum_u64(sum);
     ties = __reduce_add_sync(0xffffffffu, ties);
-    __syncthreads();
     if (lane == 0) s.redc[warp] = ties, s.red[warp] = sum;
     __syncthreads();
-    uint64_t of_block = 0, before = 0;  // without ties
-    uint32_t ties_of_block = 0, ties_before = 0;
-    for (int i = 0; i < kSmpWarps; ++i) {
-        if (i < warp) before += s.red[i], ties_before += s.redc[i];
-        of_block += s.red[i], ties_of_block += s.redc[i];
-    }
-    uint64_t total = of_block;
-    uint32_t all_ties = ties_of_block;
+    // sums without ties: before this warp, of all
+    uint64_t total = lane < kSmpWarps ? s.red[lane] : 0, before = lane < warp ? total : 0;
+    uint32_t all_ties = lane < kSmpWarps ? s.redc[lane] : 0, ties_before = lane < warp ? all_ties : 0;
+    before = warp_sum_u64(before), ties_before = __reduce_add_sync(0xffffffffu, ties_before);
+    total = warp_sum_u64(total), all_ties = __reduce_add_sync(0xffffffffu, all_ties);
     if (blocks > 1) {
-        tell(&s.of_sum[0][rank], of_block);
-        tell(&s.of_n[rank], ties_of_block);
+        if (tid == 0) s.kept = total, s.kept_ties = all_ties;
         cluster.sync();
-        total = 0, all_ties = 0;
-        for (int i = 0; i < blocks; ++i) {
-            if (i < rank) before += s.of_sum[0][i], ties_before += s.of_n[i];
-            total += s.of_sum[0][i], all_ties += s.of_n[i];
-        }
+        const int i = lane < blocks ? lane : 0;
+        total = of(&s.kept, i), all_ties = of(&s.kept_ties, i);
+        if (lane >= blocks) total = 0, all_ties = 0;
+        before += warp_sum_u64(lane < rank ? total : 0);
+        ties_before += __reduce_add_sync(0xffffffffu, lane < rank ? all_ties : 0);
+        total = warp_sum_u64(total), all_ties = __reduce_add_sync(0xffffffffu, all_ties);
+        // no block leaves while another may read from it
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     }
-    const uint64_t wk = r.ties ? r.weight(r.key) : 0;
-    const uint32_t quota = r.ties > ties_before ? min(r.ties - ties_before, ties) : 0;  // this warp's kept ties
-    before += min(ties_before, r.ties) * wk;
-    total += min(all_ties, r.ties) * wk;
+    const uint64_t wk = key_ties ? smp_weight(s, key) : 0;
+    const uint32_t quota = key_ties > ties_before ? min(key_ties - ties_before, ties) : 0;  // this warp's kept ties
+    before += min(ties_before, key_ties) * wk;
+    total += min(all_ties, key_ties) * wk;
     sum += quota * wk;
-    const double ud = fmin(fmax((double)__ldg(a.u + row), 0.0), 1.0);
+    if (mx == -INFINITY) {  // nothing to draw from
+        if (rank == 0 && tid == 0) a.out[row] = -1;
+        total = sum = 0;
+    }
     // first index whose running sum exceeds u * total; u = 1 takes the last kept one
-    const uint64_t target = min((uint64_t)(ud * (double)total), total - 1);
+    const uint64_t target = total ? min((uint64_t)(ud * (double)total), total - 1) : 0;
     if (target >= before && target < before + sum) {  // one warp of the cluster
         uint32_t left = quota;
         uint64_t at = before;
+#pragma unroll 1
         for (int j = 0; j < a.steps; ++j) {
-            const uint4 u = mine[j * 32];
-            if (!__any_sync(0xffffffffu, K::max(u) >= r.key)) continue;
-            float v[K::N];
-            K::get(u, v);
-            uint64_t w[K::N], own = 0;
-            uint32_t eq = 0;
-#pragma unroll
-            for (int i = 0; i < K::N; ++i) {
-                w[i] = v[i] > r.key && (r.place(v[i]) < (float)kSmpBuckets || v[i] == r.max) ? r.weight(v[i]) : 0;
-                eq += r.ties && v[i] == r.key ? 1 : 0;
-            }
-            uint32_t eq_before = eq;  // ties in lower lanes
+            const float top = K::max(mine[j * 32]);
+            if (!__any_sync(0xffffffffu, top >= key && r.place(top) < (float)kSmpUnits)) continue;
+            const T* e = reinterpret_cast<const T*>(mine + j * 32);
+            auto weigh = [&](float v, uint32_t& eq, uint32_t ahead) -> uint64_t {
+                if (v > key) return r.place(v) < (float)kSmpUnits ? smp_weight(s, v) : 0;
+                if (!key_ties || v != key) return 0;
+                return ahead + eq++ < left ? wk : 0;
+            };
+            uint32_t eq = 0, eq_before = 0;  // ties of this lane; of lower lanes
+#pragma unroll 1
+            for (int i = 0; i < K::N; ++i) eq += key_ties && (float)e[i] == key ? 1 : 0;
+            eq_before = eq;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const uint32_t n = __shfl_up_sync(0xffffffffu, eq_before, o);
@@ -672,12 +796,10 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
             }
             const uint32_t eq_all = __shfl_sync(0xffffffffu, eq_before, 31);
             eq_before -= eq;
-#pragma unroll
-            for (int i = 0; i < K::N; ++i) {
-                if (r.ties && v[i] == r.key && eq_before++ < left) w[i] = wk;
-                own += w[i];
-            }
-            left -= min(left, eq_all);
+            uint64_t own = 0;
+            eq = 0;
+#pragma unroll 1
+            for (int i = 0; i < K::N; ++i) own += weigh((float)e[i], eq, eq_before);
             uint64_t inc = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -688,20 +810,25 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
             if (hit) {
                 if (lane == __ffs(hit) - 1) {
                     uint64_t run = at + inc - own;
-                    int token = -1;
-#pragma unroll
-                    for (int i = 0; i < K::N; ++i) {
-                        run += w[i];
-                        if (token < 0 && run > target) token = (chunk0 + j * 32) * K::N - shift + i;
+                    eq = 0;
+                    int i = 0;
+#pragma unroll 1
+                    for (; i < K::N; ++i) {
+                        run += weigh((float)e[i], eq, eq_before);
+                        if (run > target) break;
                     }
-                    a.out[row] = token;
+                    a.out[row] = (chunk0 + j * 32) * K::N - shift + i;
                 }
                 break;
             }
+            left -= min(left, eq_all);
             at += __shfl_sync(0xffffffffu, inc, 31);
         }
     }
-    if (blocks > 1) cluster.sync();  // no block leaves while another may write to it
+    if (blocks > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
 }
 
 template <typename T>
