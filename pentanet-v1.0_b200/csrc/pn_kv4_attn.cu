@@ -64,7 +64,6 @@ struct Kv4AttnArgs {
     float* part;       // workspace: partial results of two segments per block
 };
 
-constexpr int kAttnTokens = 128;  // tokens of a unit: 32 per warp
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 
@@ -100,14 +99,16 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
-// Row tiles of RT query rows and the units of sequence b (every row tile is
+// Row tiles and the units of sequence b (every row tile is
 // walked over all of the sequence's tokens; what a tile may not see is skipped
 // when it is met).  The host has checked that all units together fit 31 bits.
-__device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, uint32_t rt_rows, uint32_t& nt) {
+// C: the kernel's configuration, with kRows query rows to a row tile and kTokens tokens to a unit.
+template <typename C>
+__device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, uint32_t& nt) {
     int64_t first, n;
     kv4_rows(a.s, b, first, n);
-    nt = max((kv4_len(a.s, b) + kAttnTokens - 1) / kAttnTokens, 1);
-    return ((uint32_t)n * a.G + rt_rows - 1) / rt_rows * nt * a.s.Hk;
+    nt = max((kv4_len(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
+    return ((uint32_t)n * a.G + C::kRows - 1) / C::kRows * nt * a.s.Hk;
 }
 
 // The units of the call, and this block's run [begin, end): all threads of the
@@ -118,13 +119,14 @@ struct AttnRun {
 __device__ __forceinline__ uint32_t attn_begin(uint32_t total, uint32_t blocks, uint32_t c) {
     return total / blocks * c + min(c, total % blocks);
 }
-__device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a, uint32_t rt_rows) {
+template <typename C>
+__device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
     __shared__ uint32_t sums[kAttnWarps], start[2];
     // thread t takes sequences [t * per, (t + 1) * per)
     const uint32_t B = (uint32_t)a.s.B, per = (B + kAttnThreads - 1) / kAttnThreads;
     const uint32_t b0 = min(threadIdx.x * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0, nt;
-    for (uint32_t b = b0; b < b1; ++b) sum += attn_units(a, b, rt_rows, nt);
+    for (uint32_t b = b0; b < b1; ++b) sum += attn_units<C>(a, b, nt);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     uint32_t inc = sum;
 #pragma unroll
@@ -147,7 +149,7 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a, uint32_t rt_r
     if (run.begin >= at && run.begin < at + sum) {
         uint32_t b = b0;
         for (; b < b1; ++b) {
-            const uint32_t n = attn_units(a, b, rt_rows, nt);
+            const uint32_t n = attn_units<C>(a, b, nt);
             if (run.begin < at + n) break;
             at += n;
         }
@@ -170,23 +172,25 @@ struct AttnSeg {
     int lim_min;             // the last position that its first row sees
 
     // Advances `in_seq` to its sequence first.
-    __device__ __forceinline__ AttnSeg(const Kv4AttnArgs& a, uint32_t rt_rows, uint32_t& seq, uint32_t& in_seq,
-                                       uint32_t left) {
-        uint32_t n = attn_units(a, seq, rt_rows, nt);
+    template <typename C>
+    __device__ __forceinline__ AttnSeg(const Kv4AttnArgs& a, const C&, uint32_t& seq, uint32_t& in_seq, uint32_t left) {
+        uint32_t n = attn_units<C>(a, seq, nt);
         while (in_seq >= n) {  // past the sequence (or one without rows)
             in_seq -= n;
             ++seq;
-            n = attn_units(a, seq, rt_rows, nt);
+            n = attn_units<C>(a, seq, nt);
         }
         b = seq;
         // a row tile's units are consecutive: (head, row tile, token tile)
         int64_t n_rows;
         kv4_rows(a.s, b, row0, n_rows);
-        const uint32_t q_rows = (uint32_t)n_rows * a.G, n_rt = (q_rows + rt_rows - 1) / rt_rows;
+        const uint32_t q_rows = (uint32_t)n_rows * a.G, n_rt = (q_rows + C::kRows - 1) / C::kRows;
         const uint32_t tile = in_seq / nt;
         head = (int)(tile / n_rt);
-        r0 = (tile - head * n_rt) * rt_rows;
-        rows = (int)min(rt_rows, q_rows - (uint32_t)r0);
+        // first and last row tiles in turn: of a long prompt the first see few tokens, the last many
+        const uint32_t i = tile - head * n_rt;
+        r0 = (i & 1 ? n_rt - 1 - (i >> 1) : i >> 1) * C::kRows;
+        rows = (int)min((uint32_t)C::kRows, q_rows - (uint32_t)r0);
         t0 = in_seq - tile * nt;
         t1 = min(nt, t0 + left);
         pos0 = kv4_len(a.s, b) - (int)n_rows;
@@ -199,6 +203,16 @@ struct AttnSeg {
         return (a.s.cu ? (row0 + i) * a.q_sl : b * a.q_sb + i * a.q_sl) + (head * a.G + (rr - i * a.G)) * a.q_sh;
     }
 };
+
+// Leaves the joining kernel a note where a row tile ends in this block and began
+// in an earlier one.
+__device__ __forceinline__ void attn_note(const Kv4AttnArgs& a, const AttnRun& run, const AttnSeg& sg, uint32_t unit) {
+    if (sg.t0 == 0 || sg.t1 != sg.nt) return;
+    // the block that holds the tile's first unit: the first `rem` blocks hold one more
+    const uint32_t u0 = unit - sg.t0, each = run.total / gridDim.x, rem = run.total % gridDim.x;
+    const uint32_t c0 = u0 < (each + 1) * rem ? u0 / (each + 1) : rem + (u0 - (each + 1) * rem) / each;
+    a.notes[blockIdx.x] = {sg.rows, (int)c0, attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0, a.G, sg.row0, sg.r0, sg.head};
+}
 
 // Looks up the pages of a sequence, 32 pieces of 16 tokens at a time: lane l
 // holds where piece (base + l)'s keys begin.
@@ -286,14 +300,15 @@ template <int D, int NT>
 struct AttnCfg {
     static constexpr int W = D / 32;             // words per thread and token
     static constexpr int kRows = 8 * NT;         // query rows of a row tile
-    static constexpr int kStages = NT == 4 ? 8 : 6;
+    static constexpr int kTokens = 128;          // tokens of a unit: 32 per warp
+    static constexpr int kStages = 6;
     static constexpr int kCodes = 16 * (D / 2);  // bytes of one 16-token piece of keys or values
     static constexpr int kStage = 2 * kCodes + 128;
     static constexpr int kRing = kStages * kStage;  // per warp
     static constexpr int kSmem = kAttnWarps * kRing;
     static constexpr int kPitch = D + 8;         // floats per row of the join buffer (over the warp's own ring)
     static constexpr int kPart = kRows * (D + 2);  // floats of one partial result
-    static constexpr int kBlocks = NT <= 2 ? 3 : 2;  // per SM
+    static constexpr int kBlocks = 3;  // per SM
     static_assert(kRows * kPitch * 4 <= kRing, "the join buffer lies over the ring");
 };
 
@@ -332,7 +347,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    AttnRun run = attn_plan(a, RT);
+    AttnRun run = attn_plan<C>(a);
     if (tid == 0) a.notes[blockIdx.x].rows = 0;
     const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
     // a lane's part of a piece: 16-byte chunks of codes, and of the pairs (lanes 0-3 keys, 4-7 values)
@@ -343,17 +358,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 
     uint32_t seq = run.seq, in_seq = run.in_seq;
     for (uint32_t unit = run.begin; unit < run.end;) {
-        const AttnSeg sg(a, RT, seq, in_seq, run.end - unit);
+        const AttnSeg sg(a, C{}, seq, in_seq, run.end - unit);
 
         // ---- the warp's runs: tokens [128 * tile + 32 * warp, + 32), two pieces each
-        const int used = min((int)sg.t1, (sg.kv_end + kAttnTokens - 1) / kAttnTokens);  // tiles behind it are skipped
+        const int used = min((int)sg.t1, (sg.kv_end + C::kTokens - 1) / C::kTokens);  // tiles behind it are skipped
         const int count = used - (int)sg.t0;
-        const int tok_base = (int)sg.t0 * kAttnTokens + warp * 32;
+        const int tok_base = (int)sg.t0 * C::kTokens + warp * 32;
         AttnPages pages;
         uint32_t dead = 0;  // ring of flags: the piece is not there
         auto issue = [&](int i, uint32_t slot) {  // run i; slot: its first stage's offset in the ring
             if ((i & 15) == 0) {  // lane 2 k + j looks up piece j of run i + k
-                const int k = i + (lane >> 1), tok = tok_base + k * kAttnTokens + (lane & 1) * 16;
+                const int k = i + (lane >> 1), tok = tok_base + k * C::kTokens + (lane & 1) * 16;
                 pages.look_up(a, sg.b, sg.head, block, tok, k < count && tok < sg.kv_end);
             }
 #pragma unroll
@@ -448,7 +463,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
             float top = -INFINITY, vtop = 0.0f, rel[2][NT][4];  // rel: logit - m
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int tok0 = tok_base + i * kAttnTokens + j * 16;
+                const int tok0 = tok_base + i * C::kTokens + j * 16;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const uint32_t kp = *reinterpret_cast<const uint32_t*>(st[j] + 2 * C::kCodes + (g + 8 * k) * 4);
@@ -564,7 +579,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
             issue(i + ST / 2 - 1, fill);
             cp_wait<ST / 2 - 1>();
             __syncwarp();
-            const bool mask = (dead >> (2 * (i & 15)) & 3u) || tok_base + i * kAttnTokens + 31 > sg.lim_min;
+            const bool mask = (dead >> (2 * (i & 15)) & 3u) || tok_base + i * C::kTokens + 31 > sg.lim_min;
             if (mask)
                 pieces(i, slot, std::true_type{});
             else
@@ -628,14 +643,293 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                 if (d == 0) part[RT * D + r * 2] = mx, part[RT * D + r * 2 + 1] = sum;
             }
         }
-        if (tid == 0 && sg.t0 > 0 && sg.t1 == sg.nt) {  // the tile ends here and began in an earlier block
-            // the block that holds the tile's first unit: the first `rem` blocks hold one more
-            const uint32_t u0 = unit - sg.t0, each = run.total / gridDim.x, rem = run.total % gridDim.x;
-            const uint32_t c0 = u0 < (each + 1) * rem ? u0 / (each + 1) : rem + (u0 - (each + 1) * rem) / each;
-            a.notes[blockIdx.x] = {sg.rows, (int)c0, attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0, a.G,
-                                   sg.row0, sg.r0, sg.head};
-        }
+        if (tid == 0) attn_note(a, run, sg, unit);
         __syncthreads();
+        unit += sg.t1 - sg.t0;
+        in_seq += sg.t1 - sg.t0;
+    }
+}
+
+// Prompts and chunks of them: 64 query rows per block, 16 per warp, which share
+// the tokens' pieces in shared memory.  Here the rows are the 16-row operand, the
+// codes the 8-column one: the same words and masks give it (the first operand's
+// registers are two of the second's).  A block steps through 64 tokens at a time,
+// a warp through 32 of them at once; rows meet the softmax as they lie in the
+// accumulators, and their weights go back in as they come out.
+//
+// What bounds it: m16n8k16 runs at one per ten cycles on each quarter of an SM
+// (measured; 460 TFLOP/s over the device), 128 of them to a warp's 64 tokens at
+// d = 128, against 320 mask and shift instructions at two cycles each.
+template <int D>
+struct ChunkCfg {
+    static constexpr int W = D / 32;
+    static constexpr int kRows = 64, kTokens = 64;
+    static constexpr int kStages = 3;
+    static constexpr int kCodes = 16 * (D / 2);
+    static constexpr int kPiece = 2 * kCodes + 128;  // 16 tokens, as in AttnCfg
+    static constexpr int kTile = 4 * kPiece;
+    static constexpr int kSmem = kStages * kTile;
+    static constexpr int kPart = kRows * (D + 2);
+    static constexpr int kBlocks = 3;  // per SM
+};
+
+template <int D>
+__global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_kernel(const Kv4AttnArgs a) {
+    using C = ChunkCfg<D>;
+    constexpr int W = C::W, ST = C::kStages;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint8_t dead[ST][4];  // the piece is not there
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int g = lane >> 2, t = lane & 3;
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const AttnRun run = attn_plan<C>(a);
+    if (tid == 0) a.notes[blockIdx.x].rows = 0;
+    const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
+    const uint32_t pair_off = (uint32_t)a.s.page * (D / 2) + (lane & 3) * 16 + (lane & 4 ? (uint32_t)block : 0u);
+    const uint32_t base_u = smem_u32(smem) + warp * C::kPiece;  // this warp copies piece `warp` of every tile
+    const uint32_t dst_k = base_u + lane * 16, dst_v = base_u + C::kCodes + v_chunk<D>(lane / (D / 16), lane % (D / 16)),
+                   dst_p = base_u + 2 * C::kCodes + lane * 16;
+
+    uint32_t seq = run.seq, in_seq = run.in_seq;
+    for (uint32_t unit = run.begin; unit < run.end;) {
+        const AttnSeg sg(a, C{}, seq, in_seq, run.end - unit);
+        const int used = min((int)sg.t1, (sg.kv_end + C::kTokens - 1) / C::kTokens);
+        const int count = used - (int)sg.t0;
+        const int tok_base = (int)sg.t0 * C::kTokens;
+        AttnPages pages;
+        auto issue = [&](int i, int stage) {
+            if ((i & 31) == 0) {
+                const int tok = tok_base + (i + lane) * C::kTokens + warp * 16;
+                pages.look_up(a, sg.b, sg.head, block, tok, i + lane < count && tok < sg.kv_end);
+            }
+            const uint64_t addr = __shfl_sync(0xffffffffu, pages.addr, i & 31);
+            const uint32_t off = __shfl_sync(0xffffffffu, pages.off, i & 31);
+            if (lane == 0) dead[stage][warp] = addr == 0;
+            if (addr) {
+                const uint8_t* kc = reinterpret_cast<const uint8_t*>(addr) + (off * (D / 2) + lane * 16);
+                const uint8_t* vc = kc + block;
+                const uint32_t st = stage * C::kTile;
+#pragma unroll
+                for (int c = 0; c < C::kCodes / 512; ++c) {
+                    cp_async16(dst_k + st + c * 512, kc + c * 512);
+                    cp_async16(dst_v + st + c * 512, vc + c * 512);
+                }
+                if (lane < 8) cp_async16(dst_p + st, reinterpret_cast<const uint8_t*>(addr) + (pair_off + off * 4));
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < ST - 1; ++i) issue(i, i);
+
+        // ---- this warp's rows: g and g + 8
+        const int w_rows = min(sg.rows - warp * 16, 16);  // none: the warp only copies
+        uint32_t qa[D / 8], qc[D / 8];
+        float ca[2], cb[2];
+        int lim[2], w_end = 0, w_min = 0;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int r = warp * 16 + k * 8 + g;
+            const char* row = nullptr;
+            if (r < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, r) * (a.q_f32 ? 4 : 2);
+            load_query<D>(a, row, t, k ? qc : qa, ca[k], cb[k]);
+            lim[k] = r < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + r) / a.G) : sg.kv_end - 1;
+        }
+        if (w_rows > 0) {
+            w_min = sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16) / a.G);
+            w_end = max(sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16 + w_rows - 1) / a.G) + 1, 0);
+            // a padding row sees what the warp's last one does
+            if (warp * 16 + g >= sg.rows) lim[0] = w_end - 1;
+            if (warp * 16 + 8 + g >= sg.rows) lim[1] = w_end - 1;
+        }
+
+        float o[D / 8][4], neg_m[2] = {INFINITY, INFINITY};
+        float2 l[2], zs[2];
+        float S = 0.0f, inv_S = 0.0f;  // as in the decode kernel
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[j][k] = 0.0f;
+        l[0] = l[1] = zs[0] = zs[1] = make_float2(0.0f, 0.0f);
+
+        // 32 tokens from tok on, pieces `st` and the next.
+        auto half = [&](const uint8_t* st, int tok, bool dead0, bool dead1, auto mask) {
+            constexpr bool kMask = decltype(mask)::value;
+            float acc[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[j][k] = 0.0f;
+            }
+#pragma unroll
+            for (int w = 0; w < W; w += 2) {  // two words of each token at a time, the tokens' chains in turn
+                uint32_t kw[4][2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(st + (j >> 1) * C::kPiece + ((j & 1) * 8 + g) * (D / 2) + t * 4 * W + w * 4);
+                    kw[j][0] = u.x, kw[j][1] = u.y;
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t u = h ? kw[j][x] >> 8 : kw[j][x];
+                            const int q = (w + x) * 4 + h * 2;
+                            mma_f16(acc[j], qa[q], qc[q], qa[q + 1], qc[q + 1], u & 0x000F000Fu, u & 0x00F000F0u);
+                        }
+            }
+            // ---- logits; columns 2t, 2t + 1 of n-tile j are tokens 8 j + 2 t, + 1
+            float top = -INFINITY, vtop = 0.0f;
+            uint2 vp[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint8_t* pairs = st + (j >> 1) * C::kPiece + 2 * C::kCodes + ((j & 1) * 8 + 2 * t) * 4;
+                const uint2 kp = *reinterpret_cast<const uint2*>(pairs);
+                vp[j] = *reinterpret_cast<const uint2*>(pairs + 64);
+                const int tk = tok + j * 8 + 2 * t;
+                const bool gone = kMask && (j < 2 ? dead0 : dead1);
+                if constexpr (kMask) {
+                    if (gone || tk >= w_end) vp[j].x = 0;  // whatever lies behind the sequence
+                    if (gone || tk + 1 >= w_end) vp[j].y = 0;
+                }
+                const float2 ks = make_float2(pair_lo(kp.x), pair_lo(kp.y)), kz = make_float2(pair_hi(kp.x), pair_hi(kp.y));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float2 x = make_float2(acc[j][2 * k], acc[j][2 * k + 1]);
+                    x = fma2(ks, mul2(x, make_float2(ca[k], ca[k])), mul2(kz, make_float2(cb[k], cb[k])));
+                    if constexpr (kMask) {
+                        if (gone || tk > lim[k]) x.x = -INFINITY;
+                        if (gone || tk + 1 > lim[k]) x.y = -INFINITY;
+                    }
+                    acc[j][2 * k] = x.x, acc[j][2 * k + 1] = x.y;
+                    const float2 d = add2(x, make_float2(neg_m[k], neg_m[k]));
+                    top = fmaxf(top, fmaxf(d.x, d.y));
+                }
+                vtop = fmaxf(vtop, fmaxf(pair_lo(vp[j].x), pair_lo(vp[j].y)));
+            }
+            if (__any_sync(0xffffffffu, top > 8.0f || vtop > S)) {  // seldom: see the decode kernel
+                vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
+                vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
+                float fs = 1.0f;
+                if (vtop > S) {
+                    const int e = min(max((int)(__float_as_uint(vtop) >> 23) - 126, -100), 102);
+                    const float was = S;
+                    S = pow2i(e);
+                    inv_S = pow2i(-e);
+                    fs = was * inv_S;
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float x = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x = fmaxf(x, fmaxf(acc[j][2 * k], acc[j][2 * k + 1]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    const float was = neg_m[k], now = fminf(was, -x);
+                    const float f = now == was ? 1.0f : ex2f(now - was);
+                    neg_m[k] = now;
+                    l[k] = mul2(l[k], make_float2(f, f));
+                    zs[k] = mul2(zs[k], make_float2(f, f));
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) o[j][2 * k] *= f * fs, o[j][2 * k + 1] *= f * fs;
+                }
+            }
+            // ---- weights, in place as the first operand of the output's products
+            uint32_t pa[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 vn = mul2(make_float2(pair_lo(vp[j].x), pair_lo(vp[j].y)), make_float2(inv_S, inv_S));
+                const float2 vz = make_float2(pair_hi(vp[j].x), pair_hi(vp[j].y));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float2 d = add2(make_float2(acc[j][2 * k], acc[j][2 * k + 1]), make_float2(neg_m[k], neg_m[k]));
+                    float2 p = make_float2(ex2f(d.x), ex2f(d.y)), pv;
+                    if constexpr (kMask) {  // a token that a row does not see adds nothing, whatever its pair holds
+                        const bool n0 = acc[j][2 * k] == -INFINITY, n1 = acc[j][2 * k + 1] == -INFINITY;
+                        p = make_float2(n0 ? 0.0f : p.x, n1 ? 0.0f : p.y);
+                        zs[k] = add2(zs[k], make_float2(n0 ? 0.0f : p.x * vz.x, n1 ? 0.0f : p.y * vz.y));
+                        pv = make_float2(n0 ? 0.0f : p.x * vn.x, n1 ? 0.0f : p.y * vn.y);
+                    } else {
+                        zs[k] = fma2(p, vz, zs[k]);
+                        pv = mul2(p, vn);
+                    }
+                    l[k] = add2(l[k], p);
+                    pa[j][k] = pack_f16(pv.x, pv.y);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // 16 tokens each
+                uint32_t va[W], vb[W];
+                const uint8_t* sv = st + x * C::kPiece + C::kCodes;
+                lds_words<W>(sv + (W == 4 ? v_chunk<D>(t, g) : v_chunk<D>(t, g >> 1) + (g & 1) * 8), va);
+                lds_words<W>(sv + (W == 4 ? v_chunk<D>(t + 4, g) : v_chunk<D>(t + 4, g >> 1) + (g & 1) * 8), vb);
+#pragma unroll
+                for (int w = 0; w < W; ++w)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t u = h ? va[w] >> 8 : va[w], v = h ? vb[w] >> 8 : vb[w];
+                        mma_f16(o[w * 4 + h * 2], pa[2 * x][0], pa[2 * x][1], pa[2 * x + 1][0], pa[2 * x + 1][1], u & 0x000F000Fu,
+                                v & 0x000F000Fu);
+                        mma_f16(o[w * 4 + h * 2 + 1], pa[2 * x][0], pa[2 * x][1], pa[2 * x + 1][0], pa[2 * x + 1][1],
+                                u & 0x00F000F0u, v & 0x00F000F0u);
+                    }
+            }
+        };
+        int stage = 0;
+        for (int i = 0; i < count; ++i) {
+            cp_wait<ST - 2>();
+            __syncthreads();  // tile i is there for all; all are done with the stage that is filled next
+            issue(i + ST - 1, stage == 0 ? ST - 1 : stage - 1);
+            const uint8_t* tile = smem + stage * C::kTile;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+                const int tok = tok_base + i * C::kTokens + h * 32;
+                if (tok >= w_end) break;
+                const bool d0 = dead[stage][2 * h], d1 = dead[stage][2 * h + 1];
+                if (d0 || d1 || tok + 31 > w_min)
+                    half(tile + 2 * h * C::kPiece, tok, d0, d1, std::true_type{});
+                else
+                    half(tile + 2 * h * C::kPiece, tok, false, false, std::false_type{});
+            }
+            stage = stage == ST - 1 ? 0 : stage + 1;
+        }
+
+        // ---- results: row g's columns 2t and 2t + 1 are 4 W dims each
+        const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
+        float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
+        const float up = S * 16777216.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float sum = l[k].x + l[k].y, z = zs[k].x + zs[k].y;
+#pragma unroll
+            for (int d = 1; d < 4; d <<= 1) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                z += __shfl_xor_sync(0xffffffffu, z, d);
+            }
+            const int r = warp * 16 + k * 8 + g;
+            if (r >= sg.rows) continue;
+            const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
+            const int64_t at = (((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G) * D;
+            const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const int d = 4 * ((2 * t + c) * W + w);
+                    const float4 y = make_float4(fmaf(o[w * 4][2 * k + c], up, z), fmaf(o[w * 4 + 1][2 * k + c], up * 0.0625f, z),
+                                                 fmaf(o[w * 4 + 2][2 * k + c], up, z), fmaf(o[w * 4 + 3][2 * k + c], up * 0.0625f, z));
+                    if (whole)
+                        store_out(a, at + d, y, inv);
+                    else
+                        *reinterpret_cast<float4*>(part + r * D + d) = y;
+                }
+            if (!whole && t == 0) part[C::kRows * D + r * 2] = -neg_m[k], part[C::kRows * D + r * 2 + 1] = sum;
+        }
+        if (tid == 0) attn_note(a, run, sg, unit);
+        __syncthreads();  // nobody reads a stage any more
         unit += sg.t1 - sg.t0;
         in_seq += sg.t1 - sg.t0;
     }
@@ -716,35 +1010,36 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
     }
 }
 
-// 8 NT query rows per tile: the fewest that hold a sequence's rows on average.
-static int attn_nt(int64_t B, int64_t T, int64_t G) {
+// The kernel by the query rows that a sequence has on average for one kv head: up
+// to 8 and up to 16 in the decode kernel, more in the chunk kernel.
+enum AttnKind { kAttn8, kAttn16, kAttnChunk };
+static AttnKind attn_kind(int64_t B, int64_t T, int64_t G) {
     const int64_t rows = (T + B - 1) / B * G;
-    return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    return rows <= 8 ? kAttn8 : rows <= 16 ? kAttn16 : kAttnChunk;
 }
-static int attn_blocks(int nt) {  // blocks that the device holds at once
+static int attn_blocks() {  // blocks that the device holds at once (kBlocks of every configuration)
     const int sms = device_sm_count();
-    return (sms > 0 ? sms : 148) * (nt <= 2 ? 3 : 2);  // AttnCfg::kBlocks
+    return (sms > 0 ? sms : 148) * 3;
 }
 static size_t attn_notes_bytes(int blocks) { return ((size_t)blocks * sizeof(Kv4Join) + 255) / 256 * 256; }
 static size_t attn_workspace(int64_t B, int64_t T, int64_t G, int64_t D) {
     if (B == 0 || T == 0) return 0;
-    const int nt = attn_nt(B, T, G), blocks = attn_blocks(nt);
-    return attn_notes_bytes(blocks) + (size_t)blocks * 2 * (8 * nt) * (D + 2) * 4;
+    const int blocks = attn_blocks();
+    const AttnKind kind = attn_kind(B, T, G);
+    return attn_notes_bytes(blocks) + (size_t)blocks * 2 * (kind == kAttn8 ? 8 : kind == kAttn16 ? 16 : 64) * (D + 2) * 4;
 }
 
-template <int D, int NT>
-static cudaError_t launch_attn(const Kv4AttnArgs& a, cudaStream_t s) {
-    using C = AttnCfg<D, NT>;
+template <int D, typename C>
+static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a, cudaStream_t s) {
     static bool done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !done[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   C::kSmem);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    const int blocks = attn_blocks(NT);
+    const int blocks = attn_blocks();
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -755,7 +1050,7 @@ static cudaError_t launch_attn(const Kv4AttnArgs& a, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<D, NT>, a);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
     if (e != cudaSuccess) return e;
     // Few tiles have many partial results each: more blocks and warps per tile.
     // Many tiles: fewer, most blocks find nothing to join.  (8 tiles of 55
@@ -795,7 +1090,7 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     const size_t e = q_dtype == PN_F32 ? 4 : 2;
     if (!aligned(q, e) || !aligned(out, 16)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: misaligned pointer");
     // an upper bound on the units that the kernels count in 31 bits
-    if (B > 0 && ((double)T * (q_heads / kv_heads) / 8 + B) * kv_heads * ((double)table_w * page / pn::kAttnTokens + 1) > 2e9)
+    if (B > 0 && ((double)T * (q_heads / kv_heads) / 8 + B) * kv_heads * ((double)table_w * page / 64 + 1) > 2e9)
         return fail(PN_ERR_SHAPE, "pn_kv4_attention: %lld rows over tables of %lld tokens are too much for one call",
                     (long long)T, (long long)(table_w * page));
     if (int st = check_device()) return st;
@@ -812,15 +1107,18 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     a.G = (int)(q_heads / kv_heads);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.out = out;
-    const int nt = pn::attn_nt(B, T, a.G);
     a.notes = static_cast<pn::Kv4Join*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_notes_bytes(pn::attn_blocks(nt)));
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_notes_bytes(pn::attn_blocks()));
     const cudaStream_t s = (cudaStream_t)stream;
-    cudaError_t err;
-    if (head_dim == 64)
-        err = nt == 1 ? pn::launch_attn<64, 1>(a, s) : nt == 2 ? pn::launch_attn<64, 2>(a, s) : pn::launch_attn<64, 4>(a, s);
-    else
-        err = nt == 1 ? pn::launch_attn<128, 1>(a, s) : nt == 2 ? pn::launch_attn<128, 2>(a, s) : pn::launch_attn<128, 4>(a, s);
+    auto go = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        switch (pn::attn_kind(B, T, a.G)) {
+            case pn::kAttn8: return pn::launch_attn<D, pn::AttnCfg<D, 1>>(pn::kv4_decode_kernel<D, 1>, a, s);
+            case pn::kAttn16: return pn::launch_attn<D, pn::AttnCfg<D, 2>>(pn::kv4_decode_kernel<D, 2>, a, s);
+            default: return pn::launch_attn<D, pn::ChunkCfg<D>>(pn::kv4_chunk_kernel<D>, a, s);
+        }
+    };
+    const cudaError_t err = head_dim == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
     return err == cudaSuccess ? ok() : cuda_fail(err, "pn_kv4_attention");
 }
 
