@@ -300,8 +300,7 @@ int pn_rms_norm_i8(const void *x, int x_dtype, const void *residual, int64_t M, 
  * the page of its positions [i * page, (i + 1) * page).  seq_lens: (B) int32, the
  * sequences' lengths WITH the rows of this call, taken as at most table_w * page
  * (at most 2^30).  The T rows of a call are the newest positions of their sequences: T / B rows
- * each, or rows [cu_q[b], cu_q[b + 1]) with cu_q (B + 1) int32.  Rows behind
- * cu_q[B] are not touched.  Entries used that are no page of the cache are
+ * each, or rows [cu_q[b], cu_q[b + 1]) with cu_q (B + 1) int32.  Entries used that are no page of the cache are
  * skipped (nothing is stored; their tokens read as zeros and are not attended
  * to) and recorded as PN_ERR_ARG in the device status word.
  * Strides are in elements: of a sequence, a row and a head (the first is not
@@ -309,14 +308,15 @@ int pn_rms_norm_i8(const void *x, int x_dtype, const void *residual, int64_t M, 
 int64_t pn_kv4_block_bytes(int64_t page, int64_t head_dim);
 
 /* Quantise and store the rows' keys and values (PN_BF16 or PN_F32).  A row at
- * a negative position (more rows than the sequence is long) is dropped. */
+ * a negative position (more rows than the sequence is long), or behind cu_q[B], is
+ * dropped. */
 int pn_kv4_append(const void *k, int64_t k_sb, int64_t k_sl, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sl,
                   int64_t v_sh, int kv_dtype, void *cache, int64_t n_pages, int64_t kv_heads, int64_t page,
                   int64_t head_dim, const int32_t *block_table, int64_t table_ld, int64_t table_w,
                   const int32_t *seq_lens, const int32_t *cu_q, int64_t B, int64_t T, void *stream);
 
 /* Read the rows' keys and values back: k, v (T, kv_heads, head_dim) of kv_dtype,
- * contiguous, 16-byte aligned; zeros at negative positions. */
+ * contiguous, 16-byte aligned; zeros at negative positions and behind cu_q[B]. */
 int pn_kv4_gather(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
                   const int32_t *block_table, int64_t table_ld, int64_t table_w, const int32_t *seq_lens,
                   const int32_t *cu_q, int64_t B, int64_t T, void *k, void *v, int kv_dtype, void *stream);
@@ -324,7 +324,8 @@ int pn_kv4_gather(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t 
 /* Causal attention: row i of sequence b (of L_b rows) sees the cached positions
  * up to seq_lens[b] - L_b + i, its own included (store the rows' keys and values
  * first).  out (T, q_heads, head_dim) of q's type (PN_BF16 or PN_F32),
- * contiguous, 16-byte aligned; zeros for a row that sees nothing.  Query head
+ * contiguous, 16-byte aligned; zeros for a row that sees nothing; rows behind
+ * cu_q[B] are left as they were.  Query head
  * h reads kv head h / (q_heads / kv_heads).  The logits are scale * q . k.
  * Queries enter the products as fp16 relative to the row's largest (bf16 ones
  * exactly), weights as fp16; sums and the softmax are fp32.

@@ -116,7 +116,7 @@ __device__ __forceinline__ void kv4_load8(const T* p, bool vec, float (&v)[8]) {
 // Where a row lives, looked up once per row and block.
 struct Kv4Row {
     int64_t src[2];  // first element of its keys and values in the inputs
-    int64_t page;    // page of the cache; -1: none; -2: behind the last sequence
+    int64_t dst;     // its page's first byte in the cache; -1: none
     int tok;         // its place in the page
 };
 constexpr int kKv4Threads = 256;
@@ -125,8 +125,9 @@ constexpr int kKv4MaxRows = 8;  // rows per block
 // A block's vectors are numbered row by row, a row's keys before its values; a
 // thread steps from one to the next without a division.
 struct Kv4Step {
+    int block;    // bytes of a page block
     int per_row;  // 2 * kv heads
-    int dr, dh;   // 256 / lanes per vector, as whole rows and the rest
+    int dr, dh;   // the vectors of a block at once, as whole rows and the rest
 };
 struct Kv4At {
     int r, hv;  // row in the block; head, or Hk + head
@@ -142,20 +143,20 @@ struct Kv4At {
 };
 
 __device__ __forceinline__ void kv4_rows_of_block(const Kv4Seq& s, int64_t row0, int n, const int64_t* sb, const int64_t* sl,
-                                                  Kv4Row* rows) {
+                                                  const Kv4Step& step, Kv4Row* rows) {
     if ((int)threadIdx.x < n) {
         Kv4Row r;
         const int64_t row = row0 + threadIdx.x;
         int64_t b, i;
-        r.page = -2;
+        r.dst = -1;
         r.tok = 0;
         if (kv4_find(s, row, b, i)) {
             int64_t first, count;
             kv4_rows(s, b, first, count);
             const int pos = (int)(kv4_len(s, b) - count + i);
-            r.page = -1;
             if (pos >= 0) {
-                r.page = kv4_page(s, b, pos);
+                const int64_t page = kv4_page(s, b, pos);
+                if (page >= 0) r.dst = page * step.per_row * step.block;
                 r.tok = pos % s.page;
             }
             if (sb)
@@ -217,14 +218,15 @@ __device__ __forceinline__ uint32_t kv4_codes8(const float (&v)[8], float s, flo
 
 // The range of VT lanes' values, a NaN among them kept: (min, max).
 template <int VT>
-__device__ __forceinline__ float2 kv4_range(const Raw8<float>& x) {
-    float v[8];
-    x.get(v);
-    float lo = v[0], hi = v[0];
+__device__ __forceinline__ float2 kv4_range(const Raw8<float> (&x)[2]) {
+    float v[2][8];
+    x[0].get(v[0]);
+    x[1].get(v[1]);
+    float lo = v[0][0], hi = v[0][0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) {
-        lo = min_nan(lo, v[j]);
-        hi = max_nan(hi, v[j]);
+    for (int j = 1; j < 16; ++j) {
+        lo = min_nan(lo, v[j >> 3][j & 7]);
+        hi = max_nan(hi, v[j >> 3][j & 7]);
     }
 #pragma unroll
     for (int o = VT / 2; o > 0; o >>= 1) {
@@ -238,79 +240,93 @@ __device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b) {
     asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+__device__ __forceinline__ uint32_t max2_nan(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
 // bf16: (min, -max) share a register, one shuffle and one minimum per step.
 template <int VT>
-__device__ __forceinline__ float2 kv4_range(const Raw8<__nv_bfloat16>& x) {
+__device__ __forceinline__ float2 kv4_range(const Raw8<__nv_bfloat16> (&x)[2]) {
     constexpr uint32_t kNeg = 0x80008000u;
-    const uint4 u = x.u;
-    const uint32_t lo = min2_nan(min2_nan(u.x, u.y), min2_nan(u.z, u.w));
-    const uint32_t hi = min2_nan(min2_nan(u.x ^ kNeg, u.y ^ kNeg), min2_nan(u.z ^ kNeg, u.w ^ kNeg));
+    const uint4 u = x[0].u, v = x[1].u;
+    const uint32_t lo = min2_nan(min2_nan(min2_nan(u.x, u.y), min2_nan(u.z, u.w)), min2_nan(min2_nan(v.x, v.y), min2_nan(v.z, v.w)));
+    const uint32_t hi = max2_nan(max2_nan(max2_nan(u.x, u.y), max2_nan(u.z, u.w)), max2_nan(max2_nan(v.x, v.y), max2_nan(v.z, v.w))) ^ kNeg;
     uint32_t r = min2_nan(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
 #pragma unroll
     for (int o = VT / 2; o > 0; o >>= 1) r = min2_nan(r, __shfl_xor_sync(0xffffffffu, r, o));
     return make_float2(__uint_as_float(r << 16), __uint_as_float((r & 0xFFFF0000u) ^ 0x80000000u));
 }
 
-// D / 8 lanes per vector, eight dims each; a block takes a few rows with all
+// D / 16 lanes per vector, sixteen dims each; a block takes a few rows with all
 // their heads, the next vector's values in flight while one is stored.  One read
-// of the inputs; what bounds it beside the bytes is the instructions per eight
-// values (the range's shuffles, scale and codes).
+// of the inputs; what bounds it beside the bytes is the instructions per vector
+// (the range's shuffles, scale, codes and addresses): with eight dims per lane
+// 9723 rows of 8 heads took 26 us, 233 instructions per eight values.
 template <typename T, int D>
 __global__ void __launch_bounds__(kKv4Threads) kv4_append_kernel(const Kv4AppendArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
-    constexpr int VT = D / 8, kVecs = kKv4Threads / VT;
+    constexpr int VT = D / 16, kVecs = kKv4Threads / VT;
     __shared__ Kv4Row rows[kKv4MaxRows];
     const int64_t row0 = (int64_t)blockIdx.x * a.rows;
     const int n_rows = (int)min((int64_t)a.rows, a.s.T - row0);
-    kv4_rows_of_block(a.s, row0, n_rows, a.sb, a.sl, rows);
+    kv4_rows_of_block(a.s, row0, n_rows, a.sb, a.sl, a.step, rows);
     const int l = threadIdx.x % VT;
-    const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
 
     Kv4At at(a.step, threadIdx.x / VT);
-    auto load = [&](Raw8<T>& x) {
-        x.zero();
-        if (at.r >= n_rows || rows[at.r].page < 0) return;
+    auto load = [&](Raw8<T> (&x)[2]) {
+        x[0].zero();
+        x[1].zero();
+        if (at.r >= n_rows || rows[at.r].dst < 0) return;
         const bool kv = at.hv >= a.s.Hk;
-        const T* p = static_cast<const T*>(kv ? a.x[1] : a.x[0]) + rows[at.r].src[kv] + l * 8 +
+        const T* p = static_cast<const T*>(kv ? a.x[1] : a.x[0]) + rows[at.r].src[kv] + l * 16 +
                      (kv ? (at.hv - a.s.Hk) * a.sh[1] : at.hv * a.sh[0]);
         if (a.vec) {
-            x.load(p);
+            x[0].load(p);
+            x[1].load(p + 8);
         } else {
             float v[8];
             kv4_load8(p, false, v);
-            x.set(v);
+            x[0].set(v);
+            kv4_load8(p + 8, false, v);
+            x[1].set(v);
         }
     };
-    Raw8<T> x;
+    Raw8<T> x[2];
     load(x);
     for (int base = 0; base < n_rows * a.step.per_row; base += kVecs) {
-        const Raw8<T> now = x;
+        const Raw8<T> now[2] = {x[0], x[1]};
         const Kv4At was = at;
         at.next(a.step);
         load(x);
         const float2 range = kv4_range<VT>(now);
-        if (was.r >= n_rows || rows[was.r].page < 0) continue;
-        const int kv = was.hv >= a.s.Hk ? 1 : 0;
+        if (was.r >= n_rows || rows[was.r].dst < 0) continue;
+        const bool kv = was.hv >= a.s.Hk;
         float z = floor_bf16(range.x);
         float s = ceil_bf16_pos(__fdiv_rn(__fsub_rn(range.y, z), 15.0f));
         if (!(s < INFINITY) || !(fabsf(z) < INFINITY)) {  // an inf or NaN in the vector: all of it reads back as NaN
             s = 0.0f;
             z = __int_as_float(0x7fc00000);
         }
-        float v[8];
-        now.get(v);
-        const uint32_t w = s > 0.0f ? kv4_codes8(v, s, z) : 0;
+        uint2 w = make_uint2(0, 0);
+        if (s > 0.0f) {
+            float v[8];
+            now[0].get(v);
+            w.x = kv4_codes8(v, s, z);
+            now[1].get(v);
+            w.y = kv4_codes8(v, s, z);
+        }
         const int tok = rows[was.r].tok;
-        uint8_t* blk = a.cache + (rows[was.r].page * a.step.per_row + (kv ? 2 * (was.hv - a.s.Hk) + 1 : 2 * was.hv)) * block;
-        if (kv == 0) {
-            *reinterpret_cast<uint32_t*>(blk + tok * (D / 2) + l * 4) = w;
+        uint8_t* blk = a.cache + rows[was.r].dst + (int64_t)(kv ? 2 * (was.hv - a.s.Hk) + 1 : 2 * was.hv) * a.step.block;
+        if (!kv) {
+            *reinterpret_cast<uint2*>(blk + tok * (D / 2) + l * 8) = w;
         } else {
-            uint8_t* p = blk + (tok >> 1) * D + l * 8 + (tok & 1) * 2;
-            *reinterpret_cast<uint16_t*>(p) = (uint16_t)w;
-            *reinterpret_cast<uint16_t*>(p + 4) = (uint16_t)(w >> 16);
+            uint16_t* p = reinterpret_cast<uint16_t*>(blk + (tok >> 1) * D + l * 16 + (tok & 1) * 2);
+            p[0] = (uint16_t)w.x, p[2] = (uint16_t)(w.x >> 16);
+            p[4] = (uint16_t)w.y, p[6] = (uint16_t)(w.y >> 16);
         }
         if (l == 0)
-            *reinterpret_cast<uint32_t*>(blk + (int64_t)a.s.page * (D / 2) + tok * 4) =
+            *reinterpret_cast<uint32_t*>(blk + a.s.page * (D / 2) + tok * 4) =
                 (__float_as_uint(s) >> 16) | (__float_as_uint(z) & 0xFFFF0000u);
     }
 }
@@ -327,60 +343,65 @@ struct Kv4GatherArgs {
 template <int D>
 __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4GatherArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
-    constexpr int VT = D / 8;
+    constexpr int VT = D / 16;
     __shared__ Kv4Row rows[kKv4MaxRows];
     const int64_t row0 = (int64_t)blockIdx.x * a.rows;
     const int n_rows = (int)min((int64_t)a.rows, a.s.T - row0);
-    kv4_rows_of_block(a.s, row0, n_rows, nullptr, nullptr, rows);
+    kv4_rows_of_block(a.s, row0, n_rows, nullptr, nullptr, a.step, rows);
     const int l = threadIdx.x % VT;
-    const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
     Kv4At at(a.step, threadIdx.x / VT);
-    uint32_t w = 0, pair = 0;  // the next vector's codes and (scale, zero)
+    uint2 w = make_uint2(0, 0);  // the next vector's codes and (scale, zero)
+    uint32_t pair = 0;
     auto load = [&]() {
-        w = pair = 0;  // stands for zeros
-        if (at.r >= n_rows || rows[at.r].page < 0) return;
+        w = make_uint2(0, 0);  // stands for zeros
+        pair = 0;
+        if (at.r >= n_rows || rows[at.r].dst < 0) return;
         const bool kv = at.hv >= a.s.Hk;
         const int tok = rows[at.r].tok;
-        const uint8_t* blk = a.cache + (rows[at.r].page * a.step.per_row + (kv ? 2 * (at.hv - a.s.Hk) + 1 : 2 * at.hv)) * block;
-        pair = *reinterpret_cast<const uint32_t*>(blk + (int64_t)a.s.page * (D / 2) + tok * 4);
+        const uint8_t* blk = a.cache + rows[at.r].dst + (int64_t)(kv ? 2 * (at.hv - a.s.Hk) + 1 : 2 * at.hv) * a.step.block;
+        pair = *reinterpret_cast<const uint32_t*>(blk + a.s.page * (D / 2) + tok * 4);
         if (!kv) {
-            w = *reinterpret_cast<const uint32_t*>(blk + tok * (D / 2) + l * 4);
+            w = *reinterpret_cast<const uint2*>(blk + tok * (D / 2) + l * 8);
         } else {
-            const uint2 two = *reinterpret_cast<const uint2*>(blk + (tok >> 1) * D + l * 8);
-            w = __byte_perm(two.x, two.y, tok & 1 ? 0x7632 : 0x5410);
+            const uint4 two = *reinterpret_cast<const uint4*>(blk + (tok >> 1) * D + l * 16);
+            const uint32_t which = tok & 1 ? 0x7632 : 0x5410;
+            w = make_uint2(__byte_perm(two.x, two.y, which), __byte_perm(two.z, two.w, which));
         }
     };
     load();
     while (at.r < n_rows) {
-        const uint32_t now_w = w, now_pair = pair;
+        const uint2 now = w;
+        const uint32_t now_pair = pair;
         const Kv4At was = at;
         at.next(a.step);
         load();
-        if (rows[was.r].page == -2) continue;
         const bool kv = was.hv >= a.s.Hk;
         const float s = __uint_as_float(now_pair << 16), z = __uint_as_float(now_pair & 0xFFFF0000u);
-        // masked into the low bits of 2^23 a code reads as 2^23 + 16^j c; s * c is exact (12 bits), so one rounding
-        float v[8];
-        const float2 z2 = make_float2(z, z), down = make_float2(-8388608.0f, -8388608.0f);
-        float sj = s;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 c = make_float2(__uint_as_float((now_w & (15u << (4 * j))) | 0x4B000000u),
-                                         __uint_as_float(((now_w >> 16) & (15u << (4 * j))) | 0x4B000000u));
-            const float2 y = fma2(add2(c, down), make_float2(sj, sj), z2);
-            v[j] = y.x, v[j + 4] = y.y;
-            sj *= 0.0625f;
-        }
-        const int64_t to = ((row0 + was.r) * a.s.Hk + was.hv - (kv ? a.s.Hk : 0)) * D + l * 8;
+        const int64_t to = ((row0 + was.r) * a.s.Hk + was.hv - (kv ? a.s.Hk : 0)) * D + l * 16;
         void* out = kv ? a.y[1] : a.y[0];
-        if (a.y_f32) {
-            Raw8<float> o;
-            o.set(v);
-            o.store(static_cast<float*>(out) + to);
-        } else {
-            Raw8<__nv_bfloat16> o;
-            o.set(v);
-            o.store(static_cast<__nv_bfloat16*>(out) + to);
+        // masked into the low bits of 2^23 a code reads as 2^23 + 16^j c; s * c is exact (12 bits), so one rounding
+        const float2 z2 = make_float2(z, z), down = make_float2(-8388608.0f, -8388608.0f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t c8 = i ? now.y : now.x;
+            float v[8], sj = s;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 c = make_float2(__uint_as_float((c8 & (15u << (4 * j))) | 0x4B000000u),
+                                             __uint_as_float(((c8 >> 16) & (15u << (4 * j))) | 0x4B000000u));
+                const float2 y = fma2(add2(c, down), make_float2(sj, sj), z2);
+                v[j] = y.x, v[j + 4] = y.y;
+                sj *= 0.0625f;
+            }
+            if (a.y_f32) {
+                Raw8<float> o;
+                o.set(v);
+                o.store(static_cast<float*>(out) + to + i * 8);
+            } else {
+                Raw8<__nv_bfloat16> o;
+                o.set(v);
+                o.store(static_cast<__nv_bfloat16*>(out) + to + i * 8);
+            }
         }
     }
 }
@@ -393,9 +414,9 @@ static int kv4_block_rows(int64_t T) {
     while (r < kKv4MaxRows && T / (2 * r) >= 8 * sms) r *= 2;
     return r;
 }
-static Kv4Step kv4_step(int Hk, int64_t D) {
-    const int vecs = kKv4Threads / (int)(D / 8), per_row = 2 * Hk;
-    return {per_row, vecs / per_row, vecs % per_row};
+static Kv4Step kv4_step(int Hk, int64_t page, int64_t D) {
+    const int vecs = kKv4Threads / (int)(D / 16), per_row = 2 * Hk;
+    return {(int)(page * (D / 2 + 4)), per_row, vecs / per_row, vecs % per_row};
 }
 
 }  // namespace pn
@@ -450,7 +471,7 @@ int pn_kv4_append(const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh, const
     };
     a.vec = whole(0) && whole(1);
     a.rows = pn::kv4_block_rows(T);
-    a.step = pn::kv4_step((int)kv_heads, head_dim);
+    a.step = pn::kv4_step((int)kv_heads, page, head_dim);
     const unsigned g = (unsigned)((T + a.rows - 1) / a.rows);
     const cudaStream_t s = (cudaStream_t)stream;
     if (kv_dtype == PN_F32) {
@@ -482,7 +503,7 @@ int pn_kv4_gather(const void* cache, int64_t n_pages, int64_t kv_heads, int64_t 
     a.y[1] = v;
     a.y_f32 = kv_dtype == PN_F32;
     a.rows = pn::kv4_block_rows(T);
-    a.step = pn::kv4_step((int)kv_heads, head_dim);
+    a.step = pn::kv4_step((int)kv_heads, page, head_dim);
     const unsigned g = (unsigned)((T + a.rows - 1) / a.rows);
     const cudaStream_t s = (cudaStream_t)stream;
     if (head_dim == 64) pn::kv4_gather_kernel<64><<<g, pn::kKv4Threads, 0, s>>>(a);

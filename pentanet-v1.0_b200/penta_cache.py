@@ -22,6 +22,8 @@ penta_native.device_status().
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 try:
@@ -47,7 +49,8 @@ def kv4_cache(n_pages: int, n_kv_heads: int, head_dim: int, page_size: int = 64,
 
 
 def _cache_args(cache, head_dim, block_table, seq_lens, cu_q, device):
-    """(n_pages, kv heads, page size) after the checks that every call shares."""
+    """(n_pages, kv heads, page size) after the checks that every call shares.
+    device: the rows' (index)."""
     assert head_dim in HEAD_DIMS, f"head_dim must be one of {HEAD_DIMS}, got {head_dim}"
     assert cache.dtype == torch.uint8 and cache.dim() == 4 and cache.shape[2] == 2 and cache.is_contiguous(), \
         "cache must be a contiguous uint8 tensor of kv4_cache"
@@ -55,17 +58,23 @@ def _cache_args(cache, head_dim, block_table, seq_lens, cu_q, device):
     page, rest = divmod(size, head_dim // 2 + 4)
     assert rest == 0 and page >= 16 and page % 16 == 0, f"cache blocks of {size} bytes do not fit head_dim {head_dim}"
     assert block_table.dtype == torch.int32 and block_table.dim() == 2, "block_table must be a (B, pages) int32 tensor"
-    B = block_table.shape[0]
-    assert block_table.stride(1) == 1 or block_table.shape[1] <= 1, "block_table rows must be contiguous"
-    assert B <= 1 or block_table.stride(0) >= block_table.shape[1], "block_table rows must not overlap"
+    B, W = block_table.shape
+    assert W <= 1 or block_table.stride(1) == 1, "block_table rows must be contiguous"
+    assert B <= 1 or block_table.stride(0) >= W, "block_table rows must not overlap"
     assert seq_lens.dtype == torch.int32 and seq_lens.shape == (B,) and seq_lens.is_contiguous(), \
         f"seq_lens must be a contiguous ({B},) int32 tensor"
-    assert cache.device == device and block_table.device == device and seq_lens.device == device, \
+    assert cache.get_device() == block_table.get_device() == seq_lens.get_device() == device, \
         "cache, block_table and seq_lens must be on the rows' device"
     if cu_q is not None:
-        assert cu_q.dtype == torch.int32 and cu_q.shape == (B + 1,) and cu_q.is_contiguous() and cu_q.device == device, \
+        assert cu_q.dtype == torch.int32 and cu_q.shape == (B + 1,) and cu_q.is_contiguous() and cu_q.get_device() == device, \
             f"cu_q must be a contiguous ({B + 1},) int32 tensor on the rows' device"
     return n, hk, page
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(B, T, H, hk, D, device_index):
+    with torch.cuda.device(device_index):
+        return int(_nat.load().pn_kv4_attention_workspace_size(B, T, H, hk, D))
 
 
 def _rows(x, B, cu_q, what):
@@ -92,10 +101,10 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, block_tabl
     """Quantise the rows' keys and values (bf16/fp32, any row and head strides)
     into the cache, at the newest positions of their sequences."""
     assert k.is_cuda, "kv4_append requires CUDA tensors"
-    assert k.dtype in _FLOATS and v.dtype == k.dtype and v.shape == k.shape and v.device == k.device, \
+    assert k.dtype in _FLOATS and v.dtype == k.dtype and v.shape == k.shape and v.get_device() == k.get_device(), \
         "k and v must be bfloat16 or float32 tensors of one shape, type and device"
     D = k.shape[-1]
-    n, hk, page = _cache_args(cache, D, block_table, seq_lens, cu_q, k.device)
+    n, hk, page = _cache_args(cache, D, block_table, seq_lens, cu_q, k.get_device())
     assert k.shape[-2] == hk, f"k has {k.shape[-2]} heads, the cache {hk}"
     k, v = _inner(k), _inner(v)
     B, W = block_table.shape
@@ -117,10 +126,9 @@ def kv4_gather(cache: torch.Tensor, head_dim: int, block_table: torch.Tensor, se
     assert cache.is_cuda, "kv4_gather requires CUDA tensors"
     assert dtype in _FLOATS
     rows = tuple(rows)
-    n, hk, page = _cache_args(cache, head_dim, block_table, seq_lens, cu_q, cache.device)
-    make = torch.empty if cu_q is None else torch.zeros
-    k = make((*rows, hk, head_dim), dtype=dtype, device=cache.device)
-    v = make((*rows, hk, head_dim), dtype=dtype, device=cache.device)
+    n, hk, page = _cache_args(cache, head_dim, block_table, seq_lens, cu_q, cache.get_device())
+    k = torch.empty((*rows, hk, head_dim), dtype=dtype, device=cache.device)
+    v = torch.empty((*rows, hk, head_dim), dtype=dtype, device=cache.device)
     B, W = block_table.shape
     T = _rows(k, B, cu_q, "rows")[3]
     with _nat.device_of(cache):
@@ -145,7 +153,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     behind cu_q[B] are left as they were (zeros where no out is given)."""
     assert q.is_cuda and q.dtype in _FLOATS, "kv4_attention takes bfloat16 or float32 CUDA queries"
     D = q.shape[-1]
-    n, hk, page = _cache_args(cache, D, block_table, seq_lens, cu_q, q.device)
+    dev = q.get_device()
+    n, hk, page = _cache_args(cache, D, block_table, seq_lens, cu_q, dev)
     H = q.shape[-2]
     assert H > 0 and H % hk == 0, f"{H} query heads are no multiple of {hk} kv heads"
     q = _inner(q)
@@ -154,14 +163,14 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     if out is None:
         out = (torch.empty if cu_q is None else torch.zeros)(q.shape, dtype=q.dtype, device=q.device)
     else:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device and out.is_contiguous(), \
+        assert out.shape == q.shape and out.dtype == q.dtype and out.get_device() == dev and out.is_contiguous(), \
             "out must be a contiguous tensor of q's shape, type and device"
-    L = _nat.load()
+    size = _attention_workspace(B, T, H, hk, D, dev)
     with _nat.device_of(q):
-        size = L.pn_kv4_attention_workspace_size(B, T, H, hk, D)
         ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-        _nat.check(L.pn_kv4_attention(q.data_ptr(), sb, sl, sh, _FLOATS[q.dtype], H, cache.data_ptr(), n, hk, page, D,
-                                      block_table.data_ptr(), max(block_table.stride(0), W), W, seq_lens.data_ptr(),
-                                      _nat.ptr(cu_q), B, T, D ** -0.5 if scale is None else scale, out.data_ptr(),
-                                      ws.data_ptr(), size, _nat.stream_of(q)), "kv4_attention")
+        _nat.check(_nat.load().pn_kv4_attention(q.data_ptr(), sb, sl, sh, _FLOATS[q.dtype], H, cache.data_ptr(), n, hk, page,
+                                                D, block_table.data_ptr(), max(block_table.stride(0), W), W,
+                                                seq_lens.data_ptr(), _nat.ptr(cu_q), B, T,
+                                                D ** -0.5 if scale is None else scale, out.data_ptr(), ws.data_ptr(), size,
+                                                _nat.stream_of(q)), "kv4_attention")
     return out

@@ -359,19 +359,20 @@ _FLOATS = {torch.float32: _nat.PN_F32, torch.bfloat16: _nat.PN_BF16}
 
 def _rms_args(x, weight, residual, what):
     """(x, residual, h, weight, rows, C) of the RMS norms, ready for the C ABI."""
-    assert x.is_cuda and x.dtype in _FLOATS, f"{what} takes a bfloat16 or float32 CUDA tensor"
-    assert x.dim() >= 1 and x.shape[-1] > 0, f"{what}: the last dimension is empty"
-    C = x.shape[-1]
+    dev, shape = x.get_device(), x.shape
+    assert dev >= 0 and x.dtype in _FLOATS, f"{what} takes a bfloat16 or float32 CUDA tensor"
+    assert len(shape) >= 1 and shape[-1] > 0, f"{what}: the last dimension is empty"
+    C = shape[-1]
     x = x.contiguous()
     r = h = w = None
     if residual is not None:
         assert residual.dtype == x.dtype, f"{what}: the residual has the type of x"
-        assert residual.device == x.device and residual.shape == x.shape, f"{what}: the residual has the shape of x"
+        assert residual.get_device() == dev and residual.shape == shape, f"{what}: the residual has the shape of x"
         r = residual.contiguous()
         h = torch.empty_like(x)
     if weight is not None:
-        w = weight.detach()
-        assert w.dtype in _FLOATS and w.device == x.device and w.numel() == C, f"{what}: weight is ({C},) on x's device"
+        w = weight
+        assert w.dtype in _FLOATS and w.get_device() == dev and w.numel() == C, f"{what}: weight is ({C},) on x's device"
         w = w.contiguous()
     return x, r, h, w, x.numel() // C, C
 
@@ -423,7 +424,7 @@ _MAX_VOCAB = 1 << 18
 def _setting(v, rows, dtype, device, what):
     """A sampling setting as (tensor or None, number)."""
     if isinstance(v, torch.Tensor):
-        assert v.dtype == dtype and v.device == device and v.shape == (rows,), \
+        assert v.dtype == dtype and v.get_device() == device and v.shape == (rows,), \
             f"sample_tokens: {what} is a number or a ({rows},) {dtype} tensor on the logits' device"
         return v.contiguous(), 0
     return None, v
@@ -448,9 +449,9 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     _require_cuda(logits, "sample_tokens")
     B, V = logits.shape
     assert 0 < V <= _MAX_VOCAB, f"the vocabulary must hold 1 to {_MAX_VOCAB} tokens, got {V}"
-    assert u.dtype == torch.float32 and u.device == logits.device and u.shape == (B,), \
+    dev = logits.get_device()
+    assert u.dtype == torch.float32 and u.get_device() == dev and u.shape == (B,), \
         f"u must be a ({B},) float32 tensor on the logits' device"
-    dev = logits.device
     t, t0 = _setting(temperature, B, torch.float32, dev, "temperature")
     k, k0 = _setting(top_k, B, torch.int32, dev, "top_k")
     p, p0 = _setting(top_p, B, torch.float32, dev, "top_p")
@@ -459,7 +460,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     if logits.stride(1) != 1 or logits.stride(0) < V:
         logits = logits.contiguous()
     u = u.contiguous()
-    out = torch.empty(B, dtype=torch.int64, device=dev)
+    out = torch.empty(B, dtype=torch.int64, device=logits.device)
     with _nat.device_of(logits):
         _nat.check(_nat.load().pn_sample_tokens(logits.data_ptr(), _FLOATS[logits.dtype], B, V, max(logits.stride(0), V),
                                                 u.data_ptr(), _nat.ptr(t), t0, _nat.ptr(k), min(int(k0), 0x7fffffff),

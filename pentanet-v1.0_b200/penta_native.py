@@ -136,7 +136,7 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
-        return _raw_stream(t.device.index)
+        return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -156,7 +156,7 @@ _same_device = _SameDevice()
 
 def device_of(t: torch.Tensor):
     """Context in which t's device is the current one (free where it already is)."""
-    return _same_device if t.device.index == _get_device() else torch.cuda.device(t.device)
+    return _same_device if t.get_device() == _get_device() else torch.cuda.device(t.device)
 
 
 @functools.lru_cache(maxsize=4096)

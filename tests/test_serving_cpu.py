@@ -143,13 +143,13 @@ def test_python_refusals():
 def test_cache_argument_checks():
     """The checks that the three cache calls share, on CPU tensors."""
     cache = pc.kv4_cache(2, 2, 64, 16, "cpu")
-    table, lens, dev = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32), torch.device("cpu")
+    table, lens, dev = torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32), -1
     assert pc._cache_args(cache, 64, table, lens, None, dev) == (2, 2, 16)
     cu = torch.zeros(3, dtype=torch.int32)
     bad = [dict(cache=cache.float()), dict(cache=cache[..., :-4]), dict(cache=cache[:, :, :1]), dict(head_dim=128),
            dict(table=table.long()), dict(table=table[0]), dict(lens=lens.long()), dict(lens=lens[:1]), dict(cu=cu.long()),
            dict(cu=cu[:2]), dict(table=torch.zeros(2, 8, dtype=torch.int32)[:, ::2]),
-           dict(table=torch.zeros(1, 8, dtype=torch.int32).expand(2, 8)), dict(dev=torch.device("meta"))]
+           dict(table=torch.zeros(1, 8, dtype=torch.int32).expand(2, 8)), dict(dev=0)]
     for kw in bad:
         a = dict(cache=cache, head_dim=64, table=table, lens=lens, cu=cu, dev=dev, **{})
         a.update(kw)
