@@ -282,6 +282,12 @@ int pn_rms_norm_i8(const void *x, int x_dtype, const void *residual, int64_t M, 
                    int w_dtype, double eps, void *h, int8_t *xq, int64_t xq_pitch, float *s_x, int32_t *rowsum,
                    void *stream);
 
+/* The values that quantised activations stand for: y[m, k] = xq[m, k] * s_x[m]
+ * for k < K, y (M, K) PN_BF16 or PN_F32; xq and s_x as pn_quant_act_i8 or
+ * pn_rms_norm_i8 write them.  No reference counterpart. */
+int pn_dequant_act_i8(const int8_t *xq, int64_t xq_pitch, const float *s_x, int64_t M, int64_t K, void *y, int y_dtype,
+                      void *stream);
+
 /* ---- a paged cache of keys and values in 4 bits, and attention over it (no
  *      reference counterpart; its GPT recomputes the whole prefix) ----------
  *

@@ -7,6 +7,8 @@
 // s = 1.  The output rows are padded with zeros to a pitch the tensor-core
 // kernel loads in 32-byte slabs, and the row sums feed its unsigned-code
 // correction (sum_k xq*(c-2) = sum_k xq*c - 2*sum_k xq).
+#include <type_traits>
+
 #include "pn_common.cuh"
 #include "pn_internal.h"
 
@@ -226,6 +228,71 @@ cudaError_t launch_quant_act_i8(const void* x, int x_dtype, int64_t M, int64_t K
     else
         quant_act_i8_kernel<__nv_bfloat16><<<(unsigned)M, kActThreads, 0, s>>>(
             static_cast<const __nv_bfloat16*>(x), K, xq, pitch, s_x, rowsum);
+    return cudaGetLastError();
+}
+
+// The values that quantised rows stand for: y = float(xq) * s_x, rounded to bf16
+// where asked for.  Sixteen codes per thread; whole 16-byte stores where the rows
+// of y allow them (K % 8 == 0).  One byte in and two out per element: bounded by
+// the bytes from about a thousand rows on.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kActThreads) dequant_act_i8_kernel(const int8_t* __restrict__ xq, int64_t pitch,
+                                                                     const float* __restrict__ s_x, int64_t M, int64_t K,
+                                                                     uint32_t pieces, T* __restrict__ y) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int64_t at = (int64_t)blockIdx.x * kActThreads + threadIdx.x;
+    const int64_t m = at / pieces;
+    if (m >= M) return;
+    const int64_t c0 = (at - m * pieces) * 16;
+    const uint4 u = *reinterpret_cast<const uint4*>(xq + m * pitch + c0);
+    const float s = s_x[m];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __fmul_rn((float)(int8_t)(w[i >> 2] >> (8 * (i & 3))), s);
+    T* row = y + m * K;
+    if constexpr (VEC) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (c0 + 8 * h >= K) break;
+            if constexpr (sizeof(T) == 4) {
+                float4* p = reinterpret_cast<float4*>(row + c0 + 8 * h);
+                p[0] = make_float4(v[8 * h], v[8 * h + 1], v[8 * h + 2], v[8 * h + 3]);
+                p[1] = make_float4(v[8 * h + 4], v[8 * h + 5], v[8 * h + 6], v[8 * h + 7]);
+            } else {
+                uint32_t o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * h + 2 * k], v[8 * h + 2 * k + 1]);
+                    o[k] = *reinterpret_cast<const uint32_t*>(&b);
+                }
+                *reinterpret_cast<uint4*>(row + c0 + 8 * h) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (c0 + i < K) row[c0 + i] = (T)v[i];
+    }
+}
+
+cudaError_t launch_dequant_act_i8(const int8_t* xq, int64_t pitch, const float* s_x, int64_t M, int64_t K, void* y,
+                                  int y_dtype, cudaStream_t s) {
+    if (M == 0) return cudaSuccess;
+    const bool vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(y) % 16 == 0;
+    const uint32_t pieces = (uint32_t)((K + 15) / 16);
+    const unsigned blocks = (unsigned)((M * pieces + kActThreads - 1) / kActThreads);
+    auto go = [&](auto* out) {
+        using T = std::remove_pointer_t<decltype(out)>;
+        if (vec)
+            dequant_act_i8_kernel<T, true><<<blocks, kActThreads, 0, s>>>(xq, pitch, s_x, M, K, pieces, out);
+        else
+            dequant_act_i8_kernel<T, false><<<blocks, kActThreads, 0, s>>>(xq, pitch, s_x, M, K, pieces, out);
+    };
+    if (y_dtype == PN_F32)
+        go(static_cast<float*>(y));
+    else
+        go(static_cast<__nv_bfloat16*>(y));
     return cudaGetLastError();
 }
 

@@ -511,4 +511,18 @@ int pn_rms_norm_i8(const void* x, int x_dtype, const void* residual, int64_t M, 
     return e == cudaSuccess ? ok() : cuda_fail(e, "pn_rms_norm_i8");
 }
 
+int pn_dequant_act_i8(const int8_t* xq, int64_t xq_pitch, const float* s_x, int64_t M, int64_t K, void* y, int y_dtype,
+                      void* stream) {
+    if (M > 0 && (!xq || !s_x || !y)) return fail(PN_ERR_ARG, "pn_dequant_act_i8: null pointer");
+    if (y_dtype != PN_F32 && y_dtype != PN_BF16) return fail(PN_ERR_DTYPE, "pn_dequant_act_i8: dtype %d", y_dtype);
+    if (M < 0 || K < 1 || xq_pitch < K || xq_pitch % 16 != 0 || K > 0x7fffffff || (double)M * (K / 16 + 1) > 5e11)
+        return fail(PN_ERR_SHAPE, "pn_dequant_act_i8: M=%lld K=%lld pitch=%lld (pitch must be >= K, multiple of 16)",
+                    (long long)M, (long long)K, (long long)xq_pitch);
+    if (!aligned(xq, 16) || !aligned(s_x, 4) || !aligned(y, y_dtype == PN_F32 ? 4 : 2))
+        return fail(PN_ERR_ALIGN, "pn_dequant_act_i8: misaligned pointer");
+    if (int st = check_device()) return st;
+    const cudaError_t e = pn::launch_dequant_act_i8(xq, xq_pitch, s_x, M, K, y, y_dtype, (cudaStream_t)stream);
+    return e == cudaSuccess ? ok() : cuda_fail(e, "pn_dequant_act_i8");
+}
+
 }  // extern "C"

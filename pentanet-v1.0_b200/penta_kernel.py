@@ -491,6 +491,23 @@ def quantize_activations_i8(x: torch.Tensor):
     return xq, s_x, rowsum
 
 
+def dequantize_activations_i8(xq: torch.Tensor, s_x: torch.Tensor, K: int, out_dtype: torch.dtype = torch.bfloat16
+                              ) -> torch.Tensor:
+    """The (M, K) values that quantised activations stand for, xq[:, :K] * s_x per
+    row: xq and s_x as quantize_activations_i8 or rms_norm_i8 return them.  Not in
+    the reference."""
+    assert xq.is_cuda and xq.dtype == torch.int8 and xq.dim() == 2 and xq.is_contiguous()
+    M, pitch = xq.shape
+    assert 0 < K <= pitch and pitch % 16 == 0, f"K={K} does not fit rows of {pitch} codes"
+    assert s_x.dtype == torch.float32 and s_x.shape == (M,) and s_x.is_contiguous() and s_x.get_device() == xq.get_device()
+    assert out_dtype in _FLOATS
+    y = torch.empty(M, K, dtype=out_dtype, device=xq.device)
+    with _nat.device_of(xq):
+        _nat.check(_nat.load().pn_dequant_act_i8(xq.data_ptr(), pitch, s_x.data_ptr(), M, K, y.data_ptr(),
+                                                 _FLOATS[out_dtype], _nat.stream_of(xq)), "dequantize_activations_i8")
+    return y
+
+
 def penta_linear_i8_prequant(xq: torch.Tensor, s_x: torch.Tensor, rowsum: torch.Tensor, K_orig: int,
                              packed_w: torch.Tensor, scale: float, bias: torch.Tensor | None = None,
                              out_dtype: torch.dtype | None = torch.bfloat16, return_acc: bool = False,

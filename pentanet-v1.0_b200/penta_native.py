@@ -33,7 +33,7 @@ EXPORTS = (
     "pn_linear_bf16_peers", "pn_peer_barrier", "pn_peer_barrier_wait", "pn_set_gemv_max_tokens",
     "pn_set_limb_max_tokens", "pn_matmul_i8w",
     "pn_words_2bit", "pn_quantize_pack_2bit", "pn_unpack_2bit", "pn_linear_bf16_2bit",
-    "pn_rms_norm", "pn_rms_norm_i8", "pn_kv4_block_bytes", "pn_kv4_append", "pn_kv4_gather",
+    "pn_rms_norm", "pn_rms_norm_i8", "pn_dequant_act_i8", "pn_kv4_block_bytes", "pn_kv4_append", "pn_kv4_gather",
     "pn_kv4_attention_workspace_size", "pn_kv4_attention", "pn_sample_tokens",
 )
 
@@ -99,6 +99,7 @@ def load() -> ctypes.CDLL:
         "pn_linear_bf16_2bit": (I, [P, I64, I64, P, I64, I64, F, P, P, I, P]),
         "pn_rms_norm": (I, [P, I, P, I64, I64, P, I, D, P, P, I, P]),
         "pn_rms_norm_i8": (I, [P, I, P, I64, I64, P, I, D, P, P, I64, P, P, P]),
+        "pn_dequant_act_i8": (I, [P, I64, P, I64, I64, P, I, P]),
         "pn_kv4_block_bytes": (I64, [I64, I64]),
         "pn_kv4_append": (I, [P, I64, I64, I64, P, I64, I64, I64, I, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64,
                               P]),

@@ -175,3 +175,16 @@ def test_side_stream_and_graph(cuda_device):
     r.copy_(r.flip(0))
     graph.replay()
     assert all(torch.equal(a, b.flip(0)) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("M,C", [(0, 8), (1, 1), (3, 31), (5, 32), (2, 768), (17, 1001), (301, 1000), (4, 8200)])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_dequantize(cuda_device, M, C, out_dtype):
+    """The values that codes stand for: one fp32 product, and one rounding where bf16 is asked for."""
+    x, _, _ = _inputs(M, C, torch.bfloat16, C, cuda_device)
+    xq, s, _ = pk.rms_norm_i8(x, None, 1e-6)
+    if M > 2:
+        s[1] = float("nan")
+    want = (xq[:, :C].float() * s[:, None]).to(out_dtype)
+    got = pk.dequantize_activations_i8(xq, s, C, out_dtype)
+    assert got.dtype == out_dtype and torch.equal(torch.nan_to_num(got, nan=123.0), torch.nan_to_num(want, nan=123.0))

@@ -47,6 +47,14 @@ def test_rms_output_refusals():
     assert rms_i8(q=P + 8) == nat.PN_ERR_ALIGN and rms_i8(s=P + 2) == nat.PN_ERR_ALIGN
 
 
+def test_dequantize_refusals():
+    call = lambda q=P, pitch=64, s=P, M=4, K=60, y=P, dt=nat.PN_BF16: nat.load().pn_dequant_act_i8(q, pitch, s, M, K, y, dt, None)
+    assert call(q=None) == call(s=None) == call(y=None) == nat.PN_ERR_ARG
+    assert call(dt=nat.PN_I8) == nat.PN_ERR_DTYPE
+    assert call(K=0) == call(K=65) == call(pitch=72) == call(M=-1) == nat.PN_ERR_SHAPE
+    assert call(q=P + 8) == call(s=P + 2) == call(y=P + 1) == nat.PN_ERR_ALIGN
+
+
 BASE = dict(cache=P, n_pages=8, hk=2, page=64, d=64, table=P, ld=4, w=4, lens=P, cu=None, B=2, T=2)
 
 
