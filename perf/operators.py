@@ -267,9 +267,7 @@ def _norm(s):
         pk = _kernel()
         if s["out"] == "i8":
             q, scale, total, *h = pk.rms_norm_i8(s["x"], s["w"], s["eps"], residual=s["r"])
-            x = s["x"]
-            y = torch.mul(q[:, :x.shape[1]], scale[:, None], out=torch.empty(x.shape, dtype=torch.bfloat16, device=x.device))
-            return {"y": y, "scale": scale, "total": total, "h": h}
+            return {"y": pk.dequantize_activations_i8(q, scale, s["width"]), "scale": scale, "total": total, "h": h}
         if s["r"] is None:
             return {"y": pk.rms_norm(s["x"], s["w"], s["eps"]), "h": []}
         y, h = pk.rms_norm(s["x"], s["w"], s["eps"], residual=s["r"])
