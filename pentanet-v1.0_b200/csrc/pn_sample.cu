@@ -398,7 +398,8 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
     const int chunks = (a.V + shift + K::N - 1) / K::N;
     const int chunk0 = (rank * kSmpWarps + warp) * a.steps * 32 + lane;  // index order: block, warp, step, lane
     uint4* mine = raw + warp * a.steps * 32 + lane;
-    const float temp = a.t ? __ldg(a.t + row) : a.t0, top_p = a.p ? __ldg(a.p + row) : a.p0,
+    const float t_in = a.t ? __ldg(a.t + row) : a.t0, temp = t_in > 1e30f ? 1e30f : t_in,  // (all finite logits weigh the same)
+                top_p = a.p ? __ldg(a.p + row) : a.p0,
                 min_p = a.m ? __ldg(a.m + row) : a.m0;
     int k = a.k ? __ldg(a.k + row) : a.k0;
     const double ud = fmin(fmax((double)__ldg(a.u + row), 0.0), 1.0);
@@ -488,6 +489,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
         }
     };
     auto push = [&](float v) {
+        if (*const_cast<volatile uint32_t*>(&s.n) > kSmpList) return;  // too many: how many does not matter
         const uint32_t at = atomicAdd(&s.n, 1);
         if (at < kSmpList) s.list[at] = v;
     };

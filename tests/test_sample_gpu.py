@@ -119,6 +119,21 @@ def test_ends_of_the_unit_interval(cuda_device):
     check(x, u, top_p=0.8)
 
 
+def test_extreme_temperatures(cuda_device):
+    """Near zero the largest logit, at infinity every finite one alike, NaN as zero."""
+    x, u = inputs(5, 3000, torch.float32, 11, cuda_device)
+    x[1, ::3] = -float("inf")
+    x[2] = x[2].round()
+    for t in (1e-30, 1e-9, 1e-3, 1e6, 1e29, 1e30):
+        check(x, u, temperature=t)
+        check(x, u, temperature=t, top_p=0.5)
+        check(x, u, temperature=t, top_k=17, top_p=0.9)
+    hot = pk.sample_tokens(x, u, temperature=float("inf"))
+    assert hot.tolist() == pk.sample_tokens(x, u, temperature=1e30).tolist()
+    nan = torch.full((5,), float("nan"), device=cuda_device)
+    assert pk.sample_tokens(x, u, temperature=nan).tolist() == x.argmax(-1).tolist()
+
+
 def test_strided_logits_and_the_models_shape(cuda_device):
     wide, u = inputs(6, 2100, torch.bfloat16, 8, cuda_device)
     for x in (wide[:, 3:2050], wide[::2], wide[:, ::2], wide.t()[:6, :6]):
