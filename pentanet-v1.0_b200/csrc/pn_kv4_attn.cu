@@ -121,9 +121,10 @@ __device__ __forceinline__ uint32_t attn_begin(uint32_t total, uint32_t blocks, 
 }
 template <typename C>
 __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
-    __shared__ uint32_t sums[kAttnWarps], start[2];
+    constexpr int kWarps = C::kThreads / 32;
+    __shared__ uint32_t sums[kWarps], start[2];
     // thread t takes sequences [t * per, (t + 1) * per)
-    const uint32_t B = (uint32_t)a.s.B, per = (B + kAttnThreads - 1) / kAttnThreads;
+    const uint32_t B = (uint32_t)a.s.B, per = (B + C::kThreads - 1) / C::kThreads;
     const uint32_t b0 = min(threadIdx.x * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0, nt;
     for (uint32_t b = b0; b < b1; ++b) sum += attn_units<C>(a, b, nt);
@@ -140,7 +141,7 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
     AttnRun run;
     run.total = 0;
 #pragma unroll
-    for (int i = 0; i < kAttnWarps; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
         if (i < w) at += sums[i];
         run.total += sums[i];
     }
@@ -244,9 +245,31 @@ __device__ __forceinline__ void store_out(const Kv4AttnArgs& a, int64_t at, cons
     }
 }
 
-// A row's query operands: scaled to the power of two that brings the row's
-// largest magnitude to [2^14, 2^15), dims base + {0,4}, {1,5} / 16, {2,6}, {3,7} / 16
-// of each word of eight dims that this thread holds (words t * W ..).
+// The exponent of a query row's scaling, which brings its largest magnitude to
+// [2^14, 2^15), kept where 2^e and 2^(24 - e) are normal numbers.
+__device__ __forceinline__ int query_exponent(float amax) {
+    const int e = 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
+    return amax > 0.0f ? min(max(e, -100), 126) : 0;
+}
+// Eight dims (a word of codes) as the operands that meet the masked codes: dims
+// {0,4}, {1,5} / 16, {2,6}, {3,7} / 16, times `up`.  Returns the sum of the rounded eight.
+__device__ __forceinline__ float pack_query(const float* v, float up, uint32_t (&p)[4]) {
+    float u[8], sum = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = v[j] * up;
+    p[0] = pack_f16(u[0], u[4]);
+    p[1] = pack_f16(u[1] * 0.0625f, u[5] * 0.0625f);
+    p[2] = pack_f16(u[2], u[6]);
+    p[3] = pack_f16(u[3] * 0.0625f, u[7] * 0.0625f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[k]));
+        sum += (f.x + f.y) * (k & 1 ? 16.0f : 1.0f);
+    }
+    return sum;
+}
+
+// A row's query operands for the words t * W .. that this thread holds.
 template <int D>
 __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row, int t, uint32_t (&qb)[D / 8], float& ca,
                                            float& cb) {
@@ -271,24 +294,15 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
     for (int j = 0; j < W * 8; ++j) amax = max_nan(amax, fabsf(v[j]));
     amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // exponent of the scaling, kept where 2^e and 2^(24 - e) are normal numbers
-    int e = 14 - ((int)(__float_as_uint(amax) >> 23) - 127);
-    e = amax > 0.0f ? min(max(e, -100), 126) : 0;
+    const int e = query_exponent(amax);
     const float up = pow2i(e);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-        float u[8];
+        uint32_t p[4];
+        sum += pack_query(v + i * 8, up, p);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = v[i * 8 + j] * up;
-        const uint32_t p[4] = {pack_f16(u[0], u[4]), pack_f16(u[1] * 0.0625f, u[5] * 0.0625f), pack_f16(u[2], u[6]),
-                               pack_f16(u[3] * 0.0625f, u[7] * 0.0625f)};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            qb[i * 4 + k] = p[k];
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p[k]));
-            sum += (f.x + f.y) * (k & 1 ? 16.0f : 1.0f);
-        }
+        for (int k = 0; k < 4; ++k) qb[i * 4 + k] = p[k];
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -296,11 +310,17 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
     cb = a.scale_log2 * (sum * pow2i(-e));
 }
 
+// Shared-memory operand in 128-byte swizzled boxes (K-major), from its address.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
+    return (uint64_t)kDescHiSW128 << 32 | 1u << 16 | (addr >> 4 & 0x3FFFu);
+}
+
 template <int D, int NT>
 struct AttnCfg {
     static constexpr int W = D / 32;             // words per thread and token
     static constexpr int kRows = 8 * NT;         // query rows of a row tile
     static constexpr int kTokens = 128;          // tokens of a unit: 32 per warp
+    static constexpr int kThreads = kAttnThreads;
     static constexpr int kStages = 6;
     static constexpr int kCodes = 16 * (D / 2);  // bytes of one 16-token piece of keys or values
     static constexpr int kStage = 2 * kCodes + 128;
@@ -663,7 +683,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 template <int D>
 struct ChunkCfg {
     static constexpr int W = D / 32;
-    static constexpr int kRows = 64, kTokens = 64;
+    static constexpr int kRows = 64, kTokens = 64, kThreads = kAttnThreads;
     static constexpr int kStages = 3;
     static constexpr int kCodes = 16 * (D / 2);
     static constexpr int kPiece = 2 * kCodes + 128;  // 16 tokens, as in AttnCfg
@@ -935,6 +955,445 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
     }
 }
 
+// Long prompts: 128 query rows per block on tcgen05.  The block's 16 warps spread a
+// tile of 128 tokens' codes into fp16 operands in shared memory (128-byte
+// swizzle; a code is still only masked), one thread has the tensor core form
+// logits = Q K^T and output += P V with the row operands (Q, P) and both results
+// in tensor memory, and the warps do the softmax between the two: thread
+// (row, quarter) takes 32 tokens of a row.
+//
+// In step i the keys of tile i + 1 are spread while P V of tile i - 1 still runs,
+// and its logits are formed while the softmax of tile i runs; buffers of keys,
+// values, logits and pairs come in twos for that.
+//
+// What bounds it: the softmax's and the spreading's instructions (about 330 per
+// thread and tile); the products take 1024 cycles per tile at the tensor core's
+// rate, hidden behind them.
+template <int D>
+struct TcCfg {
+    static constexpr int kRows = 128, kTokens = 128, kThreads = 512;
+    static constexpr int kStages = 3;
+    static constexpr int kRawK = 128 * (D / 2);          // codes of a tile's keys (or values)
+    static constexpr int kRaw = 2 * kRawK + 1024;        // and the pairs: keys' 512 bytes, values' 512 bytes
+    static constexpr int kOp = 128 * D * 2;              // one spread operand: rows of 128 bytes in boxes of 64 columns
+    static constexpr int kPairs = 4 * 128 * 4;           // key scales, key zeros, value scales, value zeros as fp32
+    static constexpr int kSmem = 4 * kOp + kStages * kRaw + 2 * kPairs + 1024;  // (+ alignment)
+    static constexpr int kPart = kRows * (D + 2);
+    static constexpr int kBlocks = 1;  // per SM
+    // tensor memory columns
+    static constexpr uint32_t kS = 0, kP = 256, kO = 320, kQ = 448;
+    // instruction descriptors, f16 x f16 -> f32, 128 rows: 128 tokens (logits), D dims (output)
+    static constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    static constexpr uint32_t kIdescO = (1u << 4) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+};
+
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+template <int D>
+__global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
+    using C = TcCfg<D>;
+    constexpr int ST = C::kStages;
+    constexpr int kCols = D / 8;   // columns of Q per quarter
+    constexpr int kDims = D / 4;   // dims of a row per quarter
+    extern __shared__ uint8_t smem_base[];
+    __shared__ uint64_t bar_s[2], bar_o;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    __shared__ uint8_t dead[ST][8];
+    __shared__ uint32_t v_top[2];       // largest value scale of a tile (bits)
+    __shared__ uint32_t gone[2];        // which pieces of a tile are not there
+    __shared__ float ex[2][4][128];     // exchange between a row's four threads
+    uint8_t* smem = smem_base + (1024 - smem_u32(smem_base) % 1024) % 1024;
+    uint8_t* kop = smem;                 // two of keys, then two of values
+    uint8_t* vop = smem + 2 * C::kOp;
+    uint8_t* raw = smem + 4 * C::kOp;
+    float* pairs = reinterpret_cast<float*>(raw + ST * C::kRaw);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int quad = warp & 3, tq = warp >> 2;  // tensor-memory lanes 32 quad ..; quarter of the tile's tokens
+    const int row = quad * 32 + lane;
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (warp == 0) tmem_alloc(&s_tmem, 512);
+    if (tid == 0) {
+        mbar_init(&bar_s[0], 1);
+        mbar_init(&bar_s[1], 1);
+        mbar_init(&bar_o, 1);
+        fence_barrier_init();
+        s_abort = 0;
+        v_top[0] = v_top[1] = 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tm = s_tmem;
+    const uint32_t tl = tm + ((uint32_t)(quad * 32) << 16);  // this warp's lanes
+    volatile int* abort = &s_abort;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const AttnRun run = attn_plan<C>(a);
+    if (tid == 0) a.notes[blockIdx.x].rows = 0;
+    const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
+    uint32_t n_s[2] = {0, 0}, n_o = 0;  // completed phases awaited so far
+
+    uint32_t seq = run.seq, in_seq = run.in_seq;
+    for (uint32_t unit = run.begin; unit < run.end;) {
+        const AttnSeg sg(a, C{}, seq, in_seq, run.end - unit);
+        const int used = min((int)sg.t1, (sg.kv_end + C::kTokens - 1) / C::kTokens);
+        const int count = used - (int)sg.t0;
+        const int tok_base = (int)sg.t0 * C::kTokens;
+
+        // ---- copies: warps 0-7 a piece's keys, warps 8-15 a piece's values
+        const int piece = warp & 7;
+        AttnPages pages;
+        auto issue = [&](int i) {
+            if ((i & 31) == 0) {
+                const int tok = tok_base + (i + lane) * C::kTokens + piece * 16;
+                pages.look_up(a, sg.b, sg.head, block, tok, i + lane < count && tok < sg.kv_end);
+            }
+            const uint64_t addr = __shfl_sync(0xffffffffu, pages.addr, i & 31);
+            const uint32_t off = __shfl_sync(0xffffffffu, pages.off, i & 31);
+            const int stage = i % ST;
+            if (warp < 8 && lane == 0) dead[stage][piece] = addr == 0;
+            if (addr) {
+                const uint8_t* from = reinterpret_cast<const uint8_t*>(addr) + (warp < 8 ? 0 : block);
+                const uint32_t to = smem_u32(raw + stage * C::kRaw) + (warp < 8 ? 0 : C::kRawK);
+#pragma unroll
+                for (int c = lane; c < D / 2; c += 32)  // 16 tokens of D / 2 bytes
+                    cp_async16(to + piece * 8 * D + c * 16, from + off * (D / 2) + c * 16);
+                if (lane < 4)
+                    cp_async16(smem_u32(raw + stage * C::kRaw) + 2 * C::kRawK + (warp < 8 ? 0 : 512) + piece * 64 + lane * 16,
+                               from + (uint32_t)a.s.page * (D / 2) + off * 4 + lane * 16);
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < ST; ++i) issue(i);
+
+        // ---- the row's query, scaled to fp16, into tensor memory
+        float ca, cb;
+        {
+            float v[kDims];
+            if (row < sg.rows) {
+                const char* q = static_cast<const char*>(a.q) + (sg.query(a, row) + tq * kDims) * (a.q_f32 ? 4 : 2);
+#pragma unroll
+                for (int i = 0; i < kDims / 8; ++i) {
+                    float u[8];
+                    if (a.q_f32)
+                        kv4_load8(reinterpret_cast<const float*>(q) + i * 8, a.q_vec, u);
+                    else
+                        kv4_load8(reinterpret_cast<const __nv_bfloat16*>(q) + i * 8, a.q_vec, u);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i * 8 + j] = u[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < kDims; ++j) v[j] = 0.0f;
+            }
+            float amax = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kDims; ++j) amax = max_nan(amax, fabsf(v[j]));
+            ex[0][tq][row] = amax;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax = max_nan(amax, ex[0][i][row]);
+            const int e = query_exponent(amax);
+            const float up = pow2i(e);
+            float sum = 0.0f;
+            uint32_t qp[kCols];
+#pragma unroll
+            for (int i = 0; i < kDims / 8; ++i) {
+                uint32_t p[4];
+                sum += pack_query(v + i * 8, up, p);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) qp[i * 4 + k] = p[k];
+            }
+            ex[1][tq][row] = sum;
+            if constexpr (kCols == 16)
+                tmem_st16(tl + C::kQ + tq * kCols, qp);
+            else
+                tmem_st8(tl + C::kQ + tq * kCols, qp);
+            tmem_wait_st();
+            __syncthreads();
+            sum = ex[1][0][row] + ex[1][1][row] + ex[1][2][row] + ex[1][3][row];
+            ca = a.scale_log2 * pow2i(24 - e);
+            cb = a.scale_log2 * (sum * pow2i(-e));
+        }
+        const int lim = row < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + row) / a.G) : sg.kv_end - 1;
+
+        // ---- spreading of a tile's codes
+        auto spread_keys = [&](int i) {
+            const uint8_t* st = raw + (i % ST) * C::kRaw;
+            uint8_t* op = kop + (i & 1) * C::kOp;
+            constexpr int kQuads = D / 32;  // groups of four words (32 dims) per token
+            if (tid < 128 * kQuads) {
+                const int tok = tid / kQuads, qr = tid % kQuads;
+                uint4 u = *reinterpret_cast<const uint4*>(st + tok * (D / 2) + qr * 16);
+                // lanes of one store phase: two tokens, all quads; the upper two write their words in
+                // the order 2, 3, 0, 1, so that all eight meet different banks
+                const bool swap = qr & 2;
+                if (swap) u = make_uint4(u.z, u.w, u.x, u.y);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int j = qr * 4 + (swap ? k ^ 2 : k);  // the word: eight dims, one 16-byte chunk
+                    const uint32_t x = w[k], y = x >> 8;
+                    *reinterpret_cast<uint4*>(op + (j >> 3) * 16384 + tok * 128 + (((j & 7) ^ (tok & 7)) * 16)) =
+                        make_uint4(x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
+                }
+            }
+            if (tid == 256) {
+                uint32_t m = 0;
+                for (int k = 0; k < 8; ++k) m |= (uint32_t)dead[i % ST][k] << k;
+                gone[i & 1] = m;
+            }
+            // the pairs as fp32: 128 threads the keys', 128 the values'
+            if (tid < 256) {
+                const int tok = tid & 127, kv = tid >> 7;
+                const uint32_t p = *reinterpret_cast<const uint32_t*>(st + 2 * C::kRawK + kv * 512 + tok * 4);
+                float* to = pairs + (i & 1) * 512 + kv * 256 + tok;
+                const bool none = dead[i % ST][tok >> 4] || tok_base + i * C::kTokens + tok >= sg.kv_end;
+                to[0] = none ? 0.0f : pair_lo(p);  // whatever lies behind the sequence
+                to[128] = none ? 0.0f : pair_hi(p);
+                if (kv) {
+                    const float top = none ? 0.0f : fmaxf(pair_lo(p), 0.0f);  // (a NaN does not count)
+                    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                    if (lane == 0) atomicMax(&v_top[i & 1], bits);
+                }
+            }
+        };
+        auto spread_values = [&](int i) {
+            const uint8_t* st = raw + (i % ST) * C::kRaw + C::kRawK;
+            uint8_t* op = vop + (i & 1) * C::kOp;
+            constexpr int kWords = D / 4;  // words (four dims) of a token pair
+            if (tid < 16 * kWords) {
+                const int j = tid % kWords, q = tid / kWords;  // dims 4 j .. 4 j + 3, tokens 8 q .. 8 q + 7
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w[k] = *reinterpret_cast<const uint32_t*>(st + (4 * q + k) * D + j * 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int n = (k + (j >> 1)) & 3;  // the dim in turn, so that eight lanes meet different banks
+                    const uint32_t sh = (n & 2) * 4, mask = n & 1 ? 0x00F000F0u : 0x000F000Fu;
+                    const int r = 4 * j + n;
+                    *reinterpret_cast<uint4*>(op + (q >> 3) * (D * 128) + r * 128 + (((q & 7) ^ (r & 7)) * 16)) =
+                        make_uint4(w[0] >> sh & mask, w[1] >> sh & mask, w[2] >> sh & mask, w[3] >> sh & mask);
+                }
+            }
+        };
+        auto logits = [&](int i) {  // warp 0: S[i & 1] = Q K^T
+            const uint32_t op = smem_u32(kop + (i & 1) * C::kOp);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+                mma_f16_ts_warp(tm + C::kS + (i & 1) * 128, tm + C::kQ + k * 8, desc_sw128(op + (k >> 2) * 16384 + (k & 3) * 32),
+                                C::kIdescS, k > 0);
+            tc_commit_warp(&bar_s[i & 1]);
+        };
+
+        float neg_m = INFINITY, l = 0.0f, zs = 0.0f;  // minus the row's running maximum; sums over this thread's tokens
+        float S = 0.0f, inv_S = 0.0f;
+        float2 l2 = make_float2(0.0f, 0.0f), z2 = make_float2(0.0f, 0.0f);
+        if (count > 0) {
+            cp_wait<ST - 1>();
+            __syncthreads();  // tile 0 is there for all
+            spread_keys(0);
+            spread_values(0);
+            proxy_fence();
+            tc_fence_before();
+            __syncthreads();
+            tc_fence_after();
+            if (warp == 0) logits(0);
+        }
+        for (int i = 0; i < count; ++i) {
+            const int b = i & 1;
+            // ---- tile i + 1: keys now, values once the output of tile i - 1 is formed
+            cp_wait<ST - 2>();
+            __syncthreads();  // tile i + 1 is there; all are done with tile i's raw stage
+            issue(i + ST);
+            const bool next = i + 1 < count;
+            if (next) spread_keys(i + 1);
+            if (i > 0) {
+                mbar_wait(&bar_o, n_o & 1, abort);
+                ++n_o;
+                tc_fence_after();
+            }
+            if (next) {
+                spread_values(i + 1);
+                proxy_fence();
+                __syncthreads();
+                if (warp == 0) {
+                    tc_fence_after();
+                    logits(i + 1);
+                }
+            }
+
+            // ---- softmax of tile i
+            mbar_wait(&bar_s[b], n_s[b] & 1, abort);
+            ++n_s[b];
+            __syncwarp();
+            tc_fence_after();
+            float2 x[16];
+            {
+                uint32_t u[16];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    tmem_ld16(tl + C::kS + b * 128 + tq * 32 + h * 16, u);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[h * 8 + k] = make_float2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
+                }
+            }
+            const float* pk = pairs + b * 512 + tq * 32;
+            const int tok = tok_base + i * C::kTokens + tq * 32;
+            const bool d0 = gone[b] >> (tq * 2) & 1u, d1 = gone[b] >> (tq * 2 + 1) & 1u;
+            float top = -INFINITY;
+            const float2 ca2 = make_float2(ca, ca), cb2 = make_float2(cb, cb);
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+                const float4 ks = *reinterpret_cast<const float4*>(pk + 2 * k), kz = *reinterpret_cast<const float4*>(pk + 128 + 2 * k);
+                x[k] = fma2(mul2(make_float2(ks.x, ks.y), ca2), x[k], mul2(make_float2(kz.x, kz.y), cb2));
+                x[k + 1] = fma2(mul2(make_float2(ks.z, ks.w), ca2), x[k + 1], mul2(make_float2(kz.z, kz.w), cb2));
+            }
+            const bool mask = d0 || d1 || tok + 31 > sg.lim_min;  // the warp's threads agree
+            if (mask) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const bool none = k < 8 ? d0 : d1;
+                    if (none || tok + 2 * k > lim) x[k].x = -INFINITY;
+                    if (none || tok + 2 * k + 1 > lim) x[k].y = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
+            const float vt = __uint_as_float(v_top[b]);
+            if (__syncthreads_or(top + neg_m > 8.0f || vt > S)) {  // seldom: see the decode kernel
+                ex[0][tq][row] = top;
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) top = fmaxf(top, ex[0][k][row]);
+                float fs = 1.0f;
+                if (vt > S) {
+                    const int e = min(max((int)(__float_as_uint(vt) >> 23) - 126, -100), 102);
+                    const float was = S;
+                    S = pow2i(e);
+                    inv_S = pow2i(-e);
+                    fs = was * inv_S;
+                }
+                const float now = fminf(neg_m, -top), f = now == neg_m ? 1.0f : ex2f(now - neg_m);
+                neg_m = now;
+                l2 = mul2(l2, make_float2(f, f));
+                z2 = mul2(z2, make_float2(f, f));
+                if (i > 0) {  // the output so far (P V of tile i - 1 is done)
+#pragma unroll
+                    for (int h = 0; h < kDims / 16; ++h) {
+                        uint32_t u[16];
+                        tmem_ld16(tl + C::kO + tq * kDims + h * 16, u);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * (f * fs));
+                        tmem_st16(tl + C::kO + tq * kDims + h * 16, u);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            if (tid == 0) v_top[b] = 0;  // all have read it
+            {
+                const float2 m2 = make_float2(neg_m, neg_m), is2 = make_float2(inv_S, inv_S);
+                uint32_t pw[16];
+#pragma unroll
+                for (int k = 0; k < 16; k += 2) {
+                    const float4 vs = *reinterpret_cast<const float4*>(pk + 256 + 2 * k), vz = *reinterpret_cast<const float4*>(pk + 384 + 2 * k);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float2 y = x[k + c], d = add2(y, m2);
+                        float2 p = make_float2(ex2f(d.x), ex2f(d.y));
+                        const float2 s2 = mul2(c ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y), is2);
+                        const float2 zz = c ? make_float2(vz.z, vz.w) : make_float2(vz.x, vz.y);
+                        float2 pv;
+                        if (mask) {  // a token that a row does not see adds nothing, whatever its pair holds
+                            const bool n0 = y.x == -INFINITY, n1 = y.y == -INFINITY;
+                            p = make_float2(n0 ? 0.0f : p.x, n1 ? 0.0f : p.y);
+                            z2 = add2(z2, make_float2(n0 ? 0.0f : p.x * zz.x, n1 ? 0.0f : p.y * zz.y));
+                            pv = make_float2(n0 ? 0.0f : p.x * s2.x, n1 ? 0.0f : p.y * s2.y);
+                        } else {
+                            z2 = fma2(p, zz, z2);
+                            pv = mul2(p, s2);
+                        }
+                        l2 = add2(l2, p);
+                        pw[k + c] = pack_f16(pv.x, pv.y);
+                    }
+                }
+                tmem_st16(tl + C::kP + tq * 16, pw);
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            __syncthreads();
+            if (warp == 0) {  // O += P V
+                tc_fence_after();
+                const uint32_t op = smem_u32(vop + b * C::kOp);
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    mma_f16_ts_warp(tm + C::kO, tm + C::kP + k * 8, desc_sw128(op + (k >> 2) * (D * 128) + (k & 3) * 32), C::kIdescO,
+                                    i > 0 || k > 0);
+                tc_commit_warp(&bar_o);
+            }
+        }
+
+        // ---- results
+        l = l2.x + l2.y, zs = z2.x + z2.y;
+        if (count > 0) {
+            mbar_wait(&bar_o, n_o & 1, abort);
+            ++n_o;
+            __syncwarp();
+            tc_fence_after();
+        }
+        ex[0][tq][row] = l;
+        ex[1][tq][row] = zs;
+        __syncthreads();
+        l = ex[0][0][row] + ex[0][1][row] + ex[0][2][row] + ex[0][3][row];
+        zs = ex[1][0][row] + ex[1][1][row] + ex[1][2][row] + ex[1][3][row];
+        const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
+        float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
+        const float up = S * 16777216.0f, inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        const uint32_t rr = (uint32_t)sg.r0 + row, ri = rr / a.G;
+        const int64_t at = (((sg.row0 + ri) * a.s.Hk + sg.head) * a.G + rr - ri * a.G) * D + tq * kDims;
+#pragma unroll
+        for (int h = 0; h < kDims / 16; ++h) {
+            uint32_t u[16];
+            if (count > 0) {
+                tmem_ld16(tl + C::kO + tq * kDims + h * 16, u);
+                tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) u[k] = 0;
+            }
+            if (row < sg.rows) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    const float4 y = make_float4(fmaf(__uint_as_float(u[k]), up, zs), fmaf(__uint_as_float(u[k + 1]), up * 0.0625f, zs),
+                                                 fmaf(__uint_as_float(u[k + 2]), up, zs), fmaf(__uint_as_float(u[k + 3]), up * 0.0625f, zs));
+                    if (whole)
+                        store_out(a, at + h * 16 + k, y, inv);
+                    else
+                        *reinterpret_cast<float4*>(part + row * D + tq * kDims + h * 16 + k) = y;
+                }
+            }
+        }
+        if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = -neg_m, part[C::kRows * D + row * 2 + 1] = l;
+        if (tid == 0) attn_note(a, run, sg, unit);
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        unit += sg.t1 - sg.t0;
+        in_seq += sg.t1 - sg.t0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        tmem_relinquish();
+        tmem_dealloc(tm, 512);
+    }
+}
+
 // Joins the partial results of a row tile that several blocks share: block c of
 // this grid those of the tile that ends in block c of the other, gridDim.y blocks
 // sharing its rows.  The warps of a block are shared out over its rows; those of
@@ -1011,22 +1470,23 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 }
 
 // The kernel by the query rows that a sequence has on average for one kv head: up
-// to 8 and up to 16 in the decode kernel, more in the chunk kernel.
-enum AttnKind { kAttn8, kAttn16, kAttnChunk };
+// to 8 and up to 16 in the decode kernel, up to 64 in the chunk kernel, more in
+// the one on tcgen05.
+enum AttnKind { kAttn8, kAttn16, kAttnChunk, kAttnLong };
 static AttnKind attn_kind(int64_t B, int64_t T, int64_t G) {
     const int64_t rows = (T + B - 1) / B * G;
-    return rows <= 8 ? kAttn8 : rows <= 16 ? kAttn16 : kAttnChunk;
+    return rows <= 8 ? kAttn8 : rows <= 16 ? kAttn16 : rows <= 64 ? kAttnChunk : kAttnLong;
 }
-static int attn_blocks() {  // blocks that the device holds at once (kBlocks of every configuration)
+static int attn_blocks(AttnKind kind) {  // blocks that the device holds at once
     const int sms = device_sm_count();
-    return (sms > 0 ? sms : 148) * 3;
+    return (sms > 0 ? sms : 148) * (kind == kAttnLong ? TcCfg<128>::kBlocks : AttnCfg<128, 1>::kBlocks);
 }
 static size_t attn_notes_bytes(int blocks) { return ((size_t)blocks * sizeof(Kv4Join) + 255) / 256 * 256; }
 static size_t attn_workspace(int64_t B, int64_t T, int64_t G, int64_t D) {
     if (B == 0 || T == 0) return 0;
-    const int blocks = attn_blocks();
     const AttnKind kind = attn_kind(B, T, G);
-    return attn_notes_bytes(blocks) + (size_t)blocks * 2 * (kind == kAttn8 ? 8 : kind == kAttn16 ? 16 : 64) * (D + 2) * 4;
+    const int blocks = attn_blocks(kind), rows[4] = {8, 16, 64, 128};
+    return attn_notes_bytes(blocks) + (size_t)blocks * 2 * rows[kind] * (D + 2) * 4;
 }
 
 template <int D, typename C>
@@ -1039,13 +1499,13 @@ static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    const int blocks = attn_blocks();
+    const int blocks = attn_blocks(attn_kind(a.s.B, a.s.T, a.G));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3(kAttnThreads);
+    cfg.blockDim = dim3(C::kThreads);
     cfg.dynamicSmemBytes = C::kSmem;
     cfg.stream = s;
     cfg.attrs = attr;
@@ -1107,15 +1567,17 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     a.G = (int)(q_heads / kv_heads);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.out = out;
+    const pn::AttnKind kind = pn::attn_kind(B, T, a.G);
     a.notes = static_cast<pn::Kv4Join*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_notes_bytes(pn::attn_blocks()));
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_notes_bytes(pn::attn_blocks(kind)));
     const cudaStream_t s = (cudaStream_t)stream;
     auto go = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
-        switch (pn::attn_kind(B, T, a.G)) {
+        switch (kind) {
             case pn::kAttn8: return pn::launch_attn<D, pn::AttnCfg<D, 1>>(pn::kv4_decode_kernel<D, 1>, a, s);
             case pn::kAttn16: return pn::launch_attn<D, pn::AttnCfg<D, 2>>(pn::kv4_decode_kernel<D, 2>, a, s);
-            default: return pn::launch_attn<D, pn::ChunkCfg<D>>(pn::kv4_chunk_kernel<D>, a, s);
+            case pn::kAttnChunk: return pn::launch_attn<D, pn::ChunkCfg<D>>(pn::kv4_chunk_kernel<D>, a, s);
+            default: return pn::launch_attn<D, pn::TcCfg<D>>(pn::kv4_long_kernel<D>, a, s);
         }
     };
     const cudaError_t err = head_dim == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
