@@ -955,68 +955,80 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
     }
 }
 
-// Long prompts: 128 query rows per block on tcgen05.  The block's 16 warps spread a
-// tile of 128 tokens' codes into fp16 operands in shared memory (128-byte
-// swizzle; a code is still only masked), one thread has the tensor core form
-// logits = Q K^T and output += P V with the row operands (Q, P) and both results
-// in tensor memory, and the warps do the softmax between the two: thread
-// (row, quarter) takes 32 tokens of a row.
+// Long prompts: 128 query rows per block on tcgen05, two blocks to an SM.  The
+// block's eight warps spread 64 tokens' codes into fp16 operands in shared memory
+// (128-byte swizzle; a code is still only masked), one thread has the tensor core
+// form output += P V of one tile and logits = Q K^T of the next, with both results
+// and P in tensor memory, and the warps do the softmax: thread (row, half) takes 32
+// tokens of a row.
 //
-// In step i the keys of tile i + 1 are spread while P V of tile i - 1 still runs,
-// and its logits are formed while the softmax of tile i runs; buffers of keys,
-// values, logits and pairs come in twos for that.
+// A step waits for the products of the one before, so operands and logits need no
+// second buffer; the other block of the SM fills the wait.  (One block of 16 warps
+// with doubled buffers and 128 tokens per step took 278 us where this takes 231 us:
+// its warps met at five barriers per step with nothing else to run.)
 //
-// What bounds it: the softmax's and the spreading's instructions (about 330 per
-// thread and tile); the products take 1024 cycles per tile at the tensor core's
-// rate, hidden behind them.
+// What bounds it: the softmax's and the spreading's instructions (about 350 per
+// thread and step); the products take 512 cycles per step at the tensor core's
+// rate.
 template <int D>
 struct TcCfg {
-    static constexpr int kRows = 128, kTokens = 128, kThreads = 512;
+    static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
     static constexpr int kStages = 3;
-    static constexpr int kRawK = 128 * (D / 2);          // codes of a tile's keys (or values)
-    static constexpr int kRaw = 2 * kRawK + 1024;        // and the pairs: keys' 512 bytes, values' 512 bytes
-    static constexpr int kOp = 128 * D * 2;              // one spread operand: rows of 128 bytes in boxes of 64 columns
-    static constexpr int kPairs = 4 * 128 * 4;           // key scales, key zeros, value scales, value zeros as fp32
-    static constexpr int kSmem = 4 * kOp + kStages * kRaw + 2 * kPairs + 1024;  // (+ alignment)
+    static constexpr int kRawK = kTokens * (D / 2);      // codes of a tile's keys (or values)
+    static constexpr int kRaw = 2 * kRawK + 8 * kTokens; // and the pairs: the keys', then the values'
+    static constexpr int kQ = kRows * D * 2;             // operands: rows of 128 bytes, in boxes of 64 columns
+    static constexpr int kK = kTokens * D * 2, kV = D * kTokens * 2;
+    static constexpr int kPairs = 4 * kTokens * 4;       // key scales, key zeros, value scales, value zeros as fp32
+    static constexpr int kSmem = kQ + kK + kV + kStages * kRaw + 2 * kPairs + 1024;  // (+ alignment)
     static constexpr int kPart = kRows * (D + 2);
-    static constexpr int kBlocks = 1;  // per SM
-    // tensor memory columns
-    static constexpr uint32_t kS = 0, kP = 256, kO = 320, kQ = 448;
-    // instruction descriptors, f16 x f16 -> f32, 128 rows: 128 tokens (logits), D dims (output)
-    static constexpr uint32_t kIdescS = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+    static constexpr int kBlocks = 2;  // per SM
+    // tensor memory columns: logits, weights, output
+    static constexpr uint32_t kColS = 0, kColP = 64, kColO = 128, kCols = 256;
+    // instruction descriptors, f16 x f16 -> f32, 128 rows: 64 tokens (logits), D dims (output)
+    static constexpr uint32_t kIdescS = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
     static constexpr uint32_t kIdescO = (1u << 4) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
 };
 
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// D[tmem] (+)= A[smem] x B[smem], kind::f16, issued by one lane of a converged warp.
+__device__ __forceinline__ void mma_f16_ss_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 
 template <int D>
-__global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
     using C = TcCfg<D>;
     constexpr int ST = C::kStages;
-    constexpr int kCols = D / 8;   // columns of Q per quarter
-    constexpr int kDims = D / 4;   // dims of a row per quarter
+    constexpr int kDims = D / 2;  // dims of a row per thread
     extern __shared__ uint8_t smem_base[];
-    __shared__ uint64_t bar_s[2], bar_o;
+    __shared__ uint64_t bar;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
-    __shared__ uint8_t dead[ST][8];
+    __shared__ uint8_t dead[ST][4];     // pieces that are not there
     __shared__ uint32_t v_top[2];       // largest value scale of a tile (bits)
-    __shared__ uint32_t gone[2];        // which pieces of a tile are not there
-    __shared__ float ex[2][4][128];     // exchange between a row's four threads
-    uint8_t* smem = smem_base + (1024 - smem_u32(smem_base) % 1024) % 1024;
-    uint8_t* kop = smem;                 // two of keys, then two of values
-    uint8_t* vop = smem + 2 * C::kOp;
-    uint8_t* raw = smem + 4 * C::kOp;
+    __shared__ float ex[2][2][128];     // exchange between a row's two threads
+    uint8_t* qop = smem_base + (1024 - smem_u32(smem_base) % 1024) % 1024;
+    uint8_t* kop = qop + C::kQ;
+    uint8_t* vop = kop + C::kK;
+    uint8_t* raw = vop + C::kV;
     float* pairs = reinterpret_cast<float*>(raw + ST * C::kRaw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int quad = warp & 3, tq = warp >> 2;  // tensor-memory lanes 32 quad ..; quarter of the tile's tokens
+    const int quad = warp & 3, tq = warp >> 2;  // tensor-memory lanes 32 quad ..; half of the tile's tokens
     const int row = quad * 32 + lane;
     asm volatile("griddepcontrol.launch_dependents;");
-    if (warp == 0) tmem_alloc(&s_tmem, 512);
+    if (warp == 0) {
+        tmem_alloc(&s_tmem, C::kCols);
+        tmem_relinquish();  // (the SM's other block allocates too)
+    }
     if (tid == 0) {
-        mbar_init(&bar_s[0], 1);
-        mbar_init(&bar_s[1], 1);
-        mbar_init(&bar_o, 1);
+        mbar_init(&bar, 1);
         fence_barrier_init();
         s_abort = 0;
         v_top[0] = v_top[1] = 0;
@@ -1032,7 +1044,7 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
     const AttnRun run = attn_plan<C>(a);
     if (tid == 0) a.notes[blockIdx.x].rows = 0;
     const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
-    uint32_t n_s[2] = {0, 0}, n_o = 0;  // completed phases awaited so far
+    uint32_t phase = 0;  // of bar
 
     uint32_t seq = run.seq, in_seq = run.in_seq;
     for (uint32_t unit = run.begin; unit < run.end;) {
@@ -1041,34 +1053,34 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
         const int count = used - (int)sg.t0;
         const int tok_base = (int)sg.t0 * C::kTokens;
 
-        // ---- copies: warps 0-7 a piece's keys, warps 8-15 a piece's values
-        const int piece = warp & 7;
+        // ---- copies: warps 0-3 a piece's keys, warps 4-7 a piece's values
+        const int piece = warp & 3;
         AttnPages pages;
-        auto issue = [&](int i) {
+        auto issue = [&](int i, int stage) {
             if ((i & 31) == 0) {
                 const int tok = tok_base + (i + lane) * C::kTokens + piece * 16;
                 pages.look_up(a, sg.b, sg.head, block, tok, i + lane < count && tok < sg.kv_end);
             }
             const uint64_t addr = __shfl_sync(0xffffffffu, pages.addr, i & 31);
             const uint32_t off = __shfl_sync(0xffffffffu, pages.off, i & 31);
-            const int stage = i % ST;
-            if (warp < 8 && lane == 0) dead[stage][piece] = addr == 0;
+            if (warp < 4 && lane == 0) dead[stage][piece] = addr == 0;
             if (addr) {
-                const uint8_t* from = reinterpret_cast<const uint8_t*>(addr) + (warp < 8 ? 0 : block);
-                const uint32_t to = smem_u32(raw + stage * C::kRaw) + (warp < 8 ? 0 : C::kRawK);
+                const uint8_t* from = reinterpret_cast<const uint8_t*>(addr) + (warp < 4 ? 0 : block);
+                const uint32_t to = smem_u32(raw) + stage * C::kRaw;
 #pragma unroll
-                for (int c = lane; c < D / 2; c += 32)  // 16 tokens of D / 2 bytes
-                    cp_async16(to + piece * 8 * D + c * 16, from + off * (D / 2) + c * 16);
+                for (int c = 0; c < D / 64; ++c)  // 16 tokens of D / 2 bytes
+                    cp_async16(to + (warp < 4 ? 0 : C::kRawK) + piece * 8 * D + (lane + 32 * c) * 16,
+                               from + off * (D / 2) + (lane + 32 * c) * 16);
                 if (lane < 4)
-                    cp_async16(smem_u32(raw + stage * C::kRaw) + 2 * C::kRawK + (warp < 8 ? 0 : 512) + piece * 64 + lane * 16,
+                    cp_async16(to + 2 * C::kRawK + (warp < 4 ? 0 : 4 * C::kTokens) + piece * 64 + lane * 16,
                                from + (uint32_t)a.s.page * (D / 2) + off * 4 + lane * 16);
             }
             cp_commit();
         };
-#pragma unroll
-        for (int i = 0; i < ST; ++i) issue(i);
+        issue(0, 0);
+        issue(1, 1);
 
-        // ---- the row's query, scaled to fp16, into tensor memory
+        // ---- the row's query, scaled, as an operand: rows of 128 bytes, 64 dims each
         float ca, cb;
         {
             float v[kDims];
@@ -1093,38 +1105,31 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
             for (int j = 0; j < kDims; ++j) amax = max_nan(amax, fabsf(v[j]));
             ex[0][tq][row] = amax;
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) amax = max_nan(amax, ex[0][i][row]);
+            amax = max_nan(ex[0][0][row], ex[0][1][row]);
             const int e = query_exponent(amax);
             const float up = pow2i(e);
             float sum = 0.0f;
-            uint32_t qp[kCols];
 #pragma unroll
             for (int i = 0; i < kDims / 8; ++i) {
                 uint32_t p[4];
                 sum += pack_query(v + i * 8, up, p);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) qp[i * 4 + k] = p[k];
+                const int j = tq * (kDims / 8) + i;
+                *reinterpret_cast<uint4*>(qop + (j >> 3) * 16384 + row * 128 + (((j & 7) ^ (row & 7)) * 16)) =
+                    make_uint4(p[0], p[1], p[2], p[3]);
             }
             ex[1][tq][row] = sum;
-            if constexpr (kCols == 16)
-                tmem_st16(tl + C::kQ + tq * kCols, qp);
-            else
-                tmem_st8(tl + C::kQ + tq * kCols, qp);
-            tmem_wait_st();
             __syncthreads();
-            sum = ex[1][0][row] + ex[1][1][row] + ex[1][2][row] + ex[1][3][row];
+            sum = ex[1][0][row] + ex[1][1][row];
             ca = a.scale_log2 * pow2i(24 - e);
             cb = a.scale_log2 * (sum * pow2i(-e));
         }
         const int lim = row < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + row) / a.G) : sg.kv_end - 1;
 
         // ---- spreading of a tile's codes
-        auto spread_keys = [&](int i) {
-            const uint8_t* st = raw + (i % ST) * C::kRaw;
-            uint8_t* op = kop + (i & 1) * C::kOp;
+        auto spread_keys = [&](int i, int stage) {
+            const uint8_t* st = raw + stage * C::kRaw;
             constexpr int kQuads = D / 32;  // groups of four words (32 dims) per token
-            if (tid < 128 * kQuads) {
+            if (tid < C::kTokens * kQuads) {
                 const int tok = tid / kQuads, qr = tid % kQuads;
                 uint4 u = *reinterpret_cast<const uint4*>(st + tok * (D / 2) + qr * 16);
                 // lanes of one store phase: two tokens, all quads; the upper two write their words in
@@ -1136,23 +1141,19 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
                 for (int k = 0; k < 4; ++k) {
                     const int j = qr * 4 + (swap ? k ^ 2 : k);  // the word: eight dims, one 16-byte chunk
                     const uint32_t x = w[k], y = x >> 8;
-                    *reinterpret_cast<uint4*>(op + (j >> 3) * 16384 + tok * 128 + (((j & 7) ^ (tok & 7)) * 16)) =
+                    *reinterpret_cast<uint4*>(kop + (j >> 3) * (C::kTokens * 128) + tok * 128 + (((j & 7) ^ (tok & 7)) * 16)) =
                         make_uint4(x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u);
                 }
             }
-            if (tid == 256) {
-                uint32_t m = 0;
-                for (int k = 0; k < 8; ++k) m |= (uint32_t)dead[i % ST][k] << k;
-                gone[i & 1] = m;
-            }
-            // the pairs as fp32: 128 threads the keys', 128 the values'
-            if (tid < 256) {
-                const int tok = tid & 127, kv = tid >> 7;
-                const uint32_t p = *reinterpret_cast<const uint32_t*>(st + 2 * C::kRawK + kv * 512 + tok * 4);
-                float* to = pairs + (i & 1) * 512 + kv * 256 + tok;
-                const bool none = dead[i % ST][tok >> 4] || tok_base + i * C::kTokens + tok >= sg.kv_end;
+            // the pairs as fp32: 64 threads the keys', 64 the values'
+            if (tid < 2 * C::kTokens) {
+                const int tok = tid % C::kTokens, kv = tid / C::kTokens;
+                const uint32_t p = *reinterpret_cast<const uint32_t*>(st + 2 * C::kRawK + kv * 4 * C::kTokens + tok * 4);
+                float* to = pairs + (i & 1) * 4 * C::kTokens + kv * 2 * C::kTokens + tok;
+                const bool none = dead[stage][tok >> 4] || tok_base + i * C::kTokens + tok >= sg.kv_end;
                 to[0] = none ? 0.0f : pair_lo(p);  // whatever lies behind the sequence
-                to[128] = none ? 0.0f : pair_hi(p);
+                // (a dead piece's tokens are told by a zero of +inf: their logits are dropped)
+                to[C::kTokens] = !none ? pair_hi(p) : !kv && dead[stage][tok >> 4] ? INFINITY : 0.0f;
                 if (kv) {
                     const float top = none ? 0.0f : fmaxf(pair_lo(p), 0.0f);  // (a NaN does not count)
                     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
@@ -1160,100 +1161,112 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
                 }
             }
         };
-        auto spread_values = [&](int i) {
-            const uint8_t* st = raw + (i % ST) * C::kRaw + C::kRawK;
-            uint8_t* op = vop + (i & 1) * C::kOp;
+        auto spread_values = [&](int stage) {
+            const uint8_t* st = raw + stage * C::kRaw + C::kRawK;
             constexpr int kWords = D / 4;  // words (four dims) of a token pair
-            if (tid < 16 * kWords) {
+            if (tid < 8 * kWords) {
                 const int j = tid % kWords, q = tid / kWords;  // dims 4 j .. 4 j + 3, tokens 8 q .. 8 q + 7
                 uint32_t w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) w[k] = *reinterpret_cast<const uint32_t*>(st + (4 * q + k) * D + j * 4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int n = (k + (j >> 1)) & 3;  // the dim in turn, so that eight lanes meet different banks
+                    const int n = (k + (j >> 1)) & 3;  // the dims in turn, so that eight lanes meet different banks
                     const uint32_t sh = (n & 2) * 4, mask = n & 1 ? 0x00F000F0u : 0x000F000Fu;
                     const int r = 4 * j + n;
-                    *reinterpret_cast<uint4*>(op + (q >> 3) * (D * 128) + r * 128 + (((q & 7) ^ (r & 7)) * 16)) =
+                    *reinterpret_cast<uint4*>(vop + r * 128 + ((q ^ (r & 7)) * 16)) =
                         make_uint4(w[0] >> sh & mask, w[1] >> sh & mask, w[2] >> sh & mask, w[3] >> sh & mask);
                 }
             }
         };
-        auto logits = [&](int i) {  // warp 0: S[i & 1] = Q K^T
-            const uint32_t op = smem_u32(kop + (i & 1) * C::kOp);
+        auto logits = [&]() {  // warp 0
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-                mma_f16_ts_warp(tm + C::kS + (i & 1) * 128, tm + C::kQ + k * 8, desc_sw128(op + (k >> 2) * 16384 + (k & 3) * 32),
-                                C::kIdescS, k > 0);
-            tc_commit_warp(&bar_s[i & 1]);
+                mma_f16_ss_warp(tm + C::kColS, desc_sw128(smem_u32(qop) + (k >> 2) * 16384 + (k & 3) * 32),
+                                desc_sw128(smem_u32(kop) + (k >> 2) * (C::kTokens * 128) + (k & 3) * 32), C::kIdescS, k > 0);
         };
 
-        float neg_m = INFINITY, l = 0.0f, zs = 0.0f;  // minus the row's running maximum; sums over this thread's tokens
+        float neg_m = INFINITY;  // minus the row's running maximum
         float S = 0.0f, inv_S = 0.0f;
-        float2 l2 = make_float2(0.0f, 0.0f), z2 = make_float2(0.0f, 0.0f);
+        float2 l2 = make_float2(0.0f, 0.0f), z2 = make_float2(0.0f, 0.0f);  // sums over this thread's tokens
+        float2 x[16];
+        // weights of tile i into tensor memory; kMask: some token is not seen by some row
+        auto weights = [&](const float* pk, auto mask) {
+            constexpr bool kMask = decltype(mask)::value;
+            const float2 m2 = make_float2(neg_m, neg_m), is2 = make_float2(inv_S, inv_S);
+            uint32_t pw[16];
+#pragma unroll
+            for (int k = 0; k < 16; k += 2) {
+                const float4 vs = *reinterpret_cast<const float4*>(pk + 2 * C::kTokens + 2 * k),
+                             vz = *reinterpret_cast<const float4*>(pk + 3 * C::kTokens + 2 * k);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float2 y = x[k + c], d = add2(y, m2);
+                    float2 p = make_float2(ex2f(d.x), ex2f(d.y));
+                    const float2 s2 = mul2(c ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y), is2);
+                    const float2 zz = c ? make_float2(vz.z, vz.w) : make_float2(vz.x, vz.y);
+                    float2 pv;
+                    if constexpr (kMask) {  // a token that a row does not see adds nothing, whatever its pair holds
+                        const bool n0 = y.x == -INFINITY, n1 = y.y == -INFINITY;
+                        p = make_float2(n0 ? 0.0f : p.x, n1 ? 0.0f : p.y);
+                        z2 = add2(z2, make_float2(n0 ? 0.0f : p.x * zz.x, n1 ? 0.0f : p.y * zz.y));
+                        pv = make_float2(n0 ? 0.0f : p.x * s2.x, n1 ? 0.0f : p.y * s2.y);
+                    } else {
+                        z2 = fma2(p, zz, z2);
+                        pv = mul2(p, s2);
+                    }
+                    l2 = add2(l2, p);
+                    pw[k + c] = pack_f16(pv.x, pv.y);
+                }
+            }
+            tmem_st16(tl + C::kColP + tq * 16, pw);
+            tmem_wait_st();
+        };
         if (count > 0) {
-            cp_wait<ST - 1>();
+            cp_wait<1>();
             __syncthreads();  // tile 0 is there for all
-            spread_keys(0);
-            spread_values(0);
+            spread_keys(0, 0);
             proxy_fence();
             tc_fence_before();
             __syncthreads();
-            tc_fence_after();
-            if (warp == 0) logits(0);
+            if (warp == 0) {
+                tc_fence_after();
+                logits();
+                tc_commit_warp(&bar);
+            }
         }
+        int stage = 0, ahead = 1, fill = 2;  // of tiles i, i + 1, i + 2
         for (int i = 0; i < count; ++i) {
             const int b = i & 1;
-            // ---- tile i + 1: keys now, values once the output of tile i - 1 is formed
-            cp_wait<ST - 2>();
-            __syncthreads();  // tile i + 1 is there; all are done with tile i's raw stage
-            issue(i + ST);
-            const bool next = i + 1 < count;
-            if (next) spread_keys(i + 1);
-            if (i > 0) {
-                mbar_wait(&bar_o, n_o & 1, abort);
-                ++n_o;
-                tc_fence_after();
-            }
-            if (next) {
-                spread_values(i + 1);
-                proxy_fence();
-                __syncthreads();
-                if (warp == 0) {
-                    tc_fence_after();
-                    logits(i + 1);
-                }
-            }
-
-            // ---- softmax of tile i
-            mbar_wait(&bar_s[b], n_s[b] & 1, abort);
-            ++n_s[b];
+            issue(i + 2, fill);  // (the stage of tile i - 1, done with before the last barrier)
+            // ---- softmax of tile i, once its logits and the output of tile i - 1 are there
+            mbar_wait(&bar, phase & 1, abort);
+            ++phase;
             __syncwarp();
             tc_fence_after();
-            float2 x[16];
             {
-                uint32_t u[16];
+                uint32_t u[2][16];
+                tmem_ld16(tl + C::kColS + tq * 32, u[0]);
+                tmem_ld16(tl + C::kColS + tq * 32 + 16, u[1]);
+                tmem_wait_ld();
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    tmem_ld16(tl + C::kS + b * 128 + tq * 32 + h * 16, u);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) x[h * 8 + k] = make_float2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]));
-                }
+                for (int k = 0; k < 16; ++k)
+                    x[k] = make_float2(__uint_as_float(u[k >> 3][2 * (k & 7)]), __uint_as_float(u[k >> 3][2 * (k & 7) + 1]));
             }
-            const float* pk = pairs + b * 512 + tq * 32;
+            const float* pk = pairs + b * 4 * C::kTokens + tq * 32;
             const int tok = tok_base + i * C::kTokens + tq * 32;
-            const bool d0 = gone[b] >> (tq * 2) & 1u, d1 = gone[b] >> (tq * 2 + 1) & 1u;
             float top = -INFINITY;
             const float2 ca2 = make_float2(ca, ca), cb2 = make_float2(cb, cb);
+            const bool lost = pk[C::kTokens] == INFINITY || pk[C::kTokens + 16] == INFINITY;
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
-                const float4 ks = *reinterpret_cast<const float4*>(pk + 2 * k), kz = *reinterpret_cast<const float4*>(pk + 128 + 2 * k);
+                const float4 ks = *reinterpret_cast<const float4*>(pk + 2 * k), kz = *reinterpret_cast<const float4*>(pk + C::kTokens + 2 * k);
                 x[k] = fma2(mul2(make_float2(ks.x, ks.y), ca2), x[k], mul2(make_float2(kz.x, kz.y), cb2));
                 x[k + 1] = fma2(mul2(make_float2(ks.z, ks.w), ca2), x[k + 1], mul2(make_float2(kz.z, kz.w), cb2));
             }
-            const bool mask = d0 || d1 || tok + 31 > sg.lim_min;  // the warp's threads agree
+            const bool mask = lost || tok + 31 > sg.lim_min;  // the warp's threads agree
             if (mask) {
+                const bool d0 = pk[C::kTokens] == INFINITY, d1 = pk[C::kTokens + 16] == INFINITY;
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     const bool none = k < 8 ? d0 : d1;
@@ -1264,11 +1277,11 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
             const float vt = __uint_as_float(v_top[b]);
+            cp_wait<1>();  // tile i + 1 (visible to all behind the barrier)
             if (__syncthreads_or(top + neg_m > 8.0f || vt > S)) {  // seldom: see the decode kernel
                 ex[0][tq][row] = top;
                 __syncthreads();
-#pragma unroll
-                for (int k = 0; k < 4; ++k) top = fmaxf(top, ex[0][k][row]);
+                top = fmaxf(ex[0][0][row], ex[0][1][row]);
                 float fs = 1.0f;
                 if (vt > S) {
                     const int e = min(max((int)(__float_as_uint(vt) >> 23) - 126, -100), 102);
@@ -1281,75 +1294,53 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
                 neg_m = now;
                 l2 = mul2(l2, make_float2(f, f));
                 z2 = mul2(z2, make_float2(f, f));
-                if (i > 0) {  // the output so far (P V of tile i - 1 is done)
-#pragma unroll
+                if (i > 0) {  // the output so far
+#pragma unroll 1
                     for (int h = 0; h < kDims / 16; ++h) {
                         uint32_t u[16];
-                        tmem_ld16(tl + C::kO + tq * kDims + h * 16, u);
+                        tmem_ld16(tl + C::kColO + tq * kDims + h * 16, u);
                         tmem_wait_ld();
 #pragma unroll
                         for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * (f * fs));
-                        tmem_st16(tl + C::kO + tq * kDims + h * 16, u);
+                        tmem_st16(tl + C::kColO + tq * kDims + h * 16, u);
                     }
                     tmem_wait_st();
                 }
             }
             if (tid == 0) v_top[b] = 0;  // all have read it
-            {
-                const float2 m2 = make_float2(neg_m, neg_m), is2 = make_float2(inv_S, inv_S);
-                uint32_t pw[16];
-#pragma unroll
-                for (int k = 0; k < 16; k += 2) {
-                    const float4 vs = *reinterpret_cast<const float4*>(pk + 256 + 2 * k), vz = *reinterpret_cast<const float4*>(pk + 384 + 2 * k);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const float2 y = x[k + c], d = add2(y, m2);
-                        float2 p = make_float2(ex2f(d.x), ex2f(d.y));
-                        const float2 s2 = mul2(c ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y), is2);
-                        const float2 zz = c ? make_float2(vz.z, vz.w) : make_float2(vz.x, vz.y);
-                        float2 pv;
-                        if (mask) {  // a token that a row does not see adds nothing, whatever its pair holds
-                            const bool n0 = y.x == -INFINITY, n1 = y.y == -INFINITY;
-                            p = make_float2(n0 ? 0.0f : p.x, n1 ? 0.0f : p.y);
-                            z2 = add2(z2, make_float2(n0 ? 0.0f : p.x * zz.x, n1 ? 0.0f : p.y * zz.y));
-                            pv = make_float2(n0 ? 0.0f : p.x * s2.x, n1 ? 0.0f : p.y * s2.y);
-                        } else {
-                            z2 = fma2(p, zz, z2);
-                            pv = mul2(p, s2);
-                        }
-                        l2 = add2(l2, p);
-                        pw[k + c] = pack_f16(pv.x, pv.y);
-                    }
-                }
-                tmem_st16(tl + C::kP + tq * 16, pw);
-                tmem_wait_st();
-            }
+            if (mask)
+                weights(pk, std::true_type{});
+            else
+                weights(pk, std::false_type{});
+            // ---- the operands of the next products
+            spread_values(stage);
+            if (i + 1 < count) spread_keys(i + 1, ahead);
+            proxy_fence();
             tc_fence_before();
             __syncthreads();
-            if (warp == 0) {  // O += P V
+            if (warp == 0) {
                 tc_fence_after();
-                const uint32_t op = smem_u32(vop + b * C::kOp);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    mma_f16_ts_warp(tm + C::kO, tm + C::kP + k * 8, desc_sw128(op + (k >> 2) * (D * 128) + (k & 3) * 32), C::kIdescO,
-                                    i > 0 || k > 0);
-                tc_commit_warp(&bar_o);
+                for (int k = 0; k < C::kTokens / 16; ++k)
+                    mma_f16_ts_warp(tm + C::kColO, tm + C::kColP + k * 8, desc_sw128(smem_u32(vop) + k * 32), C::kIdescO, i > 0 || k > 0);
+                if (i + 1 < count) logits();
+                tc_commit_warp(&bar);
             }
+            const int done = stage;
+            stage = ahead, ahead = fill, fill = done;
         }
 
         // ---- results
-        l = l2.x + l2.y, zs = z2.x + z2.y;
         if (count > 0) {
-            mbar_wait(&bar_o, n_o & 1, abort);
-            ++n_o;
+            mbar_wait(&bar, phase & 1, abort);
+            ++phase;
             __syncwarp();
             tc_fence_after();
         }
-        ex[0][tq][row] = l;
-        ex[1][tq][row] = zs;
+        ex[0][tq][row] = l2.x + l2.y;
+        ex[1][tq][row] = z2.x + z2.y;
         __syncthreads();
-        l = ex[0][0][row] + ex[0][1][row] + ex[0][2][row] + ex[0][3][row];
-        zs = ex[1][0][row] + ex[1][1][row] + ex[1][2][row] + ex[1][3][row];
+        const float l = ex[0][0][row] + ex[0][1][row], zs = ex[1][0][row] + ex[1][1][row];
         const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
         const float up = S * 16777216.0f, inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
@@ -1359,7 +1350,7 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
         for (int h = 0; h < kDims / 16; ++h) {
             uint32_t u[16];
             if (count > 0) {
-                tmem_ld16(tl + C::kO + tq * kDims + h * 16, u);
+                tmem_ld16(tl + C::kColO + tq * kDims + h * 16, u);
                 tmem_wait_ld();
             } else {
 #pragma unroll
@@ -1389,8 +1380,7 @@ __global__ void __launch_bounds__(512, 1) kv4_long_kernel(const Kv4AttnArgs a) {
     __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        tmem_relinquish();
-        tmem_dealloc(tm, 512);
+        tmem_dealloc(tm, C::kCols);
     }
 }
 
