@@ -332,7 +332,7 @@ int pn_kv4_gather(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t 
  * first).  out (T, q_heads, head_dim) of q's type (PN_BF16 or PN_F32),
  * contiguous, 16-byte aligned; zeros for a row that sees nothing; rows behind
  * cu_q[B] are left as they were.  Query head
- * h reads kv head h / (q_heads / kv_heads).  The logits are scale * q . k.
+ * h reads kv head h / (q_heads / kv_heads).  The logits are scale * q . k, scale > 0.
  * Queries enter the products as fp16 relative to the row's largest (bf16 ones
  * exactly), weights as fp16; sums and the softmax are fp32.
  * Workspace: pn_kv4_attention_workspace_size bytes, 256-byte aligned, no

@@ -962,9 +962,15 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
 // and P in tensor memory, and the warps do the softmax: thread (row, half) takes 32
 // tokens of a row.
 //
+// Here a row's logits stay in units of its query's scaling until the exponent (the
+// factor joins the maximum in one fma), and the largest value scale is taken into
+// the maximum: weights and totals are all relative to 2^m S, which cancels in the
+// end.
+//
 // A step waits for the products of the one before, so operands and logits need no
 // second buffer; the other block of the SM fills the wait.  (One block of 16 warps
-// with doubled buffers and 128 tokens per step took 278 us where this takes 231 us:
+// with doubled buffers and 128 tokens per step took 278 us for the ragged
+// chunks where this takes 225 us:
 // its warps met at five barriers per step with nothing else to run.)
 //
 // What bounds it: the softmax's and the spreading's instructions (about 350 per
@@ -1081,7 +1087,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         issue(1, 1);
 
         // ---- the row's query, scaled, as an operand: rows of 128 bytes, 64 dims each
-        float ca, cb;
+        float ca, cb;  // logit = ca * (s_k * S + z_k * cb)
         {
             float v[kDims];
             if (row < sg.rows) {
@@ -1121,7 +1127,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             __syncthreads();
             sum = ex[1][0][row] + ex[1][1][row];
             ca = a.scale_log2 * pow2i(24 - e);
-            cb = a.scale_log2 * (sum * pow2i(-e));
+            cb = sum * 0x1p-24f;
         }
         const int lim = row < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + row) / a.G) : sg.kv_end - 1;
 
@@ -1187,13 +1193,13 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         };
 
         float neg_m = INFINITY;  // minus the row's running maximum
-        float S = 0.0f, inv_S = 0.0f;
+        float S = 0.0f, log_S = 0.0f;  // power of two not below the largest value scale seen
         float2 l2 = make_float2(0.0f, 0.0f), z2 = make_float2(0.0f, 0.0f);  // sums over this thread's tokens
         float2 x[16];
         // weights of tile i into tensor memory; kMask: some token is not seen by some row
         auto weights = [&](const float* pk, auto mask) {
             constexpr bool kMask = decltype(mask)::value;
-            const float2 m2 = make_float2(neg_m, neg_m), is2 = make_float2(inv_S, inv_S);
+            const float2 m2 = make_float2(neg_m - log_S, neg_m - log_S), ca2 = make_float2(ca, ca);
             uint32_t pw[16];
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
@@ -1201,9 +1207,9 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                              vz = *reinterpret_cast<const float4*>(pk + 3 * C::kTokens + 2 * k);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const float2 y = x[k + c], d = add2(y, m2);
+                    const float2 y = x[k + c], d = fma2(y, ca2, m2);
                     float2 p = make_float2(ex2f(d.x), ex2f(d.y));
-                    const float2 s2 = mul2(c ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y), is2);
+                    const float2 s2 = c ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y);
                     const float2 zz = c ? make_float2(vz.z, vz.w) : make_float2(vz.x, vz.y);
                     float2 pv;
                     if constexpr (kMask) {  // a token that a row does not see adds nothing, whatever its pair holds
@@ -1256,13 +1262,13 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             const float* pk = pairs + b * 4 * C::kTokens + tq * 32;
             const int tok = tok_base + i * C::kTokens + tq * 32;
             float top = -INFINITY;
-            const float2 ca2 = make_float2(ca, ca), cb2 = make_float2(cb, cb);
+            const float2 cb2 = make_float2(cb, cb);
             const bool lost = pk[C::kTokens] == INFINITY || pk[C::kTokens + 16] == INFINITY;
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
                 const float4 ks = *reinterpret_cast<const float4*>(pk + 2 * k), kz = *reinterpret_cast<const float4*>(pk + C::kTokens + 2 * k);
-                x[k] = fma2(mul2(make_float2(ks.x, ks.y), ca2), x[k], mul2(make_float2(kz.x, kz.y), cb2));
-                x[k + 1] = fma2(mul2(make_float2(ks.z, ks.w), ca2), x[k + 1], mul2(make_float2(kz.z, kz.w), cb2));
+                x[k] = fma2(make_float2(ks.x, ks.y), x[k], mul2(make_float2(kz.x, kz.y), cb2));
+                x[k + 1] = fma2(make_float2(ks.z, ks.w), x[k + 1], mul2(make_float2(kz.z, kz.w), cb2));
             }
             const bool mask = lost || tok + 31 > sg.lim_min;  // the warp's threads agree
             if (mask) {
@@ -1276,6 +1282,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             }
 #pragma unroll
             for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
+            top *= ca;
             const float vt = __uint_as_float(v_top[b]);
             cp_wait<1>();  // tile i + 1 (visible to all behind the barrier)
             if (__syncthreads_or(top + neg_m > 8.0f || vt > S)) {  // seldom: see the decode kernel
@@ -1284,13 +1291,12 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 top = fmaxf(ex[0][0][row], ex[0][1][row]);
                 float fs = 1.0f;
                 if (vt > S) {
-                    const int e = min(max((int)(__float_as_uint(vt) >> 23) - 126, -100), 102);
-                    const float was = S;
+                    const int e = min(max((int)(__float_as_uint(vt) >> 23) - 126, -100), 100);
+                    fs = ex2f(log_S - (float)e);  // (before the first: weights relative to 1)
                     S = pow2i(e);
-                    inv_S = pow2i(-e);
-                    fs = was * inv_S;
+                    log_S = (float)e;
                 }
-                const float now = fminf(neg_m, -top), f = now == neg_m ? 1.0f : ex2f(now - neg_m);
+                const float now = fminf(neg_m, -top), f = (now == neg_m ? 1.0f : ex2f(now - neg_m)) * fs;
                 neg_m = now;
                 l2 = mul2(l2, make_float2(f, f));
                 z2 = mul2(z2, make_float2(f, f));
@@ -1301,7 +1307,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                         tmem_ld16(tl + C::kColO + tq * kDims + h * 16, u);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * (f * fs));
+                        for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * f);
                         tmem_st16(tl + C::kColO + tq * kDims + h * 16, u);
                     }
                     tmem_wait_st();
@@ -1343,7 +1349,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         const float l = ex[0][0][row] + ex[0][1][row], zs = ex[1][0][row] + ex[1][1][row];
         const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
-        const float up = S * 16777216.0f, inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        const float up = 16777216.0f, inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         const uint32_t rr = (uint32_t)sg.r0 + row, ri = rr / a.G;
         const int64_t at = (((sg.row0 + ri) * a.s.Hk + sg.head) * a.G + rr - ri * a.G) * D + tq * kDims;
 #pragma unroll
@@ -1368,7 +1374,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 }
             }
         }
-        if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = -neg_m, part[C::kRows * D + row * 2 + 1] = l;
+        if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = log_S - neg_m, part[C::kRows * D + row * 2 + 1] = l;
         if (tid == 0) attn_note(a, run, sg, unit);
         tc_fence_before();
         __syncthreads();
@@ -1537,6 +1543,7 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
         return fail(PN_ERR_SHAPE, "pn_kv4_attention: %lld query heads over %lld kv heads", (long long)q_heads,
                     (long long)kv_heads);
     if (T > 0 && B > 0 && (!q || !out)) return fail(PN_ERR_ARG, "pn_kv4_attention: null pointer");
+    if (!(scale > 0.0f && scale < INFINITY)) return fail(PN_ERR_ARG, "pn_kv4_attention: scale must be positive");
     const size_t e = q_dtype == PN_F32 ? 4 : 2;
     if (!aligned(q, e) || !aligned(out, 16)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: misaligned pointer");
     // an upper bound on the units that the kernels count in 31 bits

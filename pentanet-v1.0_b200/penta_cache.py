@@ -148,7 +148,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     shape and type.
 
     Query heads are a multiple of the cache's kv heads; head h reads kv head
-    h // (heads / kv heads).  scale defaults to head_dim ** -0.5.  A row that sees
+    h // (heads / kv heads).  scale > 0 defaults to head_dim ** -0.5.  A row that sees
     nothing gives zeros.  out: a contiguous tensor to write to; rows of it
     behind cu_q[B] are left as they were (zeros where no out is given)."""
     assert q.is_cuda and q.dtype in _FLOATS, "kv4_attention takes bfloat16 or float32 CUDA queries"

@@ -203,6 +203,21 @@ def test_peaked_and_shifted_logits(cuda_device):
         s.attend([rows] * 4, 4, seed=rows)
 
 
+@pytest.mark.parametrize("d,G", [(64, 1), (128, 4), (128, 8)])
+def test_value_scales_from_zero_up(cuda_device, d, G):
+    """Constant values first (their scale is zero), then ever larger ones, and the reverse."""
+    n = 900
+    s = Batch([n, n, n], 2, d, 64, cuda_device, seed=12)
+    grow = torch.logspace(-6, 3, n)[:, None, None]
+    s.v[0] = (s.v[0].float() * grow).to(torch.bfloat16)
+    s.v[0][:300] = 0.75
+    s.v[1] = (s.v[1].float() * grow.flip(0)).to(torch.bfloat16)
+    s.v[2][:] = torch.arange(n)[:, None, None] % 7
+    s.store([n] * 3)
+    for rows in (1, 3, 20, 150):
+        s.attend([rows] * 3, G, seed=rows)
+
+
 def test_tables_wider_than_the_sequences(cuda_device):
     """Entries behind a sequence's end are never looked at."""
     s = Batch([100, 3], 2, 128, 16, cuda_device, width=4096)

@@ -73,11 +73,11 @@ def gather(**kw):
 
 
 def attention(**kw):
-    a = dict(BASE, k=P, v=P, dt=nat.PN_BF16, heads=4, ws=P, size=1 << 30)
+    a = dict(BASE, k=P, v=P, dt=nat.PN_BF16, heads=4, ws=P, size=1 << 30, scale=1.0)
     a.update(kw)
     return nat.load().pn_kv4_attention(a["k"], 1, 1, 1, a["dt"], a["heads"], a["cache"], a["n_pages"], a["hk"], a["page"],
                                        a["d"], a["table"], a["ld"], a["w"], a["lens"], a["cu"], a["B"], a["T"],
-                                       ctypes.c_float(1.0), a["v"], a["ws"], a["size"], None)
+                                       ctypes.c_float(a["scale"]), a["v"], a["ws"], a["size"], None)
 
 
 @pytest.mark.parametrize("call", [append, gather, attention])
@@ -99,6 +99,8 @@ def test_kv4_attention_refusals():
     L = nat.load()
     for heads in (0, 1, 3, 1 << 20):
         assert attention(heads=heads) == nat.PN_ERR_SHAPE
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        assert attention(scale=scale) == nat.PN_ERR_ARG
     assert attention(v=P + 8) == nat.PN_ERR_ALIGN
     need = L.pn_kv4_attention_workspace_size(2, 2, 4, 2, 64)
     assert need > 0 and L.pn_kv4_attention_workspace_size(0, 0, 4, 2, 64) == 0
