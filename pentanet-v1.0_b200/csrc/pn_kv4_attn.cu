@@ -310,11 +310,6 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
     cb = a.scale_log2 * (sum * pow2i(-e));
 }
 
-// Shared-memory operand in 128-byte swizzled boxes (K-major), from its address.
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr) {
-    return (uint64_t)kDescHiSW128 << 32 | 1u << 16 | (addr >> 4 & 0x3FFFu);
-}
-
 template <int D, int NT>
 struct AttnCfg {
     static constexpr int W = D / 32;             // words per thread and token
@@ -996,17 +991,44 @@ struct TcCfg {
 };
 
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// D[tmem] (+)= A[smem] x B[smem], kind::f16, issued by one lane of a converged warp.
-__device__ __forceinline__ void mma_f16_ss_warp(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                                uint32_t accumulate) {
+// Four K-steps over one 64-column box from a converged warp, kind::f16, with one
+// election and 32-bit descriptor arithmetic (an election and a 64-bit descriptor per
+// product took 58 cycles each, on the path of every step): D[tmem] (+)= A B^T, B in
+// shared memory, A in shared memory (ss) or tensor memory (ts).  a, b: low words of
+// the descriptors, or A's column; the steps lie 32 bytes, or 8 columns, apart.
+__device__ __forceinline__ void mma4_ss_warp(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\t.reg .b32 r;\n\t"
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 r, a1, a2, a3, b1, b2, b3;\n\t.reg .b64 x0, x1, x2, x3, y0, y1, y2, y3;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
+        "add.u32 a1, %1, 2;\n\tadd.u32 a2, %1, 4;\n\tadd.u32 a3, %1, 6;\n\t"
+        "add.u32 b1, %2, 2;\n\tadd.u32 b2, %2, 4;\n\tadd.u32 b3, %2, 6;\n\t"
+        "mov.b64 x0, {%1, %5};\n\tmov.b64 x1, {a1, %5};\n\tmov.b64 x2, {a2, %5};\n\tmov.b64 x3, {a3, %5};\n\t"
+        "mov.b64 y0, {%2, %5};\n\tmov.b64 y1, {b1, %5};\n\tmov.b64 y2, {b2, %5};\n\tmov.b64 y3, {b3, %5};\n\t"
         "elect.sync r|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x0, y0, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x1, y1, %3, 1;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x2, y2, %3, 1;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], x3, y3, %3, 1;\n\t}" ::"r"(d_tmem),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHiSW128)
         : "memory");
 }
+__device__ __forceinline__ void mma4_ts_warp(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b32 r, a1, a2, a3, b1, b2, b3;\n\t.reg .b64 y0, y1, y2, y3;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "add.u32 a1, %1, 8;\n\tadd.u32 a2, %1, 16;\n\tadd.u32 a3, %1, 24;\n\t"
+        "add.u32 b1, %2, 2;\n\tadd.u32 b2, %2, 4;\n\tadd.u32 b3, %2, 6;\n\t"
+        "mov.b64 y0, {%2, %5};\n\tmov.b64 y1, {b1, %5};\n\tmov.b64 y2, {b2, %5};\n\tmov.b64 y3, {b3, %5};\n\t"
+        "elect.sync r|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y0, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], y1, %3, 1;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], y2, %3, 1;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], y3, %3, 1;\n\t}" ::"r"(d_tmem),
+        "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHiSW128)
+        : "memory");
+}
+// The low word of a 128-byte swizzled operand's descriptor.
+__device__ __forceinline__ uint32_t desc_lo(const void* p) { return 1u << 16 | (smem_u32(p) >> 4 & 0x3FFFu); }
 
 template <int D>
 __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
@@ -1045,6 +1067,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
     const uint32_t tm = s_tmem;
     const uint32_t tl = tm + ((uint32_t)(quad * 32) << 16);  // this warp's lanes
     volatile int* abort = &s_abort;
+    const uint32_t q_lo = desc_lo(qop), k_lo = desc_lo(kop), v_lo = desc_lo(vop);
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const AttnRun run = attn_plan<C>(a);
@@ -1187,9 +1210,8 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         };
         auto logits = [&]() {  // warp 0
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-                mma_f16_ss_warp(tm + C::kColS, desc_sw128(smem_u32(qop) + (k >> 2) * 16384 + (k & 3) * 32),
-                                desc_sw128(smem_u32(kop) + (k >> 2) * (C::kTokens * 128) + (k & 3) * 32), C::kIdescS, k > 0);
+            for (int k = 0; k < D / 64; ++k)
+                mma4_ss_warp(tm + C::kColS, q_lo + k * (16384 >> 4), k_lo + k * (C::kTokens * 128 >> 4), C::kIdescS, k);
         };
 
         float neg_m = INFINITY;  // minus the row's running maximum
@@ -1326,9 +1348,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             __syncthreads();
             if (warp == 0) {
                 tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < C::kTokens / 16; ++k)
-                    mma_f16_ts_warp(tm + C::kColO, tm + C::kColP + k * 8, desc_sw128(smem_u32(vop) + k * 32), C::kIdescO, i > 0 || k > 0);
+                mma4_ts_warp(tm + C::kColO, tm + C::kColP, v_lo, C::kIdescO, i > 0);
                 if (i + 1 < count) logits();
                 tc_commit_warp(&bar);
             }
