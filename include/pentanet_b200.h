@@ -304,11 +304,13 @@ int pn_dequant_act_i8(const int8_t *xq, int64_t xq_pitch, const float *s_x, int6
  *
  * block_table: (B, table_w) int32, rows table_ld apart: entry i of sequence b is
  * the page of its positions [i * page, (i + 1) * page).  seq_lens: (B) int32, the
- * sequences' lengths WITH the rows of this call, taken as at most table_w * page
- * (at most 2^30).  The T rows of a call are the newest positions of their sequences: T / B rows
- * each, or rows [cu_q[b], cu_q[b + 1]) with cu_q (B + 1) int32.  Entries used that are no page of the cache are
- * skipped (nothing is stored; their tokens read as zeros and are not attended
- * to) and recorded as PN_ERR_ARG in the device status word.
+ * sequences' lengths WITH the rows of this call (table_w * page is at most 2^30).
+ * The T rows of a call are the newest positions of their sequences: T / B rows
+ * each, or rows [cu_q[b], cu_q[b + 1]) with cu_q (B + 1) int32.  Positions behind
+ * the table's end, and entries used that are no page of the cache, are skipped
+ * (nothing is stored; their tokens read as zeros and are not attended to) and
+ * recorded as PN_ERR_ARG in the device status word (not where the cache or the
+ * table is empty: such a call finds nothing).
  * Strides are in elements: of a sequence, a row and a head (the first is not
  * used with cu_q); the last dimension is contiguous. */
 int64_t pn_kv4_block_bytes(int64_t page, int64_t head_dim);

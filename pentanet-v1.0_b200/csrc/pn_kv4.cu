@@ -30,7 +30,7 @@ namespace pn {
 struct Kv4Seq {
     const int32_t* table;  // (B, table_ld): page of tokens [i * page, (i + 1) * page)
     int64_t table_ld;
-    int table_w;           // pages per sequence in the table
+    int table_w;           // pages per sequence in the table; 0 where there are no pages at all
     const int32_t* lens;   // (B)
     const int32_t* cu;     // (B + 1) first row of each sequence, or null: L rows each
     int64_t B, T;          // sequences, rows
@@ -39,10 +39,9 @@ struct Kv4Seq {
     int Hk, page;
 };
 
-__device__ __forceinline__ int kv4_len(const Kv4Seq& s, int64_t b) {
-    const int64_t cap = (int64_t)s.table_w * s.page;
-    return (int)min(max((int64_t)__ldg(s.lens + b), (int64_t)0), cap);
-}
+// The length of sequence b, and how much of it its table has room for.
+__device__ __forceinline__ int kv4_len(const Kv4Seq& s, int64_t b) { return min(max(__ldg(s.lens + b), 0), 1 << 30); }
+__device__ __forceinline__ int kv4_held(const Kv4Seq& s, int64_t b) { return min(kv4_len(s, b), s.table_w * s.page); }
 
 // First row and number of rows of sequence b.
 __device__ __forceinline__ void kv4_rows(const Kv4Seq& s, int64_t b, int64_t& first, int64_t& n) {
@@ -78,11 +77,12 @@ __device__ __forceinline__ bool kv4_find(const Kv4Seq& s, int64_t row, int64_t& 
 }
 
 // The page block that holds position pos of sequence b, or -1 (and the device
-// status word) when the table's entry is no page of the cache.
+// status word) when the table has no entry for it, or one that is no page of the
+// cache.  (A table without any entry is no mistake of an index: nothing is reported.)
 __device__ __forceinline__ int64_t kv4_page(const Kv4Seq& s, int64_t b, int pos) {
-    const int p = __ldg(s.table + b * s.table_ld + pos / s.page);
+    const int p = pos < s.table_w * s.page ? __ldg(s.table + b * s.table_ld + pos / s.page) : -1;
     if (p >= 0 && p < s.n_pages) return p;
-    record_status(PN_ERR_ARG);
+    if (s.table_w > 0) record_status(PN_ERR_ARG);
     return -1;
 }
 
@@ -439,7 +439,7 @@ static int check_kv4(const char* name, const void* cache, int64_t n_pages, int64
         return fail(PN_ERR_ARG, "%s: null pointer", name);
     if (!aligned(cache, 16)) return fail(PN_ERR_ALIGN, "%s: the cache needs 16-byte alignment", name);
     if (!aligned(table, 4) || !aligned(lens, 4) || !aligned(cu, 4)) return fail(PN_ERR_ALIGN, "%s: misaligned pointer", name);
-    *s = pn::Kv4Seq{table, table_ld, (int)table_w, lens, cu, B, T, B > 0 ? T / B : 0, n_pages, (int)Hk, (int)page};
+    *s = pn::Kv4Seq{table, table_ld, n_pages > 0 ? (int)table_w : 0, lens, cu, B, T, B > 0 ? T / B : 0, n_pages, (int)Hk, (int)page};
     return PN_OK;
 }
 
@@ -461,7 +461,6 @@ int pn_kv4_append(const void* k, int64_t k_sb, int64_t k_sl, int64_t k_sh, const
     if (!aligned(k, e) || !aligned(v, e)) return fail(PN_ERR_ALIGN, "pn_kv4_append: misaligned pointer");
     if (int st = check_device()) return st;
     if (T == 0 || B == 0) return ok();
-    if (n_pages == 0 || table_w == 0) return ok();  // no room for any token
     a.x[0] = k, a.sb[0] = k_sb, a.sl[0] = k_sl, a.sh[0] = k_sh;
     a.x[1] = v, a.sb[1] = v_sb, a.sl[1] = v_sl, a.sh[1] = v_sh;
     a.cache = static_cast<uint8_t*>(cache);
@@ -497,7 +496,6 @@ int pn_kv4_gather(const void* cache, int64_t n_pages, int64_t kv_heads, int64_t 
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(PN_ERR_ALIGN, "pn_kv4_gather: k and v need 16-byte alignment");
     if (int st = check_device()) return st;
     if (T == 0 || B == 0) return ok();
-    if (n_pages == 0) a.s.table_w = 0;  // every length counts as zero
     a.cache = static_cast<const uint8_t*>(cache);
     a.y[0] = k;
     a.y[1] = v;

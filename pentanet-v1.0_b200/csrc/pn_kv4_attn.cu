@@ -107,7 +107,7 @@ template <typename C>
 __device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, uint32_t& nt) {
     int64_t first, n;
     kv4_rows(a.s, b, first, n);
-    nt = max((kv4_len(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
+    nt = max((kv4_held(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
     return ((uint32_t)n * a.G + C::kRows - 1) / C::kRows * nt * a.s.Hk;
 }
 
@@ -169,8 +169,8 @@ struct AttnSeg {
     int head, rows;          // kv head; query rows in the tile
     int64_t row0, r0;        // first row of the sequence; first query row of the tile
     int pos0;                // query row r sees positions up to pos0 + r / G
-    int kv_end;              // tokens that the tile's last row sees
-    int lim_min;             // the last position that its first row sees
+    int kv_end;              // tokens that the tile's last row sees (and the table has room for)
+    int lim_min;             // the last position that its first row sees (at most kv_end - 1)
 
     // Advances `in_seq` to its sequence first.
     template <typename C>
@@ -195,8 +195,9 @@ struct AttnSeg {
         t0 = in_seq - tile * nt;
         t1 = min(nt, t0 + left);
         pos0 = kv4_len(a.s, b) - (int)n_rows;
-        kv_end = max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0);
-        lim_min = pos0 + (int)((uint32_t)r0 / a.G);
+        kv_end = min(max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0), kv4_held(a.s, b));
+        if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && pos0 + (int)n_rows > kv4_held(a.s, b)) record_status(PN_ERR_ARG);
+        lim_min = min(pos0 + (int)((uint32_t)r0 / a.G), kv_end - 1);
     }
     // Where query row r of the tile (r < rows) lies in q, in elements.
     __device__ __forceinline__ int64_t query(const Kv4AttnArgs& a, int r) const {
@@ -1566,8 +1567,9 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     if (!(scale > 0.0f && scale < INFINITY)) return fail(PN_ERR_ARG, "pn_kv4_attention: scale must be positive");
     const size_t e = q_dtype == PN_F32 ? 4 : 2;
     if (!aligned(q, e) || !aligned(out, 16)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: misaligned pointer");
-    // an upper bound on the units that the kernels count in 31 bits
-    if (B > 0 && ((double)T * (q_heads / kv_heads) / 8 + B) * kv_heads * ((double)table_w * page / 64 + 1) > 2e9)
+    // upper bounds on the rows and units that the kernels count in 31 bits
+    if (B > 0 && ((double)T * (q_heads / kv_heads) > 2e9 ||
+                  ((double)T * (q_heads / kv_heads) / 8 + B) * kv_heads * ((double)table_w * page / 64 + 1) > 2e9))
         return fail(PN_ERR_SHAPE, "pn_kv4_attention: %lld rows over tables of %lld tokens are too much for one call",
                     (long long)T, (long long)(table_w * page));
     if (int st = check_device()) return st;
@@ -1576,7 +1578,6 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     if (!workspace || workspace_bytes < need)
         return fail(PN_ERR_WORKSPACE, "pn_kv4_attention: workspace needs %zu bytes", need);
     if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: the workspace needs 256-byte alignment");
-    if (n_pages == 0) a.s.table_w = 0;  // every length counts as zero
     a.q = q, a.q_f32 = q_dtype == PN_F32, a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh;
     const int64_t n = 16 / (int64_t)e;
     a.q_vec = aligned(q, 16) && q_sb % n == 0 && q_sl % n == 0 && q_sh % n == 0;

@@ -268,6 +268,29 @@ def test_block_table_entries_outside_the_cache(cuda_device):
     assert nat.device_status() == 0
 
 
+@pytest.mark.parametrize("rows", [3, 20, 90])
+def test_lengths_past_the_table(cuda_device, rows):
+    """Positions that the table has no entry for are not stored, not attended to and
+    reported; what lies in the table stays as it was."""
+    n, held, page, hk, G = 200, 160, 16, 2, 4
+    s = Batch([n, 50], hk, 128, page, cuda_device, seed=rows)
+    s.table = s.table[:, :held // page].contiguous()
+    before = s.cache.clone()
+    s.store([rows, 0])  # of its positions 200 - rows .. 199 those below 160 are there already
+    assert torch.equal(before, s.cache)
+    assert nat.device_status(reset=True) == nat.PN_ERR_ARG
+    k, _ = pc.kv4_gather(s.cache, 128, s.table, s.lens, (n,), cu_q=torch.tensor([0, n, n], dtype=torch.int32, device=cuda_device))
+    assert not k[held:].any() and k[held - 1].any() and nat.device_status(reset=True) == nat.PN_ERR_ARG
+    q = torch.randn(rows, hk * G, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    cu = torch.tensor([0, rows, rows], dtype=torch.int32, device=cuda_device)
+    y = pc.kv4_attention(q.to(cuda_device), s.cache, s.table, s.lens, cu_q=cu)
+    assert nat.device_status(reset=True) == nat.PN_ERR_ARG
+    for r in range(rows):  # a row at position p sees positions up to min(p, 159)
+        end = min(n - rows + r + 1, held)
+        want, bound = oracle.attention(q[r:r + 1], s.k[0][:end], s.v[0][:end])
+        assert ((y[r].double().cpu() - want[0]).abs() <= bound[0] + 2.0 ** -8 * (want[0].abs() + bound[0])).all(), r
+
+
 def test_rows_behind_the_last_sequence(cuda_device):
     s = Batch([30, 20], 2, 64, 16, cuda_device)
     cu = torch.tensor([0, 1, 3], dtype=torch.int32, device=cuda_device)
