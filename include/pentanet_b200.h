@@ -306,7 +306,9 @@ int pn_dequant_act_i8(const int8_t *xq, int64_t xq_pitch, const float *s_x, int6
  * the page of its positions [i * page, (i + 1) * page).  seq_lens: (B) int32, the
  * sequences' lengths WITH the rows of this call (table_w * page is at most 2^30).
  * The T rows of a call are the newest positions of their sequences: T / B rows
- * each, or rows [cu_q[b], cu_q[b + 1]) with cu_q (B + 1) int32.  Positions behind
+ * each, or rows [cu_q[b], cu_q[b + 1]) with cu_q (B + 1) int32, which does not
+ * fall (attention over rows of one that does computes nothing and records
+ * PN_ERR_ARG in the device status word).  Positions behind
  * the table's end, and entries used that are no page of the cache, are skipped
  * (nothing is stored; their tokens read as zeros and are not attended to) and
  * recorded as PN_ERR_ARG in the device status word (not where the cache or the

@@ -127,7 +127,11 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
     const uint32_t B = (uint32_t)a.s.B, per = (B + C::kThreads - 1) / C::kThreads;
     const uint32_t b0 = min(threadIdx.x * per, B), b1 = min(b0 + per, B);
     uint32_t sum = 0, nt;
-    for (uint32_t b = b0; b < b1; ++b) sum += attn_units<C>(a, b, nt);
+    bool falls = false;  // cu_q does: its rows, and so the units, may be more than the host counted on
+    for (uint32_t b = b0; b < b1; ++b) {
+        sum += attn_units<C>(a, b, nt);
+        falls |= a.s.cu && __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
+    }
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     uint32_t inc = sum;
 #pragma unroll
@@ -136,10 +140,14 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
         if (lane >= o) inc += v;
     }
     if (lane == 31) sums[w] = inc;
-    __syncthreads();
-    uint32_t at = inc - sum;
     AttnRun run;
     run.total = 0;
+    if (__syncthreads_or(falls)) {  // nothing is computed
+        if (threadIdx.x == 0) record_status(PN_ERR_ARG);
+        run.begin = run.end = run.seq = run.in_seq = 0;
+        return run;
+    }
+    uint32_t at = inc - sum;
 #pragma unroll
     for (int i = 0; i < kWarps; ++i) {
         if (i < w) at += sums[i];

@@ -15,7 +15,8 @@ A sequence's page i (block_table[b, i]) holds its positions [i * page_size,
 (i + 1) * page_size).  seq_lens[b] counts the sequence's tokens WITH the rows of
 the call: the rows are its newest positions.  Rows come as (B, L, heads,
 head_dim), L for each sequence, or as (T, heads, head_dim) with cu_q (B + 1)
-int32, sequence b having rows [cu_q[b], cu_q[b + 1]) (without cu_q: T / B each).
+int32, never falling, sequence b having rows [cu_q[b], cu_q[b + 1]) (without cu_q:
+T / B each).
 Lengths, tables and cu_q are read on the GPU, so a captured CUDA graph follows
 their contents.  A block-table entry outside the cache, and a position behind the
 table's end, is skipped (not stored, not attended to) and shows in

@@ -291,6 +291,18 @@ def test_lengths_past_the_table(cuda_device, rows):
         assert ((y[r].double().cpu() - want[0]).abs() <= bound[0] + 2.0 ** -8 * (want[0].abs() + bound[0])).all(), r
 
 
+@pytest.mark.parametrize("rows", [4, 40, 100])
+def test_row_starts_that_fall(cuda_device, rows):
+    """Reported, and nothing is computed."""
+    s = Batch([50, 60, 20], 1, 64, 16, cuda_device)
+    q = torch.randn(3 * rows, 2, 64, device=cuda_device).to(torch.bfloat16)
+    out = torch.full_like(q, 7.0)
+    assert nat.device_status() == 0
+    cu = torch.tensor([0, 3 * rows, rows, 3 * rows], dtype=torch.int32, device=cuda_device)
+    pc.kv4_attention(q, s.cache, s.table, s.lens, cu_q=cu, out=out)
+    assert (out == 7).all() and nat.device_status(reset=True) == nat.PN_ERR_ARG
+
+
 def test_rows_behind_the_last_sequence(cuda_device):
     s = Batch([30, 20], 2, 64, 16, cuda_device)
     cu = torch.tensor([0, 1, 3], dtype=torch.int32, device=cuda_device)
