@@ -973,13 +973,13 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
 //
 // A step waits for the products of the one before, so operands and logits need no
 // second buffer; the other block of the SM fills the wait.  (One block of 16 warps
-// with doubled buffers and 128 tokens per step took 278 us for the ragged
-// chunks where this takes 225 us:
-// its warps met at five barriers per step with nothing else to run.)
+// with doubled buffers and 128 tokens per step took 278 us where this takes 223 us,
+// chunks of 1 to 512 tokens: its warps met at five barriers per step with
+// nothing else to run.)
 //
-// What bounds it: the softmax's and the spreading's instructions (about 350 per
-// thread and step); the products take 512 cycles per step at the tensor core's
-// rate.
+// What bounds it: the softmax's and the spreading's instructions, about 500 per
+// thread and step (3500 to 4500 cycles for an SM's two blocks); the products take
+// 512 cycles of a step at the tensor core's rate.
 template <int D>
 struct TcCfg {
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
@@ -1494,22 +1494,40 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
     }
 }
 
-// The kernel by the query rows that a sequence has on average for one kv head: up
-// to 8 and up to 16 in the decode kernel, up to 64 in the chunk kernel, more in
-// the one on tcgen05.
+// The kernel by the query rows that a sequence has on average for one kv head, and
+// by the row tiles that this makes of the call.  A small tile reads and unpacks the
+// cache more often, but gives the SMs more to share: up to four tiles of 16 rows
+// per SM the 16-row kernel wins whatever the number of rows, from eight per SM
+// on the larger one of the others.  In us for d = 128 (16 rows / chunk / tcgen05):
+//   4 sequences x 128 rows x 8 heads of 2048 tokens (256 tiles)      44 /  63 /  92
+//   one prompt of 500 tokens, 512 rows x 8 heads (256 tiles)         28 /  44 /  70
+//   8 x 144 x 8 heads of 2048 tokens (576 tiles)                     72 /  78 /  78
+//   one prompt of 768 tokens, 12 heads (576 tiles)                   37 /  39 /  71
+//   64 x 96 x 2 heads of 1024 tokens (768 tiles)                     61 /  64 /  66
+//   32 prompts of 24 tokens, 12 heads (768 tiles)                    22 /  12 /  19
+//   64 x 64 x 4 heads of 1024 tokens (1024 tiles)                    77 /  73 /  77
+//   64 x 96 x 4 heads of 1024 tokens (1536 tiles)                   106 /  93 /  81
+//   16 x 512 x 8 heads of 1024 tokens (4096 tiles)                  239 / 165 / 121
+// and at 8 rows 24 against 34 (64 heads of 4096 tokens: the 8-row kernel, the 16-row
+// one).  Where the rule is wrong: few tiles over very long sequences (290
+// tokens x 4 behind 8192, 584 tiles: 190 / 176 / 152), many prompts of 128 to 512
+// tokens (32 x 128, 12 heads: 79 / 36 / 51; d = 64, 16 x 512: 116 / 67 / 75); the
+// host does not know the lengths.
 enum AttnKind { kAttn8, kAttn16, kAttnChunk, kAttnLong };
-static AttnKind attn_kind(int64_t B, int64_t T, int64_t G) {
-    const int64_t rows = (T + B - 1) / B * G;
-    return rows <= 8 ? kAttn8 : rows <= 16 ? kAttn16 : rows <= 64 ? kAttnChunk : kAttnLong;
+static AttnKind attn_kind(int64_t B, int64_t T, int64_t Hk, int64_t G) {
+    const int64_t rows = (T + B - 1) / B * G, tiles = (rows + 15) / 16 * B * Hk;
+    const int64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    if (rows <= 16 || tiles <= 4 * sms) return rows <= 8 ? kAttn8 : kAttn16;
+    return rows <= 64 || tiles <= 8 * sms ? kAttnChunk : kAttnLong;
 }
 static int attn_blocks(AttnKind kind) {  // blocks that the device holds at once
     const int sms = device_sm_count();
     return (sms > 0 ? sms : 148) * (kind == kAttnLong ? TcCfg<128>::kBlocks : AttnCfg<128, 1>::kBlocks);
 }
 static size_t attn_notes_bytes(int blocks) { return ((size_t)blocks * sizeof(Kv4Join) + 255) / 256 * 256; }
-static size_t attn_workspace(int64_t B, int64_t T, int64_t G, int64_t D) {
+static size_t attn_workspace(int64_t B, int64_t T, int64_t Hk, int64_t G, int64_t D) {
     if (B == 0 || T == 0) return 0;
-    const AttnKind kind = attn_kind(B, T, G);
+    const AttnKind kind = attn_kind(B, T, Hk, G);
     const int blocks = attn_blocks(kind), rows[4] = {8, 16, 64, 128};
     return attn_notes_bytes(blocks) + (size_t)blocks * 2 * rows[kind] * (D + 2) * 4;
 }
@@ -1524,7 +1542,7 @@ static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    const int blocks = attn_blocks(attn_kind(a.s.B, a.s.T, a.G));
+    const int blocks = attn_blocks(attn_kind(a.s.B, a.s.T, a.s.Hk, a.G));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1555,7 +1573,7 @@ extern "C" {
 
 size_t pn_kv4_attention_workspace_size(int64_t B, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
     if (B < 0 || T < 0 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
-    return pn::attn_workspace(B, T, q_heads / kv_heads, head_dim);
+    return pn::attn_workspace(B, T, kv_heads, q_heads / kv_heads, head_dim);
 }
 
 int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
@@ -1582,7 +1600,7 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
                     (long long)T, (long long)(table_w * page));
     if (int st = check_device()) return st;
     if (T == 0 || B == 0) return ok();
-    const size_t need = pn::attn_workspace(B, T, q_heads / kv_heads, head_dim);
+    const size_t need = pn::attn_workspace(B, T, kv_heads, q_heads / kv_heads, head_dim);
     if (!workspace || workspace_bytes < need)
         return fail(PN_ERR_WORKSPACE, "pn_kv4_attention: workspace needs %zu bytes", need);
     if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: the workspace needs 256-byte alignment");
@@ -1593,7 +1611,7 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     a.G = (int)(q_heads / kv_heads);
     a.scale_log2 = scale * 1.4426950408889634f;
     a.out = out;
-    const pn::AttnKind kind = pn::attn_kind(B, T, a.G);
+    const pn::AttnKind kind = pn::attn_kind(B, T, kv_heads, a.G);
     a.notes = static_cast<pn::Kv4Join*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_notes_bytes(pn::attn_blocks(kind)));
     const cudaStream_t s = (cudaStream_t)stream;

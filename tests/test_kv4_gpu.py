@@ -385,3 +385,108 @@ def test_empty_calls(cuda_device):
     none = torch.zeros(0, 3, dtype=torch.int32, device=cuda_device)
     assert pc.kv4_attention(q[:0], cache, none, lens[:0]).shape == (0, 1, 4, 64)
     assert nat.device_status() == 0
+
+
+# Calls of many row tiles (more than four per SM) take larger ones: 64 rows up to 64 rows
+# per sequence and head (here 12 x 4), 128 above (21 x 4).
+def wide(device, d, rows, **kw):
+    g = torch.Generator().manual_seed(rows + d)
+    lengths = torch.randint(1, 260, (32,), generator=g).tolist()
+    lengths[:4] = [300, 255, 64, 5]
+    return Batch(lengths, 8, d, kw.pop("page", 64), device, seed=rows, **kw)
+
+
+def wide_rows(rows):
+    """`rows` each on average: long ones, single ones, none, more than the sequence has."""
+    r = [rows] * 32
+    r[:6] = [3 * rows, 1, 0, rows, rows - 1, 2]
+    r[6] += 6 * rows - sum(r[:6])
+    assert sum(r) == 32 * rows and min(r) >= 0
+    return r
+
+
+@pytest.mark.parametrize("d,page", [(64, 64), (128, 16), (128, 48), (64, 128)])
+@pytest.mark.parametrize("rows", [12, 21])
+def test_many_row_tiles(cuda_device, d, page, rows):
+    s = wide(cuda_device, d, rows, page=page)
+    s.attend(wide_rows(rows), 4)
+    s.attend(wide_rows(rows), 4, dtype=torch.float32, scale=0.2)
+    assert nat.device_status() == 0
+
+
+@pytest.mark.parametrize("rows", [12, 21])
+def test_many_row_tiles_hard_values(cuda_device, rows):
+    """Growing maxima and value scales, one dominant token, constant vectors."""
+    s = wide(cuda_device, 128, rows)
+    n = s.lengths
+    s.k[0] = (s.k[0].float() * 0.1 + torch.linspace(-6, 6, n[0])[:, None, None]).to(torch.bfloat16)
+    s.k[1][n[1] // 2] = 20.0
+    s.v[0] = (s.v[0].float() * torch.logspace(-6, 3, n[0])[:, None, None]).to(torch.bfloat16)
+    s.v[0][:100] = 0.75
+    s.v[1] = (s.v[1].float() * torch.logspace(-4, 4, n[1]).flip(0)[:, None, None]).to(torch.bfloat16)
+    s.k[3] = torch.ones_like(s.k[3])
+    s.v[3] = torch.full_like(s.v[3], 0.37)
+    s.store(n)
+    s.attend([rows] * 32, 4)
+    s.attend(wide_rows(rows), 4)
+
+
+@pytest.mark.parametrize("rows", [12, 21])
+def test_many_row_tiles_not_finite(cuda_device, rows):
+    """Only rows that see a vector that is not finite turn NaN."""
+    s = wide(cuda_device, 64, rows)
+    s.v[0][290, 3, 5] = float("inf")
+    s.k[1][250, 2, 0] = float("nan")
+    s.store(s.lengths)
+    q = torch.randn(32, rows, 32, 64, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(cuda_device)
+    y = pc.kv4_attention(q, s.cache, s.table, s.lens).view(32, rows, 8, 4, 64)
+    bad = torch.zeros(32, rows, 8, dtype=torch.bool, device=cuda_device)
+    for r in range(rows):
+        bad[0, r, 3] = 300 - rows + r >= 290
+        bad[1, r, 2] = 255 - rows + r >= 250
+    assert bad.any() and torch.equal(torch.isnan(y).all(-1).all(-1), bad)
+    assert torch.equal(~torch.isfinite(y).all(-1).all(-1), bad)
+
+
+@pytest.mark.parametrize("rows", [12, 21])
+def test_many_row_tiles_lost_pages(cuda_device, rows):
+    """Entries outside the cache and lengths past the table: skipped and reported."""
+    s = wide(cuda_device, 128, rows, page=16)
+    q = torch.randn(32, rows, 32, 128, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    s.table[0, 2] = -1
+    s.table[1, 0] = s.cache.shape[0]
+    table = s.table[:, :256 // 16].contiguous()  # sequence 0 has 300 tokens
+    assert nat.device_status() == 0
+    y = pc.kv4_attention(q.to(cuda_device), s.cache, table, s.lens)
+    assert nat.device_status(reset=True) == nat.PN_ERR_ARG
+    near = lambda got, want, bound: ((got.double().cpu() - want).abs() <= bound + 2.0 ** -8 * (want.abs() + bound)).all().item()
+    behind = set(range(256, 300))
+    for i, n in enumerate(s.lengths):
+        lost = behind | (set(range(32, 48)) if i == 0 else set(range(16)) if i == 1 else set())
+        if lost.isdisjoint(range(n)):
+            lead = max(rows - n, 0)
+            assert not y[i, :lead].any() and near(y[i, lead:], *oracle.attention(q[i, lead:], s.k[i], s.v[i])), i
+            continue
+        for r in range(max(rows - n, 0), rows):
+            keep = [t for t in range(n - rows + r + 1) if t not in lost]
+            want, bound = oracle.attention(q[i, r:r + 1], s.k[i][keep], s.v[i][keep])
+            assert near(y[i, r], want[0], bound[0]), (i, r)
+
+
+@pytest.mark.parametrize("rows", [12, 21])
+def test_many_row_tiles_captured(cuda_device, rows):
+    """Strided queries of a joint projection; replays follow the lengths; twice the same bits."""
+    s = wide(cuda_device, 128, rows)
+    qkv = torch.randn(32, rows, 48 * 128, device=cuda_device).to(torch.bfloat16)
+    q = qkv[..., :32 * 128].view(32, rows, 32, 128)
+    want = pc.kv4_attention(q.contiguous(), s.cache, s.table, s.lens)
+    assert torch.equal(pc.kv4_attention(q, s.cache, s.table, s.lens), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = pc.kv4_attention(q, s.cache, s.table, s.lens)
+    for _ in range(2):
+        graph.replay()
+        assert torch.equal(y, want)
+        s.lens -= 3
+        s.lens.clamp_(min=0)
+        want = pc.kv4_attention(q, s.cache, s.table, s.lens)
