@@ -335,8 +335,8 @@ int pn_kv4_gather(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t 
  * up to seq_lens[b] - L_b + i, its own included (store the rows' keys and values
  * first).  out (T, q_heads, head_dim) of q's type (PN_BF16 or PN_F32),
  * contiguous, 16-byte aligned; zeros for a row that sees nothing; rows behind
- * cu_q[B] are left as they were.  Query head
- * h reads kv head h / (q_heads / kv_heads).  The logits are scale * q . k, scale > 0.
+ * cu_q[B] are left as they were.  Query head h reads kv head
+ * h / (q_heads / kv_heads).  The logits are scale * q . k, scale > 0.
  * Queries enter the products as fp16 relative to the row's largest (bf16 ones
  * exactly), weights as fp16; sums and the softmax are fp32.
  * Workspace: pn_kv4_attention_workspace_size bytes, 256-byte aligned, no
@@ -353,8 +353,8 @@ int pn_kv4_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
  *   w_i = exp((x_i - max) / T); keep the top_k largest logits (ties: lowest
  *   index first; <= 0: all), of them those with w_i >= min_p, of them the
  *   smallest prefix in that order whose sum reaches top_p of the sum of all
- *   left (top_p >= 1: all; never less than one token); the token is the first index whose running sum of
- *   the kept w exceeds u * their sum.
+ *   left (top_p >= 1: all; never less than one token); the token is the first
+ *   index whose running sum of the kept w exceeds u * their sum.
  * T <= 0 takes the first largest logit.  A NaN logit counts as -inf; a row with
  * nothing above -inf gives -1; logits of +inf share all the weight.  Each
  * setting is a device array of one value per row, or, where its pointer is

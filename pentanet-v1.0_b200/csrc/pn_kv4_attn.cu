@@ -319,6 +319,12 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
     cb = a.scale_log2 * (sum * pow2i(-e));
 }
 
+// What bounds the decode kernel: not the cache's bytes but unpacking them, about 270
+// instructions per piece of 16 tokens and warp (d = 128, up to 8 rows: 64 masks and
+// shifts, 32 products, the softmax of 16 x 8 logits), issued at two per cycle and SM.
+// 32 sequences of up to 8191 tokens, 8 heads: 48 us, 3.3 TB/s; one of 131072: 41 us,
+// 3.4 TB/s (half of the copy's rate).  Three blocks of six stages per SM: two, four or
+// five blocks, and more stages in two, are all slower.
 template <int D, int NT>
 struct AttnCfg {
     static constexpr int W = D / 32;             // words per thread and token
@@ -683,7 +689,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 //
 // What bounds it: m16n8k16 runs at one per ten cycles on each quarter of an SM
 // (measured; 460 TFLOP/s over the device), 128 of them to a warp's 64 tokens at
-// d = 128, against 320 mask and shift instructions at two cycles each.
+// d = 128, against 320 mask and shift instructions at two cycles each.  64
+// sequences x 64 rows x 4 heads over 1024 tokens: 72 us (two blocks to an SM: 2 %
+// slower than three).
 template <int D>
 struct ChunkCfg {
     static constexpr int W = D / 32;
@@ -979,7 +987,8 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
 //
 // What bounds it: the softmax's and the spreading's instructions, about 500 per
 // thread and step (3500 to 4500 cycles for an SM's two blocks); the products take
-// 512 cycles of a step at the tensor core's rate.
+// 512 cycles of a step at the tensor core's rate.  16 sequences x 512 rows x 8
+// heads over 1024 tokens: 120 us (the chunk kernel 165).
 template <int D>
 struct TcCfg {
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;

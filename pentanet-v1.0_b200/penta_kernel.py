@@ -438,8 +438,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=
     With w = exp((x - max) / temperature): the top_k largest logits are kept
     (ties: lowest index first; 0 keeps all), of them those with w >= min_p, of
     them the smallest prefix in that order whose sum reaches top_p of the sum of
-    all left (at least one); the token is the first index whose running sum of kept w exceeds
-    u times their sum.  The same inputs always give the same token.
+    all left (at least one); the token is the first index whose running sum of
+    kept w exceeds u times their sum.  The same inputs always give the same token.
 
     temperature (0 takes the first largest logit), top_p and min_p are numbers or
     (B,) float32 tensors, top_k a number or a (B,) int32 tensor.  NaN logits are
