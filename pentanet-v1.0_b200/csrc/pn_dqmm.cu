@@ -1429,12 +1429,9 @@ static EncodeTiledFn get_encode_fn() {
 }
 
 int device_sm_count() {
-    static int known[64] = {};
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (dev >= 0 && dev < 64 && known[dev] > 0) return known[dev];
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    if (dev >= 0 && dev < 64) known[dev] = n;
     return n;
 }
 

@@ -1,5 +1,6 @@
 // pn_internal.h -- launchers shared between the kernel files and the C ABI.
 #pragma once
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <cuda_runtime.h>
@@ -63,6 +64,20 @@ int launch_linear(const LinearArgs& a, cudaStream_t s, cudaError_t* cuda_err, co
 cudaError_t launch_linear_simt_bf16(const LinearArgs& a, cudaStream_t s);
 
 int device_sm_count();
+// The same, asked of each device once, for launches that size their grids by it; 148
+// where it cannot be had.
+inline int sm_count() {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        n = device_sm_count();
+        if (n <= 0) return 148;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
 
 // Limb decode (bf16 products of at most l8_max_tokens() tokens, 0..16) on the
 // kind::i8 tensor cores; set_l8_max_tokens clamps to that range.

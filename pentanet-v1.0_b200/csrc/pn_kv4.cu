@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4Gather
 // first), one where there are few.  (9723 rows: 21 us with 8 rows to a block, 23
 // with 4, 28 with 2.)
 static int kv4_block_rows(int64_t T) {
-    const int64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    const int64_t sms = sm_count();
     int r = 1;
     while (r < kKv4MaxRows && T / (2 * r) >= 8 * sms) r *= 2;
     return r;

@@ -1525,13 +1525,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 enum AttnKind { kAttn8, kAttn16, kAttnChunk, kAttnLong };
 static AttnKind attn_kind(int64_t B, int64_t T, int64_t Hk, int64_t G) {
     const int64_t rows = (T + B - 1) / B * G, tiles = (rows + 15) / 16 * B * Hk;
-    const int64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    const int64_t sms = sm_count();
     if (rows <= 16 || tiles <= 4 * sms) return rows <= 8 ? kAttn8 : kAttn16;
     return rows <= 64 || tiles <= 8 * sms ? kAttnChunk : kAttnLong;
 }
 static int attn_blocks(AttnKind kind) {  // blocks that the device holds at once
-    const int sms = device_sm_count();
-    return (sms > 0 ? sms : 148) * (kind == kAttnLong ? TcCfg<128>::kBlocks : AttnCfg<128, 1>::kBlocks);
+    return sm_count() * (kind == kAttnLong ? TcCfg<128>::kBlocks : AttnCfg<128, 1>::kBlocks);
 }
 static size_t attn_notes_bytes(int blocks) { return ((size_t)blocks * sizeof(Kv4Join) + 255) / 256 * 256; }
 static size_t attn_workspace(int64_t B, int64_t T, int64_t Hk, int64_t G, int64_t D) {
@@ -1543,7 +1542,7 @@ static size_t attn_workspace(int64_t B, int64_t T, int64_t Hk, int64_t G, int64_
 
 template <int D, typename C>
 static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a, cudaStream_t s) {
-    static bool done[64] = {};
+    static std::atomic<bool> done[64];  // false at first
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !done[dev]) {

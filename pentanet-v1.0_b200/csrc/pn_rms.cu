@@ -447,7 +447,7 @@ static cudaError_t launch_rms_t(const RmsArgs& a, cudaStream_t s) {
     // Few rows: a piece per thread, for latency.  Many: 64 bytes per thread
     // (fewer threads to reduce over, as many loads in flight).
     constexpr int kMany = sizeof(T) == 2 ? 4 : 2;
-    const int64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    const int64_t sms = sm_count();
     int pc = a.M <= 2 * sms ? 1 : kMany;
     if (pieces > 1024 * pc) pc = kMany;
     int tpt = 32;

@@ -840,7 +840,7 @@ template <typename T>
 static cudaError_t launch_sample(SampleArgs a, int64_t rows, cudaStream_t s) {
     // chunks of a row, wherever its first byte lies
     const int64_t chunks = (a.V + 2 * SmpChunk<T>::N - 2) / SmpChunk<T>::N;
-    const int64_t sms = device_sm_count() > 0 ? device_sm_count() : 148;
+    const int64_t sms = sm_count();
     // Blocks per row: at least what holds it at 8 chunks per thread (64 KB, two
     // blocks per SM) or, beyond eight blocks, more chunks per thread; more blocks
     // while a row more or less would leave SMs idle, down to one chunk per thread.
@@ -850,7 +850,7 @@ static cudaError_t launch_sample(SampleArgs a, int64_t rows, cudaStream_t s) {
     if (blocks > kSmpBlocks) blocks = kSmpBlocks;
     a.steps = (int)((chunks + blocks * kSmpThreads - 1) / (blocks * kSmpThreads));
     const size_t smem = (size_t)a.steps * kSmpThreads * 16 + sizeof(SampleShared);
-    static bool done[64] = {};
+    static std::atomic<bool> done[64];  // false at first
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !done[dev]) {
