@@ -20,7 +20,8 @@ T / B each).
 Lengths, tables and cu_q are read on the GPU, so a captured CUDA graph follows
 their contents.  A block-table entry outside the cache, and a position behind the
 table's end, is skipped (not stored, not attended to) and shows in
-penta_native.device_status().
+penta_native.device_status().  Sequences may share a page that the call stores
+nothing to.
 """
 from __future__ import annotations
 

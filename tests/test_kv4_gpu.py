@@ -1,5 +1,7 @@
 """The 4-bit cache (penta_cache): what is stored, what is read back, and attention
 over it, against the definition (kv4_oracle)."""
+import threading
+
 import pytest
 import torch
 
@@ -490,3 +492,26 @@ def test_many_row_tiles_captured(cuda_device, rows):
         s.lens -= 3
         s.lens.clamp_(min=0)
         want = pc.kv4_attention(q, s.cache, s.table, s.lens)
+
+
+def test_calls_of_several_threads(cuda_device):
+    """Each on a stream of its own, all kernels at once: every call gives its own result."""
+    s = wide(cuda_device, 128, 21)
+    q = torch.randn(32, 21, 32, 128, device=cuda_device).to(torch.bfloat16)
+    calls = [q[:, :n] for n in (1, 4, 12, 21)]
+    want = [pc.kv4_attention(x, s.cache, s.table, s.lens) for x in calls]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                wrong.extend(n for n, x in enumerate(calls)
+                             if not torch.equal(pc.kv4_attention(x, s.cache, s.table, s.lens), want[n]))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and nat.device_status() == 0
