@@ -185,7 +185,9 @@ __device__ __noinline__ uint64_t smp_weight(const SampleShared& s, float x) {
     return w >= s.row.floor ? w : 0;
 }
 
-// 16 bytes of logits as fp32.
+// 16 bytes of logits as fp32.  clean: a NaN becomes -inf, and -0 becomes +0 (the sum
+// with +0), so that equal logits have one bit pattern and the order of patterns is that of
+// the logits.
 template <typename T>
 struct SmpChunk;
 template <>
@@ -198,8 +200,8 @@ struct SmpChunk<float> {
     static __device__ __forceinline__ float max(const uint4& u) {
         return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
     }
-    static __device__ __forceinline__ uint32_t no_nan(uint32_t w) {
-        return __float_as_uint(fmaxf(__uint_as_float(w), -INFINITY));
+    static __device__ __forceinline__ uint32_t clean(uint32_t w) {
+        return __float_as_uint(__fadd_rn(fmaxf(__uint_as_float(w), -INFINITY), 0.0f));
     }
     static __device__ __forceinline__ void set_none(uint8_t* p) { *reinterpret_cast<uint32_t*>(p) = kNone; }
 };
@@ -224,7 +226,11 @@ struct SmpChunk<__nv_bfloat16> {
         const uint32_t m = max2(max2(u.x, u.y), max2(u.z, u.w));
         return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
     }
-    static __device__ __forceinline__ uint32_t no_nan(uint32_t w) { return max2(w, kNone); }
+    static __device__ __forceinline__ uint32_t clean(uint32_t w) {
+        uint32_t r;
+        asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(max2(w, kNone)), "r"(0));
+        return r;
+    }
     static __device__ __forceinline__ void set_none(uint8_t* p) { *reinterpret_cast<uint16_t*>(p) = 0xFF80; }
 };
 
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(kSmpThreads, 2) sample_kernel(const SampleArgs
         uint4 u = make_uint4(K::kNone, K::kNone, K::kNone, K::kNone);
         if (c < chunks) {
             u = __ldg(src + c);
-            u.x = K::no_nan(u.x), u.y = K::no_nan(u.y), u.z = K::no_nan(u.z), u.w = K::no_nan(u.w);
+            u.x = K::clean(u.x), u.y = K::clean(u.y), u.z = K::clean(u.z), u.w = K::clean(u.w);
         }
         mine[j * 32] = u;
         if (c == 0 || c == chunks - 1) {  // what lies beside the row in its first and last chunk

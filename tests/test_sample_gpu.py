@@ -86,6 +86,24 @@ def test_ties(cuda_device, V):
         check(few.to(torch.bfloat16), u, **kw)
 
 
+@pytest.mark.parametrize("V", [20, 1000, 50257])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("share", [0.03, 0.5, 0.97])
+def test_zeros_of_both_signs(cuda_device, V, dtype, share):
+    """-0 and +0 are equal logits, the lowest index first whatever their signs; the
+    border among them lies in a short list, a long one and a row too long for it."""
+    u = torch.tensor([0.0, 0.25, 0.5, 0.999, 1.0 - 2.0 ** -24], device=cuda_device)
+    x = torch.rand(5, V, generator=torch.Generator().manual_seed(V)).to(cuda_device)
+    x = torch.where(x < share, 0.0, -0.0).to(dtype)
+    for rest in (0, 7):  # zeros alone; every seventh logit below them, one above
+        if rest:
+            x[:, ::rest] = -1.0
+            x[:, V // 2] = 1.0
+        for kw in (dict(top_k=V * 2 // 5), dict(top_p=0.37), dict(top_k=V // 2, top_p=0.6), dict(top_k=3), dict(temperature=0.0),
+                   dict()):
+            check(x, u, **kw)
+
+
 def test_masked_and_special_logits(cuda_device):
     inf, nan, low = float("inf"), float("nan"), torch.finfo(torch.float32).min
     x, u = inputs(12, 700, torch.float32, 3, cuda_device)
