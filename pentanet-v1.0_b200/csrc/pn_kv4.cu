@@ -497,10 +497,18 @@ int pn_kv4_gather(const void* cache, int64_t n_pages, int64_t kv_heads, int64_t 
                            seq_lens, cu_q, B, T, &a.s))
         return st;
     if (kv_dtype != PN_F32 && kv_dtype != PN_BF16) return fail(PN_ERR_DTYPE, "pn_kv4_gather: dtype %d", kv_dtype);
-    if (T > 0 && B > 0 && (!k || !v)) return fail(PN_ERR_ARG, "pn_kv4_gather: null pointer");
+    if (T > 0 && (!k || !v)) return fail(PN_ERR_ARG, "pn_kv4_gather: null pointer");
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(PN_ERR_ALIGN, "pn_kv4_gather: k and v need 16-byte alignment");
     if (int st = check_device()) return st;
-    if (T == 0 || B == 0) return ok();
+    if (T == 0) return ok();
+    if (B == 0) {  // every row lies behind the last sequence
+        const size_t bytes = (size_t)T * kv_heads * head_dim * (kv_dtype == PN_F32 ? 4 : 2);
+        for (void* y : {k, v}) {
+            const cudaError_t err = cudaMemsetAsync(y, 0, bytes, (cudaStream_t)stream);
+            if (err != cudaSuccess) return cuda_fail(err, "pn_kv4_gather");
+        }
+        return ok();
+    }
     a.cache = static_cast<const uint8_t*>(cache);
     a.y[0] = k;
     a.y[1] = v;

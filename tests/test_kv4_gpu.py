@@ -389,6 +389,30 @@ def test_empty_calls(cuda_device):
     assert nat.device_status() == 0
 
 
+def test_no_sequences(cuda_device):
+    """Rows behind the last sequence, of which there is none: zeros."""
+    cache = pc.kv4_cache(3, 2, 64, 16, cuda_device)
+    table = torch.zeros(0, 3, dtype=torch.int32, device=cuda_device)
+    lens = torch.zeros(0, dtype=torch.int32, device=cuda_device)
+    cu = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    for dtype in (torch.bfloat16, torch.float32):
+        junk = [torch.full((40, 2, 64), 7.0, dtype=dtype, device=cuda_device) for _ in range(4)]
+        torch.cuda.synchronize()
+        del junk  # what the allocator hands out next
+        k, v = pc.kv4_gather(cache, 64, table, lens, (40,), cu_q=cu, dtype=dtype)
+        assert k.shape == v.shape == (40, 2, 64) and not k.any() and not v.any()
+        k, v = (torch.full((5, 2, 64), 7.0, dtype=dtype, device=cuda_device) for _ in range(2))
+        st = nat.load().pn_kv4_gather(cache.data_ptr(), 3, 2, 16, 64, None, 3, 3, None, cu.data_ptr(), 0, 4, k.data_ptr(),
+                                      v.data_ptr(), nat.PN_F32 if dtype == torch.float32 else nat.PN_BF16, nat.stream_of(k))
+        assert st == nat.PN_OK
+        assert not k[:4].any() and not v[:4].any() and (k[4] == 7).all() and (v[4] == 7).all()
+        x = torch.ones(40, 2, 64, dtype=dtype, device=cuda_device)
+        before = cache.clone()
+        pc.kv4_append(x, x, cache, table, lens, cu_q=cu)
+        assert torch.equal(before, cache) and not pc.kv4_attention(x, cache, table, lens, cu_q=cu).any()
+    assert nat.device_status() == 0
+
+
 # Calls of many row tiles (more than four per SM) take larger ones: 64 rows up to 64 rows
 # per sequence and head (here 12 x 4), 128 above (21 x 4).
 def wide(device, d, rows, **kw):
