@@ -11,10 +11,10 @@
 // the query is divided by 16 there, on the value side the output is).  Five
 // integer operations give four fp16 pairs.  A row's query is scaled by a power
 // of two to a largest magnitude in [2^14, 2^15), so bf16 queries stay exact in fp16 down
-// to 2^-32 of the largest (fp32 queries are rounded to 11 bits).  The weights
+// to 2^-28 of the largest (fp32 queries are rounded to 11 bits).  The weights
 // p_t * s_v are rounded to fp16 (11 bits, more than the bf16 output keeps)
-// relative to the largest s_v seen; sums, the softmax's maximum and total, and
-// the z term are fp32.
+// relative to the largest s_v that the row has seen; sums, the softmax's maximum
+// and total, and the z term are fp32.
 //
 // Shape of the decode kernel.  Keys are the 16-row operand of m16n8k16 (16
 // tokens), the query rows of one kv head (group x new tokens) its 8 columns,
@@ -98,6 +98,27 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+// A row's reference, 2^m S: m its running maximum, S a power of two not below the value
+// scales of the tokens that it has seen (and no others: what a row may not see must not cost
+// it bits).  Weights, totals and outputs are relative to it, so that the weights times the
+// value scales fit fp16.  neg_r is minus its logarithm.  The maximum need not be exact: a
+// weight may exceed 1 / S by up to 2^8 before the sums are rescaled (fp16 holds 2^15), so most
+// tokens skip that; `limit`, 8 - log2 S, is what a logit may exceed the reference by.
+constexpr int kScaleLeast = -60, kScaleMost = 100;  // exponents of S: sums of weights over 2^30 tokens stay normal numbers
+constexpr float kFirstScale = 0x1p-60f, kFirstLimit = 8 - kScaleLeast;
+__device__ __forceinline__ float scale_of(float limit) { return pow2i(8 - (int)limit); }
+// Takes the logit x and the value scale vt into a row's reference; returns the factor that
+// brings earlier sums to it.
+__device__ __forceinline__ float raise_reference(float x, float vt, float& neg_r, float& limit) {
+    const float neg_m = neg_r + (8.0f - limit);
+    const bool louder = vt > scale_of(limit);
+    if (!louder && !(-x < neg_m)) return 1.0f;
+    if (louder) limit = (float)(8 - min(max((int)(__float_as_uint(vt) >> 23) - 126, kScaleLeast), kScaleMost));
+    const float was = neg_r;
+    neg_r = fminf(neg_m, -x) - (8.0f - limit);
+    return neg_r == was ? 1.0f : ex2f(neg_r - was);
+}
 
 // Row tiles and the units of sequence b (every row tile is
 // walked over all of the sequence's tokens; what a tile may not see is skipped
@@ -450,11 +471,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
         }
 
         float o[NT][D / 16][4];
-        float2 neg_m[NT], l[NT], zs[NT];  // minus the running maximum; totals of p and of p z (this lane's tokens)
-        float S = 0.0f, inv_S = 0.0f;  // power of two not below the largest value scale seen, and its inverse
+        float2 neg_r[NT], limit[NT], l[NT], zs[NT];  // the rows' references; totals of p and of p z (this lane's tokens)
+        float S = kFirstScale;  // the least of the rows'
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            neg_m[n] = make_float2(INFINITY, INFINITY), l[n] = zs[n] = make_float2(0.0f, 0.0f);
+            neg_r[n] = make_float2(INFINITY, INFINITY), limit[n] = make_float2(kFirstLimit, kFirstLimit);
+            l[n] = zs[n] = make_float2(0.0f, 0.0f);
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
 #pragma unroll
@@ -490,7 +512,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                         for (int n = 0; n < NT; ++n)
                             mma_f16(acc[j][n], a0, a1, a2, a3, qb[n][w * 4 + h * 2], qb[n][w * 4 + h * 2 + 1]);
                     }
-            float top = -INFINITY, vtop = 0.0f, rel[2][NT][4];  // rel: logit - m
+            float rel[2][NT][4], vtop = 0.0f;  // rel: logit - reference
+            float2 top[NT];                    // a row's largest
+#pragma unroll
+            for (int n = 0; n < NT; ++n) top[n] = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int tok0 = tok_base + i * C::kTokens + j * 16;
@@ -510,50 +535,47 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                             if (none || tok0 + g + 8 * k > lim[n][1]) x.y = -INFINITY;
                         }
                         acc[j][n][2 * k] = x.x, acc[j][n][2 * k + 1] = x.y;
-                        x = add2(x, neg_m[n]);
+                        x = add2(x, neg_r[n]);
                         rel[j][n][2 * k] = x.x, rel[j][n][2 * k + 1] = x.y;
-                        top = fmaxf(top, fmaxf(x.x, x.y));
+                        top[n] = make_float2(fmaxf(top[n].x, x.x), fmaxf(top[n].y, x.y));
                     }
                     vtop = fmaxf(vtop, pair_lo(vp[j][k]));
                 }
             }
-            // The maximum need not be exact: a weight may exceed 1 by up to 2^8
-            // before the sums are rescaled (fp16 holds 2^15), so most pieces
-            // skip this.  (The first one does not: m is -inf there.)
-            if (__any_sync(0xffffffffu, top > 8.0f || vtop > S)) {
+            bool raise = vtop > S;
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
-                float fs = 1.0f;
-                if (vtop > S) {
-                    // next power of two, kept where the inverse and 2^24 times it are normal numbers
-                    const int e = min(max((int)(__float_as_uint(vtop) >> 23) - 126, -100), 102);
-                    const float was = S;
-                    S = pow2i(e);
-                    inv_S = pow2i(-e);
-                    fs = was * inv_S;
-                }
+            for (int n = 0; n < NT; ++n) raise |= top[n].x > limit[n].x || top[n].y > limit[n].y;
+            if (__any_sync(0xffffffffu, raise)) {  // (for the first piece it is true: m is -inf there)
+                S = INFINITY;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float f[2];
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         float x = fmaxf(fmaxf(acc[0][n][k], acc[0][n][2 + k]), fmaxf(acc[1][n][k], acc[1][n][2 + k]));
+                        float vt = kMask ? 0.0f : vtop;
+                        if constexpr (kMask) {  // of the tokens that the row sees
 #pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                        const float was = k ? neg_m[n].y : neg_m[n].x, now = fminf(was, -x);
-                        f[k] = now == was ? 1.0f : ex2f(now - was);
+                            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+                                    if (acc[j][n][2 * c + k] != -INFINITY) vt = fmaxf(vt, pair_lo(vp[j][c]));
+                        }
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) {
+                            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                            vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
+                        }
+                        f[k] = k ? raise_reference(x, vt, neg_r[n].y, limit[n].y) : raise_reference(x, vt, neg_r[n].x, limit[n].x);
+                        S = fminf(S, scale_of(k ? limit[n].y : limit[n].x));
+                        const float now = k ? neg_r[n].y : neg_r[n].x;
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
 #pragma unroll
                             for (int c = 0; c < 2; ++c) rel[j][n][2 * c + k] = acc[j][n][2 * c + k] + now;
-                        if (k == 0)
-                            neg_m[n].x = now;
-                        else
-                            neg_m[n].y = now;
                     }
                     l[n] = mul2(l[n], make_float2(f[0], f[1]));
                     zs[n] = mul2(zs[n], make_float2(f[0], f[1]));
-                    f[0] *= fs, f[1] *= fs;
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
@@ -564,7 +586,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint32_t pb[NT][2];
-                const float vn[2] = {pair_lo(vp[j][0]) * inv_S, pair_lo(vp[j][1]) * inv_S};
+                const float vs[2] = {pair_lo(vp[j][0]), pair_lo(vp[j][1])};
                 const float vz[2] = {pair_hi(vp[j][0]), pair_hi(vp[j][1])};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -577,11 +599,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                             const bool n0 = acc[j][n][2 * k] == -INFINITY, n1 = acc[j][n][2 * k + 1] == -INFINITY;
                             p.x = n0 ? 0.0f : p.x, p.y = n1 ? 0.0f : p.y;
                             pz = make_float2(n0 ? 0.0f : p.x * vz[k], n1 ? 0.0f : p.y * vz[k]);
-                            pv = make_float2(n0 ? 0.0f : p.x * vn[k], n1 ? 0.0f : p.y * vn[k]);
+                            pv = make_float2(n0 ? 0.0f : p.x * vs[k], n1 ? 0.0f : p.y * vs[k]);
                             zs[n] = add2(zs[n], pz);
                         } else {
                             zs[n] = fma2(p, make_float2(vz[k], vz[k]), zs[n]);
-                            pv = mul2(p, make_float2(vn[k], vn[k]));
+                            pv = mul2(p, make_float2(vs[k], vs[k]));
                         }
                         l[n] = add2(l[n], p);
                         wgt[k] = pack_f16(pv.x, pv.y);
@@ -621,7 +643,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 
         // ---- join the four warps
         float* mine = reinterpret_cast<float*>(ring);  // nothing is in flight
-        const float up = S * 16777216.0f;              // the codes' 2^-24 and the weights' scale
+        const float up = 16777216.0f;                  // the codes' 2^-24
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -640,7 +662,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                     *reinterpret_cast<float2*>(mine + r * C::kPitch + 4 * (g * W + j / 2) + 2 * (j & 1)) =
                         make_float2(fmaf(o[n][j][k], up, z), fmaf(o[n][j][2 + k], up * 0.0625f, z));
                 if (g == 0) {
-                    join_ml[(warp * RT + r) * 2] = k ? -neg_m[n].y : -neg_m[n].x;
+                    join_ml[(warp * RT + r) * 2] = k ? -neg_r[n].y : -neg_r[n].x;
                     join_ml[(warp * RT + r) * 2 + 1] = k ? l[n].y : l[n].x;
                 }
             }
@@ -776,9 +798,8 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
             if (warp * 16 + 8 + g >= sg.rows) lim[1] = w_end - 1;
         }
 
-        float o[D / 8][4], neg_m[2] = {INFINITY, INFINITY};
+        float o[D / 8][4], neg_r[2] = {INFINITY, INFINITY}, limit[2] = {kFirstLimit, kFirstLimit}, S = kFirstScale;
         float2 l[2], zs[2];
-        float S = 0.0f, inv_S = 0.0f;  // as in the decode kernel
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
 #pragma unroll
@@ -814,7 +835,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                         }
             }
             // ---- logits; columns 2t, 2t + 1 of n-tile j are tokens 8 j + 2 t, + 1
-            float top = -INFINITY, vtop = 0.0f;
+            float top[2] = {-INFINITY, -INFINITY}, vtop = 0.0f;  // as in the decode kernel
             uint2 vp[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -837,56 +858,55 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                         if (gone || tk + 1 > lim[k]) x.y = -INFINITY;
                     }
                     acc[j][2 * k] = x.x, acc[j][2 * k + 1] = x.y;
-                    const float2 d = add2(x, make_float2(neg_m[k], neg_m[k]));
-                    top = fmaxf(top, fmaxf(d.x, d.y));
+                    const float2 d = add2(x, make_float2(neg_r[k], neg_r[k]));
+                    top[k] = fmaxf(top[k], fmaxf(d.x, d.y));
                 }
                 vtop = fmaxf(vtop, fmaxf(pair_lo(vp[j].x), pair_lo(vp[j].y)));
             }
-            if (__any_sync(0xffffffffu, top > 8.0f || vtop > S)) {  // seldom: see the decode kernel
-                vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 1));
-                vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, 2));
-                float fs = 1.0f;
-                if (vtop > S) {
-                    const int e = min(max((int)(__float_as_uint(vtop) >> 23) - 126, -100), 102);
-                    const float was = S;
-                    S = pow2i(e);
-                    inv_S = pow2i(-e);
-                    fs = was * inv_S;
-                }
+            if (__any_sync(0xffffffffu, top[0] > limit[0] || top[1] > limit[1] || vtop > S)) {  // seldom
+                S = INFINITY;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    float x = -INFINITY;
+                    float x = -INFINITY, vt = kMask ? 0.0f : vtop;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x = fmaxf(x, fmaxf(acc[j][2 * k], acc[j][2 * k + 1]));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-                    const float was = neg_m[k], now = fminf(was, -x);
-                    const float f = now == was ? 1.0f : ex2f(now - was);
-                    neg_m[k] = now;
+                    for (int j = 0; j < 4; ++j) {
+                        x = fmaxf(x, fmaxf(acc[j][2 * k], acc[j][2 * k + 1]));
+                        if constexpr (kMask) {  // of the tokens that the row sees
+                            if (acc[j][2 * k] != -INFINITY) vt = fmaxf(vt, pair_lo(vp[j].x));
+                            if (acc[j][2 * k + 1] != -INFINITY) vt = fmaxf(vt, pair_lo(vp[j].y));
+                        }
+                    }
+#pragma unroll
+                    for (int d = 1; d < 4; d <<= 1) {
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                        vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
+                    }
+                    const float f = raise_reference(x, vt, neg_r[k], limit[k]);
+                    S = fminf(S, scale_of(limit[k]));
                     l[k] = mul2(l[k], make_float2(f, f));
                     zs[k] = mul2(zs[k], make_float2(f, f));
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j) o[j][2 * k] *= f * fs, o[j][2 * k + 1] *= f * fs;
+                    for (int j = 0; j < D / 8; ++j) o[j][2 * k] *= f, o[j][2 * k + 1] *= f;
                 }
             }
             // ---- weights, in place as the first operand of the output's products
             uint32_t pa[4][2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 vn = mul2(make_float2(pair_lo(vp[j].x), pair_lo(vp[j].y)), make_float2(inv_S, inv_S));
+                const float2 vs = make_float2(pair_lo(vp[j].x), pair_lo(vp[j].y));
                 const float2 vz = make_float2(pair_hi(vp[j].x), pair_hi(vp[j].y));
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const float2 d = add2(make_float2(acc[j][2 * k], acc[j][2 * k + 1]), make_float2(neg_m[k], neg_m[k]));
+                    const float2 d = add2(make_float2(acc[j][2 * k], acc[j][2 * k + 1]), make_float2(neg_r[k], neg_r[k]));
                     float2 p = make_float2(ex2f(d.x), ex2f(d.y)), pv;
                     if constexpr (kMask) {  // a token that a row does not see adds nothing, whatever its pair holds
                         const bool n0 = acc[j][2 * k] == -INFINITY, n1 = acc[j][2 * k + 1] == -INFINITY;
                         p = make_float2(n0 ? 0.0f : p.x, n1 ? 0.0f : p.y);
                         zs[k] = add2(zs[k], make_float2(n0 ? 0.0f : p.x * vz.x, n1 ? 0.0f : p.y * vz.y));
-                        pv = make_float2(n0 ? 0.0f : p.x * vn.x, n1 ? 0.0f : p.y * vn.y);
+                        pv = make_float2(n0 ? 0.0f : p.x * vs.x, n1 ? 0.0f : p.y * vs.y);
                     } else {
                         zs[k] = fma2(p, vz, zs[k]);
-                        pv = mul2(p, vn);
+                        pv = mul2(p, vs);
                     }
                     l[k] = add2(l[k], p);
                     pa[j][k] = pack_f16(pv.x, pv.y);
@@ -932,7 +952,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
         // ---- results: row g's columns 2t and 2t + 1 are 4 W dims each
         const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
-        const float up = S * 16777216.0f;
+        const float up = 16777216.0f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             float sum = l[k].x + l[k].y, z = zs[k].x + zs[k].y;
@@ -958,7 +978,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                     else
                         *reinterpret_cast<float4*>(part + r * D + d) = y;
                 }
-            if (!whole && t == 0) part[C::kRows * D + r * 2] = -neg_m[k], part[C::kRows * D + r * 2 + 1] = sum;
+            if (!whole && t == 0) part[C::kRows * D + r * 2] = -neg_r[k], part[C::kRows * D + r * 2 + 1] = sum;
         }
         if (tid == 0) attn_note(a, run, sg, unit);
         __syncthreads();  // nobody reads a stage any more
@@ -975,9 +995,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
 // tokens of a row.
 //
 // Here a row's logits stay in units of its query's scaling until the exponent (the
-// factor joins the maximum in one fma), and the largest value scale is taken into
-// the maximum: weights and totals are all relative to 2^m S, which cancels in the
-// end.
+// factor joins the reference in one fma).
 //
 // A step waits for the products of the one before, so operands and logits need no
 // second buffer; the other block of the SM fills the wait.  (One block of 16 warps
@@ -1058,7 +1076,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     __shared__ uint8_t dead[ST][4];     // pieces that are not there
-    __shared__ uint32_t v_top[2];       // largest value scale of a tile (bits)
+    __shared__ uint32_t v_top[2][2];    // largest value scale of a tile's halves (bits)
     __shared__ float ex[2][2][128];     // exchange between a row's two threads
     uint8_t* qop = smem_base + (1024 - smem_u32(smem_base) % 1024) % 1024;
     uint8_t* kop = qop + C::kQ;
@@ -1077,7 +1095,6 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         mbar_init(&bar, 1);
         fence_barrier_init();
         s_abort = 0;
-        v_top[0] = v_top[1] = 0;
     }
     tc_fence_before();
     __syncthreads();
@@ -1204,7 +1221,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 if (kv) {
                     const float top = none ? 0.0f : fmaxf(pair_lo(p), 0.0f);  // (a NaN does not count)
                     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-                    if (lane == 0) atomicMax(&v_top[i & 1], bits);
+                    if (lane == 0) v_top[i & 1][tok / 32] = bits;  // (a warp has one half's tokens)
                 }
             }
         };
@@ -1232,14 +1249,13 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 mma4_ss_warp(tm + C::kColS, q_lo + k * (16384 >> 4), k_lo + k * (C::kTokens * 128 >> 4), C::kIdescS, k);
         };
 
-        float neg_m = INFINITY;  // minus the row's running maximum
-        float S = 0.0f, log_S = 0.0f;  // power of two not below the largest value scale seen
+        float neg_r = INFINITY, limit = kFirstLimit, S = kFirstScale;  // the row's reference
         float2 l2 = make_float2(0.0f, 0.0f), z2 = make_float2(0.0f, 0.0f);  // sums over this thread's tokens
         float2 x[16];
         // weights of tile i into tensor memory; kMask: some token is not seen by some row
         auto weights = [&](const float* pk, auto mask) {
             constexpr bool kMask = decltype(mask)::value;
-            const float2 m2 = make_float2(neg_m - log_S, neg_m - log_S), ca2 = make_float2(ca, ca);
+            const float2 m2 = make_float2(neg_r, neg_r), ca2 = make_float2(ca, ca);
             uint32_t pw[16];
 #pragma unroll
             for (int k = 0; k < 16; k += 2) {
@@ -1301,7 +1317,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             }
             const float* pk = pairs + b * 4 * C::kTokens + tq * 32;
             const int tok = tok_base + i * C::kTokens + tq * 32;
-            float top = -INFINITY;
+            float top = -INFINITY, vt = __uint_as_float(v_top[b][tq]);
             const float2 cb2 = make_float2(cb, cb);
             const bool lost = pk[C::kTokens] == INFINITY || pk[C::kTokens + 16] == INFINITY;
 #pragma unroll
@@ -1323,21 +1339,24 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
             top *= ca;
-            const float vt = __uint_as_float(v_top[b]);
             cp_wait<1>();  // tile i + 1 (visible to all behind the barrier)
-            if (__syncthreads_or(top + neg_m > 8.0f || vt > S)) {  // seldom: see the decode kernel
+            if (__syncthreads_or(top + neg_r > limit || vt > S)) {  // seldom
+                if (mask) {  // the scales of the tokens that the row sees
+                    vt = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 vs = *reinterpret_cast<const float2*>(pk + 2 * C::kTokens + 2 * k);
+                        if (x[k].x != -INFINITY) vt = fmaxf(vt, vs.x);
+                        if (x[k].y != -INFINITY) vt = fmaxf(vt, vs.y);
+                    }
+                }
                 ex[0][tq][row] = top;
+                ex[1][tq][row] = vt;
                 __syncthreads();
                 top = fmaxf(ex[0][0][row], ex[0][1][row]);
-                float fs = 1.0f;
-                if (vt > S) {
-                    const int e = min(max((int)(__float_as_uint(vt) >> 23) - 126, -100), 100);
-                    fs = ex2f(log_S - (float)e);  // (before the first: weights relative to 1)
-                    S = pow2i(e);
-                    log_S = (float)e;
-                }
-                const float now = fminf(neg_m, -top), f = (now == neg_m ? 1.0f : ex2f(now - neg_m)) * fs;
-                neg_m = now;
+                vt = fmaxf(ex[1][0][row], ex[1][1][row]);
+                const float f = raise_reference(top, vt, neg_r, limit);
+                S = scale_of(limit);
                 l2 = mul2(l2, make_float2(f, f));
                 z2 = mul2(z2, make_float2(f, f));
                 if (i > 0) {  // the output so far
@@ -1353,7 +1372,6 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                     tmem_wait_st();
                 }
             }
-            if (tid == 0) v_top[b] = 0;  // all have read it
             if (mask)
                 weights(pk, std::true_type{});
             else
@@ -1412,7 +1430,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 }
             }
         }
-        if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = log_S - neg_m, part[C::kRows * D + row * 2 + 1] = l;
+        if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = -neg_r, part[C::kRows * D + row * 2 + 1] = l;
         if (tid == 0) attn_note(a, run, sg, unit);
         tc_fence_before();
         __syncthreads();

@@ -153,7 +153,11 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     Query heads are a multiple of the cache's kv heads; head h reads kv head
     h // (heads / kv heads).  scale > 0 defaults to head_dim ** -0.5.  A row that sees
     nothing gives zeros.  out: a contiguous tensor to write to; rows of it
-    behind cu_q[B] are left as they were (zeros where no out is given)."""
+    behind cu_q[B] are left as they were (zeros where no out is given).
+
+    The products take 11 bits of fp32 queries (all of bf16 ones) and 11 of a token's
+    weight times its value scale, relative to the largest such scale that the row
+    sees; sums and the softmax are fp32."""
     assert q.is_cuda and q.dtype in _FLOATS, "kv4_attention takes bfloat16 or float32 CUDA queries"
     D = q.shape[-1]
     dev = q.get_device()

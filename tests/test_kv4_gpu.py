@@ -518,6 +518,50 @@ def test_many_row_tiles_captured(cuda_device, rows):
         want = pc.kv4_attention(q, s.cache, s.table, s.lens)
 
 
+def check_rows_apart(y, q, k, v):
+    """Every row against the tokens that it sees, as if there were no others: the
+    oracle's bound then knows the value ranges of these alone."""
+    r, n = q.shape[0], k.shape[0]
+    for i in range(max(r - n, 0), r):
+        end = n - r + i + 1
+        want, bound = oracle.attention(q[i:i + 1], k[:end], v[:end])
+        assert ((y[i].double().cpu() - want[0]).abs() <= bound[0] + 2.0 ** -8 * (want[0].abs() + bound[0])).all(), i
+
+
+@pytest.mark.parametrize("d,rows,G", [(64, 6, 1), (128, 7, 1), (64, 5, 3), (128, 4, 4), (128, 30, 4), (64, 150, 1)])
+def test_values_that_a_row_does_not_see(cuda_device, d, rows, G):
+    """However large, they cost it nothing (few row tiles)."""
+    lengths = [rows, rows + 40, 200, 333]
+    s = Batch(lengths, 2, d, 16, cuda_device, seed=rows + d)
+    for i, n in enumerate(lengths):
+        for back, up in ((1, 2.0 ** 27), (2, 2.0 ** 24), (3, 2.0 ** 20), (4, 2.0 ** 12)):
+            s.v[i][n - back] *= up
+    s.store(lengths)
+    q = torch.randn(4, rows, 2 * G, d, generator=torch.Generator().manual_seed(rows)).to(torch.bfloat16)
+    y = pc.kv4_attention(q.to(cuda_device), s.cache, s.table, s.lens)
+    for i in range(4):
+        check_rows_apart(y[i], q[i], s.k[i], s.v[i])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [12, 21])
+def test_values_that_a_row_does_not_see_many_row_tiles(cuda_device, d, rows):
+    s = wide(cuda_device, d, rows)
+    for i, n in enumerate(s.lengths):
+        for back in range(1, min(rows, n)):
+            s.v[i][n - back] *= 2.0 ** (9 * (-back % 4))  # up to 2^27 between rows of one warp
+    s.store(s.lengths)
+    q = torch.randn(32, rows, 32, d, generator=torch.Generator().manual_seed(rows)).to(torch.bfloat16)
+    y = pc.kv4_attention(q.to(cuda_device), s.cache, s.table, s.lens)
+    for i in range(8):
+        check_rows_apart(y[i], q[i], s.k[i], s.v[i])
+    # the same rows before the last token is there
+    s.lens -= 1
+    again = pc.kv4_attention(q[:, :-1].contiguous().to(cuda_device), s.cache, s.table, s.lens)
+    for i in range(8):
+        check_rows_apart(again[i], q[i, :-1], s.k[i][:-1], s.v[i][:-1])
+
+
 def test_calls_of_several_threads(cuda_device):
     """Each on a stream of its own, all kernels at once: every call gives its own result."""
     s = wide(cuda_device, 128, 21)
