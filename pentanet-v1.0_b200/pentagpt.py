@@ -102,7 +102,12 @@ class _Block(nn.Module):
 class PentaGPTCache:
     """The past tokens of a batch: a 4-bit cache per layer (penta_cache), their
     pages and the sequences' lengths.  The pages are handed out up front;
-    seq_lens lives on the GPU, so a captured step goes on where it stands."""
+    seq_lens lives on the GPU, so a captured step goes on where it stands.
+
+    A capture stores nothing, and replays advance seq_lens alone; so once a step
+    was captured over the cache, eager calls read the length from there (a
+    synchronisation each).  A replay past the capacity stores no more tokens and
+    shows in penta_native.device_status()."""
 
     def __init__(self, cfg: PentaGPTConfig, batch: int, device, max_tokens: int | None = None, page_size: int = 64):
         self.capacity = cfg.block_size if max_tokens is None else max_tokens
@@ -111,10 +116,25 @@ class PentaGPTCache:
                        for _ in range(cfg.n_layer)]
         self.block_table = torch.arange(batch * pages, dtype=torch.int32, device=device).view(batch, pages)
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
-        self.length = 0  # what the host knows: tokens appended so far
+        self.length = 0  # what the host knows: tokens appended so far (of the longest sequence)
+        self.captured = False  # replays may have advanced seq_lens since
+
+    def known_length(self) -> int:
+        """length, brought up to what replays of captured steps left on the GPU (not
+        while a step is being captured)."""
+        if self.captured and self.seq_lens.numel() and not torch.cuda.is_current_stream_capturing():
+            self.length = int(self.seq_lens.max())
+        return self.length
+
+    def rewind(self, length: int) -> None:
+        """Forget the tokens behind the first `length` of each sequence (their pages
+        are written over)."""
+        assert length >= 0
+        self.length = min(self.known_length(), length)
+        self.seq_lens.clamp_(max=length)
 
     def reset(self) -> None:
-        """Forget all tokens (their pages are written over)."""
+        """Forget all tokens."""
         self.seq_lens.zero_()
         self.length = 0
 
@@ -165,18 +185,35 @@ class PentaGPTFast(nn.Module):
     def forward(self, idx: torch.Tensor, all_logits: bool = False, cache: PentaGPTCache | None = None) -> torch.Tensor:
         """Logits of the last position (all with all_logits).  With a cache, idx
         holds the tokens that follow those in it; their keys and values are added
-        and attention runs over the cache."""
+        and attention runs over the cache.  Where that raises, none were added."""
         B, T = idx.shape
         if cache is None:
             assert T <= self.cfg.block_size
-            pos = torch.arange(T, device=idx.device)
+            return self._logits(idx, torch.arange(T, device=idx.device), all_logits)
+        assert B == cache.seq_lens.shape[0], f"{B} sequences, the cache holds {cache.seq_lens.shape[0]}"
+        assert cache.known_length() + T <= min(cache.capacity, self.cfg.block_size), "the cache is full"
+        return self._append(idx, cache, all_logits)
+
+    def _append(self, idx: torch.Tensor, cache: PentaGPTCache, all_logits: bool = False) -> torch.Tensor:
+        T = idx.shape[1]
+        capturing = torch.cuda.is_current_stream_capturing()
+        # (a captured step replayed past the block stays at its last position)
+        pos = (cache.seq_lens[:, None] + torch.arange(T, device=idx.device)).clamp(max=self.cfg.block_size - 1)
+        cache.seq_lens += T
+        try:
+            logits = self._logits(idx, pos, all_logits, cache)
+        except BaseException:
+            if not capturing:
+                cache.seq_lens -= T
+            raise
+        if capturing:
+            cache.captured = True
         else:
-            assert B == cache.seq_lens.shape[0], f"{B} sequences, the cache holds {cache.seq_lens.shape[0]}"
-            assert cache.length + T <= min(cache.capacity, self.cfg.block_size), "the cache is full"
-            # (a captured step replayed past the block stays at its last position)
-            pos = (cache.seq_lens[:, None] + torch.arange(T, device=idx.device)).clamp(max=self.cfg.block_size - 1)
-            cache.seq_lens += T
             cache.length += T
+        return logits
+
+    def _logits(self, idx: torch.Tensor, pos: torch.Tensor, all_logits: bool, cache: PentaGPTCache | None = None
+                ) -> torch.Tensor:
         x = (self.wte(idx) + self.wpe(pos)).to(torch.bfloat16)
         for i, block in enumerate(self.h):
             x = block(x) if cache is None else block(x, cache.layers[i], cache)
@@ -196,11 +233,12 @@ class PentaGPTFast(nn.Module):
         B, T = idx.shape
         assert T >= 1 and max_new_tokens >= 0
         cache = cache if cache is not None else self.new_cache(B, min(T + max_new_tokens, self.cfg.block_size))
-        assert cache.length + T + max(max_new_tokens - 1, 0) <= min(cache.capacity, self.cfg.block_size), \
-            f"{cache.length} + {T} + {max_new_tokens} tokens do not fit the model's block or the cache"
+        held = cache.known_length()
+        assert held + T + max(max_new_tokens - 1, 0) <= min(cache.capacity, self.cfg.block_size), \
+            f"{held} + {T} + {max_new_tokens} tokens do not fit the model's block or the cache"
         out = [idx]
         u = torch.rand(max_new_tokens, B, device=idx.device, generator=generator)
         for i in range(max_new_tokens):
-            logits = self(out[-1].clamp(min=0), cache=cache)  # -1: a row of NaN logits has no token
+            logits = self._append(out[-1].clamp(min=0), cache)  # -1: a row of NaN logits has no token
             out.append(pk.sample_tokens(logits[:, 0], u[i], temperature, top_k, top_p, min_p)[:, None])
         return torch.cat(out, dim=1)

@@ -8,6 +8,7 @@ import torch
 import torch.nn.functional as F
 
 import penta_kernel as pk
+import penta_native as nat
 from pentagpt import PentaGPTConfig, PentaGPTFast
 
 pytestmark = pytest.mark.gpu
@@ -244,3 +245,71 @@ def test_captured_decode_step(cuda_device):
         graph.replay()
         got.append(tok.clone())
     assert torch.equal(torch.cat(got, 1), want[:, 16:])
+
+
+def _small(device):
+    cfg = PentaGPTConfig(n_layer=2, n_head=2, n_embd=128, block_size=96, vocab_size=700)
+    return PentaGPTFast.random(cfg, seed=3, device=device)
+
+
+def test_cache_after_replays(cuda_device):
+    """Replays advance the lengths on the GPU alone; eager calls after them go on from
+    there, and know when the cache is full."""
+    model = _small(cuda_device)
+    idx = torch.randint(0, 700, (2, 15), generator=torch.Generator().manual_seed(5)).to(cuda_device)
+    want = model.generate(idx, 12, temperature=0.0)
+    cache = model.new_cache(2, 24)
+    tok, u = model.generate(idx, 1, temperature=0.0, cache=cache)[:, -1:].clone(), torch.zeros(2, device=cuda_device)
+    first = tok.clone()
+
+    def step():
+        tok.copy_(pk.sample_tokens(model(tok, cache=cache)[:, 0], u, temperature=0.0)[:, None])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert cache.length == 16
+    cache.rewind(15)
+    assert cache.length == 15 and cache.seq_lens.tolist() == [15, 15]
+    tok.copy_(first)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    assert cache.length == 15  # nothing was stored
+    got = [first]
+    for _ in range(5):
+        graph.replay()
+        got.append(tok.clone())
+    for i in range(4):  # eager
+        step()
+        got.append(tok.clone())
+        assert cache.length == 21 + i and cache.seq_lens.tolist() == [21 + i] * 2
+    assert torch.equal(torch.cat(got, 1), want[:, 15:25])
+    with pytest.raises(AssertionError, match="do not fit"):
+        model.generate(tok, 2, cache=cache)
+    assert cache.length == 24
+    with pytest.raises(AssertionError, match="full"):
+        model(tok, cache=cache)
+    assert cache.seq_lens.tolist() == [24, 24] and nat.device_status() == 0
+
+
+def test_cache_after_a_block_that_raises(cuda_device, monkeypatch):
+    """Tokens without keys are not counted."""
+    model = _small(cuda_device)
+    idx = torch.randint(0, 700, (2, 15), generator=torch.Generator().manual_seed(5)).to(cuda_device)
+    cache = model.new_cache(2)
+    want = model(idx, cache=cache), model(idx[:, :3], cache=cache)
+    cache.reset()
+    assert torch.equal(model(idx, cache=cache), want[0])
+
+    def broken(*args):
+        raise RuntimeError("out of something")
+
+    with monkeypatch.context() as m:
+        m.setattr(model.h[1], "forward", broken)
+        with pytest.raises(RuntimeError, match="something"):
+            model(idx[:, 3:9], cache=cache)
+    assert cache.length == 15 and cache.seq_lens.tolist() == [15, 15]
+    assert torch.equal(model(idx[:, :3], cache=cache), want[1])
