@@ -229,7 +229,12 @@ class PentaGPTFast(nn.Module):
         max_new_tokens).  The settings are those of penta_kernel.sample_tokens
         (temperature=0: the most likely token), its uniform numbers come from
         `generator`.  With a cache from an earlier call, idx holds what follows
-        the tokens in it (the last token returned is not in it yet)."""
+        the tokens in it (the last token returned is not in it yet).
+
+        Past keys and values are held in 4 bits, which costs accuracy (attention
+        outputs move by 13 % in norm and more; penta_cache says what that depends
+        on): forward(idx) over the whole prefix is the way to bf16 attention.  Heads of
+        64 or 128 dims."""
         B, T = idx.shape
         assert T >= 1 and max_new_tokens >= 0
         cache = cache if cache is not None else self.new_cache(B, min(T + max_new_tokens, self.cfg.block_size))

@@ -413,6 +413,40 @@ def test_no_sequences(cuda_device):
     assert nat.device_status() == 0
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("loud", [1.0, 5.0, 12.0])
+def test_what_four_bits_cost(cuda_device, d, loud):
+    """Against attention over the keys and values as they were given, before rounding to 4 bits.
+
+    Rounding moves each value by an error of variance s^2 / 12.  A logit then moves by D of
+    variance (scale |q| s_k)^2 / 12 and its weight by the factor 1 + D, so with independent
+    errors the output sum_t p_t v_t moves by sum_t p_t (D_t v_t + e_t): relative to p_t and
+    the values' mean square, by D^2 + s_v^2 / (12 mean v^2) in the square.  The bound allows a
+    quarter more than that root (products of the two, the exponential's curvature)."""
+    n, hk, G, rows = 1024, 2, 4, 8
+    s = Batch([n], hk, d, 64, cuda_device, seed=3)
+    g = torch.Generator().manual_seed(11)
+    k, v = (torch.randn(n, hk, d, generator=g) for _ in range(2))
+    k[:, :, [3, d // 2]] *= loud
+    s.k, s.v = [k.to(torch.bfloat16)], [v.to(torch.bfloat16)]
+    s.store([n])
+    q = torch.randn(rows, hk * G, d, generator=g).to(torch.bfloat16)
+    cu = torch.tensor([0, rows], dtype=torch.int32, device=cuda_device)
+    y = pc.kv4_attention(q.to(cuda_device), s.cache, s.table, s.lens, cu_q=cu).double().cpu().view(rows, hk, G, d)
+    qq, kk, vv = q.double().view(rows, hk, G, d), s.k[0].double(), s.v[0].double()
+    logit = torch.einsum("rhgd,nhd->hgrn", qq, kk) * d ** -0.5
+    logit.masked_fill_(torch.arange(n) > (n - rows + torch.arange(rows))[:, None], -float("inf"))
+    p = torch.softmax(logit, -1)
+    want = torch.einsum("hgrn,nhd->rhgd", p, vv)
+    sk, sv = (oracle.quantise(x)[1].double() for x in (s.k[0], s.v[0]))  # (n, hk)
+    moved = qq.square().sum(-1).permute(1, 2, 0)[..., None] / d * (sk * sk).t()[:, None, None] / 12  # D^2: (hk, G, rows, n)
+    part = moved + ((sv * sv).t() / (12 * vv.square().mean((0, 2)))[:, None])[:, None, None]
+    part = (p * p * part).sum() / (p * p).sum()
+    off, cost = ((y - want).norm() / want.norm()).item(), 1.25 * part.sqrt().item()
+    print(f"\n4 bits, head_dim {d}, two key dims {loud:g}x louder: {off:.3f} of the output's norm (bound {cost:.3f})")
+    assert off <= cost
+
+
 # Calls of many row tiles (more than four per SM) take larger ones: 64 rows up to 64 rows
 # per sequence and head (here 12 x 4), 128 above (21 x 4).
 def wide(device, d, rows, **kw):

@@ -313,3 +313,24 @@ def test_cache_after_a_block_that_raises(cuda_device, monkeypatch):
             model(idx[:, 3:9], cache=cache)
     assert cache.length == 15 and cache.seq_lens.tolist() == [15, 15]
     assert torch.equal(model(idx[:, :3], cache=cache), want[1])
+
+
+def test_what_the_cache_costs(cuda_device):
+    """Logits over the 4-bit cache against those of forward(idx), whose attention is bf16.
+
+    Attention outputs move by 13 % in norm for keys and values without loud dims (see
+    test_kv4_gpu.test_what_four_bits_cost), and with them what attention adds to the logits:
+    bounded here by a fifth of the difference that leaving it out makes, plus 2^-7 of the
+    logits for the bf16 roundings that differ (some ten per layer, 2^-9 each, as a root of
+    their sum of squares)."""
+    model = _small(cuda_device)
+    idx = torch.randint(0, 700, (3, 83), generator=torch.Generator().manual_seed(1)).to(cuda_device)
+    dense = model(idx, all_logits=True).double()
+    cached = model(idx, all_logits=True, cache=model.new_cache(3)).double()
+    hooks = [b.attn_proj.register_forward_hook(lambda m, args, y: torch.zeros_like(y)) for b in model.h]
+    without = model(idx, all_logits=True).double()
+    for h in hooks:
+        h.remove()
+    off, share = (cached - dense).norm() / dense.norm(), (without - dense).norm() / dense.norm()
+    print(f"\nlogits over the 4-bit cache: {off:.4f} of their norm from forward(idx); attention adds {share:.4f}")
+    assert off <= 0.2 * share + 2.0 ** -7
