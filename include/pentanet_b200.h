@@ -339,9 +339,9 @@ int pn_kv4_gather(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t 
  * h / (q_heads / kv_heads).  The logits are scale * q . k, scale > 0.
  * Queries enter the products as fp16 relative to the row's largest (bf16 ones
  * exactly down to 2^-28 of it; magnitudes from 2^116 on overflow), a token's weight
- * times its value scale s as fp16 relative to the largest s among the tokens that the
- * row sees (and to 2^-60 at least; s from 2^115 on overflows): what is below 2^-24 of
- * that is lost.  Sums and the softmax are fp32.
+ * times its value scale s as fp16: 11 bits down to 2^-20 of the largest s among the tokens
+ * that the row sees (counted as 2^-54 at least; s from 2^107 on overflows), fewer below, none
+ * below 2^-31.  Sums and the softmax are fp32.
  * Workspace: pn_kv4_attention_workspace_size bytes, 256-byte aligned, no
  * initialisation needed; calls that may overlap need one each. */
 size_t pn_kv4_attention_workspace_size(int64_t B, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim);

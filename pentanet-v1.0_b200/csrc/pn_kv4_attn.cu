@@ -99,22 +99,25 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
-// A row's reference, 2^m S: m its running maximum, S a power of two not below the value
-// scales of the tokens that it has seen (and no others: what a row may not see must not cost
-// it bits).  Weights, totals and outputs are relative to it, so that the weights times the
-// value scales fit fp16.  neg_r is minus its logarithm.  The maximum need not be exact: a
-// weight may exceed 1 / S by up to 2^8 before the sums are rescaled (fp16 holds 2^15), so most
-// tokens skip that; `limit`, 8 - log2 S, is what a logit may exceed the reference by.
+// A row's reference, 2^m S: m its running maximum, S a power of two 2^6 to 2^7 below the
+// largest value scale of the tokens that it has seen (and of no others: what a row may not
+// see must not cost it bits).  Weights, totals and outputs are relative to it.  neg_r is minus
+// its logarithm.  The maximum need not be exact: a weight may exceed 1 / S by up to 2^8 before
+// the sums are rescaled, so most tokens skip that; weights times value scales then stay below
+// 2^15 in fp16, with the smallest ones as far above its last bit, 2^-24, as that allows.
+// `limit`, 8 - log2 S, is what a logit may exceed the reference by.
 constexpr int kScaleLeast = -60, kScaleMost = 100;  // exponents of S: sums of weights over 2^30 tokens stay normal numbers
-constexpr float kFirstScale = 0x1p-60f, kFirstLimit = 8 - kScaleLeast;
-__device__ __forceinline__ float scale_of(float limit) { return pow2i(8 - (int)limit); }
+constexpr float kFirstLimit = 8 - kScaleLeast;
+// The value scale from which on S is raised.
+__device__ __forceinline__ float loud_of(float limit) { return pow2i(15 - (int)limit); }
+constexpr float kFirstLoud = 0x1p-53f;  // loud_of(kFirstLimit)
 // Takes the logit x and the value scale vt into a row's reference; returns the factor that
 // brings earlier sums to it.
 __device__ __forceinline__ float raise_reference(float x, float vt, float& neg_r, float& limit) {
     const float neg_m = neg_r + (8.0f - limit);
-    const bool louder = vt > scale_of(limit);
+    const bool louder = vt >= loud_of(limit);
     if (!louder && !(-x < neg_m)) return 1.0f;
-    if (louder) limit = (float)(8 - min(max((int)(__float_as_uint(vt) >> 23) - 126, kScaleLeast), kScaleMost));
+    if (louder) limit = (float)(8 - min(max((int)(__float_as_uint(vt) >> 23) - 133, kScaleLeast), kScaleMost));
     const float was = neg_r;
     neg_r = fminf(neg_m, -x) - (8.0f - limit);
     return neg_r == was ? 1.0f : ex2f(neg_r - was);
@@ -472,7 +475,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 
         float o[NT][D / 16][4];
         float2 neg_r[NT], limit[NT], l[NT], zs[NT];  // the rows' references; totals of p and of p z (this lane's tokens)
-        float S = kFirstScale;  // the least of the rows'
+        float loud = kFirstLoud;  // the least of the rows'
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             neg_r[n] = make_float2(INFINITY, INFINITY), limit[n] = make_float2(kFirstLimit, kFirstLimit);
@@ -542,11 +545,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                     vtop = fmaxf(vtop, pair_lo(vp[j][k]));
                 }
             }
-            bool raise = vtop > S;
+            bool raise = vtop >= loud;
 #pragma unroll
             for (int n = 0; n < NT; ++n) raise |= top[n].x > limit[n].x || top[n].y > limit[n].y;
             if (__any_sync(0xffffffffu, raise)) {  // (for the first piece it is true: m is -inf there)
-                S = INFINITY;
+                loud = INFINITY;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float f[2];
@@ -567,7 +570,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                             vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
                         }
                         f[k] = k ? raise_reference(x, vt, neg_r[n].y, limit[n].y) : raise_reference(x, vt, neg_r[n].x, limit[n].x);
-                        S = fminf(S, scale_of(k ? limit[n].y : limit[n].x));
+                        loud = fminf(loud, loud_of(k ? limit[n].y : limit[n].x));
                         const float now = k ? neg_r[n].y : neg_r[n].x;
 #pragma unroll
                         for (int j = 0; j < 2; ++j)
@@ -798,7 +801,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
             if (warp * 16 + 8 + g >= sg.rows) lim[1] = w_end - 1;
         }
 
-        float o[D / 8][4], neg_r[2] = {INFINITY, INFINITY}, limit[2] = {kFirstLimit, kFirstLimit}, S = kFirstScale;
+        float o[D / 8][4], neg_r[2] = {INFINITY, INFINITY}, limit[2] = {kFirstLimit, kFirstLimit}, loud = kFirstLoud;
         float2 l[2], zs[2];
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
@@ -863,8 +866,8 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                 }
                 vtop = fmaxf(vtop, fmaxf(pair_lo(vp[j].x), pair_lo(vp[j].y)));
             }
-            if (__any_sync(0xffffffffu, top[0] > limit[0] || top[1] > limit[1] || vtop > S)) {  // seldom
-                S = INFINITY;
+            if (__any_sync(0xffffffffu, top[0] > limit[0] || top[1] > limit[1] || vtop >= loud)) {  // seldom
+                loud = INFINITY;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     float x = -INFINITY, vt = kMask ? 0.0f : vtop;
@@ -882,7 +885,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                         vt = fmaxf(vt, __shfl_xor_sync(0xffffffffu, vt, d));
                     }
                     const float f = raise_reference(x, vt, neg_r[k], limit[k]);
-                    S = fminf(S, scale_of(limit[k]));
+                    loud = fminf(loud, loud_of(limit[k]));
                     l[k] = mul2(l[k], make_float2(f, f));
                     zs[k] = mul2(zs[k], make_float2(f, f));
 #pragma unroll
@@ -1249,7 +1252,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 mma4_ss_warp(tm + C::kColS, q_lo + k * (16384 >> 4), k_lo + k * (C::kTokens * 128 >> 4), C::kIdescS, k);
         };
 
-        float neg_r = INFINITY, limit = kFirstLimit, S = kFirstScale;  // the row's reference
+        float neg_r = INFINITY, limit = kFirstLimit, loud = kFirstLoud;  // the row's reference
         float2 l2 = make_float2(0.0f, 0.0f), z2 = make_float2(0.0f, 0.0f);  // sums over this thread's tokens
         float2 x[16];
         // weights of tile i into tensor memory; kMask: some token is not seen by some row
@@ -1340,7 +1343,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
             top *= ca;
             cp_wait<1>();  // tile i + 1 (visible to all behind the barrier)
-            if (__syncthreads_or(top + neg_r > limit || vt > S)) {  // seldom
+            if (__syncthreads_or(top + neg_r > limit || vt >= loud)) {  // seldom
                 if (mask) {  // the scales of the tokens that the row sees
                     vt = 0.0f;
 #pragma unroll
@@ -1356,7 +1359,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 top = fmaxf(ex[0][0][row], ex[0][1][row]);
                 vt = fmaxf(ex[1][0][row], ex[1][1][row]);
                 const float f = raise_reference(top, vt, neg_r, limit);
-                S = scale_of(limit);
+                loud = loud_of(limit);
                 l2 = mul2(l2, make_float2(f, f));
                 z2 = mul2(z2, make_float2(f, f));
                 if (i > 0) {  // the output so far

@@ -596,6 +596,19 @@ def test_values_that_a_row_does_not_see_many_row_tiles(cuda_device, d, rows):
         check_rows_apart(again[i], q[i, :-1], s.k[i][:-1], s.v[i][:-1])
 
 
+@pytest.mark.parametrize("rows,G", [(1, 4), (2, 4), (2, 8), (2, 40)])
+def test_quiet_values_beside_loud_ones(cuda_device, rows, G):
+    """A few tokens whose values lie 2^16 to 2^24 below those of others but carry the weight:
+    within the bound that counts an error of 2^-25 of the largest scale per token."""
+    lengths = [2 + i % 5 for i in range(96)]
+    s = Batch(lengths, 3, 64, 16, cuda_device, seed=G)
+    for i, n in enumerate(lengths):
+        s.v[i][i % n] *= 2.0 ** (16 + i % 9)
+        s.v[i] *= 2.0 ** -20
+    s.store(lengths)
+    s.attend([rows] * 96, G, scale=1.0, seed=G)
+
+
 def test_calls_of_several_threads(cuda_device):
     """Each on a stream of its own, all kernels at once: every call gives its own result."""
     s = wide(cuda_device, 128, 21)
