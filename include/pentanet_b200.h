@@ -300,7 +300,8 @@ int pn_dequant_act_i8(const int8_t *xq, int64_t xq_pitch, const float *s_x, int6
  * of token 2i + 1 in its high half, four bits per dim, the first dim lowest.
  * z is the vector's minimum rounded down to bf16, s = (max - z) / 15 rounded up
  * to bf16, c = clamp(rint((x - z) / s), 0, 15) in fp32; a vector that holds an
- * inf or NaN reads back as NaN.  head_dim: 64 or 128.  page: a multiple of 16.
+ * inf or NaN, or whose z or s is no finite number, reads back as NaN.  head_dim: 64 or 128.
+ * page: a multiple of 16.
  *
  * block_table: (B, table_w) int32, rows table_ld apart: entry i of sequence b is
  * the page of its positions [i * page, (i + 1) * page).  seq_lens: (B) int32, the

@@ -261,7 +261,8 @@ __device__ __forceinline__ float2 kv4_range(const Raw8<__nv_bfloat16> (&x)[2]) {
 // D / 16 lanes per vector, sixteen dims each; a block takes a few rows with all
 // their heads, the next vector's values in flight while one is stored.  One read
 // of the inputs; what bounds it beside the bytes is the instructions per vector
-// (the range's shuffles, scale, codes and addresses).  9723 bf16 rows of 8 heads,
+// (the range's shuffles, scale, codes and addresses: 61 % of the issue slots) and the
+// barrier behind each block's look-up, its largest stall.  9723 bf16 rows of 8 heads,
 // d = 128: 21 us, 2.4 TB/s (8 us at the copy's rate); with eight dims per lane, 233
 // instructions per eight values, it took 26 us.
 template <typename T, int D>
@@ -342,8 +343,9 @@ struct Kv4GatherArgs {
 };
 
 // The reverse, zeros for rows that are not there: a code is masked into the low
-// bits of 2^23, one fma per value.  Bound by the bytes written and, as the append, by the
-// instructions per vector; the same rows 15 us, 3.4 TB/s.
+// bits of 2^23, one fma per value.  Bound by latency: the rows' look-up, a barrier and the
+// codes' loads stand before a block's first store (43 % of the issue slots used); the same
+// rows 15.3 us, 3.4 TB/s.
 template <int D>
 __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4GatherArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");

@@ -343,12 +343,16 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
     cb = a.scale_log2 * (sum * pow2i(-e));
 }
 
-// What bounds the decode kernel: not the cache's bytes but unpacking them, about 270
-// instructions per piece of 16 tokens and warp (d = 128, up to 8 rows: 64 masks and
-// shifts, 32 products, the softmax of 16 x 8 logits), issued at two per cycle and SM.
-// 32 sequences of up to 8191 tokens, 8 heads: 48 us, 3.3 TB/s; one of 131072: 41 us,
+// What bounds the decode kernel: neither the cache's bytes nor a pipe, but latency.  A
+// piece of 16 tokens takes a warp about 260 instructions (d = 128, up to 8 rows: 64 masks
+// and shifts, 32 products, the softmax of 16 x 8 logits), each waiting for the one
+// before, and the registers leave room for twelve warps to an SM: they issue 1.9
+// instructions of four possible per cycle, the ALU pipe is 45 % and the tensor
+// pipe 24 % busy.
+// 32 sequences of up to 8191 tokens, 8 heads: 49 us, 3.3 TB/s; one of 131072: 41 us,
 // 3.4 TB/s (half of the copy's rate).  Three blocks of six stages per SM: two, four or
-// five blocks, and more stages in two, are all slower.
+// five blocks, and more stages in two, are all slower.  With 16 rows at d = 128 the
+// registers do not suffice (372 bytes spilled per thread).
 template <int D, int NT>
 struct AttnCfg {
     static constexpr int W = D / 32;             // words per thread and token
@@ -714,9 +718,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 //
 // What bounds it: m16n8k16 runs at one per ten cycles on each quarter of an SM
 // (measured; 460 TFLOP/s over the device), 128 of them to a warp's 64 tokens at
-// d = 128, against 320 mask and shift instructions at two cycles each.  64
-// sequences x 64 rows x 4 heads over 1024 tokens: 72 us (two blocks to an SM: 2 %
-// slower than three).
+// d = 128, and 320 mask and shift instructions; but the tensor pipe is only 34 % busy
+// and 41 % of the issue slots are used: as in the decode kernel the warps (twelve to
+// an SM) wait for their own last instruction.  64 sequences x 64 rows x 4 heads over 1024
+// tokens: 72 us (two blocks to an SM: 2 % slower than three); 148 bytes spilled per thread.
 template <int D>
 struct ChunkCfg {
     static constexpr int W = D / 32;
@@ -1006,10 +1011,11 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
 // chunks of 1 to 512 tokens: its warps met at five barriers per step with
 // nothing else to run.)
 //
-// What bounds it: the softmax's and the spreading's instructions, about 500 per
-// thread and step (3500 to 4500 cycles for an SM's two blocks); the products take
+// What bounds it: the latency of the softmax's and the spreading's instructions, about
+// 500 per thread and step, which all warps do in turn between the block's barriers (3500 to
+// 4500 cycles for an SM's two blocks, 47 % of the issue slots used); the products take
 // 512 cycles of a step at the tensor core's rate.  16 sequences x 512 rows x 8
-// heads over 1024 tokens: 120 us (the chunk kernel 165).
+// heads over 1024 tokens: 115 us (the chunk kernel 146).
 template <int D>
 struct TcCfg {
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
@@ -1529,20 +1535,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 // cache more often, but gives the SMs more to share: up to four tiles of 16 rows
 // per SM the 16-row kernel wins whatever the number of rows, from eight per SM
 // on the larger one of the others.  In us for d = 128 (16 rows / chunk / tcgen05):
-//   4 sequences x 128 rows x 8 heads of 2048 tokens (256 tiles)      44 /  63 /  92
-//   one prompt of 500 tokens, 512 rows x 8 heads (256 tiles)         28 /  44 /  70
-//   8 x 144 x 8 heads of 2048 tokens (576 tiles)                     72 /  78 /  78
-//   one prompt of 768 tokens, 12 heads (576 tiles)                   37 /  39 /  71
-//   64 x 96 x 2 heads of 1024 tokens (768 tiles)                     61 /  64 /  66
-//   32 prompts of 24 tokens, 12 heads (768 tiles)                    22 /  12 /  19
-//   64 x 64 x 4 heads of 1024 tokens (1024 tiles)                    77 /  73 /  77
-//   64 x 96 x 4 heads of 1024 tokens (1536 tiles)                   106 /  93 /  81
-//   16 x 512 x 8 heads of 1024 tokens (4096 tiles)                  239 / 165 / 121
-// and at 8 rows 24 against 34 (64 heads of 4096 tokens: the 8-row kernel, the 16-row
+//   4 sequences x 128 rows x 8 heads of 2048 tokens (256 tiles)      46 /  61 /  94
+//   one prompt of 500 tokens, 8 heads (256 tiles)                    29 /  44 /  37
+//   8 x 144 x 8 heads of 2048 tokens (576 tiles)                     74 /  78 /  80
+//   one prompt of 768 tokens, 12 heads (576 tiles)                   40 /  40 /  73
+//   64 x 96 x 2 heads of 1024 tokens (768 tiles)                     65 /  63 /  67
+//   32 prompts of 24 tokens, 12 heads (768 tiles)                    24 /  13 /  20
+//   64 x 64 x 4 heads of 1024 tokens (1024 tiles)                    83 /  72 /  77
+//   64 x 96 x 4 heads of 1024 tokens (1536 tiles)                   110 /  93 /  82
+//   16 x 512 x 8 heads of 1024 tokens (4096 tiles)                  227 / 146 / 115
+// and at 8 rows 23 against 34 (64 heads of 4096 tokens: the 8-row kernel, the 16-row
 // one).  Where the rule is wrong: few tiles over very long sequences (290
-// tokens x 4 behind 8192, 584 tiles: 190 / 176 / 152), many prompts of 128 to 512
-// tokens (32 x 128, 12 heads: 79 / 36 / 51; d = 64, 16 x 512: 116 / 67 / 75); the
-// host does not know the lengths.
+// tokens x 4 behind 8192, 584 tiles: 196 / 179 / 152), many prompts of 128 to 512
+// tokens (32 x 128, 12 heads: 81 / 38 / 52; d = 64, 16 x 512: 125 / 67 / 75), and a
+// prompt among single tokens, whose sequences all go to the kernel that their mean
+// asks for; the host knows neither lengths nor rows.
 enum AttnKind { kAttn8, kAttn16, kAttnChunk, kAttnLong };
 static AttnKind attn_kind(int64_t B, int64_t T, int64_t Hk, int64_t G) {
     const int64_t rows = (T + B - 1) / B * G, tiles = (rows + 15) / 16 * B * Hk;

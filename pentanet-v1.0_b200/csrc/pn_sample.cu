@@ -28,13 +28,14 @@
 // the logits' ordered bit patterns: on a list of them or, where one bucket holds too
 // many (all logits nearly alike), over the runs themselves.
 //
-// What bounds it: large batches the weights, about thirty instructions each (six of
-// them fp64; the split into table index and rest runs in fp32), and the histogram's
-// atomics where it covers whole runs; small ones the chain of short steps, each
-// behind a barrier of the cluster (1 to 2 us).  One bf16 row of 50257, top-k 50 and
-// top-p: 18.5 us; 64 fp32 rows with settings of their own: 25 us; 256 rows of 131071
-// with top-p alone over a flat distribution: 218 us (a histogram of all weights in the
-// first pass: 302 us; candidates down to 2^-16 of the largest: 236 us).
+// What bounds it: the chain of short steps, each behind a barrier of the block or the
+// cluster (1 to 2 us); in large batches over flat distributions also the weights, about
+// thirty instructions each (six of them fp64; the split into table index and rest runs in
+// fp32), computed up to three times (sum, histogram, draw: 84 instructions per logit, 45 % of
+// the issue slots used), and the histogram's atomics.  One bf16 row of 50257, top-k 50
+// and top-p: 18.6 us; 64 fp32 rows with settings of their own: 25.6 us; 256 rows of 131071
+// with top-p alone over a flat distribution: 219 us, five waves of clusters (a histogram of
+// all weights in the first pass: 302 us; candidates down to 2^-16 of the largest: 236 us).
 #include <cooperative_groups.h>
 
 #include "pn_common.cuh"

@@ -14,7 +14,7 @@ what four bits cost depends on how alike a vector's dims are.  Measured on norma
 random data (1024 tokens), the attention output moves against unquantised keys and
 values by 13 % (head_dim 64) or 14 % (128) of its norm; with two key dims 5x louder
 than the rest, which take the range of every key, by 28 % or 26 %, 12x louder by 46 %
-or 63 %.  A vector whose range is no finite fp32 number reads back as NaN.
+or 63 %.  A vector whose range is no finite number reads back as NaN.
 
 A sequence's page i (block_table[b, i]) holds its positions [i * page_size,
 (i + 1) * page_size).  seq_lens[b] counts the sequence's tokens WITH the rows of
