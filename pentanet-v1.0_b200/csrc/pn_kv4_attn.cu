@@ -1096,6 +1096,10 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
     const int quad = warp & 3, tq = warp >> 2;  // tensor-memory lanes 32 quad ..; half of the tile's tokens
     const int row = quad * 32 + lane;
     asm volatile("griddepcontrol.launch_dependents;");
+    // Tensor memory is taken only when the grid before this one is done: one that allocates
+    // after its own trigger (the product kernel does) could otherwise wait for columns that
+    // this block holds while it waits for that grid.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp == 0) {
         tmem_alloc(&s_tmem, C::kCols);
         tmem_relinquish();  // (the SM's other block allocates too)
@@ -1112,7 +1116,6 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
     const uint32_t tl = tm + ((uint32_t)(quad * 32) << 16);  // this warp's lanes
     volatile int* abort = &s_abort;
     const uint32_t q_lo = desc_lo(qop), k_lo = desc_lo(kop), v_lo = desc_lo(vop);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 
     const AttnRun run = attn_plan<C>(a);
     if (tid == 0) a.notes[blockIdx.x].rows = 0;

@@ -7,6 +7,7 @@ import torch
 
 import kv4_oracle as oracle
 import penta_cache as pc
+import penta_kernel as pk
 import penta_native as nat
 
 pytestmark = pytest.mark.gpu
@@ -607,6 +608,36 @@ def test_quiet_values_beside_loud_ones(cuda_device, rows, G):
         s.v[i] *= 2.0 ** -20
     s.store(lengths)
     s.attend([rows] * 96, G, scale=1.0, seed=G)
+
+
+@pytest.mark.parametrize("rows", [1, 12, 21])
+def test_between_products(cuda_device, rows):
+    """Queries straight from a packed product, the output straight into the next, on two
+    streams at once: both kernels start before the one before them ends and take tensor memory."""
+    s = wide(cuda_device, 64, rows)
+    g = torch.Generator().manual_seed(rows)
+    w_q = pk.quantize_and_pack(torch.randn(32 * 64, 256, generator=g).to(cuda_device))
+    w_o = pk.quantize_and_pack(torch.randn(256, 32 * 64, generator=g).to(cuda_device))
+    x = torch.randn(32 * rows, 256, generator=g).to(torch.bfloat16).to(cuda_device)
+
+    def block(wait=lambda: None):
+        q = pk.penta_linear(x, w_q[0], w_q[2], w_q[1])
+        wait()
+        y = pc.kv4_attention(q.view(32, rows, 32, 64), s.cache, s.table, s.lens)
+        wait()
+        return pk.penta_linear(y.view(32 * rows, 32 * 64), w_o[0], w_o[2], w_o[1])
+
+    want = block(torch.cuda.synchronize)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for side in streams:
+        side.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for side in streams:
+            with torch.cuda.stream(side):
+                got.append(block())
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y in got) and nat.device_status() == 0
 
 
 def test_calls_of_several_threads(cuda_device):
