@@ -192,10 +192,6 @@ class PentaGPTFast(nn.Module):
             return self._logits(idx, torch.arange(T, device=idx.device), all_logits)
         assert B == cache.seq_lens.shape[0], f"{B} sequences, the cache holds {cache.seq_lens.shape[0]}"
         assert cache.known_length() + T <= min(cache.capacity, self.cfg.block_size), "the cache is full"
-        return self._append(idx, cache, all_logits)
-
-    def _append(self, idx: torch.Tensor, cache: PentaGPTCache, all_logits: bool = False) -> torch.Tensor:
-        T = idx.shape[1]
         capturing = torch.cuda.is_current_stream_capturing()
         # (a captured step replayed past the block stays at its last position)
         pos = (cache.seq_lens[:, None] + torch.arange(T, device=idx.device)).clamp(max=self.cfg.block_size - 1)
@@ -243,7 +239,11 @@ class PentaGPTFast(nn.Module):
             f"{held} + {T} + {max_new_tokens} tokens do not fit the model's block or the cache"
         out = [idx]
         u = torch.rand(max_new_tokens, B, device=idx.device, generator=generator)
-        for i in range(max_new_tokens):
-            logits = self._append(out[-1].clamp(min=0), cache)  # -1: a row of NaN logits has no token
-            out.append(pk.sample_tokens(logits[:, 0], u[i], temperature, top_k, top_p, min_p)[:, None])
+        captured, cache.captured = cache.captured, False  # (nothing is replayed in between: one look at seq_lens will do)
+        try:
+            for i in range(max_new_tokens):
+                logits = self(out[-1].clamp(min=0), cache=cache)  # -1: a row of NaN logits has no token
+                out.append(pk.sample_tokens(logits[:, 0], u[i], temperature, top_k, top_p, min_p)[:, None])
+        finally:
+            cache.captured |= captured
         return torch.cat(out, dim=1)

@@ -295,6 +295,17 @@ def test_cache_after_replays(cuda_device):
     assert cache.seq_lens.tolist() == [24, 24] and nat.device_status() == 0
 
 
+def test_cache_of_another_batch(cuda_device):
+    model = _small(cuda_device)
+    idx = torch.randint(0, 700, (4, 5), generator=torch.Generator().manual_seed(5)).to(cuda_device)
+    for batch, n in ((1, 4), (4, 1), (3, 2)):
+        cache = model.new_cache(batch)
+        for call in (lambda: model(idx[:n], cache=cache), lambda: model.generate(idx[:n], 3, cache=cache)):
+            with pytest.raises(AssertionError, match="the cache holds"):
+                call()
+        assert cache.length == 0 and not cache.seq_lens.any()
+
+
 def test_cache_after_a_block_that_raises(cuda_device, monkeypatch):
     """Tokens without keys are not counted."""
     model = _small(cuda_device)
