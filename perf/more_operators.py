@@ -367,7 +367,7 @@ def _sparse(s):
         pc.kv4_page_means(s["cache"], s["means"], s["table"], s["lens"], s["q"].shape[:-2], cu_q=s["cu"])
         y, pages = pc.kv4_sparse_attention(s["q"], s["cache"], s["means"], s["table"], s["lens"], top, first_pages=first,
                                            last_pages=last, cu_q=s["cu"], return_pages=True)
-        return {"y": y, "pages": pages, "means": s["means"]}
+        return {"y": y, "pages": pages.flatten(0, -3), "means": s["means"]}
     b, hk, group, d, page = s["batch"], s["kv_heads"], s["group"], s["head_dim"], s["page"]
     # the means of the pages that the rows are in, over the tokens held so far
     seq, i = _touched(s)
