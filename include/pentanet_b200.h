@@ -352,6 +352,68 @@ int pn_kv4_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
                      const int32_t *cu_q, int64_t B, int64_t T, float scale, void *out, void *workspace,
                      size_t workspace_bytes, void *stream);
 
+/* pn_kv4_append of keys whose positions are rotated on the way, with the rows' queries
+ * (q_heads of them, all three of one type): of the first `rotated` dims of a head
+ * (a multiple of 16 up to head_dim; the rest pass as they are) pair (a, b) becomes
+ * (a cos - b sin, b cos + a sin), each product and sum rounded to fp32; pairs are
+ * (i, i + rotated / 2), or (2i, 2i + 1) with interleaved != 0.  cos, sin: (n_pos,
+ * rotated / 2) fp32, rows table_stride apart; a row at position p of sequence b takes
+ * entry p + offsets[b] (int32; p where offsets is NULL).  The rotated queries go to
+ * q_out (T, q_heads, head_dim), contiguous, 16-byte aligned, rounded once (q_out may be
+ * q itself, where q is contiguous; other overlaps of the two are not allowed).  Keys
+ * are quantised from fp32, values as pn_kv4_append does.  Rows behind cu_q[B] are left as
+ * they were in q_out; a row at a negative position gives zeros there, and one whose
+ * entry is outside the tables zeros, nothing stored and PN_ERR_ARG in the device
+ * status word. */
+int pn_kv4_append_rotary(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int64_t q_heads, const void *k, int64_t k_sb,
+                         int64_t k_sl, int64_t k_sh, const void *v, int64_t v_sb, int64_t v_sl, int64_t v_sh, int dtype,
+                         const float *cos, const float *sin, int64_t n_pos, int64_t table_stride, int64_t rotated,
+                         int interleaved, const int32_t *offsets, void *cache, int64_t n_pages, int64_t kv_heads, int64_t page,
+                         int64_t head_dim, const int32_t *block_table, int64_t table_ld, int64_t table_w,
+                         const int32_t *seq_lens, const int32_t *cu_q, int64_t B, int64_t T, void *q_out, void *stream);
+
+/* pn_kv4_attention of sequences behind shared prefixes: the rows of sequences
+ * [cu_prefix[g], cu_prefix[g + 1]) see all prefix_lens[g] tokens of prefix g (pages of
+ * the same cache, prefix_table (n_prefixes, prefix_w), rows prefix_ld apart) before
+ * their sequence's own, which block_table and seq_lens count from 0.  cu_prefix:
+ * (n_prefixes + 1) int32 that do not fall (one that does: nothing is computed and
+ * PN_ERR_ARG recorded), or NULL: B / n_prefixes sequences each.  Sequences before
+ * cu_prefix[0] or behind cu_prefix[n_prefixes] have no prefix.  A row sees its prefix
+ * also where it sees none of its sequence.  A prefix's tokens are read once for all
+ * rows that see them. */
+size_t pn_kv4_prefix_attention_workspace_size(int64_t B, int64_t T, int64_t n_prefixes, int64_t q_heads, int64_t kv_heads,
+                                              int64_t head_dim);
+int pn_kv4_prefix_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
+                            const void *cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
+                            const int32_t *block_table, int64_t table_ld, int64_t table_w, const int32_t *seq_lens,
+                            const int32_t *cu_q, int64_t B, int64_t T, const int32_t *prefix_table, int64_t prefix_ld,
+                            int64_t prefix_w, const int32_t *prefix_lens, const int32_t *cu_prefix, int64_t n_prefixes,
+                            float scale, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The mean keys of the pages that the rows of a call are in, over the tokens that
+ * each holds: means (n_pages, kv_heads, head_dim) bf16, 16-byte aligned; sums in fp64,
+ * rounded to fp32 and to bf16.  Other pages' means are left as they were. */
+int pn_kv4_page_means(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
+                      const int32_t *block_table, int64_t table_ld, int64_t table_w, const int32_t *seq_lens,
+                      const int32_t *cu_q, int64_t B, int64_t T, void *means, void *stream);
+
+/* pn_kv4_attention over chosen pages: a row whose position is in page j of its sequence
+ * attends, in each kv head, to pages 0 .. first_pages - 1, to j - last_pages + 1 .. j
+ * (last_pages >= 1) and to the top_pages of the others with the largest scores (sum
+ * of the kv head's queries) . means[page], in fp64, ties by the lowest page; a NaN, and
+ * an entry that is no page of the cache, come last.  Of page j it sees the tokens up to
+ * its own.  chosen: NULL, or (T, kv_heads, width) int32 with width = first_pages +
+ * last_pages + top_pages: the pages' numbers in the sequence, ascending, then -1 (all -1 for
+ * rows that are no sequence's). */
+size_t pn_kv4_sparse_attention_workspace_size(int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t table_w,
+                                              int64_t width);
+int pn_kv4_sparse_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
+                            const void *cache, const void *means, int64_t n_pages, int64_t kv_heads, int64_t page,
+                            int64_t head_dim, const int32_t *block_table, int64_t table_ld, int64_t table_w,
+                            const int32_t *seq_lens, const int32_t *cu_q, int64_t B, int64_t T, int64_t first_pages,
+                            int64_t last_pages, int64_t top_pages, float scale, void *out, int32_t *chosen, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
 /* One token per row of logits ((rows, vocab) PN_BF16 or PN_F32, rows ld elements
  * apart, vocab <= 2^18) from a uniform number u[row] in [0, 1):
  *   w_i = exp((x_i - max) / T); keep the top_k largest logits (ties: lowest

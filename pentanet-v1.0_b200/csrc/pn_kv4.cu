@@ -37,6 +37,12 @@ struct Kv4Seq {
     int64_t L;
     int64_t n_pages;
     int Hk, page;
+    int64_t table_hd;    // entries between the tables of a sequence's kv heads; 0: they share one
+    // Shared prefixes: the B "sequences" are prefixes, with a table and a length each, whose
+    // rows are those of sequences [grp[b], grp[b + 1]) of `grouped` (grp null: equally many
+    // each).  0: the sequences are themselves.
+    int64_t grouped;
+    const int32_t* grp;  // (B + 1)
 };
 
 // The length of sequence b, and how much of it its table has room for.
@@ -45,6 +51,16 @@ __device__ __forceinline__ int kv4_held(const Kv4Seq& s, int64_t b) { return min
 
 // First row and number of rows of sequence b.
 __device__ __forceinline__ void kv4_rows(const Kv4Seq& s, int64_t b, int64_t& first, int64_t& n) {
+    if (s.grouped) {
+        int64_t b0 = b * (s.grouped / s.B), b1 = b0 + s.grouped / s.B;
+        if (s.grp) {
+            b0 = min(max((int64_t)__ldg(s.grp + b), (int64_t)0), s.grouped);
+            b1 = min(max((int64_t)__ldg(s.grp + b + 1), b0), s.grouped);
+        }
+        first = s.cu ? min(max((int64_t)__ldg(s.cu + b0), (int64_t)0), s.T) : b0 * s.L;
+        n = (s.cu ? min(max((int64_t)__ldg(s.cu + b1), first), s.T) : b1 * s.L) - first;
+        return;
+    }
     if (!s.cu) {
         first = b * s.L;
         n = s.L;

@@ -48,7 +48,8 @@ struct Kv4Join {
     int G;
     int64_t row0;    // first row of the tile's sequence
     int64_t r0;      // first query row of the tile
-    int64_t head;
+    int head;
+    int joins;       // the rows have a prefix's results to join
 };
 
 struct Kv4AttnArgs {
@@ -56,12 +57,22 @@ struct Kv4AttnArgs {
     const void* q;
     int q_f32, q_vec;
     int64_t q_sb, q_sl, q_sh;
+    int64_t q_l;       // rows between the strides q_sb where the call's "sequences" are not those of q; 0: they are
     const uint8_t* cache;
     int G;             // query heads per kv head
     float scale_log2;  // softmax scale * log2(e)
     void* out;         // (T, Hk * G, D), q's type
+    int out_f32;
     Kv4Join* notes;    // workspace: one per block
     float* part;       // workspace: partial results of two segments per block
+    // Rows that attend to a shared prefix and to their own sequence.  The call over the
+    // prefixes writes fp32 results with the logarithms (base 2) of their totals (lse), that over
+    // the sequences joins them to its own (pre, pre_lse), for the sequences that have a prefix:
+    // [grp[0], grp[n_grp]), or all.
+    float* lse;              // (T, Hk * G), or null
+    const float *pre, *pre_lse;
+    const int32_t* grp;      // (n_grp + 1), or null
+    int n_grp;
 };
 
 constexpr int kAttnWarps = 4;
@@ -131,6 +142,7 @@ template <typename C>
 __device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, uint32_t& nt) {
     int64_t first, n;
     kv4_rows(a.s, b, first, n);
+    if (a.s.table_hd && __ldg(a.s.lens + b) < 0) n = 0;  // (of chosen pages: a row that is no sequence's)
     nt = max((kv4_held(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
     return ((uint32_t)n * a.G + C::kRows - 1) / C::kRows * nt * a.s.Hk;
 }
@@ -154,8 +166,12 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
     bool falls = false;  // cu_q does: its rows, and so the units, may be more than the host counted on
     for (uint32_t b = b0; b < b1; ++b) {
         sum += attn_units<C>(a, b, nt);
-        falls |= a.s.cu && __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
+        falls |= !a.s.grouped && a.s.cu && __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
     }
+    if (a.s.grouped && a.s.cu)
+        for (uint32_t b = threadIdx.x; b < a.s.grouped; b += C::kThreads) falls |= __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
+    if (a.grp)
+        for (uint32_t b = threadIdx.x; b < (uint32_t)a.n_grp; b += C::kThreads) falls |= __ldg(a.grp + b + 1) < __ldg(a.grp + b);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     uint32_t inc = sum;
 #pragma unroll
@@ -200,7 +216,7 @@ struct AttnSeg {
     uint32_t b, nt, t0, t1;  // sequence; token tiles of it, and the segment's [t0, t1)
     int head, rows;          // kv head; query rows in the tile
     int64_t row0, r0;        // first row of the sequence; first query row of the tile
-    int pos0;                // query row r sees positions up to pos0 + r / G
+    int pos0;                // query row r sees positions up to pos0 + r / G (of a prefix: all)
     int kv_end;              // tokens that the tile's last row sees (and the table has room for)
     int lim_min;             // the last position that its first row sees (at most kv_end - 1)
 
@@ -226,15 +242,32 @@ struct AttnSeg {
         rows = (int)min((uint32_t)C::kRows, q_rows - (uint32_t)r0);
         t0 = in_seq - tile * nt;
         t1 = min(nt, t0 + left);
-        pos0 = kv4_len(a.s, b) - (int)n_rows;
+        pos0 = a.s.grouped ? kv4_held(a.s, b) - 1 : kv4_len(a.s, b) - (int)n_rows;
         kv_end = min(max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0), kv4_held(a.s, b));
-        if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && pos0 + (int)n_rows > kv4_held(a.s, b)) record_status(PN_ERR_ARG);
-        lim_min = min(pos0 + (int)((uint32_t)r0 / a.G), kv_end - 1);
+        if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && kv4_len(a.s, b) > kv4_held(a.s, b)) record_status(PN_ERR_ARG);
+        lim_min = last_seen(a, 0);
+    }
+    // The last position that query row r of the tile sees.
+    __device__ __forceinline__ int last_seen(const Kv4AttnArgs& a, int r) const {
+        return min(pos0 + (int)(((uint32_t)r0 + r) / a.G), kv_end - 1);
+    }
+    // Whether the rows have a prefix's results to join.
+    __device__ __forceinline__ bool joins(const Kv4AttnArgs& a) const {
+        return a.pre && (!a.grp || ((int)b >= __ldg(a.grp) && (int)b < __ldg(a.grp + a.n_grp)));
     }
     // Where query row r of the tile (r < rows) lies in q, in elements.
     __device__ __forceinline__ int64_t query(const Kv4AttnArgs& a, int r) const {
         const uint32_t rr = (uint32_t)r0 + r, i = rr / a.G;
-        return (a.s.cu ? (row0 + i) * a.q_sl : b * a.q_sb + i * a.q_sl) + (head * a.G + (rr - i * a.G)) * a.q_sh;
+        int64_t at;
+        if (a.s.cu) {
+            at = (row0 + i) * a.q_sl;
+        } else if (a.q_l) {
+            const int64_t of = (row0 + i) / a.q_l;
+            at = of * a.q_sb + (row0 + i - of * a.q_l) * a.q_sl;
+        } else {
+            at = b * a.q_sb + i * a.q_sl;
+        }
+        return at + (head * a.G + (rr - i * a.G)) * a.q_sh;
     }
 };
 
@@ -245,7 +278,7 @@ __device__ __forceinline__ void attn_note(const Kv4AttnArgs& a, const AttnRun& r
     // the block that holds the tile's first unit: the first `rem` blocks hold one more
     const uint32_t u0 = unit - sg.t0, each = run.total / gridDim.x, rem = run.total % gridDim.x;
     const uint32_t c0 = u0 < (each + 1) * rem ? u0 / (each + 1) : rem + (u0 - (each + 1) * rem) / each;
-    a.notes[blockIdx.x] = {sg.rows, (int)c0, attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0, a.G, sg.row0, sg.r0, sg.head};
+    a.notes[blockIdx.x] = {sg.rows, (int)c0, attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0, a.G, sg.row0, sg.r0, sg.head, sg.joins(a)};
 }
 
 // Looks up the pages of a sequence, 32 pieces of 16 tokens at a time: lane l
@@ -259,7 +292,7 @@ struct AttnPages {
         off = 0;
         if (!want) return;
         const uint32_t i = (uint32_t)tok / (uint32_t)a.s.page;
-        const int p = __ldg(a.s.table + b * a.s.table_ld + i);
+        const int p = __ldg(a.s.table + b * a.s.table_ld + head * a.s.table_hd + i);
         off = tok - (int)i * a.s.page;
         if (p >= 0 && p < a.s.n_pages)
             addr = (uint64_t)(a.cache + ((int64_t)p * a.s.Hk + head) * 2 * block);
@@ -268,13 +301,37 @@ struct AttnPages {
     }
 };
 
-__device__ __forceinline__ void store_out(const Kv4AttnArgs& a, int64_t at, const float4& y, float inv) {
-    if (a.q_f32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+// How a row's sums y (relative to 2^m, their total `sum`) become its result: y * k1 + pre * k2,
+// with the row of a prefix's results where it joins them.  (A total of 0: nothing was seen.)
+struct RowScale {
+    float k1, k2;
+    bool add;  // whether there is a prefix's row (k2 may be 0, its values not be finite)
+    __device__ __forceinline__ RowScale(const Kv4AttnArgs& a, int64_t row, float m, float sum, bool joins) {
+        k1 = sum == 0.0f ? 0.0f : 1.0f / sum;
+        k2 = 0.0f;
+        add = false;
+        if (!joins) return;
+        const float l1 = a.pre_lse[row], l2 = lse(m, sum), top = fmaxf(l1, l2);
+        if (l1 == -INFINITY) return;
+        const float w1 = ex2f(l1 - top), w2 = sum == 0.0f ? 0.0f : ex2f(l2 - top), each = 1.0f / (w1 + w2);
+        add = true;
+        k1 *= w2 * each;
+        k2 = w1 * each;
+    }
+    static __device__ __forceinline__ float lse(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
+};
+__device__ __forceinline__ void store_out(const Kv4AttnArgs& a, int64_t at, const float4& y, const RowScale& k) {
+    float4 v = make_float4(y.x * k.k1, y.y * k.k1, y.z * k.k1, y.w * k.k1);
+    if (k.add) {
+        const float4 u = *reinterpret_cast<const float4*>(a.pre + at);
+        v = make_float4(fmaf(u.x, k.k2, v.x), fmaf(u.y, k.k2, v.y), fmaf(u.z, k.k2, v.z), fmaf(u.w, k.k2, v.w));
+    }
+    if (a.out_f32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
     } else {
-        const __nv_bfloat162 u = __floats2bfloat162_rn(y.x * inv, y.y * inv), v = __floats2bfloat162_rn(y.z * inv, y.w * inv);
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
+            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
     }
 }
 
@@ -473,7 +530,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                 else
                     ca[n].y = va, cb[n].y = vb;
                 const int rl = n * 8 + 2 * t + k;
-                lim[n][k] = rl < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + rl) / a.G) : sg.kv_end - 1;
+                lim[n][k] = rl < sg.rows ? sg.last_seen(a, rl) : sg.kv_end - 1;
             }
         }
 
@@ -675,7 +732,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
             }
         }
         __syncthreads();
-        const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
+        const bool whole = sg.t0 == 0 && sg.t1 == sg.nt, joins = whole && sg.joins(a);
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
         for (int idx = tid; idx < sg.rows * (D / 4); idx += kAttnThreads) {
             const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
@@ -694,9 +751,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                 y.x = fmaf(f, u.x, y.x), y.y = fmaf(f, u.y, y.y), y.z = fmaf(f, u.z, y.z), y.w = fmaf(f, u.w, y.w);
             }
             if (whole) {
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
-                store_out(a, (((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G) * D + d, y, inv);
+                const int64_t at = ((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G;
+                store_out(a, at * D + d, y, RowScale(a, at, mx, sum, joins));
+                if (a.lse && d == 0) a.lse[at] = RowScale::lse(mx, sum);
             } else {
                 *reinterpret_cast<float4*>(part + r * D + d) = y;
                 if (d == 0) part[RT * D + r * 2] = mx, part[RT * D + r * 2 + 1] = sum;
@@ -796,11 +854,11 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
             const char* row = nullptr;
             if (r < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, r) * (a.q_f32 ? 4 : 2);
             load_query<D>(a, row, t, k ? qc : qa, ca[k], cb[k]);
-            lim[k] = r < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + r) / a.G) : sg.kv_end - 1;
+            lim[k] = r < sg.rows ? sg.last_seen(a, r) : sg.kv_end - 1;
         }
         if (w_rows > 0) {
-            w_min = sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16) / a.G);
-            w_end = max(sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16 + w_rows - 1) / a.G) + 1, 0);
+            w_min = sg.last_seen(a, warp * 16);
+            w_end = max(sg.last_seen(a, warp * 16 + w_rows - 1) + 1, 0);
             // a padding row sees what the warp's last one does
             if (warp * 16 + g >= sg.rows) lim[0] = w_end - 1;
             if (warp * 16 + 8 + g >= sg.rows) lim[1] = w_end - 1;
@@ -972,8 +1030,8 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
             const int r = warp * 16 + k * 8 + g;
             if (r >= sg.rows) continue;
             const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
-            const int64_t at = (((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G) * D;
-            const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int64_t row = ((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G, at = row * D;
+            const RowScale scale(a, row, -neg_r[k], sum, whole && sg.joins(a));
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -982,10 +1040,11 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                     const float4 y = make_float4(fmaf(o[w * 4][2 * k + c], up, z), fmaf(o[w * 4 + 1][2 * k + c], up * 0.0625f, z),
                                                  fmaf(o[w * 4 + 2][2 * k + c], up, z), fmaf(o[w * 4 + 3][2 * k + c], up * 0.0625f, z));
                     if (whole)
-                        store_out(a, at + d, y, inv);
+                        store_out(a, at + d, y, scale);
                     else
                         *reinterpret_cast<float4*>(part + r * D + d) = y;
                 }
+            if (whole && a.lse && t == 0) a.lse[row] = RowScale::lse(-neg_r[k], sum);
             if (!whole && t == 0) part[C::kRows * D + r * 2] = -neg_r[k], part[C::kRows * D + r * 2 + 1] = sum;
         }
         if (tid == 0) attn_note(a, run, sg, unit);
@@ -1199,7 +1258,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             ca = a.scale_log2 * pow2i(24 - e);
             cb = sum * 0x1p-24f;
         }
-        const int lim = row < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + row) / a.G) : sg.kv_end - 1;
+        const int lim = row < sg.rows ? sg.last_seen(a, row) : sg.kv_end - 1;
 
         // ---- spreading of a tile's codes
         auto spread_keys = [&](int i, int stage) {
@@ -1417,9 +1476,10 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         const float l = ex[0][0][row] + ex[0][1][row], zs = ex[1][0][row] + ex[1][1][row];
         const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
-        const float up = 16777216.0f, inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+        const float up = 16777216.0f;
         const uint32_t rr = (uint32_t)sg.r0 + row, ri = rr / a.G;
-        const int64_t at = (((sg.row0 + ri) * a.s.Hk + sg.head) * a.G + rr - ri * a.G) * D + tq * kDims;
+        const int64_t out_row = ((sg.row0 + ri) * a.s.Hk + sg.head) * a.G + rr - ri * a.G, at = out_row * D + tq * kDims;
+        const RowScale scale(a, out_row, -neg_r, l, row < sg.rows && whole && sg.joins(a));
 #pragma unroll
         for (int h = 0; h < kDims / 16; ++h) {
             uint32_t u[16];
@@ -1436,12 +1496,13 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                     const float4 y = make_float4(fmaf(__uint_as_float(u[k]), up, zs), fmaf(__uint_as_float(u[k + 1]), up * 0.0625f, zs),
                                                  fmaf(__uint_as_float(u[k + 2]), up, zs), fmaf(__uint_as_float(u[k + 3]), up * 0.0625f, zs));
                     if (whole)
-                        store_out(a, at + h * 16 + k, y, inv);
+                        store_out(a, at + h * 16 + k, y, scale);
                     else
                         *reinterpret_cast<float4*>(part + row * D + tq * kDims + h * 16 + k) = y;
                 }
             }
         }
+        if (whole && a.lse && tq == 0 && row < sg.rows) a.lse[out_row] = RowScale::lse(-neg_r, l);
         if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = -neg_r, part[C::kRows * D + row * 2 + 1] = l;
         if (tid == 0) attn_note(a, run, sg, unit);
         tc_fence_before();
@@ -1518,18 +1579,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 #pragma unroll
                 for (int e = 0; e < E; ++e) y[e] = fmaf(f, sh[warp + w][e * 32 + lane], y[e]);
             }
+            mx = top;
         }
         if (r >= to) continue;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const uint32_t rr = (uint32_t)j.r0 + r, i = rr / j.G;
-        const int64_t at = (((j.row0 + i) * a.s.Hk + j.head) * j.G + rr - i * j.G) * D + lane;
+        const int64_t row = ((j.row0 + i) * a.s.Hk + j.head) * j.G + rr - i * j.G, at = row * D + lane;
+        const RowScale k(a, row, mx, sum, j.joins);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (a.q_f32)
-                static_cast<float*>(a.out)[at + e * 32] = y[e] * inv;
+            float v = y[e] * k.k1;
+            if (k.add) v = fmaf(a.pre[at + e * 32], k.k2, v);
+            if (a.out_f32)
+                static_cast<float*>(a.out)[at + e * 32] = v;
             else
-                static_cast<__nv_bfloat16*>(a.out)[at + e * 32] = __float2bfloat16_rn(y[e] * inv);
+                static_cast<__nv_bfloat16*>(a.out)[at + e * 32] = __float2bfloat16_rn(v);
         }
+        if (a.lse && lane == 0) a.lse[row] = RowScale::lse(mx, sum);
     }
 }
 
@@ -1564,15 +1629,20 @@ static int attn_blocks(AttnKind kind) {  // blocks that the device holds at once
     return sm_count() * (kind == kAttnLong ? TcCfg<128>::kBlocks : AttnCfg<128, 1>::kBlocks);
 }
 static size_t attn_notes_bytes(int blocks) { return ((size_t)blocks * sizeof(Kv4Join) + 255) / 256 * 256; }
+static size_t attn_part_bytes(AttnKind kind, int64_t D) {
+    constexpr int rows[4] = {8, 16, 64, 128};
+    return (size_t)attn_blocks(kind) * 2 * rows[kind] * (D + 2) * 4;
+}
+// Bytes of the notes and partial results of one pass.
+static size_t attn_workspace(AttnKind kind, int64_t D) {
+    return attn_notes_bytes(attn_blocks(kind)) + attn_part_bytes(kind, D);
+}
 static size_t attn_workspace(int64_t B, int64_t T, int64_t Hk, int64_t G, int64_t D) {
-    if (B == 0 || T == 0) return 0;
-    const AttnKind kind = attn_kind(B, T, Hk, G);
-    const int blocks = attn_blocks(kind), rows[4] = {8, 16, 64, 128};
-    return attn_notes_bytes(blocks) + (size_t)blocks * 2 * rows[kind] * (D + 2) * 4;
+    return B == 0 || T == 0 ? 0 : attn_workspace(attn_kind(B, T, Hk, G), D);
 }
 
 template <int D, typename C>
-static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a, cudaStream_t s) {
+static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a, AttnKind kind, cudaStream_t s) {
     static std::atomic<bool> done[64];  // false at first
     int dev = 0;
     cudaGetDevice(&dev);
@@ -1581,7 +1651,7 @@ static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a
         if (e != cudaSuccess) return e;
         if (dev >= 0 && dev < 64) done[dev] = true;
     }
-    const int blocks = attn_blocks(attn_kind(a.s.B, a.s.T, a.s.Hk, a.G));
+    const int blocks = attn_blocks(kind);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -1606,7 +1676,61 @@ static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a
     return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, a, (int)C::kRows);
 }
 
+// One pass: its kernel and the one that joins, with notes and partial results at ws.
+static cudaError_t attn_pass(Kv4AttnArgs& a, AttnKind kind, int64_t head_dim, void* ws, cudaStream_t s) {
+    a.notes = static_cast<Kv4Join*>(ws);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + attn_notes_bytes(attn_blocks(kind)));
+    auto go = [&](auto dim) {
+        constexpr int D = decltype(dim)::value;
+        switch (kind) {
+            case kAttn8: return launch_attn<D, AttnCfg<D, 1>>(kv4_decode_kernel<D, 1>, a, kind, s);
+            case kAttn16: return launch_attn<D, AttnCfg<D, 2>>(kv4_decode_kernel<D, 2>, a, kind, s);
+            case kAttnChunk: return launch_attn<D, ChunkCfg<D>>(kv4_chunk_kernel<D>, a, kind, s);
+            default: return launch_attn<D, TcCfg<D>>(kv4_long_kernel<D>, a, kind, s);
+        }
+    };
+    return head_dim == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
+}
+
+// The kernel for the rows of shared prefixes: here the host knows that the rows walk long
+// sequences together, but no more of the prefixes' lengths than the table's width.
+static AttnKind prefix_kind(int64_t P, int64_t T, int64_t Hk, int64_t G) {
+    const int64_t rows = (T + P - 1) / P * G;
+    return rows <= 8 ? kAttn8 : rows <= 16 ? kAttn16 : rows <= 64 ? kAttnChunk : kAttnLong;
+}
+static size_t prefix_rows_bytes(int64_t T, int64_t H, int64_t D) {
+    return ((size_t)T * H * (D + 1) * 4 + 255) / 256 * 256;
+}
+
 }  // namespace pn
+
+// The queries and outputs of an attention call, a.s being there already.
+static int check_attn(const char* name, const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
+                      const void* cache, float scale, void* out, pn::Kv4AttnArgs* a) {
+    const pn::Kv4Seq& s = a->s;
+    if (q_dtype != PN_F32 && q_dtype != PN_BF16) return fail(PN_ERR_DTYPE, "%s: dtype %d", name, q_dtype);
+    if (q_heads < 1 || q_heads % s.Hk != 0 || q_heads > 65536)
+        return fail(PN_ERR_SHAPE, "%s: %lld query heads over %d kv heads", name, (long long)q_heads, s.Hk);
+    if (s.T > 0 && s.B > 0 && (!q || !out)) return fail(PN_ERR_ARG, "%s: null pointer", name);
+    if (!(scale > 0.0f && scale < INFINITY)) return fail(PN_ERR_ARG, "%s: scale must be positive", name);
+    const size_t e = q_dtype == PN_F32 ? 4 : 2;
+    if (!aligned(q, e) || !aligned(out, 16)) return fail(PN_ERR_ALIGN, "%s: misaligned pointer", name);
+    a->q = q, a->q_f32 = a->out_f32 = q_dtype == PN_F32, a->q_sb = q_sb, a->q_sl = q_sl, a->q_sh = q_sh;
+    const int64_t n = 16 / (int64_t)e;
+    a->q_vec = aligned(q, 16) && q_sb % n == 0 && q_sl % n == 0 && q_sh % n == 0;
+    a->cache = static_cast<const uint8_t*>(cache);
+    a->G = (int)(q_heads / s.Hk);
+    a->scale_log2 = scale * 1.4426950408889634f;
+    a->out = out;
+    return PN_OK;
+}
+// Upper bounds on the rows and units that the kernels count in 31 bits.
+static int check_attn_units(const char* name, const pn::Kv4Seq& s, int64_t G, int64_t tokens) {
+    if (s.B > 0 && ((double)s.T * G > 2e9 || ((double)s.T * G / 8 + s.B) * s.Hk * ((double)tokens / 64 + 1) > 2e9))
+        return fail(PN_ERR_SHAPE, "%s: %lld rows over tables of %lld tokens are too much for one call", name, (long long)s.T,
+                    (long long)tokens);
+    return PN_OK;
+}
 
 extern "C" {
 
@@ -1624,47 +1748,78 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     if (int st = check_kv4("pn_kv4_attention", cache, n_pages, kv_heads, page, head_dim, block_table, table_ld, table_w,
                            seq_lens, cu_q, B, T, &a.s))
         return st;
-    if (q_dtype != PN_F32 && q_dtype != PN_BF16) return fail(PN_ERR_DTYPE, "pn_kv4_attention: dtype %d", q_dtype);
-    if (q_heads < 1 || q_heads % kv_heads != 0 || q_heads > 65536)
-        return fail(PN_ERR_SHAPE, "pn_kv4_attention: %lld query heads over %lld kv heads", (long long)q_heads,
-                    (long long)kv_heads);
-    if (T > 0 && B > 0 && (!q || !out)) return fail(PN_ERR_ARG, "pn_kv4_attention: null pointer");
-    if (!(scale > 0.0f && scale < INFINITY)) return fail(PN_ERR_ARG, "pn_kv4_attention: scale must be positive");
-    const size_t e = q_dtype == PN_F32 ? 4 : 2;
-    if (!aligned(q, e) || !aligned(out, 16)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: misaligned pointer");
-    // upper bounds on the rows and units that the kernels count in 31 bits
-    if (B > 0 && ((double)T * (q_heads / kv_heads) > 2e9 ||
-                  ((double)T * (q_heads / kv_heads) / 8 + B) * kv_heads * ((double)table_w * page / 64 + 1) > 2e9))
-        return fail(PN_ERR_SHAPE, "pn_kv4_attention: %lld rows over tables of %lld tokens are too much for one call",
-                    (long long)T, (long long)(table_w * page));
+    if (int st = check_attn("pn_kv4_attention", q, q_sb, q_sl, q_sh, q_dtype, q_heads, cache, scale, out, &a)) return st;
+    if (int st = check_attn_units("pn_kv4_attention", a.s, a.G, table_w * page)) return st;
     if (int st = check_device()) return st;
     if (T == 0 || B == 0) return ok();
-    const size_t need = pn::attn_workspace(B, T, kv_heads, q_heads / kv_heads, head_dim);
+    const pn::AttnKind kind = pn::attn_kind(B, T, kv_heads, a.G);
+    const size_t need = pn::attn_workspace(kind, head_dim);
     if (!workspace || workspace_bytes < need)
         return fail(PN_ERR_WORKSPACE, "pn_kv4_attention: workspace needs %zu bytes", need);
     if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: the workspace needs 256-byte alignment");
-    a.q = q, a.q_f32 = q_dtype == PN_F32, a.q_sb = q_sb, a.q_sl = q_sl, a.q_sh = q_sh;
-    const int64_t n = 16 / (int64_t)e;
-    a.q_vec = aligned(q, 16) && q_sb % n == 0 && q_sl % n == 0 && q_sh % n == 0;
-    a.cache = static_cast<const uint8_t*>(cache);
-    a.G = (int)(q_heads / kv_heads);
-    a.scale_log2 = scale * 1.4426950408889634f;
-    a.out = out;
-    const pn::AttnKind kind = pn::attn_kind(B, T, kv_heads, a.G);
-    a.notes = static_cast<pn::Kv4Join*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + pn::attn_notes_bytes(pn::attn_blocks(kind)));
-    const cudaStream_t s = (cudaStream_t)stream;
-    auto go = [&](auto dim) {
-        constexpr int D = decltype(dim)::value;
-        switch (kind) {
-            case pn::kAttn8: return pn::launch_attn<D, pn::AttnCfg<D, 1>>(pn::kv4_decode_kernel<D, 1>, a, s);
-            case pn::kAttn16: return pn::launch_attn<D, pn::AttnCfg<D, 2>>(pn::kv4_decode_kernel<D, 2>, a, s);
-            case pn::kAttnChunk: return pn::launch_attn<D, pn::ChunkCfg<D>>(pn::kv4_chunk_kernel<D>, a, s);
-            default: return pn::launch_attn<D, pn::TcCfg<D>>(pn::kv4_long_kernel<D>, a, s);
-        }
-    };
-    const cudaError_t err = head_dim == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
+    const cudaError_t err = pn::attn_pass(a, kind, head_dim, workspace, (cudaStream_t)stream);
     return err == cudaSuccess ? ok() : cuda_fail(err, "pn_kv4_attention");
+}
+
+size_t pn_kv4_prefix_attention_workspace_size(int64_t B, int64_t T, int64_t n_prefixes, int64_t q_heads, int64_t kv_heads,
+                                              int64_t head_dim) {
+    if (B < 1 || T < 1 || n_prefixes < 0 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
+    const size_t own = pn::attn_workspace(B, T, kv_heads, q_heads / kv_heads, head_dim);
+    if (n_prefixes == 0) return own;
+    const size_t prefix = pn::attn_workspace(pn::prefix_kind(n_prefixes, T, kv_heads, q_heads / kv_heads), head_dim);
+    return pn::prefix_rows_bytes(T, q_heads, head_dim) + (prefix + 255) / 256 * 256 + own;
+}
+
+int pn_kv4_prefix_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
+                            const void* cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
+                            const int32_t* block_table, int64_t table_ld, int64_t table_w, const int32_t* seq_lens,
+                            const int32_t* cu_q, int64_t B, int64_t T, const int32_t* prefix_table, int64_t prefix_ld,
+                            int64_t prefix_w, const int32_t* prefix_lens, const int32_t* cu_prefix, int64_t n_prefixes,
+                            float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* name = "pn_kv4_prefix_attention";
+    pn::Kv4AttnArgs a{}, p{};
+    if (int st = check_kv4(name, cache, n_pages, kv_heads, page, head_dim, block_table, table_ld, table_w, seq_lens, cu_q, B, T,
+                           &a.s))
+        return st;
+    if (int st = check_attn(name, q, q_sb, q_sl, q_sh, q_dtype, q_heads, cache, scale, out, &a)) return st;
+    // (the rows of a prefix are any number of sequences': cu_q or not is the sequences' matter)
+    if (int st = check_kv4(name, cache, n_pages, kv_heads, page, head_dim, prefix_table, prefix_ld, prefix_w, prefix_lens, cu_prefix,
+                           n_prefixes, n_prefixes > 0 ? T / n_prefixes * n_prefixes : T, &p.s))
+        return st;
+    if (!cu_prefix && n_prefixes > 0 && B % n_prefixes != 0)
+        return fail(PN_ERR_SHAPE, "%s: %lld sequences over %lld prefixes need cu_prefix", name, (long long)B, (long long)n_prefixes);
+    if (T > 0 && B > 0 && n_prefixes > 0 && (!prefix_lens || (!prefix_table && prefix_w > 0)))
+        return fail(PN_ERR_ARG, "%s: null pointer", name);
+    if (int st = check_attn_units(name, a.s, a.G, table_w * page)) return st;
+    const pn::Kv4Seq own = a.s;
+    p.s.T = T, p.s.cu = cu_q, p.s.L = own.L, p.s.grouped = B, p.s.grp = cu_prefix;
+    if (int st = check_attn_units(name, p.s, a.G, prefix_w * page)) return st;
+    if (int st = check_device()) return st;
+    if (T == 0 || B == 0) return ok();
+    const size_t need = pn_kv4_prefix_attention_workspace_size(B, T, n_prefixes, q_heads, kv_heads, head_dim);
+    if (!workspace || workspace_bytes < need) return fail(PN_ERR_WORKSPACE, "%s: workspace needs %zu bytes", name, need);
+    if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "%s: the workspace needs 256-byte alignment", name);
+    const cudaStream_t s = (cudaStream_t)stream;
+    char* ws = static_cast<char*>(workspace);
+    if (n_prefixes > 0) {
+        const pn::Kv4Seq seq = p.s;
+        p = a;
+        p.s = seq;
+        p.q_l = cu_q ? 0 : own.L;
+        p.out = ws, p.out_f32 = 1;
+        p.lse = reinterpret_cast<float*>(ws) + (size_t)T * q_heads * head_dim;
+        p.grp = a.grp = cu_prefix;
+        p.n_grp = a.n_grp = (int)n_prefixes;
+        a.pre = reinterpret_cast<const float*>(ws);
+        a.pre_lse = p.lse;
+        ws += pn::prefix_rows_bytes(T, q_heads, head_dim);
+        const pn::AttnKind kind = pn::prefix_kind(n_prefixes, T, kv_heads, a.G);
+        const cudaError_t err = pn::attn_pass(p, kind, head_dim, ws, s);
+        if (err != cudaSuccess) return cuda_fail(err, name);
+        ws += (pn::attn_workspace(kind, head_dim) + 255) / 256 * 256;
+    }
+    const cudaError_t err = pn::attn_pass(a, pn::attn_kind(B, T, kv_heads, a.G), head_dim, ws, s);
+    return err == cudaSuccess ? ok() : cuda_fail(err, name);
 }
 
 }  // extern "C"

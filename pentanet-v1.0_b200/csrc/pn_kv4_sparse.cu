@@ -1,0 +1,474 @@
+// pn_kv4_sparse.cu -- attention over chosen pages of the 4-bit paged cache (layout:
+// pn_kv4.cu): the mean key of each page, a score of the means for each row, the choice,
+// and the attention kernels of pn_kv4_attn.cu over the pages chosen.
+//
+// Mathematics.  A page's mean key in a head is (sum_t s_t c_t + z_t) / n over its n tokens,
+// rounded to bf16; page i scores (sum of the group's queries) . mean_i for a row.  The
+// first and the last pages that the row sees are taken, and of the others the `top` largest
+// scores, ties by the lowest page.  Two scores that are close decide which page is read,
+// so sums and scores are fp64: a choice then depends on no order of summing short of
+// scores that agree to 2^-45 or so, and is the formula's.
+//
+// The chosen pages become a block table of the row's own, one for each kv head, in ascending
+// order, so the row's last page is the last and the only one that it may see in part;
+// the attention kernels walk it as any table, a row as a sequence of one.
+#include "pn_common.cuh"
+#include "pn_internal.h"
+
+namespace pn {
+
+// ---- means ------------------------------------------------------------------
+
+struct Kv4MeansArgs {
+    Kv4Seq s;
+    const uint8_t* cache;
+    __nv_bfloat16* means;  // (n_pages, Hk, D)
+    int rows;              // per block
+};
+constexpr int kMeansThreads = 128;
+constexpr int kMeansRows = 64;  // per block, at most
+
+// A block looks at a few rows: one that is its sequence's last, or whose successor starts a
+// page, stands for its page.  The block's warps share the tokens of each such page, lane
+// (token parity, word of eight dims), in fp64 (a code times its scale is exact in fp32).
+template <int D>
+__global__ void __launch_bounds__(kMeansThreads) kv4_means_kernel(const Kv4MeansArgs a) {
+    constexpr int WORDS = D / 8, TP = 32 / WORDS, WARPS = kMeansThreads / 32;  // words of a key, tokens per warp and step
+    __shared__ int64_t at[kMeansRows];
+    __shared__ int held[kMeansRows];
+    __shared__ int count;
+    __shared__ double sums[WARPS * TP][D + 1];
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    const int64_t row = (int64_t)blockIdx.x * a.rows + tid;
+    int64_t b, i;
+    if (tid < a.rows && row < a.s.T && kv4_find(a.s, row, b, i)) {
+        int64_t first, n;
+        kv4_rows(a.s, b, first, n);
+        const int len = kv4_len(a.s, b);
+        const int64_t pos = len - n + i;
+        if (pos >= 0 && (i == n - 1 || (pos + 1) % a.s.page == 0)) {
+            const int64_t page = kv4_page(a.s, b, (int)pos);
+            if (page >= 0) {
+                const int k = atomicAdd(&count, 1);  // (pages are done one by one: their order does not matter)
+                at[k] = page;
+                held[k] = (int)min((int64_t)a.s.page, len - pos / a.s.page * a.s.page);
+            }
+        }
+    }
+    __syncthreads();
+    const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
+    const int word = lane % WORDS, sub = warp * TP + lane / WORDS;
+    for (int k = 0; k < count; ++k) {
+        const int64_t head = at[k] * a.s.Hk + blockIdx.y;
+        const uint8_t* p = a.cache + head * 2 * block;
+        const int n = held[k];
+        double acc[8], zeros = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = 0.0;
+#pragma unroll 4
+        for (int t = sub; t < n; t += WARPS * TP) {
+            const uint32_t c = *reinterpret_cast<const uint32_t*>(p + t * (D / 2) + word * 4);
+            const uint32_t pair = *reinterpret_cast<const uint32_t*>(p + a.s.page * (D / 2) + t * 4);
+            const float s = __uint_as_float(pair << 16), z = __uint_as_float(pair & 0xFFFF0000u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[j] += (double)(s * (float)(c >> (4 * j) & 15));
+            zeros += (double)z;
+        }
+        __syncthreads();  // the sums of the page before are read
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[sub][word * 8 + j] = acc[j] + zeros;
+        __syncthreads();
+        for (int d = tid; d < D; d += kMeansThreads) {
+            double sum = 0.0;
+#pragma unroll
+            for (int w = 0; w < WARPS * TP; ++w) sum += sums[w][d];
+            a.means[head * D + d] = __float2bfloat16_rn(__double2float_rn(sum / n));
+        }
+    }
+}
+
+// ---- scores -----------------------------------------------------------------
+
+// Scores as keys whose order as integers is theirs as numbers; 0: a NaN, or a page that is not
+// there, taken last.
+__device__ __forceinline__ uint64_t score_key(double v) {
+    if (v != v) return 0;
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);  // -0 counts as 0
+    return u >> 63 ? ~u : u | 0x8000000000000000ull;
+}
+
+struct Kv4SelectArgs {
+    Kv4Seq s;
+    const void* q;
+    int q_f32, q_vec;
+    int64_t q_sb, q_sl, q_sh;
+    int G;
+    const __nv_bfloat16* means;
+    int first, last, top;
+    int width;            // first + last + top: pages of a row's table
+    uint64_t* keys;       // workspace (T, Hk, table_w): scores
+    int32_t* pages;       // workspace (T, Hk, width): the chosen pages, as entries of the block table
+    int32_t* lens;        // workspace (T): tokens of them; -1: no row
+    int32_t* chosen;      // (T, Hk, width): their numbers in the sequence, or null
+    int tile;             // rows of a block of the score kernel
+    int splits;           // blocks that share the pages
+};
+constexpr int kScoreThreads = 128;
+constexpr int kScoreTile = 8;
+
+// Where a row is: its sequence, and the pages [0, first), [first, free_end) and
+// [free_end, seen) that are taken, may be chosen, and are taken.
+struct SelectRow {
+    int64_t b, i;
+    int seen, free_end, len;  // len: tokens that the row sees; -1: no row
+    bool over;                // the table has no room for all of them
+    __device__ __forceinline__ SelectRow(const Kv4SelectArgs& a, int64_t row)
+        : b(0), i(0), seen(0), free_end(0), len(-1), over(false) {
+        if (row >= a.s.T || !kv4_find(a.s, row, b, i)) return;
+        int64_t at, n;
+        kv4_rows(a.s, b, at, n);
+        const int64_t pos = (int64_t)kv4_len(a.s, b) - n + i;
+        len = (int)min(max(pos + 1, (int64_t)0), (int64_t)a.s.table_w * a.s.page);
+        over = pos >= (int64_t)a.s.table_w * a.s.page && a.s.table_w > 0;
+        seen = (len + a.s.page - 1) / a.s.page;
+        free_end = max(seen - a.last, 0);
+    }
+};
+
+// A block scores some pages for up to `tile` rows of one kv head.  Four lanes share a page's
+// mean, held as fp64 for all rows of a sequence in turn; the group's queries are summed
+// once per block.
+template <int D>
+__global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4SelectArgs a) {
+    constexpr int E = D / 4;  // dims per lane: chunks of 8, four lanes in turn
+    __shared__ double q[kScoreTile][D];
+    __shared__ int seq[kScoreTile], from[kScoreTile], to[kScoreTile];
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row0 = (int64_t)blockIdx.x * a.tile;
+    const int head = blockIdx.y;
+    for (int r = 0; r < a.tile; ++r) {
+        const SelectRow at(a, row0 + r);
+        const int n = max(at.free_end - a.first, 0);
+        if (tid == 0) {
+            seq[r] = n > a.top ? (int)at.b : -1;  // (with fewer pages all are taken)
+            from[r] = a.first, to[r] = at.free_end;
+        }
+        if (n <= a.top) continue;
+        const int64_t base = a.s.cu ? (row0 + r) * a.q_sl : at.b * a.q_sb + at.i * a.q_sl;
+        for (int d = tid; d < D; d += kScoreThreads) {
+            double sum = 0.0;
+            for (int g = 0; g < a.G; ++g) {
+                const int64_t p = base + (int64_t)(head * a.G + g) * a.q_sh + d;
+                sum += (double)(a.q_f32 ? static_cast<const float*>(a.q)[p]
+                                        : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[p]));
+            }
+            q[r][d] = sum;
+        }
+    }
+    __syncthreads();
+    const int part = lane & 3, sub = warp * 8 + (lane >> 2);
+    for (int r0 = 0; r0 < a.tile;) {
+        if (seq[r0] < 0) {
+            ++r0;
+            continue;
+        }
+        int r1 = r0 + 1, lo = from[r0], hi = to[r0];
+        for (; r1 < a.tile && seq[r1] == seq[r0]; ++r1) hi = max(hi, to[r1]);
+        const int64_t b = seq[r0];
+        // the pages [lo, hi) in runs of 32 to a block
+        for (int base = lo + blockIdx.z * 32; base < hi; base += a.splits * 32) {
+            const int i = base + sub;
+            const int p = i < hi ? __ldg(a.s.table + b * a.s.table_ld + i) : -1;
+            const bool there = p >= 0 && p < a.s.n_pages;
+            double m[E];
+            const uint4* src = reinterpret_cast<const uint4*>(a.means + ((int64_t)p * a.s.Hk + head) * D);
+#pragma unroll
+            for (int c = 0; c < E / 8; ++c) {
+                const uint4 u = there ? src[c * 4 + part] : make_uint4(0, 0, 0, 0);
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    m[c * 8 + 2 * j] = (double)__uint_as_float(w[j] << 16);
+                    m[c * 8 + 2 * j + 1] = (double)__uint_as_float(w[j] & 0xFFFF0000u);
+                }
+            }
+            for (int r = r0; r < r1; ++r) {
+                double sum = 0.0, sum2 = 0.0;
+#pragma unroll
+                for (int c = 0; c < E / 8; ++c)
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const double2 x = *reinterpret_cast<const double2*>(&q[r][(c * 4 + part) * 8 + j]);
+                        sum = fma(x.x, m[c * 8 + j], sum);
+                        sum2 = fma(x.y, m[c * 8 + j + 1], sum2);
+                    }
+                sum += sum2;
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (part == 0 && i < to[r])
+                    a.keys[((row0 + r) * a.s.Hk + head) * a.s.table_w + i] = there ? score_key(sum) : 0;
+            }
+        }
+        r0 = r1;
+    }
+}
+
+// ---- choice -----------------------------------------------------------------
+
+constexpr int kSelectThreads = 256;
+constexpr int kSelectBins = 2048;
+
+// The threshold of the `top` largest of n keys by their digits from the highest: a histogram
+// of the digit among the keys that share the digits before, the bin where the count from
+// above reaches `need`, and so on, until that bin is taken whole (most often at the second
+// digit) or the digits are out.  Then one pass over the pages in order writes those above the
+// threshold and the first `need` of those at it.  One block per row and kv head.
+__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Kv4SelectArgs a) {
+    __shared__ int bins[kSelectBins];
+    __shared__ int warp_sums[kSelectThreads / 32];
+    __shared__ int border[2];  // the bin, and how many of it are needed
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = blockIdx.x / a.s.Hk;
+    const int head = (int)(blockIdx.x - row * a.s.Hk);
+    SelectRow at(a, row);
+    if (a.s.cu) {  // row starts that fall: nothing is computed
+        bool falls = false;
+        for (int b = tid; b < a.s.B; b += kSelectThreads) falls |= __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
+        if (__syncthreads_or(falls)) {
+            at.len = -1, at.seen = at.free_end = 0, at.over = true;
+        }
+    }
+    if (at.over && head == 0 && tid == 0) record_status(PN_ERR_ARG);
+    const int64_t list = (row * a.s.Hk + head) * a.width;
+    const int n = max(at.free_end - a.first, 0);
+    uint64_t edge = 0;  // taken: keys whose digits above `shift` exceed it, and `need` of those that equal it
+    int shift = 0, need = 0;
+    const uint64_t* keys = a.keys + (row * a.s.Hk + head) * a.s.table_w + a.first;
+    const bool choose = n > a.top;
+    if (choose && a.top > 0) {
+        need = a.top;
+        shift = 64;
+        for (int width = 11; shift > 0; shift -= width) {
+            if (shift < width) width = shift;
+            for (int i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
+            __syncthreads();
+            const int low = shift - width;
+            for (int i = tid; i < n; i += kSelectThreads) {
+                const uint64_t k = keys[i];
+                if (shift == 64 || k >> shift == edge) atomicAdd(&bins[(k >> low) & ((1 << width) - 1)], 1);
+            }
+            __syncthreads();
+            // thread t has bins [8 (255 - t), + 8): counts from above
+            constexpr int PER = kSelectBins / kSelectThreads;
+            int mine = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) mine += bins[(kSelectThreads - 1 - tid) * PER + j];
+            int inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            if (lane == 31) warp_sums[warp] = inc;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) inc += warp_sums[w];
+            int above = inc - mine;
+            if (above < need && need <= inc) {
+                int j = PER - 1;
+                for (;; --j) {
+                    const int c = bins[(kSelectThreads - 1 - tid) * PER + j];
+                    if (above + c >= need) break;
+                    above += c;
+                }
+                border[0] = (kSelectThreads - 1 - tid) * PER + j;
+                border[1] = need - above;
+            }
+            __syncthreads();
+            edge = (shift == 64 ? 0 : edge << width) | (uint32_t)border[0];
+            need = border[1];
+            const bool whole = bins[border[0]] == need;
+            __syncthreads();
+            if (whole) {
+                shift = low;
+                break;
+            }
+        }
+    }
+    // the pages in order
+    if (head == 0 && tid == 0) {
+        const int kept = choose ? min(a.first, at.seen) + a.top + (at.seen - at.free_end) : at.seen;
+        // all pages but the last are whole
+        a.lens[row] = at.len <= 0 ? at.len : (kept - 1) * a.s.page + at.len - (at.seen - 1) * a.s.page;
+    }
+    int done = 0, equal = 0;  // pages written, keys at the edge met so far
+    for (int base = 0; base < at.seen; base += kSelectThreads) {
+        const int i = base + tid;
+        bool take = false, tie = false;
+        if (i < at.seen) {
+            if (!choose || i < a.first || i >= at.free_end) {
+                take = true;
+            } else if (a.top > 0) {
+                const uint64_t k = keys[i - a.first] >> shift;
+                take = k > edge;
+                tie = k == edge;
+            }
+        }
+        // how many of either lie before: taken ones in the low half, ties in the high one
+        const uint32_t m_take = __ballot_sync(0xffffffffu, take), m_tie = __ballot_sync(0xffffffffu, tie);
+        const uint32_t under = (1u << lane) - 1;
+        __syncthreads();
+        if (lane == 0) warp_sums[warp] = __popc(m_take) | __popc(m_tie) << 16;
+        __syncthreads();
+        int taken = __popc(m_take & under), ties = __popc(m_tie & under), all_taken = 0, all_ties = 0;
+#pragma unroll
+        for (int w = 0; w < kSelectThreads / 32; ++w) {
+            const int v = warp_sums[w];
+            if (w < warp) taken += v & 0xFFFF, ties += v >> 16;
+            all_taken += v & 0xFFFF, all_ties += v >> 16;
+        }
+        const int ties_before = min(equal + ties, need);
+        if (take || (tie && equal + ties < need)) {
+            const int slot = done + taken + ties_before - min(equal, need);
+            a.pages[list + slot] = i < a.s.table_w ? __ldg(a.s.table + at.b * a.s.table_ld + i) : -1;
+            if (a.chosen) a.chosen[list + slot] = i;
+        }
+        done += all_taken + min(equal + all_ties, need) - min(equal, need);
+        equal += all_ties;
+    }
+    for (int i = done + tid; i < a.width; i += kSelectThreads) {
+        a.pages[list + i] = -1;
+        if (a.chosen) a.chosen[list + i] = -1;
+    }
+}
+
+struct SparseLayout {  // of the workspace
+    size_t keys, pages, lens, total;
+    SparseLayout(int64_t T, int64_t Hk, int64_t G, int64_t D, int64_t table_w, int64_t width) {
+        keys = 0;
+        pages = keys + round256((size_t)T * Hk * table_w * 8);
+        lens = pages + round256((size_t)T * Hk * width * 4);
+        total = lens + round256((size_t)T * 4);
+        attn = total;
+        total += attn_workspace(T, T, Hk, G, D);
+    }
+    size_t attn;
+};
+
+template <typename... Args>
+static cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, unsigned threads, cudaStream_t s, const Args&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+}  // namespace pn
+
+extern "C" {
+
+int pn_kv4_page_means(const void* cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
+                      const int32_t* block_table, int64_t table_ld, int64_t table_w, const int32_t* seq_lens,
+                      const int32_t* cu_q, int64_t B, int64_t T, void* means, void* stream) {
+    const char* name = "pn_kv4_page_means";
+    pn::Kv4MeansArgs a{};
+    if (int st = check_kv4(name, cache, n_pages, kv_heads, page, head_dim, block_table, table_ld, table_w, seq_lens, cu_q, B, T,
+                           &a.s))
+        return st;
+    if (T > 0 && B > 0 && !means && n_pages > 0) return fail(PN_ERR_ARG, "%s: null pointer", name);
+    if (!aligned(means, 16)) return fail(PN_ERR_ALIGN, "%s: means needs 16-byte alignment", name);
+    if (kv_heads > 65535) return fail(PN_ERR_SHAPE, "%s: %lld kv heads", name, (long long)kv_heads);
+    if (int st = check_device()) return st;
+    if (T == 0 || B == 0) return ok();
+    a.cache = static_cast<const uint8_t*>(cache);
+    a.means = static_cast<__nv_bfloat16*>(means);
+    // as many rows to a block as leave four blocks to an SM
+    a.rows = pn::kMeansRows;
+    while (a.rows > 1 && T / a.rows * kv_heads < 4 * pn::sm_count()) a.rows /= 2;
+    const dim3 grid((unsigned)((T + a.rows - 1) / a.rows), (unsigned)kv_heads);
+    const cudaError_t err = head_dim == 64 ? pn::launch_dependent(pn::kv4_means_kernel<64>, grid, pn::kMeansThreads, (cudaStream_t)stream, a)
+                                           : pn::launch_dependent(pn::kv4_means_kernel<128>, grid, pn::kMeansThreads, (cudaStream_t)stream, a);
+    return err == cudaSuccess ? ok() : cuda_fail(err, name);
+}
+
+size_t pn_kv4_sparse_attention_workspace_size(int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t table_w,
+                                              int64_t width) {
+    if (T < 1 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1 || table_w < 0 || width < 1) return 0;
+    return pn::SparseLayout(T, kv_heads, q_heads / kv_heads, head_dim, table_w, width).total;
+}
+
+int pn_kv4_sparse_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
+                            const void* cache, const void* means, int64_t n_pages, int64_t kv_heads, int64_t page,
+                            int64_t head_dim, const int32_t* block_table, int64_t table_ld, int64_t table_w,
+                            const int32_t* seq_lens, const int32_t* cu_q, int64_t B, int64_t T, int64_t first_pages,
+                            int64_t last_pages, int64_t top_pages, float scale, void* out, int32_t* chosen, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+    const char* name = "pn_kv4_sparse_attention";
+    pn::Kv4AttnArgs a{};
+    if (int st = check_kv4(name, cache, n_pages, kv_heads, page, head_dim, block_table, table_ld, table_w, seq_lens, cu_q, B, T,
+                           &a.s))
+        return st;
+    if (int st = check_attn(name, q, q_sb, q_sl, q_sh, q_dtype, q_heads, cache, scale, out, &a)) return st;
+    if (first_pages < 0 || last_pages < 1 || top_pages < 0 || first_pages > 1 << 30 || last_pages > 1 << 30 || top_pages > 1 << 30)
+        return fail(PN_ERR_SHAPE, "%s: first=%lld last=%lld top=%lld pages", name, (long long)first_pages, (long long)last_pages,
+                    (long long)top_pages);
+    const int64_t width = first_pages + last_pages + top_pages;
+    if (width > (1 << 30) / page) return fail(PN_ERR_SHAPE, "%s: %lld pages to a row", name, (long long)width);
+    if (T > 0 && B > 0 && !means && n_pages > 0) return fail(PN_ERR_ARG, "%s: null pointer", name);
+    if (!aligned(means, 16)) return fail(PN_ERR_ALIGN, "%s: means needs 16-byte alignment", name);
+    if (!aligned(chosen, 4)) return fail(PN_ERR_ALIGN, "%s: misaligned pointer", name);
+    if (kv_heads > 65535 || (double)T * kv_heads > 2e9) return fail(PN_ERR_SHAPE, "%s: %lld rows of %lld kv heads", name, (long long)T, (long long)kv_heads);
+    if ((double)T * kv_heads * ((double)table_w + width) * 8 > 6e10)
+        return fail(PN_ERR_SHAPE, "%s: %lld rows over tables of %lld pages are too much for one call", name, (long long)T, (long long)table_w);
+    if (int st = check_attn_units(name, a.s, a.G, std::min(width, table_w) * page)) return st;
+    if (int st = check_device()) return st;
+    if (T == 0 || B == 0) return ok();
+    const pn::SparseLayout lay(T, kv_heads, a.G, head_dim, a.s.table_w, width);
+    if (!workspace || workspace_bytes < lay.total) return fail(PN_ERR_WORKSPACE, "%s: workspace needs %zu bytes", name, lay.total);
+    if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "%s: the workspace needs 256-byte alignment", name);
+    char* ws = static_cast<char*>(workspace);
+    pn::Kv4SelectArgs c{};
+    c.s = a.s;
+    c.q = q, c.q_f32 = a.q_f32, c.q_vec = a.q_vec, c.q_sb = q_sb, c.q_sl = q_sl, c.q_sh = q_sh, c.G = a.G;
+    c.means = static_cast<const __nv_bfloat16*>(means);
+    c.first = (int)first_pages, c.last = (int)last_pages, c.top = (int)top_pages, c.width = (int)width;
+    c.keys = reinterpret_cast<uint64_t*>(ws + lay.keys);
+    c.pages = reinterpret_cast<int32_t*>(ws + lay.pages);
+    c.lens = reinterpret_cast<int32_t*>(ws + lay.lens);
+    c.chosen = chosen;
+    const cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t err = cudaSuccess;
+    if (top_pages > 0 && a.s.table_w > width) {  // (else every page is taken)
+        c.tile = 1;
+        while (c.tile < pn::kScoreTile && 2 * c.tile <= T / B) c.tile *= 2;
+        const int64_t tiles = (T + c.tile - 1) / c.tile, runs = (a.s.table_w + 31) / 32;
+        c.splits = (int)std::min<int64_t>(std::max<int64_t>(8 * pn::sm_count() / (tiles * kv_heads), 1), std::min<int64_t>(runs, 65535));
+        const dim3 grid((unsigned)tiles, (unsigned)kv_heads, (unsigned)c.splits);
+        err = head_dim == 64 ? pn::launch_dependent(pn::kv4_score_kernel<64>, grid, pn::kScoreThreads, s, c)
+                             : pn::launch_dependent(pn::kv4_score_kernel<128>, grid, pn::kScoreThreads, s, c);
+        if (err != cudaSuccess) return cuda_fail(err, name);
+    }
+    err = pn::launch_dependent(pn::kv4_select_kernel, dim3((unsigned)(T * kv_heads)), pn::kSelectThreads, s, c);
+    if (err != cudaSuccess) return cuda_fail(err, name);
+    // every row a sequence of its own
+    a.q_l = cu_q ? T : a.s.L;  // (with cu_q rows lie one after another)
+    a.s.table = c.pages, a.s.table_hd = width, a.s.table_ld = kv_heads * width, a.s.table_w = n_pages > 0 ? (int)width : 0;
+    a.s.lens = c.lens, a.s.cu = nullptr, a.s.B = T, a.s.L = 1;
+    err = pn::attn_pass(a, pn::attn_kind(T, T, kv_heads, a.G), head_dim, ws + lay.attn, s);
+    return err == cudaSuccess ? ok() : cuda_fail(err, name);
+}
+
+}  // extern "C"

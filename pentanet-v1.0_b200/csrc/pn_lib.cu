@@ -18,5 +18,7 @@
 #include "pn_ternary2.cu"
 #include "pn_rms.cu"
 #include "pn_kv4.cu"
+#include "pn_kv4_rotary.cu"
 #include "pn_kv4_attn.cu"
+#include "pn_kv4_sparse.cu"
 #include "pn_sample.cu"

@@ -35,6 +35,8 @@ EXPORTS = (
     "pn_words_2bit", "pn_quantize_pack_2bit", "pn_unpack_2bit", "pn_linear_bf16_2bit",
     "pn_rms_norm", "pn_rms_norm_i8", "pn_dequant_act_i8", "pn_kv4_block_bytes", "pn_kv4_append", "pn_kv4_gather",
     "pn_kv4_attention_workspace_size", "pn_kv4_attention", "pn_sample_tokens",
+    "pn_kv4_append_rotary", "pn_kv4_prefix_attention_workspace_size", "pn_kv4_prefix_attention", "pn_kv4_page_means",
+    "pn_kv4_sparse_attention_workspace_size", "pn_kv4_sparse_attention",
 )
 
 _lib = None
@@ -107,6 +109,15 @@ def load() -> ctypes.CDLL:
         "pn_kv4_attention_workspace_size": (SZ, [I64, I64, I64, I64, I64]),
         "pn_kv4_attention": (I, [P, I64, I64, I64, I, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, F, P, P,
                                  SZ, P]),
+        "pn_kv4_append_rotary": (I, [P, I64, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I, P, P, I64, I64, I64, I, P,
+                                     P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, P]),
+        "pn_kv4_prefix_attention_workspace_size": (SZ, [I64, I64, I64, I64, I64, I64]),
+        "pn_kv4_prefix_attention": (I, [P, I64, I64, I64, I, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64,
+                                        P, I64, I64, P, P, I64, F, P, P, SZ, P]),
+        "pn_kv4_page_means": (I, [P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, P]),
+        "pn_kv4_sparse_attention_workspace_size": (SZ, [I64, I64, I64, I64, I64, I64]),
+        "pn_kv4_sparse_attention": (I, [P, I64, I64, I64, I, I64, P, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64,
+                                        I64, I64, I64, F, P, P, P, SZ, P]),
         "pn_sample_tokens": (I, [P, I, I64, I64, I64, P, P, F, P, ctypes.c_int32, P, F, P, F, P, P]),
     }
     for name, (res, args) in sig.items():
