@@ -19,7 +19,7 @@ OUT = os.path.join(HERE, "libpentanet_b200.so")
 SOURCES = ["csrc/pn_lib.cu"]
 DEPS = ["csrc/pn_common.cuh", "csrc/pn_internal.h", "csrc/pn_pack.cu", "csrc/pn_act.cu", "csrc/pn_norm.cu",
         "csrc/pn_dqmm.cu", "csrc/pn_simt.cu", "csrc/pn_gemv.cu", "csrc/pn_capi.cu", "csrc/pn_static_ws.cu", "csrc/pn_peer.cu", "csrc/pn_i8w.cu", "csrc/pn_ternary2.cu",
-        "csrc/pn_rms.cu", "csrc/pn_kv4.cu", "csrc/pn_kv4_rotary.cu", "csrc/pn_kv4_attn.cu", "csrc/pn_kv4_sparse.cu",
+        "csrc/pn_rms.cu", "csrc/pn_kv4.cu", "csrc/pn_kv4_rotary.cu", "csrc/pn_kv4_attn.cu", "csrc/pn_kv4_prefix.cu", "csrc/pn_kv4_sparse.cu",
         "csrc/pn_sample.cu",
         "csrc/pn_lib.cu", "../include/pentanet_b200.h"]
 

@@ -48,8 +48,13 @@ struct Kv4Join {
     int G;
     int64_t row0;    // first row of the tile's sequence
     int64_t r0;      // first query row of the tile
-    int head;
-    int joins;       // the rows have a prefix's results to join
+    int64_t head;
+};
+
+// Where a row tile's results are, at its first row: in `out` (last < 0), or in the partial results
+// of blocks [first, last], the first's being its first_slot-th.
+struct Kv4Where {
+    int first, first_slot, last, pad;
 };
 
 struct Kv4AttnArgs {
@@ -65,13 +70,12 @@ struct Kv4AttnArgs {
     int out_f32;
     Kv4Join* notes;    // workspace: one per block
     float* part;       // workspace: partial results of two segments per block
-    // Rows that attend to a shared prefix and to their own sequence.  The call over the
-    // prefixes writes fp32 results with the logarithms (base 2) of their totals (lse), that over
-    // the sequences joins them to its own (pre, pre_lse), for the sequences that have a prefix:
-    // [grp[0], grp[n_grp]), or all.
-    float* lse;              // (T, Hk * G), or null
-    const float *pre, *pre_lse;
-    const int32_t* grp;      // (n_grp + 1), or null
+    // A pass whose results another kernel joins with those of a second pass: out is fp32, with the
+    // logarithms (base 2) of the rows' totals in lse, and a record per row tile says where
+    // its results are.  (T, Hk * G) each; null: the pass is all there is.
+    float* lse;
+    Kv4Where* where;
+    const int32_t* grp;  // (n_grp + 1) or null: shares of prefixes that may fall, where nothing is computed
     int n_grp;
 };
 
@@ -144,6 +148,12 @@ __device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, 
     kv4_rows(a.s, b, first, n);
     if (a.s.table_hd && __ldg(a.s.lens + b) < 0) n = 0;  // (of chosen pages: a row that is no sequence's)
     nt = max((kv4_held(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
+    if constexpr (C::kPaired) {  // nt: of the last row tile, whose units are twice as long where it has half the rows
+        const uint32_t rows = (uint32_t)n * a.G, tiles = (rows + C::kRows - 1) / C::kRows, full = nt;
+        if (tiles == 0) return 0;
+        if (rows - (tiles - 1) * C::kRows <= C::kRows / 2) nt = (nt + 1) / 2;
+        return ((tiles - 1) * full + nt) * a.s.Hk;
+    }
     return ((uint32_t)n * a.G + C::kRows - 1) / C::kRows * nt * a.s.Hk;
 }
 
@@ -211,12 +221,27 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
     return run;
 }
 
+// Where query row r of a row tile lies in q, in elements.
+__device__ __forceinline__ int64_t attn_query(const Kv4AttnArgs& a, uint32_t b, int64_t row0, int64_t r0, int head, int r) {
+    const uint32_t rr = (uint32_t)r0 + r, i = rr / a.G;
+    int64_t at;
+    if (a.s.cu) {
+        at = (row0 + i) * a.q_sl;
+    } else if (a.q_l) {
+        const int64_t of = (row0 + i) / a.q_l;
+        at = of * a.q_sb + (row0 + i - of * a.q_l) * a.q_sl;
+    } else {
+        at = b * a.q_sb + i * a.q_sl;
+    }
+    return at + (head * a.G + (rr - i * a.G)) * a.q_sh;
+}
+
 // One segment: a run of units of one row tile.
 struct AttnSeg {
     uint32_t b, nt, t0, t1;  // sequence; token tiles of it, and the segment's [t0, t1)
     int head, rows;          // kv head; query rows in the tile
     int64_t row0, r0;        // first row of the sequence; first query row of the tile
-    int pos0;                // query row r sees positions up to pos0 + r / G (of a prefix: all)
+    int pos0;                // query row r sees positions up to pos0 + r / G
     int kv_end;              // tokens that the tile's last row sees (and the table has room for)
     int lim_min;             // the last position that its first row sees (at most kv_end - 1)
 
@@ -242,43 +267,33 @@ struct AttnSeg {
         rows = (int)min((uint32_t)C::kRows, q_rows - (uint32_t)r0);
         t0 = in_seq - tile * nt;
         t1 = min(nt, t0 + left);
-        pos0 = a.s.grouped ? kv4_held(a.s, b) - 1 : kv4_len(a.s, b) - (int)n_rows;
+        pos0 = kv4_len(a.s, b) - (int)n_rows;
         kv_end = min(max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0), kv4_held(a.s, b));
-        if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && kv4_len(a.s, b) > kv4_held(a.s, b)) record_status(PN_ERR_ARG);
-        lim_min = last_seen(a, 0);
+        if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && pos0 + (int)n_rows > kv4_held(a.s, b)) record_status(PN_ERR_ARG);
+        lim_min = min(pos0 + (int)((uint32_t)r0 / a.G), kv_end - 1);
     }
-    // The last position that query row r of the tile sees.
-    __device__ __forceinline__ int last_seen(const Kv4AttnArgs& a, int r) const {
-        return min(pos0 + (int)(((uint32_t)r0 + r) / a.G), kv_end - 1);
-    }
-    // Whether the rows have a prefix's results to join.
-    __device__ __forceinline__ bool joins(const Kv4AttnArgs& a) const {
-        return a.pre && (!a.grp || ((int)b >= __ldg(a.grp) && (int)b < __ldg(a.grp + a.n_grp)));
-    }
-    // Where query row r of the tile (r < rows) lies in q, in elements.
-    __device__ __forceinline__ int64_t query(const Kv4AttnArgs& a, int r) const {
-        const uint32_t rr = (uint32_t)r0 + r, i = rr / a.G;
-        int64_t at;
-        if (a.s.cu) {
-            at = (row0 + i) * a.q_sl;
-        } else if (a.q_l) {
-            const int64_t of = (row0 + i) / a.q_l;
-            at = of * a.q_sb + (row0 + i - of * a.q_l) * a.q_sl;
-        } else {
-            at = b * a.q_sb + i * a.q_sl;
-        }
-        return at + (head * a.G + (rr - i * a.G)) * a.q_sh;
-    }
+    __device__ __forceinline__ int64_t query(const Kv4AttnArgs& a, int r) const { return attn_query(a, b, row0, r0, head, r); }
 };
 
 // Leaves the joining kernel a note where a row tile ends in this block and began
 // in an earlier one.
-__device__ __forceinline__ void attn_note(const Kv4AttnArgs& a, const AttnRun& run, const AttnSeg& sg, uint32_t unit) {
-    if (sg.t0 == 0 || sg.t1 != sg.nt) return;
+template <typename Seg>
+__device__ __forceinline__ void attn_note(const Kv4AttnArgs& a, const AttnRun& run, const Seg& sg, uint32_t unit) {
+    if (sg.t1 != sg.nt || (sg.t0 == 0 && !a.where)) return;
+    const uint32_t i0 = (uint32_t)sg.r0 / a.G;
+    const int64_t row = ((sg.row0 + i0) * a.s.Hk + sg.head) * a.G + (uint32_t)sg.r0 - i0 * a.G;
+    if (sg.t0 == 0) {
+        a.where[row] = {0, 0, -1, 0};
+        return;
+    }
     // the block that holds the tile's first unit: the first `rem` blocks hold one more
     const uint32_t u0 = unit - sg.t0, each = run.total / gridDim.x, rem = run.total % gridDim.x;
     const uint32_t c0 = u0 < (each + 1) * rem ? u0 / (each + 1) : rem + (u0 - (each + 1) * rem) / each;
-    a.notes[blockIdx.x] = {sg.rows, (int)c0, attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0, a.G, sg.row0, sg.r0, sg.head, sg.joins(a)};
+    const int slot = attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0;
+    if (a.where)
+        a.where[row] = {(int)c0, slot, (int)blockIdx.x, 0};
+    else
+        a.notes[blockIdx.x] = {sg.rows, (int)c0, slot, a.G, sg.row0, sg.r0, sg.head};
 }
 
 // Looks up the pages of a sequence, 32 pieces of 16 tokens at a time: lane l
@@ -301,37 +316,15 @@ struct AttnPages {
     }
 };
 
-// How a row's sums y (relative to 2^m, their total `sum`) become its result: y * k1 + pre * k2,
-// with the row of a prefix's results where it joins them.  (A total of 0: nothing was seen.)
-struct RowScale {
-    float k1, k2;
-    bool add;  // whether there is a prefix's row (k2 may be 0, its values not be finite)
-    __device__ __forceinline__ RowScale(const Kv4AttnArgs& a, int64_t row, float m, float sum, bool joins) {
-        k1 = sum == 0.0f ? 0.0f : 1.0f / sum;
-        k2 = 0.0f;
-        add = false;
-        if (!joins) return;
-        const float l1 = a.pre_lse[row], l2 = lse(m, sum), top = fmaxf(l1, l2);
-        if (l1 == -INFINITY) return;
-        const float w1 = ex2f(l1 - top), w2 = sum == 0.0f ? 0.0f : ex2f(l2 - top), each = 1.0f / (w1 + w2);
-        add = true;
-        k1 *= w2 * each;
-        k2 = w1 * each;
-    }
-    static __device__ __forceinline__ float lse(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
-};
-__device__ __forceinline__ void store_out(const Kv4AttnArgs& a, int64_t at, const float4& y, const RowScale& k) {
-    float4 v = make_float4(y.x * k.k1, y.y * k.k1, y.z * k.k1, y.w * k.k1);
-    if (k.add) {
-        const float4 u = *reinterpret_cast<const float4*>(a.pre + at);
-        v = make_float4(fmaf(u.x, k.k2, v.x), fmaf(u.y, k.k2, v.y), fmaf(u.z, k.k2, v.z), fmaf(u.w, k.k2, v.w));
-    }
+// The logarithm of a row's total `sum`, which is relative to 2^m.
+__device__ __forceinline__ float attn_lse(float m, float sum) { return sum == 0.0f ? -INFINITY : m + log2f(sum); }
+__device__ __forceinline__ void store_out(const Kv4AttnArgs& a, int64_t at, const float4& y, float inv) {
     if (a.out_f32) {
-        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = v;
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
     } else {
-        const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x, v.y), hi = __floats2bfloat162_rn(v.z, v.w);
+        const __nv_bfloat162 u = __floats2bfloat162_rn(y.x * inv, y.y * inv), v = __floats2bfloat162_rn(y.z * inv, y.w * inv);
         *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + at) =
-            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&v));
     }
 }
 
@@ -412,6 +405,7 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
 // registers do not suffice (372 bytes spilled per thread).
 template <int D, int NT>
 struct AttnCfg {
+    static constexpr bool kPaired = false;
     static constexpr int W = D / 32;             // words per thread and token
     static constexpr int kRows = 8 * NT;         // query rows of a row tile
     static constexpr int kTokens = 128;          // tokens of a unit: 32 per warp
@@ -530,7 +524,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                 else
                     ca[n].y = va, cb[n].y = vb;
                 const int rl = n * 8 + 2 * t + k;
-                lim[n][k] = rl < sg.rows ? sg.last_seen(a, rl) : sg.kv_end - 1;
+                lim[n][k] = rl < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + rl) / a.G) : sg.kv_end - 1;
             }
         }
 
@@ -732,7 +726,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
             }
         }
         __syncthreads();
-        const bool whole = sg.t0 == 0 && sg.t1 == sg.nt, joins = whole && sg.joins(a);
+        const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
         for (int idx = tid; idx < sg.rows * (D / 4); idx += kAttnThreads) {
             const int r = idx / (D / 4), d = (idx - r * (D / 4)) * 4;
@@ -753,8 +747,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
             if (whole) {
                 const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
                 const int64_t at = ((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G;
-                store_out(a, at * D + d, y, RowScale(a, at, mx, sum, joins));
-                if (a.lse && d == 0) a.lse[at] = RowScale::lse(mx, sum);
+                store_out(a, at * D + d, y, sum == 0.0f ? 0.0f : 1.0f / sum);
+                if (a.lse && d == 0) a.lse[at] = attn_lse(mx, sum);
             } else {
                 *reinterpret_cast<float4*>(part + r * D + d) = y;
                 if (d == 0) part[RT * D + r * 2] = mx, part[RT * D + r * 2 + 1] = sum;
@@ -782,6 +776,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 // tokens: 72 us (two blocks to an SM: 2 % slower than three); 148 bytes spilled per thread.
 template <int D>
 struct ChunkCfg {
+    static constexpr bool kPaired = false;
     static constexpr int W = D / 32;
     static constexpr int kRows = 64, kTokens = 64, kThreads = kAttnThreads;
     static constexpr int kStages = 3;
@@ -854,11 +849,11 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
             const char* row = nullptr;
             if (r < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, r) * (a.q_f32 ? 4 : 2);
             load_query<D>(a, row, t, k ? qc : qa, ca[k], cb[k]);
-            lim[k] = r < sg.rows ? sg.last_seen(a, r) : sg.kv_end - 1;
+            lim[k] = r < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + r) / a.G) : sg.kv_end - 1;
         }
         if (w_rows > 0) {
-            w_min = sg.last_seen(a, warp * 16);
-            w_end = max(sg.last_seen(a, warp * 16 + w_rows - 1) + 1, 0);
+            w_min = sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16) / a.G);
+            w_end = max(sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16 + w_rows - 1) / a.G) + 1, 0);
             // a padding row sees what the warp's last one does
             if (warp * 16 + g >= sg.rows) lim[0] = w_end - 1;
             if (warp * 16 + 8 + g >= sg.rows) lim[1] = w_end - 1;
@@ -1031,7 +1026,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
             if (r >= sg.rows) continue;
             const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
             const int64_t row = ((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G, at = row * D;
-            const RowScale scale(a, row, -neg_r[k], sum, whole && sg.joins(a));
+            const float inv = !whole ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -1040,11 +1035,11 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                     const float4 y = make_float4(fmaf(o[w * 4][2 * k + c], up, z), fmaf(o[w * 4 + 1][2 * k + c], up * 0.0625f, z),
                                                  fmaf(o[w * 4 + 2][2 * k + c], up, z), fmaf(o[w * 4 + 3][2 * k + c], up * 0.0625f, z));
                     if (whole)
-                        store_out(a, at + d, y, scale);
+                        store_out(a, at + d, y, inv);
                     else
                         *reinterpret_cast<float4*>(part + r * D + d) = y;
                 }
-            if (whole && a.lse && t == 0) a.lse[row] = RowScale::lse(-neg_r[k], sum);
+            if (whole && a.lse && t == 0) a.lse[row] = attn_lse(-neg_r[k], sum);
             if (!whole && t == 0) part[C::kRows * D + r * 2] = -neg_r[k], part[C::kRows * D + r * 2 + 1] = sum;
         }
         if (tid == 0) attn_note(a, run, sg, unit);
@@ -1077,6 +1072,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
 // heads over 1024 tokens: 115 us (the chunk kernel 146).
 template <int D>
 struct TcCfg {
+    static constexpr bool kPaired = false;
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
     static constexpr int kStages = 3;
     static constexpr int kRawK = kTokens * (D / 2);      // codes of a tile's keys (or values)
@@ -1258,7 +1254,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             ca = a.scale_log2 * pow2i(24 - e);
             cb = sum * 0x1p-24f;
         }
-        const int lim = row < sg.rows ? sg.last_seen(a, row) : sg.kv_end - 1;
+        const int lim = row < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + row) / a.G) : sg.kv_end - 1;
 
         // ---- spreading of a tile's codes
         auto spread_keys = [&](int i, int stage) {
@@ -1476,10 +1472,9 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         const float l = ex[0][0][row] + ex[0][1][row], zs = ex[1][0][row] + ex[1][1][row];
         const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
-        const float up = 16777216.0f;
+        const float up = 16777216.0f, inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
         const uint32_t rr = (uint32_t)sg.r0 + row, ri = rr / a.G;
         const int64_t out_row = ((sg.row0 + ri) * a.s.Hk + sg.head) * a.G + rr - ri * a.G, at = out_row * D + tq * kDims;
-        const RowScale scale(a, out_row, -neg_r, l, row < sg.rows && whole && sg.joins(a));
 #pragma unroll
         for (int h = 0; h < kDims / 16; ++h) {
             uint32_t u[16];
@@ -1496,13 +1491,13 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                     const float4 y = make_float4(fmaf(__uint_as_float(u[k]), up, zs), fmaf(__uint_as_float(u[k + 1]), up * 0.0625f, zs),
                                                  fmaf(__uint_as_float(u[k + 2]), up, zs), fmaf(__uint_as_float(u[k + 3]), up * 0.0625f, zs));
                     if (whole)
-                        store_out(a, at + h * 16 + k, y, scale);
+                        store_out(a, at + h * 16 + k, y, inv);
                     else
                         *reinterpret_cast<float4*>(part + row * D + tq * kDims + h * 16 + k) = y;
                 }
             }
         }
-        if (whole && a.lse && tq == 0 && row < sg.rows) a.lse[out_row] = RowScale::lse(-neg_r, l);
+        if (whole && a.lse && tq == 0 && row < sg.rows) a.lse[out_row] = attn_lse(-neg_r, l);
         if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = -neg_r, part[C::kRows * D + row * 2 + 1] = l;
         if (tid == 0) attn_note(a, run, sg, unit);
         tc_fence_before();
@@ -1579,22 +1574,18 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 #pragma unroll
                 for (int e = 0; e < E; ++e) y[e] = fmaf(f, sh[warp + w][e * 32 + lane], y[e]);
             }
-            mx = top;
         }
         if (r >= to) continue;
         const uint32_t rr = (uint32_t)j.r0 + r, i = rr / j.G;
-        const int64_t row = ((j.row0 + i) * a.s.Hk + j.head) * j.G + rr - i * j.G, at = row * D + lane;
-        const RowScale k(a, row, mx, sum, j.joins);
+        const int64_t at = (((j.row0 + i) * a.s.Hk + j.head) * j.G + rr - i * j.G) * D + lane;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            float v = y[e] * k.k1;
-            if (k.add) v = fmaf(a.pre[at + e * 32], k.k2, v);
             if (a.out_f32)
-                static_cast<float*>(a.out)[at + e * 32] = v;
+                static_cast<float*>(a.out)[at + e * 32] = y[e] * inv;
             else
-                static_cast<__nv_bfloat16*>(a.out)[at + e * 32] = __float2bfloat16_rn(v);
+                static_cast<__nv_bfloat16*>(a.out)[at + e * 32] = __float2bfloat16_rn(y[e] * inv);
         }
-        if (a.lse && lane == 0) a.lse[row] = RowScale::lse(mx, sum);
     }
 }
 
@@ -1663,7 +1654,7 @@ static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-    if (e != cudaSuccess) return e;
+    if (e != cudaSuccess || a.where) return e;
     // Few tiles have many partial results each: more blocks and warps per tile.
     // Many tiles: fewer, most blocks find nothing to join.  (8 tiles of 55
     // partial results: 41 us with 8 x 8 warps, 47 us with 4 x 4; 256 tiles of 2:
@@ -1676,7 +1667,8 @@ static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a
     return cudaLaunchKernelEx(&cfg, kv4_join_kernel<D>, a, (int)C::kRows);
 }
 
-// One pass: its kernel and the one that joins, with notes and partial results at ws.
+// One pass: its kernel and (where no other kernel does) the one that joins, with notes and partial
+// results at ws.
 static cudaError_t attn_pass(Kv4AttnArgs& a, AttnKind kind, int64_t head_dim, void* ws, cudaStream_t s) {
     a.notes = static_cast<Kv4Join*>(ws);
     a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + attn_notes_bytes(attn_blocks(kind)));
@@ -1690,16 +1682,6 @@ static cudaError_t attn_pass(Kv4AttnArgs& a, AttnKind kind, int64_t head_dim, vo
         }
     };
     return head_dim == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
-}
-
-// The kernel for the rows of shared prefixes: here the host knows that the rows walk long
-// sequences together, but no more of the prefixes' lengths than the table's width.
-static AttnKind prefix_kind(int64_t P, int64_t T, int64_t Hk, int64_t G) {
-    const int64_t rows = (T + P - 1) / P * G;
-    return rows <= 8 ? kAttn8 : rows <= 16 ? kAttn16 : rows <= 64 ? kAttnChunk : kAttnLong;
-}
-static size_t prefix_rows_bytes(int64_t T, int64_t H, int64_t D) {
-    return ((size_t)T * H * (D + 1) * 4 + 255) / 256 * 256;
 }
 
 }  // namespace pn
@@ -1759,67 +1741,6 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: the workspace needs 256-byte alignment");
     const cudaError_t err = pn::attn_pass(a, kind, head_dim, workspace, (cudaStream_t)stream);
     return err == cudaSuccess ? ok() : cuda_fail(err, "pn_kv4_attention");
-}
-
-size_t pn_kv4_prefix_attention_workspace_size(int64_t B, int64_t T, int64_t n_prefixes, int64_t q_heads, int64_t kv_heads,
-                                              int64_t head_dim) {
-    if (B < 1 || T < 1 || n_prefixes < 0 || kv_heads < 1 || q_heads < kv_heads || head_dim < 1) return 0;
-    const size_t own = pn::attn_workspace(B, T, kv_heads, q_heads / kv_heads, head_dim);
-    if (n_prefixes == 0) return own;
-    const size_t prefix = pn::attn_workspace(pn::prefix_kind(n_prefixes, T, kv_heads, q_heads / kv_heads), head_dim);
-    return pn::prefix_rows_bytes(T, q_heads, head_dim) + (prefix + 255) / 256 * 256 + own;
-}
-
-int pn_kv4_prefix_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,
-                            const void* cache, int64_t n_pages, int64_t kv_heads, int64_t page, int64_t head_dim,
-                            const int32_t* block_table, int64_t table_ld, int64_t table_w, const int32_t* seq_lens,
-                            const int32_t* cu_q, int64_t B, int64_t T, const int32_t* prefix_table, int64_t prefix_ld,
-                            int64_t prefix_w, const int32_t* prefix_lens, const int32_t* cu_prefix, int64_t n_prefixes,
-                            float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
-    const char* name = "pn_kv4_prefix_attention";
-    pn::Kv4AttnArgs a{}, p{};
-    if (int st = check_kv4(name, cache, n_pages, kv_heads, page, head_dim, block_table, table_ld, table_w, seq_lens, cu_q, B, T,
-                           &a.s))
-        return st;
-    if (int st = check_attn(name, q, q_sb, q_sl, q_sh, q_dtype, q_heads, cache, scale, out, &a)) return st;
-    // (the rows of a prefix are any number of sequences': cu_q or not is the sequences' matter)
-    if (int st = check_kv4(name, cache, n_pages, kv_heads, page, head_dim, prefix_table, prefix_ld, prefix_w, prefix_lens, cu_prefix,
-                           n_prefixes, n_prefixes > 0 ? T / n_prefixes * n_prefixes : T, &p.s))
-        return st;
-    if (!cu_prefix && n_prefixes > 0 && B % n_prefixes != 0)
-        return fail(PN_ERR_SHAPE, "%s: %lld sequences over %lld prefixes need cu_prefix", name, (long long)B, (long long)n_prefixes);
-    if (T > 0 && B > 0 && n_prefixes > 0 && (!prefix_lens || (!prefix_table && prefix_w > 0)))
-        return fail(PN_ERR_ARG, "%s: null pointer", name);
-    if (int st = check_attn_units(name, a.s, a.G, table_w * page)) return st;
-    const pn::Kv4Seq own = a.s;
-    p.s.T = T, p.s.cu = cu_q, p.s.L = own.L, p.s.grouped = B, p.s.grp = cu_prefix;
-    if (int st = check_attn_units(name, p.s, a.G, prefix_w * page)) return st;
-    if (int st = check_device()) return st;
-    if (T == 0 || B == 0) return ok();
-    const size_t need = pn_kv4_prefix_attention_workspace_size(B, T, n_prefixes, q_heads, kv_heads, head_dim);
-    if (!workspace || workspace_bytes < need) return fail(PN_ERR_WORKSPACE, "%s: workspace needs %zu bytes", name, need);
-    if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "%s: the workspace needs 256-byte alignment", name);
-    const cudaStream_t s = (cudaStream_t)stream;
-    char* ws = static_cast<char*>(workspace);
-    if (n_prefixes > 0) {
-        const pn::Kv4Seq seq = p.s;
-        p = a;
-        p.s = seq;
-        p.q_l = cu_q ? 0 : own.L;
-        p.out = ws, p.out_f32 = 1;
-        p.lse = reinterpret_cast<float*>(ws) + (size_t)T * q_heads * head_dim;
-        p.grp = a.grp = cu_prefix;
-        p.n_grp = a.n_grp = (int)n_prefixes;
-        a.pre = reinterpret_cast<const float*>(ws);
-        a.pre_lse = p.lse;
-        ws += pn::prefix_rows_bytes(T, q_heads, head_dim);
-        const pn::AttnKind kind = pn::prefix_kind(n_prefixes, T, kv_heads, a.G);
-        const cudaError_t err = pn::attn_pass(p, kind, head_dim, ws, s);
-        if (err != cudaSuccess) return cuda_fail(err, name);
-        ws += (pn::attn_workspace(kind, head_dim) + 255) / 256 * 256;
-    }
-    const cudaError_t err = pn::attn_pass(a, pn::attn_kind(B, T, kv_heads, a.G), head_dim, ws, s);
-    return err == cudaSuccess ? ok() : cuda_fail(err, name);
 }
 
 }  // extern "C"

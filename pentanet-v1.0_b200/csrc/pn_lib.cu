@@ -20,5 +20,6 @@
 #include "pn_kv4.cu"
 #include "pn_kv4_rotary.cu"
 #include "pn_kv4_attn.cu"
+#include "pn_kv4_prefix.cu"
 #include "pn_kv4_sparse.cu"
 #include "pn_sample.cu"
