@@ -49,9 +49,10 @@ struct Kv4Seq {
 __device__ __forceinline__ int kv4_len(const Kv4Seq& s, int64_t b) { return min(max(__ldg(s.lens + b), 0), 1 << 30); }
 __device__ __forceinline__ int kv4_held(const Kv4Seq& s, int64_t b) { return min(kv4_len(s, b), s.table_w * s.page); }
 
-// First row and number of rows of sequence b.
+// First row and number of rows of sequence b (kMore: which may be a prefix).
+template <bool kMore = false>
 __device__ __forceinline__ void kv4_rows(const Kv4Seq& s, int64_t b, int64_t& first, int64_t& n) {
-    if (s.grouped) {
+    if (kMore && s.grouped) {
         int64_t b0 = b * (s.grouped / s.B), b1 = b0 + s.grouped / s.B;
         if (s.grp) {
             b0 = min(max((int64_t)__ldg(s.grp + b), (int64_t)0), s.grouped);

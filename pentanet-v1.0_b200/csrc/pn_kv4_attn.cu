@@ -145,15 +145,9 @@ __device__ __forceinline__ float raise_reference(float x, float vt, float& neg_r
 template <typename C>
 __device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, uint32_t& nt) {
     int64_t first, n;
-    kv4_rows(a.s, b, first, n);
-    if (a.s.table_hd && __ldg(a.s.lens + b) < 0) n = 0;  // (of chosen pages: a row that is no sequence's)
+    kv4_rows<C::kMore>(a.s, b, first, n);
+    if (C::kMore && a.s.table_hd && __ldg(a.s.lens + b) < 0) n = 0;  // (of chosen pages: a row that is no sequence's)
     nt = max((kv4_held(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
-    if constexpr (C::kPaired) {  // nt: of the last row tile, whose units are twice as long where it has half the rows
-        const uint32_t rows = (uint32_t)n * a.G, tiles = (rows + C::kRows - 1) / C::kRows, full = nt;
-        if (tiles == 0) return 0;
-        if (rows - (tiles - 1) * C::kRows <= C::kRows / 2) nt = (nt + 1) / 2;
-        return ((tiles - 1) * full + nt) * a.s.Hk;
-    }
     return ((uint32_t)n * a.G + C::kRows - 1) / C::kRows * nt * a.s.Hk;
 }
 
@@ -176,11 +170,11 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
     bool falls = false;  // cu_q does: its rows, and so the units, may be more than the host counted on
     for (uint32_t b = b0; b < b1; ++b) {
         sum += attn_units<C>(a, b, nt);
-        falls |= !a.s.grouped && a.s.cu && __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
+        falls |= !(C::kMore && a.s.grouped) && a.s.cu && __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
     }
-    if (a.s.grouped && a.s.cu)
+    if (C::kMore && a.s.grouped && a.s.cu)
         for (uint32_t b = threadIdx.x; b < a.s.grouped; b += C::kThreads) falls |= __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
-    if (a.grp)
+    if (C::kMore && a.grp)
         for (uint32_t b = threadIdx.x; b < (uint32_t)a.n_grp; b += C::kThreads) falls |= __ldg(a.grp + b + 1) < __ldg(a.grp + b);
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     uint32_t inc = sum;
@@ -221,27 +215,12 @@ __device__ __forceinline__ AttnRun attn_plan(const Kv4AttnArgs& a) {
     return run;
 }
 
-// Where query row r of a row tile lies in q, in elements.
-__device__ __forceinline__ int64_t attn_query(const Kv4AttnArgs& a, uint32_t b, int64_t row0, int64_t r0, int head, int r) {
-    const uint32_t rr = (uint32_t)r0 + r, i = rr / a.G;
-    int64_t at;
-    if (a.s.cu) {
-        at = (row0 + i) * a.q_sl;
-    } else if (a.q_l) {
-        const int64_t of = (row0 + i) / a.q_l;
-        at = of * a.q_sb + (row0 + i - of * a.q_l) * a.q_sl;
-    } else {
-        at = b * a.q_sb + i * a.q_sl;
-    }
-    return at + (head * a.G + (rr - i * a.G)) * a.q_sh;
-}
-
 // One segment: a run of units of one row tile.
 struct AttnSeg {
     uint32_t b, nt, t0, t1;  // sequence; token tiles of it, and the segment's [t0, t1)
     int head, rows;          // kv head; query rows in the tile
     int64_t row0, r0;        // first row of the sequence; first query row of the tile
-    int pos0;                // query row r sees positions up to pos0 + r / G
+    int pos0;                // query row r sees positions up to pos0 + r / G (of a prefix: all)
     int kv_end;              // tokens that the tile's last row sees (and the table has room for)
     int lim_min;             // the last position that its first row sees (at most kv_end - 1)
 
@@ -257,7 +236,7 @@ struct AttnSeg {
         b = seq;
         // a row tile's units are consecutive: (head, row tile, token tile)
         int64_t n_rows;
-        kv4_rows(a.s, b, row0, n_rows);
+        kv4_rows<C::kMore>(a.s, b, row0, n_rows);
         const uint32_t q_rows = (uint32_t)n_rows * a.G, n_rt = (q_rows + C::kRows - 1) / C::kRows;
         const uint32_t tile = in_seq / nt;
         head = (int)(tile / n_rt);
@@ -267,19 +246,32 @@ struct AttnSeg {
         rows = (int)min((uint32_t)C::kRows, q_rows - (uint32_t)r0);
         t0 = in_seq - tile * nt;
         t1 = min(nt, t0 + left);
+        const bool all = C::kMore && a.s.grouped;
         pos0 = kv4_len(a.s, b) - (int)n_rows;
-        kv_end = min(max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0), kv4_held(a.s, b));
+        kv_end = all ? kv4_held(a.s, b) : min(max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0), kv4_held(a.s, b));
         if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && pos0 + (int)n_rows > kv4_held(a.s, b)) record_status(PN_ERR_ARG);
-        lim_min = min(pos0 + (int)((uint32_t)r0 / a.G), kv_end - 1);
+        lim_min = all ? kv_end - 1 : min(pos0 + (int)((uint32_t)r0 / a.G), kv_end - 1);
     }
-    __device__ __forceinline__ int64_t query(const Kv4AttnArgs& a, int r) const { return attn_query(a, b, row0, r0, head, r); }
+    // Where query row r of the tile (r < rows) lies in q, in elements.
+    template <typename C>
+    __device__ __forceinline__ int64_t query(const Kv4AttnArgs& a, const C&, int r) const {
+        const uint32_t rr = (uint32_t)r0 + r, i = rr / a.G;
+        int64_t at = a.s.cu ? (row0 + i) * a.q_sl : b * a.q_sb + i * a.q_sl;
+        if (C::kMore && !a.s.cu && a.q_l) {
+            const int64_t of = (row0 + i) / a.q_l;
+            at = of * a.q_sb + (row0 + i - of * a.q_l) * a.q_sl;
+        }
+        return at + (head * a.G + (rr - i * a.G)) * a.q_sh;
+    }
 };
 
 // Leaves the joining kernel a note where a row tile ends in this block and began
 // in an earlier one.
-template <typename Seg>
-__device__ __forceinline__ void attn_note(const Kv4AttnArgs& a, const AttnRun& run, const Seg& sg, uint32_t unit) {
-    if (sg.t1 != sg.nt || (sg.t0 == 0 && !a.where)) return;
+template <typename C>
+__device__ __forceinline__ void attn_note(const Kv4AttnArgs& a, const C&, const AttnRun& run, const AttnSeg& sg, uint32_t unit) {
+    if (sg.t1 != sg.nt) return;
+    const bool where = C::kMore && a.where;
+    if (sg.t0 == 0 && !where) return;
     const uint32_t i0 = (uint32_t)sg.r0 / a.G;
     const int64_t row = ((sg.row0 + i0) * a.s.Hk + sg.head) * a.G + (uint32_t)sg.r0 - i0 * a.G;
     if (sg.t0 == 0) {
@@ -290,7 +282,7 @@ __device__ __forceinline__ void attn_note(const Kv4AttnArgs& a, const AttnRun& r
     const uint32_t u0 = unit - sg.t0, each = run.total / gridDim.x, rem = run.total % gridDim.x;
     const uint32_t c0 = u0 < (each + 1) * rem ? u0 / (each + 1) : rem + (u0 - (each + 1) * rem) / each;
     const int slot = attn_begin(run.total, gridDim.x, c0) < u0 ? 1 : 0;
-    if (a.where)
+    if (where)
         a.where[row] = {(int)c0, slot, (int)blockIdx.x, 0};
     else
         a.notes[blockIdx.x] = {sg.rows, (int)c0, slot, a.G, sg.row0, sg.r0, sg.head};
@@ -302,12 +294,13 @@ struct AttnPages {
     uint64_t addr;  // the page block of the keys; 0: not there
     int off;        // the piece's first token in its page
 
-    __device__ __forceinline__ void look_up(const Kv4AttnArgs& a, uint32_t b, int head, int64_t block, int tok, bool want) {
+    template <typename C>
+    __device__ __forceinline__ void look_up(const Kv4AttnArgs& a, const C&, uint32_t b, int head, int64_t block, int tok, bool want) {
         addr = 0;
         off = 0;
         if (!want) return;
         const uint32_t i = (uint32_t)tok / (uint32_t)a.s.page;
-        const int p = __ldg(a.s.table + b * a.s.table_ld + head * a.s.table_hd + i);
+        const int p = __ldg(a.s.table + b * a.s.table_ld + (C::kMore ? head * a.s.table_hd : 0) + i);
         off = tok - (int)i * a.s.page;
         if (p >= 0 && p < a.s.n_pages)
             addr = (uint64_t)(a.cache + ((int64_t)p * a.s.Hk + head) * 2 * block);
@@ -403,9 +396,9 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
 // 3.4 TB/s (half of the copy's rate).  Three blocks of six stages per SM: two, four or
 // five blocks, and more stages in two, are all slower.  With 16 rows at d = 128 the
 // registers do not suffice (372 bytes spilled per thread).
-template <int D, int NT>
+template <int D, int NT, bool M>
 struct AttnCfg {
-    static constexpr bool kPaired = false;
+    static constexpr bool kMore = M;
     static constexpr int W = D / 32;             // words per thread and token
     static constexpr int kRows = 8 * NT;         // query rows of a row tile
     static constexpr int kTokens = 128;          // tokens of a unit: 32 per warp
@@ -443,9 +436,9 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[W]) {
 __device__ __forceinline__ float pair_lo(uint32_t p) { return __uint_as_float(p << 16); }
 __device__ __forceinline__ float pair_hi(uint32_t p) { return __uint_as_float(p & 0xFFFF0000u); }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_decode_kernel(const Kv4AttnArgs a) {
-    using C = AttnCfg<D, NT>;
+template <int D, int NT, bool M>
+__global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_decode_kernel(const Kv4AttnArgs a) {
+    using C = AttnCfg<D, NT, M>;
     constexpr int W = C::W, RT = C::kRows, ST = C::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float join_ml[kAttnWarps * RT * 2];
@@ -478,7 +471,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
         auto issue = [&](int i, uint32_t slot) {  // run i; slot: its first stage's offset in the ring
             if ((i & 15) == 0) {  // lane 2 k + j looks up piece j of run i + k
                 const int k = i + (lane >> 1), tok = tok_base + k * C::kTokens + (lane & 1) * 16;
-                pages.look_up(a, sg.b, sg.head, block, tok, k < count && tok < sg.kv_end);
+                pages.look_up(a, C{}, sg.b, sg.head, block, tok, k < count && tok < sg.kv_end);
             }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -513,7 +506,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const char* row = nullptr;
-            if (n * 8 + g < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, n * 8 + g) * (a.q_f32 ? 4 : 2);
+            if (n * 8 + g < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, C{}, n * 8 + g) * (a.q_f32 ? 4 : 2);
             float fa, fb;
             load_query<D>(a, row, t, qb[n], fa, fb);
 #pragma unroll
@@ -524,7 +517,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                 else
                     ca[n].y = va, cb[n].y = vb;
                 const int rl = n * 8 + 2 * t + k;
-                lim[n][k] = rl < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + rl) / a.G) : sg.kv_end - 1;
+                lim[n][k] = rl < sg.rows && !(C::kMore && a.s.grouped) ? sg.pos0 + (int)(((uint32_t)sg.r0 + rl) / a.G) : sg.kv_end - 1;
             }
         }
 
@@ -748,13 +741,13 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
                 const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
                 const int64_t at = ((sg.row0 + i) * a.s.Hk + sg.head) * a.G + rr - i * a.G;
                 store_out(a, at * D + d, y, sum == 0.0f ? 0.0f : 1.0f / sum);
-                if (a.lse && d == 0) a.lse[at] = attn_lse(mx, sum);
+                if (C::kMore && a.lse && d == 0) a.lse[at] = attn_lse(mx, sum);
             } else {
                 *reinterpret_cast<float4*>(part + r * D + d) = y;
                 if (d == 0) part[RT * D + r * 2] = mx, part[RT * D + r * 2 + 1] = sum;
             }
         }
-        if (tid == 0) attn_note(a, run, sg, unit);
+        if (tid == 0) attn_note(a, C{}, run, sg, unit);
         __syncthreads();
         unit += sg.t1 - sg.t0;
         in_seq += sg.t1 - sg.t0;
@@ -774,9 +767,9 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT>::kBlocks) kv4_dec
 // and 41 % of the issue slots are used: as in the decode kernel the warps (twelve to
 // an SM) wait for their own last instruction.  64 sequences x 64 rows x 4 heads over 1024
 // tokens: 72 us (two blocks to an SM: 2 % slower than three); 148 bytes spilled per thread.
-template <int D>
+template <int D, bool M>
 struct ChunkCfg {
-    static constexpr bool kPaired = false;
+    static constexpr bool kMore = M;
     static constexpr int W = D / 32;
     static constexpr int kRows = 64, kTokens = 64, kThreads = kAttnThreads;
     static constexpr int kStages = 3;
@@ -788,9 +781,9 @@ struct ChunkCfg {
     static constexpr int kBlocks = 3;  // per SM
 };
 
-template <int D>
-__global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_kernel(const Kv4AttnArgs a) {
-    using C = ChunkCfg<D>;
+template <int D, bool M>
+__global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D, M>::kBlocks) kv4_chunk_kernel(const Kv4AttnArgs a) {
+    using C = ChunkCfg<D, M>;
     constexpr int W = C::W, ST = C::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint8_t dead[ST][4];  // the piece is not there
@@ -817,7 +810,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
         auto issue = [&](int i, int stage) {
             if ((i & 31) == 0) {
                 const int tok = tok_base + (i + lane) * C::kTokens + warp * 16;
-                pages.look_up(a, sg.b, sg.head, block, tok, i + lane < count && tok < sg.kv_end);
+                pages.look_up(a, C{}, sg.b, sg.head, block, tok, i + lane < count && tok < sg.kv_end);
             }
             const uint64_t addr = __shfl_sync(0xffffffffu, pages.addr, i & 31);
             const uint32_t off = __shfl_sync(0xffffffffu, pages.off, i & 31);
@@ -847,13 +840,13 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
         for (int k = 0; k < 2; ++k) {
             const int r = warp * 16 + k * 8 + g;
             const char* row = nullptr;
-            if (r < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, r) * (a.q_f32 ? 4 : 2);
+            if (r < sg.rows) row = static_cast<const char*>(a.q) + sg.query(a, C{}, r) * (a.q_f32 ? 4 : 2);
             load_query<D>(a, row, t, k ? qc : qa, ca[k], cb[k]);
-            lim[k] = r < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + r) / a.G) : sg.kv_end - 1;
+            lim[k] = r < sg.rows && !(C::kMore && a.s.grouped) ? sg.pos0 + (int)(((uint32_t)sg.r0 + r) / a.G) : sg.kv_end - 1;
         }
         if (w_rows > 0) {
-            w_min = sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16) / a.G);
-            w_end = max(sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16 + w_rows - 1) / a.G) + 1, 0);
+            w_min = C::kMore && a.s.grouped ? sg.kv_end - 1 : sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16) / a.G);
+            w_end = C::kMore && a.s.grouped ? sg.kv_end : max(sg.pos0 + (int)(((uint32_t)sg.r0 + warp * 16 + w_rows - 1) / a.G) + 1, 0);
             // a padding row sees what the warp's last one does
             if (warp * 16 + g >= sg.rows) lim[0] = w_end - 1;
             if (warp * 16 + 8 + g >= sg.rows) lim[1] = w_end - 1;
@@ -1039,10 +1032,10 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
                     else
                         *reinterpret_cast<float4*>(part + r * D + d) = y;
                 }
-            if (whole && a.lse && t == 0) a.lse[row] = attn_lse(-neg_r[k], sum);
+            if (C::kMore && whole && a.lse && t == 0) a.lse[row] = attn_lse(-neg_r[k], sum);
             if (!whole && t == 0) part[C::kRows * D + r * 2] = -neg_r[k], part[C::kRows * D + r * 2 + 1] = sum;
         }
-        if (tid == 0) attn_note(a, run, sg, unit);
+        if (tid == 0) attn_note(a, C{}, run, sg, unit);
         __syncthreads();  // nobody reads a stage any more
         unit += sg.t1 - sg.t0;
         in_seq += sg.t1 - sg.t0;
@@ -1070,9 +1063,9 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D>::kBlocks) kv4_chunk_
 // 4500 cycles for an SM's two blocks, 47 % of the issue slots used); the products take
 // 512 cycles of a step at the tensor core's rate.  16 sequences x 512 rows x 8
 // heads over 1024 tokens: 115 us (the chunk kernel 146).
-template <int D>
+template <int D, bool M>
 struct TcCfg {
-    static constexpr bool kPaired = false;
+    static constexpr bool kMore = M;
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
     static constexpr int kStages = 3;
     static constexpr int kRawK = kTokens * (D / 2);      // codes of a tile's keys (or values)
@@ -1130,9 +1123,9 @@ __device__ __forceinline__ void mma4_ts_warp(uint32_t d_tmem, uint32_t a, uint32
 // The low word of a 128-byte swizzled operand's descriptor.
 __device__ __forceinline__ uint32_t desc_lo(const void* p) { return 1u << 16 | (smem_u32(p) >> 4 & 0x3FFFu); }
 
-template <int D>
+template <int D, bool M>
 __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
-    using C = TcCfg<D>;
+    using C = TcCfg<D, M>;
     constexpr int ST = C::kStages;
     constexpr int kDims = D / 2;  // dims of a row per thread
     extern __shared__ uint8_t smem_base[];
@@ -1190,7 +1183,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         auto issue = [&](int i, int stage) {
             if ((i & 31) == 0) {
                 const int tok = tok_base + (i + lane) * C::kTokens + piece * 16;
-                pages.look_up(a, sg.b, sg.head, block, tok, i + lane < count && tok < sg.kv_end);
+                pages.look_up(a, C{}, sg.b, sg.head, block, tok, i + lane < count && tok < sg.kv_end);
             }
             const uint64_t addr = __shfl_sync(0xffffffffu, pages.addr, i & 31);
             const uint32_t off = __shfl_sync(0xffffffffu, pages.off, i & 31);
@@ -1216,7 +1209,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         {
             float v[kDims];
             if (row < sg.rows) {
-                const char* q = static_cast<const char*>(a.q) + (sg.query(a, row) + tq * kDims) * (a.q_f32 ? 4 : 2);
+                const char* q = static_cast<const char*>(a.q) + (sg.query(a, C{}, row) + tq * kDims) * (a.q_f32 ? 4 : 2);
 #pragma unroll
                 for (int i = 0; i < kDims / 8; ++i) {
                     float u[8];
@@ -1254,7 +1247,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             ca = a.scale_log2 * pow2i(24 - e);
             cb = sum * 0x1p-24f;
         }
-        const int lim = row < sg.rows ? sg.pos0 + (int)(((uint32_t)sg.r0 + row) / a.G) : sg.kv_end - 1;
+        const int lim = row < sg.rows && !(C::kMore && a.s.grouped) ? sg.pos0 + (int)(((uint32_t)sg.r0 + row) / a.G) : sg.kv_end - 1;
 
         // ---- spreading of a tile's codes
         auto spread_keys = [&](int i, int stage) {
@@ -1497,9 +1490,9 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 }
             }
         }
-        if (whole && a.lse && tq == 0 && row < sg.rows) a.lse[out_row] = attn_lse(-neg_r, l);
+        if (C::kMore && whole && a.lse && tq == 0 && row < sg.rows) a.lse[out_row] = attn_lse(-neg_r, l);
         if (!whole && tq == 0 && row < sg.rows) part[C::kRows * D + row * 2] = -neg_r, part[C::kRows * D + row * 2 + 1] = l;
-        if (tid == 0) attn_note(a, run, sg, unit);
+        if (tid == 0) attn_note(a, C{}, run, sg, unit);
         tc_fence_before();
         __syncthreads();
         tc_fence_after();
@@ -1617,7 +1610,7 @@ static AttnKind attn_kind(int64_t B, int64_t T, int64_t Hk, int64_t G) {
     return rows <= 64 || tiles <= 8 * sms ? kAttnChunk : kAttnLong;
 }
 static int attn_blocks(AttnKind kind) {  // blocks that the device holds at once
-    return sm_count() * (kind == kAttnLong ? TcCfg<128>::kBlocks : AttnCfg<128, 1>::kBlocks);
+    return sm_count() * (kind == kAttnLong ? TcCfg<128, false>::kBlocks : AttnCfg<128, 1, false>::kBlocks);
 }
 static size_t attn_notes_bytes(int blocks) { return ((size_t)blocks * sizeof(Kv4Join) + 255) / 256 * 256; }
 static size_t attn_part_bytes(AttnKind kind, int64_t D) {
@@ -1668,17 +1661,19 @@ static cudaError_t launch_attn(void (*kernel)(Kv4AttnArgs), const Kv4AttnArgs& a
 }
 
 // One pass: its kernel and (where no other kernel does) the one that joins, with notes and partial
-// results at ws.
+// results at ws.  M: whether the rows or tables are other than pn_kv4_attention's; that is a matter of the kernels'
+// type, since the tests for it made that one 3 to 10 % slower (one row of 12 heads over 513 tokens: 9.3 and 10.2 us).
+template <bool M>
 static cudaError_t attn_pass(Kv4AttnArgs& a, AttnKind kind, int64_t head_dim, void* ws, cudaStream_t s) {
     a.notes = static_cast<Kv4Join*>(ws);
     a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + attn_notes_bytes(attn_blocks(kind)));
     auto go = [&](auto dim) {
         constexpr int D = decltype(dim)::value;
         switch (kind) {
-            case kAttn8: return launch_attn<D, AttnCfg<D, 1>>(kv4_decode_kernel<D, 1>, a, kind, s);
-            case kAttn16: return launch_attn<D, AttnCfg<D, 2>>(kv4_decode_kernel<D, 2>, a, kind, s);
-            case kAttnChunk: return launch_attn<D, ChunkCfg<D>>(kv4_chunk_kernel<D>, a, kind, s);
-            default: return launch_attn<D, TcCfg<D>>(kv4_long_kernel<D>, a, kind, s);
+            case kAttn8: return launch_attn<D, AttnCfg<D, 1, M>>(kv4_decode_kernel<D, 1, M>, a, kind, s);
+            case kAttn16: return launch_attn<D, AttnCfg<D, 2, M>>(kv4_decode_kernel<D, 2, M>, a, kind, s);
+            case kAttnChunk: return launch_attn<D, ChunkCfg<D, M>>(kv4_chunk_kernel<D, M>, a, kind, s);
+            default: return launch_attn<D, TcCfg<D, M>>(kv4_long_kernel<D, M>, a, kind, s);
         }
     };
     return head_dim == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
@@ -1739,7 +1734,7 @@ int pn_kv4_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
     if (!workspace || workspace_bytes < need)
         return fail(PN_ERR_WORKSPACE, "pn_kv4_attention: workspace needs %zu bytes", need);
     if (!aligned(workspace, 256)) return fail(PN_ERR_ALIGN, "pn_kv4_attention: the workspace needs 256-byte alignment");
-    const cudaError_t err = pn::attn_pass(a, kind, head_dim, workspace, (cudaStream_t)stream);
+    const cudaError_t err = pn::attn_pass<false>(a, kind, head_dim, workspace, (cudaStream_t)stream);
     return err == cudaSuccess ? ok() : cuda_fail(err, "pn_kv4_attention");
 }
 

@@ -467,7 +467,7 @@ int pn_kv4_sparse_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q
     a.q_l = cu_q ? T : a.s.L;  // (with cu_q rows lie one after another)
     a.s.table = c.pages, a.s.table_hd = width, a.s.table_ld = kv_heads * width, a.s.table_w = n_pages > 0 ? (int)width : 0;
     a.s.lens = c.lens, a.s.cu = nullptr, a.s.B = T, a.s.L = 1;
-    err = pn::attn_pass(a, pn::attn_kind(T, T, kv_heads, a.G), head_dim, ws + lay.attn, s);
+    err = pn::attn_pass<true>(a, pn::attn_kind(T, T, kv_heads, a.G), head_dim, ws + lay.attn, s);
     return err == cudaSuccess ? ok() : cuda_fail(err, name);
 }
 
