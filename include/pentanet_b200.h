@@ -362,7 +362,7 @@ int pn_kv4_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
  * q_out (T, q_heads, head_dim), contiguous, 16-byte aligned, rounded once (q_out may be
  * q itself, where q is contiguous; other overlaps of the two are not allowed).  Keys
  * are quantised from fp32, values as pn_kv4_append does.  Rows behind cu_q[B] are left as
- * they were in q_out; a row at a negative position gives zeros there, and one whose
+ * they were in q_out (zero_rest != 0: become zeros); a row at a negative position gives zeros there, and one whose
  * entry is outside the tables zeros, nothing stored and PN_ERR_ARG in the device
  * status word. */
 int pn_kv4_append_rotary(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int64_t q_heads, const void *k, int64_t k_sb,
@@ -370,7 +370,8 @@ int pn_kv4_append_rotary(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh
                          const float *cos, const float *sin, int64_t n_pos, int64_t table_stride, int64_t rotated,
                          int interleaved, const int32_t *offsets, void *cache, int64_t n_pages, int64_t kv_heads, int64_t page,
                          int64_t head_dim, const int32_t *block_table, int64_t table_ld, int64_t table_w,
-                         const int32_t *seq_lens, const int32_t *cu_q, int64_t B, int64_t T, void *q_out, void *stream);
+                         const int32_t *seq_lens, const int32_t *cu_q, int64_t B, int64_t T, void *q_out, int zero_rest,
+                         void *stream);
 
 /* pn_kv4_attention of sequences behind shared prefixes: the rows of sequences
  * [cu_prefix[g], cu_prefix[g + 1]) see all prefix_lens[g] tokens of prefix g (pages of

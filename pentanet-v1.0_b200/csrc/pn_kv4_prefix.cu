@@ -37,7 +37,6 @@ struct Kv4MergeArgs {
     int tile[2];               // rows of their row tiles
     void* out;
     int out_f32;
-    int zero_rest;             // rows of no sequence get zeros
 };
 constexpr int kMergeWarps = 8;
 
@@ -59,97 +58,94 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const Kv4Me
     if (h >= H) return;
     const int64_t at = row * H + h;
     int64_t b, i;
-    const bool found = !falls && kv4_find(a.s, row, b, i);
-    if (!found && !a.zero_rest) return;
+    if (falls || !kv4_find(a.s, row, b, i)) return;
     float mx = -INFINITY, sum = 0.0f, y[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] = 0.0f;
-    if (found) {
-        const int hk = h / a.G, gq = h - hk * a.G;
-        // own results
-        const int64_t r = i * a.G + gq, r0 = r / a.tile[0] * a.tile[0];
-        const Kv4Where own = a.where[0][((row - i + r0 / a.G) * a.s.Hk + hk) * a.G + r0 % a.G];
-        const int n_own = own.last < 0 ? 1 : own.last - own.first + 1;
-        // the prefix's
-        Kv4Where pre = {};
-        int n_pre = 0;
-        int64_t pr = 0;  // the row in its row tile
-        Kv4Seq p = a.s;
-        p.B = a.P, p.grouped = a.s.B, p.grp = a.grp;
-        int64_t g = -1;
-        if (!a.grp) {
-            g = b / (a.s.B / a.P);
-        } else {
-            int64_t lo = 0, hi = a.P;  // the last g with grp[g] <= b
-            while (hi - lo > 1) {
-                const int64_t mid = (lo + hi) / 2;
-                if (__ldg(a.grp + mid) <= b)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            if (b >= __ldg(a.grp + lo) && b < __ldg(a.grp + lo + 1)) g = lo;
+    const int hk = h / a.G, gq = h - hk * a.G;
+    // own results
+    const int64_t r = i * a.G + gq, r0 = r / a.tile[0] * a.tile[0];
+    const Kv4Where own = a.where[0][((row - i + r0 / a.G) * a.s.Hk + hk) * a.G + r0 % a.G];
+    const int n_own = own.last < 0 ? 1 : own.last - own.first + 1;
+    // the prefix's
+    Kv4Where pre = {};
+    int n_pre = 0;
+    int64_t pr = 0;  // the row in its row tile
+    Kv4Seq p = a.s;
+    p.B = a.P, p.grouped = a.s.B, p.grp = a.grp;
+    int64_t g = -1;
+    if (!a.grp) {
+        g = b / (a.s.B / a.P);
+    } else {
+        int64_t lo = 0, hi = a.P;  // the last g with grp[g] <= b
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (__ldg(a.grp + mid) <= b)
+                lo = mid;
+            else
+                hi = mid;
         }
-        if (g >= 0) {
-            int64_t first, n;
-            kv4_rows<true>(p, g, first, n);
-            pr = (row - first) * a.G + gq;
-            const int64_t t0 = pr / a.tile[1] * a.tile[1];
-            pre = a.where[1][((first + t0 / a.G) * a.s.Hk + hk) * a.G + t0 % a.G];
-            pr -= t0;
-            n_pre = pre.last < 0 ? 1 : pre.last - pre.first + 1;
-        }
-        for (int base = 0; base < n_own + n_pre; base += 32) {
-            const int n = min(n_own + n_pre - base, 32), j = base + lane;
-            const float* from = nullptr;
-            float m = -INFINITY, l = 0.0f;
-            if (lane < n) {
-                const int which = j < n_own ? 0 : 1, k = which ? j - n_own : j;
-                const Kv4Where w = which ? pre : own;
-                if (w.last < 0) {
-                    from = a.y[which] + at * D;
-                    m = a.lse[which][at], l = 1.0f;
-                } else {
-                    const int tile = a.tile[which];
-                    const int64_t tr = which ? pr : r - r0;
-                    const float* p0 = a.part[which] + ((int64_t)(w.first + k) * 2 + (k == 0 ? w.first_slot : 0)) * tile * (D + 2);
-                    from = p0 + tr * D;
-                    const float2 ml = *reinterpret_cast<const float2*>(p0 + tile * D + tr * 2);
-                    m = ml.x, l = ml.y;
-                }
+        if (b >= __ldg(a.grp + lo) && b < __ldg(a.grp + lo + 1)) g = lo;
+    }
+    if (g >= 0) {
+        int64_t first, n;
+        kv4_rows<true>(p, g, first, n);
+        pr = (row - first) * a.G + gq;
+        const int64_t t0 = pr / a.tile[1] * a.tile[1];
+        pre = a.where[1][((first + t0 / a.G) * a.s.Hk + hk) * a.G + t0 % a.G];
+        pr -= t0;
+        n_pre = pre.last < 0 ? 1 : pre.last - pre.first + 1;
+    }
+    for (int base = 0; base < n_own + n_pre; base += 32) {
+        const int n = min(n_own + n_pre - base, 32), j = base + lane;
+        const float* from = nullptr;
+        float m = -INFINITY, l = 0.0f;
+        if (lane < n) {
+            const int which = j < n_own ? 0 : 1, k = which ? j - n_own : j;
+            const Kv4Where w = which ? pre : own;
+            if (w.last < 0) {
+                from = a.y[which] + at * D;
+                m = a.lse[which][at], l = 1.0f;
+            } else {
+                const int tile = a.tile[which];
+                const int64_t tr = which ? pr : r - r0;
+                const float* p0 = a.part[which] + ((int64_t)(w.first + k) * 2 + (k == 0 ? w.first_slot : 0)) * tile * (D + 2);
+                from = p0 + tr * D;
+                const float2 ml = *reinterpret_cast<const float2*>(p0 + tile * D + tr * 2);
+                m = ml.x, l = ml.y;
             }
-            if (m == -INFINITY) l = 0.0f;
-            if (l == 0.0f) m = -INFINITY;  // (a total of 0: nothing was seen)
-            float top = m;
+        }
+        if (m == -INFINITY) l = 0.0f;
+        if (l == 0.0f) m = -INFINITY;  // (a total of 0: nothing was seen)
+        float top = m;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (top == -INFINITY) top = __any_sync(0xffffffffu, m != m) ? 0.0f : top;  // (totals that are NaN)
-            if (top == -INFINITY) continue;
-            const float mn = fmaxf(mx, top), f = ex2f(mx - mn), w = l == 0.0f ? 0.0f : ex2f(m - mn);
-            float lw = l * w;
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (top == -INFINITY) top = __any_sync(0xffffffffu, m != m) ? 0.0f : top;  // (totals that are NaN)
+        if (top == -INFINITY) continue;
+        const float mn = fmaxf(mx, top), f = ex2f(mx - mn), w = l == 0.0f ? 0.0f : ex2f(m - mn);
+        float lw = l * w;
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
-            sum = fmaf(sum, f, lw);
-            mx = mn;
+        for (int o = 16; o > 0; o >>= 1) lw += __shfl_xor_sync(0xffffffffu, lw, o);
+        sum = fmaf(sum, f, lw);
+        mx = mn;
 #pragma unroll
-            for (int e = 0; e < E; ++e) y[e] *= f;
-            const uint32_t some = __ballot_sync(0xffffffffu, l != 0.0f);
+        for (int e = 0; e < E; ++e) y[e] *= f;
+        const uint32_t some = __ballot_sync(0xffffffffu, l != 0.0f);
 #pragma unroll 4
-            for (int k = 0; k < n; ++k) {
-                const float wk = __shfl_sync(0xffffffffu, w, k);
-                const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), k));
-                if (!(some >> k & 1)) continue;
-                float u[E];
-                if constexpr (E == 4) {
-                    const float4 v = reinterpret_cast<const float4*>(src)[lane];
-                    u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
-                } else {
-                    const float2 v = reinterpret_cast<const float2*>(src)[lane];
-                    u[0] = v.x, u[1] = v.y;
-                }
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[e] = fmaf(wk, u[e], y[e]);
+        for (int k = 0; k < n; ++k) {
+            const float wk = __shfl_sync(0xffffffffu, w, k);
+            const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), k));
+            if (!(some >> k & 1)) continue;
+            float u[E];
+            if constexpr (E == 4) {
+                const float4 v = reinterpret_cast<const float4*>(src)[lane];
+                u[0] = v.x, u[1] = v.y, u[2] = v.z, u[3] = v.w;
+            } else {
+                const float2 v = reinterpret_cast<const float2*>(src)[lane];
+                u[0] = v.x, u[1] = v.y;
             }
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = fmaf(wk, u[e], y[e]);
         }
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;

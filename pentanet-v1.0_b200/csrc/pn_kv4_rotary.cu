@@ -27,6 +27,7 @@ struct Kv4RotaryArgs {
     const int32_t* offsets;          // (B), or null
     void* out;                       // (T, H, D), the inputs' type
     uint8_t* cache;
+    int zero_rest;                   // queries of rows of no sequence become zeros
     int parts;                       // warps that share a row
 };
 constexpr int kRotaryThreads = 128;
@@ -107,9 +108,11 @@ __device__ __forceinline__ void rotary_scale(const float (&v)[16], float& s, flo
 // D / 16 lanes per vector, two pieces of eight dims each: of rotated halves a lane holds the
 // two that meet, so that no value crosses lanes and a lane needs eight angles, which it
 // keeps for all heads of its row.  A warp takes a row (or one of `parts` shares of its
-// vectors, where there are few rows), no block-wide step anywhere.
+// vectors, where there are few rows), no block-wide step anywhere.  Its loads of the next step are in
+// flight during this one; six blocks to an SM spill 40 bytes, but have more of them: 7 ragged prompts of up to 2047
+// rows, 32 + 2 x 8 heads of 128 dims: 55 us (five blocks, no spills: 58; eight: 64), reading and writing once 31.
 template <typename T, int D>
-__global__ void __launch_bounds__(kRotaryThreads) kv4_rotary_kernel(const Kv4RotaryArgs a) {
+__global__ void __launch_bounds__(kRotaryThreads, 6) kv4_rotary_kernel(const Kv4RotaryArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     constexpr int VT = D / 16, VP = 32 / VT;  // lanes per vector, vectors per step
@@ -120,7 +123,12 @@ __global__ void __launch_bounds__(kRotaryThreads) kv4_rotary_kernel(const Kv4Rot
     if (row >= a.s.T) return;
     const int64_t block = (int64_t)a.s.page * (D / 2 + 4);
     RotaryRow r;
-    if (!rotary_row(a, row, block, r)) return;
+    if (!rotary_row(a, row, block, r)) {
+        if (!a.zero_rest) return;
+        const int64_t n = (int64_t)a.H * D * sizeof(T) / 16, from = n * part / a.parts, to = n * (part + 1) / a.parts;
+        for (int64_t i = from + lane; i < to; i += 32) static_cast<uint4*>(a.out)[row * n + i] = make_uint4(0, 0, 0, 0);
+        return;
+    }
 
     // the lane's two pieces of eight dims
     const bool turns = l * 16 < a.rotated;
@@ -243,7 +251,8 @@ int pn_kv4_append_rotary(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh
                          const float* cos, const float* sin, int64_t n_pos, int64_t table_stride, int64_t rotated,
                          int interleaved, const int32_t* offsets, void* cache, int64_t n_pages, int64_t kv_heads, int64_t page,
                          int64_t head_dim, const int32_t* block_table, int64_t table_ld, int64_t table_w,
-                         const int32_t* seq_lens, const int32_t* cu_q, int64_t B, int64_t T, void* q_out, void* stream) {
+                         const int32_t* seq_lens, const int32_t* cu_q, int64_t B, int64_t T, void* q_out, int zero_rest,
+                         void* stream) {
     const char* name = "pn_kv4_append_rotary";
     pn::Kv4RotaryArgs a{};
     if (int st = check_kv4(name, cache, n_pages, kv_heads, page, head_dim, block_table, table_ld, table_w, seq_lens, cu_q, B, T,
@@ -276,6 +285,7 @@ int pn_kv4_append_rotary(const void* q, int64_t q_sb, int64_t q_sl, int64_t q_sh
     a.table_vec = aligned(cos, 16) && aligned(sin, 16) && table_stride % 4 == 0;
     a.rotated = (int)rotated, a.interleaved = interleaved != 0, a.offsets = offsets;
     a.out = q_out;
+    a.zero_rest = zero_rest != 0;
     a.cache = static_cast<uint8_t*>(cache);
     const cudaStream_t s = (cudaStream_t)stream;
     cudaError_t err;

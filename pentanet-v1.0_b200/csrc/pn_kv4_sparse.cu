@@ -221,131 +221,324 @@ __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4Selec
 
 // ---- choice -----------------------------------------------------------------
 
-constexpr int kSelectThreads = 256;
 constexpr int kSelectBins = 2048;
+constexpr int kSelectFew = 256;  // keys that are ranked one against another
 
-// The threshold of the `top` largest of n keys by their digits from the highest: a histogram
-// of the digit among the keys that share the digits before, the bin where the count from
-// above reaches `need`, and so on, until that bin is taken whole (most often at the second
-// digit) or the digits are out.  Then one pass over the pages in order writes those above the
-// threshold and the first `need` of those at it.  One block per row and kv head.
-__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(const Kv4SelectArgs a) {
+// The score of a key, to fp32 (which keeps their order).
+__device__ __forceinline__ float score_of(uint64_t k) {
+    return __double2float_rn(__longlong_as_double((long long)(k >> 63 ? k & 0x7fffffffffffffffull : ~k)));
+}
+// Bin of a key, from evenly spaced ones between the least and the largest finite score (which are at
+// lo and lo + 2047 / each): never higher for a smaller key.
+__device__ __forceinline__ int score_bin(uint64_t k, float lo, float each) {
+    if (k == 0) return 0;
+    const float v = score_of(k);
+    if (!(v < INFINITY)) return kSelectBins - 1;
+    return (int)fminf(fmaxf((v - lo) * each, 0.0f), (float)(kSelectBins - 1));
+}
+
+// Counts from above: the bin where they reach `need`, and how many of it are needed.
+template <int THREADS>
+__device__ __forceinline__ void select_border(const int* bins, int need, int* warp_sums, int* border) {
+    constexpr int PER = kSelectBins / THREADS;  // thread t has bins [PER (THREADS - 1 - t), + PER)
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) mine += bins[(THREADS - 1 - tid) * PER + j];
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) warp_sums[warp] = inc;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) inc += warp_sums[w];
+    int above = inc - mine;
+    if (above < need && need <= inc) {
+        int j = PER - 1;
+        for (;; --j) {
+            const int c = bins[(THREADS - 1 - tid) * PER + j];
+            if (above + c >= need) break;
+            above += c;
+        }
+        border[0] = (THREADS - 1 - tid) * PER + j;
+        border[1] = need - above;
+    }
+    __syncthreads();
+}
+
+// A row's list in one kv head, and what of it does not depend on the scores.
+struct SelectList {
+    SelectRow at;
+    int64_t row, list;
+    int head, n;   // n: pages that may be chosen
+    bool choose;   // not all of them are
+    const uint64_t* keys;
+    const int32_t* table;
+    __device__ __forceinline__ SelectList(const Kv4SelectArgs& a, int64_t unit)
+        : at(a, unit / a.s.Hk), row(unit / a.s.Hk), list(unit * a.width), head((int)(unit - row * a.s.Hk)) {}
+    // falls: so do row starts, and nothing is computed
+    __device__ __forceinline__ void settle(const Kv4SelectArgs& a, bool falls, bool speaks) {
+        if (falls) at.len = -1, at.seen = at.free_end = 0, at.over = true;
+        if (at.over && head == 0 && speaks) record_status(PN_ERR_ARG);
+        n = max(at.free_end - a.first, 0);
+        choose = n > a.top;
+        keys = a.keys + (row * a.s.Hk + head) * a.s.table_w + a.first;
+        table = a.s.table + at.b * a.s.table_ld;
+    }
+    __device__ __forceinline__ void put(const Kv4SelectArgs& a, int slot, int i) const {
+        a.pages[list + slot] = i < a.s.table_w ? __ldg(table + i) : -1;
+        if (a.chosen) a.chosen[list + slot] = i;
+    }
+    // The first and the last pages (or all), the rest of the list, and the row's length; by thread `me` of `of`.
+    __device__ __forceinline__ void frame(const Kv4SelectArgs& a, int me, int of) const {
+        const int taken = choose ? a.first + a.top : at.seen, last = choose ? at.free_end : at.seen, kept = taken + at.seen - last;
+        for (int i = me; i < (choose ? a.first : taken); i += of) put(a, i, i);
+        for (int i = me; i < at.seen - last; i += of) put(a, taken + i, last + i);
+        for (int i = kept + me; i < a.width; i += of) {
+            a.pages[list + i] = -1;
+            if (a.chosen) a.chosen[list + i] = -1;
+        }
+        if (head == 0 && me == 0)  // all pages but the last are whole
+            a.lens[row] = at.len <= 0 ? at.len : (kept - 1) * a.s.page + at.len - (at.seen - 1) * a.s.page;
+    }
+};
+
+// The threshold of the `top` largest of n keys.  A histogram over evenly spaced bins leaves few
+// keys in the bin where the count from above reaches `top`; those are ranked one against
+// another.  Where that bin holds more than kSelectFew (scores that are equal, or far from evenly
+// spread), or there are few keys at all, they are taken digit by digit from the highest instead,
+// until the digits are out or a bin is taken whole.  Then the pages above the threshold and the
+// first `need` of those at it are written in order.  One block per row and kv head; the threads
+// keep HELD keys each in registers from pass to pass (more are read again), and what is counted
+// per warp is joined once for all of them: what bounds the kernel is how often it waits (8 rows of
+// 4096 pages, 1024 threads: 13 us; 256 threads, keys read for each pass, by digits alone and with
+// counts joined for 256 pages at a time: 22 us).
+template <int THREADS, int HELD>
+__global__ void __launch_bounds__(THREADS) kv4_select_kernel(const Kv4SelectArgs a) {
     __shared__ int bins[kSelectBins];
-    __shared__ int warp_sums[kSelectThreads / 32];
+    __shared__ int warp_sums[THREADS / 32];
     __shared__ int border[2];  // the bin, and how many of it are needed
+    __shared__ float range[2][THREADS / 32];
+    __shared__ int counts[HELD * (THREADS / 32)];
+    __shared__ uint64_t few[kSelectFew];
+    __shared__ uint64_t found[2];  // the threshold, and how many of those at it are needed
+    __shared__ int n_few;
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row = blockIdx.x / a.s.Hk;
-    const int head = (int)(blockIdx.x - row * a.s.Hk);
-    SelectRow at(a, row);
-    if (a.s.cu) {  // row starts that fall: nothing is computed
-        bool falls = false;
-        for (int b = tid; b < a.s.B; b += kSelectThreads) falls |= __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
-        if (__syncthreads_or(falls)) {
-            at.len = -1, at.seen = at.free_end = 0, at.over = true;
-        }
-    }
-    if (at.over && head == 0 && tid == 0) record_status(PN_ERR_ARG);
-    const int64_t list = (row * a.s.Hk + head) * a.width;
-    const int n = max(at.free_end - a.first, 0);
+    SelectList to(a, blockIdx.x);
+    bool falls = false;
+    if (a.s.cu)
+        for (int b = tid; b < a.s.B; b += THREADS) falls |= __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
+    to.settle(a, __syncthreads_or(falls), tid == 0);
+    to.frame(a, tid, THREADS);
+    const int n = to.n;
+    const uint64_t* keys = to.keys;
     uint64_t edge = 0;  // taken: keys whose digits above `shift` exceed it, and `need` of those that equal it
     int shift = 0, need = 0;
-    const uint64_t* keys = a.keys + (row * a.s.Hk + head) * a.s.table_w + a.first;
-    const bool choose = n > a.top;
-    if (choose && a.top > 0) {
-        need = a.top;
-        shift = 64;
-        for (int width = 11; shift > 0; shift -= width) {
-            if (shift < width) width = shift;
-            for (int i = tid; i < kSelectBins; i += kSelectThreads) bins[i] = 0;
-            __syncthreads();
-            const int low = shift - width;
-            for (int i = tid; i < n; i += kSelectThreads) {
-                const uint64_t k = keys[i];
-                if (shift == 64 || k >> shift == edge) atomicAdd(&bins[(k >> low) & ((1 << width) - 1)], 1);
-            }
-            __syncthreads();
-            // thread t has bins [8 (255 - t), + 8): counts from above
-            constexpr int PER = kSelectBins / kSelectThreads;
-            int mine = 0;
+    if (to.choose && a.top > 0) {
+        constexpr int RUN = THREADS * HELD;
+        const int runs = (n + RUN - 1) / RUN;
+        uint64_t k[HELD];
+        auto load = [&](int run) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) mine += bins[(kSelectThreads - 1 - tid) * PER + j];
-            int inc = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += v;
+            for (int j = 0; j < HELD; ++j) {
+                const int i = run * RUN + j * THREADS + tid;
+                k[j] = i < n ? keys[i] : 0;
             }
-            if (lane == 31) warp_sums[warp] = inc;
-            __syncthreads();
-            for (int w = 0; w < warp; ++w) inc += warp_sums[w];
-            int above = inc - mine;
-            if (above < need && need <= inc) {
-                int j = PER - 1;
-                for (;; --j) {
-                    const int c = bins[(kSelectThreads - 1 - tid) * PER + j];
-                    if (above + c >= need) break;
-                    above += c;
+        };
+        // f(key) for all keys
+        auto each_key = [&](auto f) {
+            for (int run = 0; run < runs; ++run) {
+                if (runs > 1) load(run);
+#pragma unroll
+                for (int j = 0; j < HELD; ++j) {
+                    const int i = run * RUN + j * THREADS + tid;
+                    if (i < n) f(k[j]);
                 }
-                border[0] = (kSelectThreads - 1 - tid) * PER + j;
-                border[1] = need - above;
             }
-            __syncthreads();
-            edge = (shift == 64 ? 0 : edge << width) | (uint32_t)border[0];
-            need = border[1];
-            const bool whole = bins[border[0]] == need;
-            __syncthreads();
-            if (whole) {
-                shift = low;
-                break;
-            }
-        }
-    }
-    // the pages in order
-    if (head == 0 && tid == 0) {
-        const int kept = choose ? min(a.first, at.seen) + a.top + (at.seen - at.free_end) : at.seen;
-        // all pages but the last are whole
-        a.lens[row] = at.len <= 0 ? at.len : (kept - 1) * a.s.page + at.len - (at.seen - 1) * a.s.page;
-    }
-    int done = 0, equal = 0;  // pages written, keys at the edge met so far
-    for (int base = 0; base < at.seen; base += kSelectThreads) {
-        const int i = base + tid;
-        bool take = false, tie = false;
-        if (i < at.seen) {
-            if (!choose || i < a.first || i >= at.free_end) {
-                take = true;
-            } else if (a.top > 0) {
-                const uint64_t k = keys[i - a.first] >> shift;
-                take = k > edge;
-                tie = k == edge;
-            }
-        }
-        // how many of either lie before: taken ones in the low half, ties in the high one
-        const uint32_t m_take = __ballot_sync(0xffffffffu, take), m_tie = __ballot_sync(0xffffffffu, tie);
-        const uint32_t under = (1u << lane) - 1;
-        __syncthreads();
-        if (lane == 0) warp_sums[warp] = __popc(m_take) | __popc(m_tie) << 16;
-        __syncthreads();
-        int taken = __popc(m_take & under), ties = __popc(m_tie & under), all_taken = 0, all_ties = 0;
+        };
+        load(0);
+        bool digits = true;
+        if constexpr (HELD > 2) {  // (with fewer keys that is more work than the digits')
+            float lo = INFINITY, hi = -INFINITY;
+            each_key([&](uint64_t key) {
+                const float v = score_of(key);
+                if (key != 0 && fabsf(v) < INFINITY) lo = fminf(lo, v), hi = fmaxf(hi, v);
+            });
 #pragma unroll
-        for (int w = 0; w < kSelectThreads / 32; ++w) {
-            const int v = warp_sums[w];
-            if (w < warp) taken += v & 0xFFFF, ties += v >> 16;
-            all_taken += v & 0xFFFF, all_ties += v >> 16;
+            for (int o = 16; o > 0; o >>= 1) {
+                lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            }
+            if (lane == 0) range[0][warp] = lo, range[1][warp] = hi;
+            for (int i = tid; i < kSelectBins; i += THREADS) bins[i] = 0;
+            if (tid == 0) n_few = 0;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < THREADS / 32; ++w) lo = fminf(lo, range[0][w]), hi = fmaxf(hi, range[1][w]);
+            float each = (kSelectBins - 1) / (hi - lo);
+            if (!(hi > lo) || !(each < INFINITY)) lo = 0.0f, each = 0.0f;  // (one bin but for infinities)
+            each_key([&](uint64_t key) { atomicAdd(&bins[score_bin(key, lo, each)], 1); });
+            __syncthreads();
+            select_border<THREADS>(bins, a.top, warp_sums, border);
+            const int bin = border[0], m = bins[bin];
+            need = border[1];
+            if (m <= kSelectFew) {
+                each_key([&](uint64_t key) {
+                    if (score_bin(key, lo, each) == bin) few[atomicAdd(&n_few, 1)] = key;
+                });
+                __syncthreads();
+                if (tid < m) {
+                    const uint64_t key = few[tid];
+                    int above = 0, same = 0;
+                    for (int j = 0; j < m; ++j) {
+                        above += few[j] > key;
+                        same += few[j] == key;
+                    }
+                    // (equal keys write the same)
+                    if (above < need && need <= above + same) found[0] = key, found[1] = need - above;
+                }
+                __syncthreads();
+                edge = found[0];
+                need = (int)found[1];
+                digits = false;
+            }
+            __syncthreads();  // the border is read
         }
-        const int ties_before = min(equal + ties, need);
-        if (take || (tie && equal + ties < need)) {
-            const int slot = done + taken + ties_before - min(equal, need);
-            a.pages[list + slot] = i < a.s.table_w ? __ldg(a.s.table + at.b * a.s.table_ld + i) : -1;
-            if (a.chosen) a.chosen[list + slot] = i;
+        if (digits) {
+            need = a.top;
+            shift = 64;
+            for (int width = 11; shift > 0; shift -= width) {
+                if (shift < width) width = shift;
+                for (int i = tid; i < kSelectBins; i += THREADS) bins[i] = 0;
+                __syncthreads();
+                const int low = shift - width;
+                each_key([&](uint64_t key) {
+                    if (shift == 64 || key >> shift == edge) atomicAdd(&bins[(key >> low) & ((1 << width) - 1)], 1);
+                });
+                __syncthreads();
+                select_border<THREADS>(bins, need, warp_sums, border);
+                edge = (shift == 64 ? 0 : edge << width) | (uint32_t)border[0];
+                need = border[1];
+                const bool whole = bins[border[0]] == need;
+                __syncthreads();
+                if (whole) {
+                    shift = low;
+                    break;
+                }
+            }
         }
-        done += all_taken + min(equal + all_ties, need) - min(equal, need);
-        equal += all_ties;
+        // those chosen, in order
+        int done = 0, equal = 0;  // keys above the edge and at it in the runs before
+        for (int run = 0; run < runs; ++run) {
+            if (runs > 1) load(run);
+            // how many of either a warp has in each of its rows of keys: those above in the low half
+            int before[HELD];
+            uint32_t takes = 0, ties = 0;
+            __syncthreads();  // the counts of the run before are read
+#pragma unroll
+            for (int j = 0; j < HELD; ++j) {
+                const bool there = run * RUN + j * THREADS + tid < n;
+                const uint64_t digits = k[j] >> shift;
+                const bool take = there && digits > edge, tie = there && digits == edge;
+                const uint32_t m_take = __ballot_sync(0xffffffffu, take), m_tie = __ballot_sync(0xffffffffu, tie);
+                const uint32_t under = (1u << lane) - 1;
+                before[j] = __popc(m_take & under) | __popc(m_tie & under) << 16;
+                takes |= (uint32_t)take << j, ties |= (uint32_t)tie << j;
+                if (lane == 0) counts[j * (THREADS / 32) + warp] = __popc(m_take) | __popc(m_tie) << 16;
+            }
+            __syncthreads();
+            // the counts before each, and their sum
+            constexpr int ALL = HELD * (THREADS / 32), PER = (ALL + 31) / 32;
+            if (warp == 0) {
+                int mine[PER], sum = 0;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) sum += mine[j] = lane * PER + j < ALL ? counts[lane * PER + j] : 0;
+                int inc = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                    if (lane >= o) inc += v;
+                }
+                int at = inc - sum;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    if (lane * PER + j < ALL) counts[lane * PER + j] = at;
+                    at += mine[j];
+                }
+                if (lane == 31) border[0] = inc;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < HELD; ++j) {
+                const int v = counts[j * (THREADS / 32) + warp] + before[j];
+                const int above = done + (v & 0xFFFF), same = equal + (v >> 16);
+                if ((takes >> j & 1) || ((ties >> j & 1) && same < need))
+                    to.put(a, a.first + above + min(same, need), a.first + run * RUN + j * THREADS + tid);
+            }
+            done += border[0] & 0xFFFF;
+            equal += border[0] >> 16;
+        }
     }
-    for (int i = done + tid; i < a.width; i += kSelectThreads) {
-        a.pages[list + i] = -1;
-        if (a.chosen) a.chosen[list + i] = -1;
+}
+
+// The same for tables of up to kSmallPages pages and many rows: a warp per row and kv head, its keys
+// in registers, the threshold found bit by bit from the highest in which two keys differ, until exactly
+// `top` are at or above it or the bits are out.  502 rows x 8 heads of 250 pages: 16 us, 35 with a
+// block for each; few rows wait for its steps, though (32 x 8 of up to 512: 12 us, 9 with blocks).
+constexpr int kWarpHeld = 16, kSmallPages = 32 * kWarpHeld, kWarpSelects = 4;
+__global__ void __launch_bounds__(kWarpSelects * 32) kv4_select_warp_kernel(const Kv4SelectArgs a) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (int64_t)blockIdx.x * kWarpSelects + (threadIdx.x >> 5);
+    if (unit >= a.s.T * a.s.Hk) return;
+    SelectList to(a, unit);
+    bool falls = false;
+    if (a.s.cu)
+        for (int b = lane; b < a.s.B; b += 32) falls |= __ldg(a.s.cu + b + 1) < __ldg(a.s.cu + b);
+    to.settle(a, __any_sync(0xffffffffu, falls), lane == 0);
+    to.frame(a, lane, 32);
+    if (!to.choose || a.top == 0) return;
+    uint64_t k[kWarpHeld], lo = ~0ull, hi = 0;
+#pragma unroll
+    for (int j = 0; j < kWarpHeld; ++j) k[j] = j * 32 + lane < to.n ? to.keys[j * 32 + lane] : 0;
+#pragma unroll
+    for (int j = 0; j < kWarpHeld; ++j)
+        if (j * 32 + lane < to.n) lo = min(lo, k[j]), hi = max(hi, k[j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, (uint64_t)__shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, (uint64_t)__shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    // `edge`: the largest number that at least `top` keys reach (those that are not there are 0, and reach none)
+    int bit = 64 - __clzll((long long)(lo ^ hi)), above = 0;
+    uint64_t edge = bit == 64 ? 0 : hi >> bit << bit;
+    for (bool exact = false; bit > 0 && !exact;) {
+        const uint64_t next = edge | 1ull << --bit;
+        int reach = 0;
+#pragma unroll
+        for (int j = 0; j < kWarpHeld; ++j) reach += k[j] >= next;
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        if (reach >= a.top) edge = next;
+        exact = reach == a.top;
+    }
+#pragma unroll
+    for (int j = 0; j < kWarpHeld; ++j) above += k[j] > edge;
+    const int need = a.top - __reduce_add_sync(0xffffffffu, above);  // of those at the edge, the first
+    int done = a.first, equal = 0;
+    const uint32_t under = (1u << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < kWarpHeld; ++j) {
+        const bool there = j * 32 + lane < to.n, take = there && k[j] > edge, tie = there && k[j] == edge;
+        const uint32_t m_take = __ballot_sync(0xffffffffu, take), m_tie = __ballot_sync(0xffffffffu, tie);
+        const int same = equal + __popc(m_tie & under);
+        if (take || (tie && same < need)) to.put(a, done + __popc(m_take & under) + min(same, need), a.first + j * 32 + lane);
+        done += __popc(m_take);
+        equal += __popc(m_tie);
     }
 }
 
@@ -461,7 +654,17 @@ int pn_kv4_sparse_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q
                              : pn::launch_dependent(pn::kv4_score_kernel<128>, grid, pn::kScoreThreads, s, c);
         if (err != cudaSuccess) return cuda_fail(err, name);
     }
-    err = pn::launch_dependent(pn::kv4_select_kernel, dim3((unsigned)(T * kv_heads)), pn::kSelectThreads, s, c);
+    const int64_t units = T * kv_heads;
+    const dim3 blocks((unsigned)units);
+    // (for few rows the passes of each are what takes the time)
+    if (a.s.table_w > pn::kSmallPages)
+        err = units <= pn::sm_count() ? pn::launch_dependent(pn::kv4_select_kernel<1024, 8>, blocks, 1024, s, c)
+                                      : pn::launch_dependent(pn::kv4_select_kernel<256, 8>, blocks, 256, s, c);
+    else if (units <= 8 * pn::sm_count())
+        err = pn::launch_dependent(pn::kv4_select_kernel<256, 2>, blocks, 256, s, c);
+    else
+        err = pn::launch_dependent(pn::kv4_select_warp_kernel, dim3((unsigned)((units + pn::kWarpSelects - 1) / pn::kWarpSelects)),
+                                   pn::kWarpSelects * 32, s, c);
     if (err != cudaSuccess) return cuda_fail(err, name);
     // every row a sequence of its own
     a.q_l = cu_q ? T : a.s.L;  // (with cu_q rows lie one after another)

@@ -110,7 +110,7 @@ def load() -> ctypes.CDLL:
         "pn_kv4_attention": (I, [P, I64, I64, I64, I, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, F, P, P,
                                  SZ, P]),
         "pn_kv4_append_rotary": (I, [P, I64, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I, P, P, I64, I64, I64, I, P,
-                                     P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, P]),
+                                     P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64, P, I, P]),
         "pn_kv4_prefix_attention_workspace_size": (SZ, [I64, I64, I64, I64, I64, I64]),
         "pn_kv4_prefix_attention": (I, [P, I64, I64, I64, I, I64, P, I64, I64, I64, I64, P, I64, I64, P, P, I64, I64,
                                         P, I64, I64, P, P, I64, F, P, P, SZ, P]),

@@ -21,7 +21,7 @@ def rotary(**kw):
     return nat.load().pn_kv4_append_rotary(a["q"], 1, 1, 1, a["heads"], a["k"], 1, 1, 1, a["v"], 1, 1, 1, a["dt"], a["cos"],
                                            a["sin"], a["n"], a["stride"], a["R"], 0, a["offsets"], a["cache"], a["n_pages"],
                                            a["hk"], a["page"], a["d"], a["table"], a["ld"], a["w"], a["lens"], a["cu"], a["B"],
-                                           a["T"], a["out"], None)
+                                           a["T"], a["out"], 0, None)
 
 
 def prefix(**kw):

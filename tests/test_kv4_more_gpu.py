@@ -156,6 +156,23 @@ def test_rotary_edges(cuda_device):
     assert not y.any() and nat.device_status() == nat.PN_ERR_ARG
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,rows", [(64, [1]), (128, [3, 0, 400])])
+def test_rotary_rows_of_no_sequence(cuda_device, dtype, d, rows):
+    """Behind the last sequence: zeros in a new tensor, whatever its memory held, and for calls without sequences."""
+    s = Rows([r + 3 for r in rows], rows, 3, 1, d, 16, dtype, cuda_device)
+    cos, sin = tables(500, d, cuda_device)
+    T = sum(rows)
+    dev = lambda x: torch.cat((x, x[:1].expand(37, -1, -1))).to(cuda_device)
+    junk = torch.full((T + 37, 3, d), 7.0, dtype=dtype, device=cuda_device)
+    del junk
+    got = pc.kv4_append_rotary(dev(s.q), dev(s.k), dev(s.v), cos, sin, s.empty.clone(), s.table, s.lens, cu_q=s.cu)
+    assert got[:T].any() and not got[T:].any()
+    none = pc.kv4_append_rotary(dev(s.q), dev(s.k), dev(s.v), cos, sin, s.empty.clone(), s.table[:0], s.lens[:0],
+                                cu_q=ints([0], cuda_device))
+    assert not none.any() and nat.device_status() == 0
+
+
 def test_rotary_not_finite(cuda_device):
     """A key vector with an inf or NaN reads back as NaN, and no other does."""
     s = Rows([6], [6], 2, 2, 64, 16, torch.float32, cuda_device)
@@ -349,6 +366,16 @@ def test_prefix_not_finite(cuda_device):
     assert y[0].isnan().all() and not y[1:].isnan().any()
 
 
+@pytest.mark.parametrize("B,G", [(4, 2), (8, 4), (36, 8)])
+def test_prefix_again_and_again(cuda_device, B, G):
+    """A long prefix behind few and many rows: the same bits from every call."""
+    s = Shared([9] * B, [5000], [B], 1, 128, 64, cuda_device, seed=B)
+    q = torch.randn(9 * B, G, 128, device=cuda_device, dtype=torch.bfloat16)
+    want = s.call(q, [9] * B)
+    assert all(torch.equal(s.call(q, [9] * B), want) for _ in range(10))
+    assert nat.device_status() == 0
+
+
 def test_prefix_captured(cuda_device):
     """A captured call follows lengths, tables and shares; two calls on two streams."""
     s = Shared([20, 31, 8, 40], [200, 90], [2, 2], 2, 128, 16, cuda_device)
@@ -512,6 +539,50 @@ def test_sparse_ties_and_nan(cuda_device):
     got = pages(mean, 36, lost)
     assert not (got == 7).any() and nat.device_status() == 0
     assert (pages(mean, 37, lost) == 7).any() and nat.device_status() == nat.PN_ERR_ARG
+
+
+@pytest.mark.parametrize("B,pages,top", [(1, 1, 1), (3, 512, 40), (40, 500, 1), (1300, 77, 9), (1200, 512, 100), (2, 513, 64), (200, 520, 17),
+                                         (2, 8300, 70), (160, 2100, 300)])
+@pytest.mark.parametrize("scores", ["normal", "wide", "few", "not finite"])
+def test_sparse_choice_over_many_pages(cuda_device, B, pages, top, scores):
+    """The choice alone, for every kernel of it: up to 512 pages, more, more than the threads hold, few rows and
+    many; scores that spread evenly, over many magnitudes, that are mostly equal, with infinities and NaN."""
+    d, page, first, last = 64, 16, 1, 2
+    gen = torch.Generator().manual_seed(B + pages + top)
+    means = torch.zeros(pages, 1, d)
+    q = torch.zeros(B, 1, d)
+    if scores == "normal":
+        means.normal_(generator=gen)
+        q.normal_(generator=gen)
+    else:
+        q[..., 0] = 1
+        x = torch.randn(pages, generator=gen)
+        if scores == "wide":
+            x = x.sign() * torch.exp2(x * 30)
+        elif scores == "few":
+            x = (x * 0.7).round()
+        else:
+            x[torch.rand(pages, generator=gen) < 0.3] = float("inf")
+            x[torch.rand(pages, generator=gen) < 0.2] = -float("inf")
+            x[torch.rand(pages, generator=gen) < 0.2] = float("nan")
+        means[:, 0, 0] = x
+    means = means.to(torch.bfloat16)
+    cache = pc.kv4_cache(pages, 1, d, page, cuda_device)
+    order = torch.stack([torch.randperm(pages, generator=gen) for _ in range(B)])
+    lens = torch.randint(1, pages * page + 1, (B,), generator=gen)
+    lens[0] = pages * page
+    got = pc.kv4_sparse_attention(q.to(cuda_device), cache, means.to(cuda_device), order.int().to(cuda_device),
+                                  lens.int().to(cuda_device), top, first, last, return_pages=True)[1].cpu()
+    for b in range(B):
+        seen = -(-int(lens[b]) // page)
+        score = (means[order[b, :seen], 0].double() * q[b, 0].double()).sum(-1)
+        score = torch.where(score.isnan(), torch.tensor(-torch.inf, dtype=torch.float64), score)
+        nan = means[order[b, :seen], 0, 0].isnan()
+        free = [i for i in range(first, seen - last)]
+        free.sort(key=lambda i: (bool(nan[i]), -float(score[i]), i))
+        want = sorted(set(range(min(first, seen))) | set(range(max(seen - last, 0), seen)) | set(free[:top]))
+        assert got[b, 0].tolist() == want + [-1] * (first + top + last - len(want)), (b, seen)
+    assert nat.device_status() == 0
 
 
 def test_sparse_rows_of_a_projection(cuda_device):
