@@ -14,8 +14,8 @@
 //
 // What bounds it: over the prefix, the exponentials and the unpacking of codes for every tile of
 // 128 rows.  64 sequences x 8 heads of 128 dims x 8 rows a head over 8192 tokens: 63 us of the
-// call's 112 (510 TFLOP/s from one length to the next; cuBLAS reaches 1667), the rows'
-// own 1000 tokens 38, the joining 15.  A kernel for the prefix alone was built too (256 rows to a tile,
+// call's 113 (510 TFLOP/s from one length to the next; cuBLAS reaches 1667), the rows'
+// own 1000 tokens 40, the joining 13.  A kernel for the prefix alone was built too (256 rows to a tile,
 // warps by task, the logits of a step formed while the softmax of the one before ran): 75 us
 // there and 186 over one prefix of 131071 tokens for 64 rows a head, where the chunk kernel
 // takes 148; its five kinds of warps did not fit the instruction cache, and it was given up.
@@ -131,7 +131,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const Kv4Me
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] *= f;
         const uint32_t some = __ballot_sync(0xffffffffu, l != 0.0f);
-        constexpr int AT_ONCE = 4;  // loads in flight (four, each behind a branch: 55 partial results of 512 rows took 38 us)
+        // Loads in flight.  512 rows of 55 partial results: 24 us (38 with each load behind a branch, 17 with eight
+        // at once, which cost the cases of two or three results 3 us more).
+        constexpr int AT_ONCE = 4;
 #pragma unroll 1
         for (int k = 0; k < n; k += AT_ONCE) {
             float u[AT_ONCE][E];
