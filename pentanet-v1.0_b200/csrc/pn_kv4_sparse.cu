@@ -626,7 +626,9 @@ int pn_kv4_sparse_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q
     if (kv_heads > 65535 || (double)T * kv_heads > 2e9) return fail(PN_ERR_SHAPE, "%s: %lld rows of %lld kv heads", name, (long long)T, (long long)kv_heads);
     if ((double)T * kv_heads * ((double)table_w + width) * 8 > 6e10)
         return fail(PN_ERR_SHAPE, "%s: %lld rows over tables of %lld pages are too much for one call", name, (long long)T, (long long)table_w);
-    if (int st = check_attn_units(name, a.s, a.G, std::min(width, table_w) * page)) return st;
+    pn::Kv4Seq rows = a.s;  // (every row a sequence of its own)
+    rows.B = T;
+    if (int st = check_attn_units(name, rows, a.G, std::min(width, table_w) * page)) return st;
     if (int st = check_device()) return st;
     if (T == 0 || B == 0) return ok();
     const pn::SparseLayout lay(T, kv_heads, a.G, head_dim, a.s.table_w, width);

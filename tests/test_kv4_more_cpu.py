@@ -102,7 +102,9 @@ def test_prefix_refusals(kw, want):
 @pytest.mark.parametrize("kw,want", [
     (dict(means=None), nat.PN_ERR_ARG), (dict(means=P + 8), nat.PN_ERR_ALIGN), (dict(chosen=P + 2), nat.PN_ERR_ALIGN),
     (dict(first=-1), nat.PN_ERR_SHAPE), (dict(last=0), nat.PN_ERR_SHAPE), (dict(top=-1), nat.PN_ERR_SHAPE),
-    (dict(top=1 << 31), nat.PN_ERR_SHAPE), (dict(top=1 << 24), nat.PN_ERR_SHAPE)])
+    (dict(top=1 << 31), nat.PN_ERR_SHAPE), (dict(top=1 << 24), nat.PN_ERR_SHAPE),
+    # (a row of one query head is a tile of its own: 2^20 rows x 8 heads x 401 units of 128 tokens)
+    (dict(T=1 << 20, B=1, heads=8, hk=8, page=128, top=398, w=401, ld=401), nat.PN_ERR_SHAPE)])
 def test_sparse_refusals(kw, want):
     assert sparse(**kw) == want
 

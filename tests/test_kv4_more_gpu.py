@@ -274,6 +274,23 @@ def test_prefix_many_rows(cuda_device, d):
     s.attend([9] * 33, 8)
 
 
+def test_prefix_and_own_on_the_long_kernel(cuda_device):
+    """Chunks long enough that both passes take the kernel for many rows, one right behind the other."""
+    B, L, G, hk, d = 40, 96, 2, 8, 64
+    s = Shared([L] * B, [300, 77], [30, 10], hk, d, 64, cuda_device, seed=3)
+    q = torch.randn(B * L, G * hk, d, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    y = s.call(q.to(cuda_device), [L] * B)
+    assert nat.device_status() == 0
+    some = [0, 1, 17, 29, 30, 39]  # (the 64-bit attention of all of them would take minutes)
+    for i in some:
+        k, v = (torch.cat((t[B + s.of[i]], t[i])) for t in (s.b.k, s.b.v))
+        x = q[i * L:(i + 1) * L]
+        want, bound = oracle.attention(x, k, v, None)
+        bound = bound + more.join_bound(x, k, v)
+        bound = bound + 2.0 ** -8 * (want.abs() + bound)
+        assert ((y[i * L:(i + 1) * L].double().cpu() - want).abs() <= bound + 1e-30).all(), i
+
+
 def test_prefix_equal_shares(cuda_device):
     """Without cu_prefix; (B, L) rows of a projection; against the same tokens laid out as whole sequences."""
     B, L, H, hk, d, page = 6, 2, 8, 2, 128, 16
