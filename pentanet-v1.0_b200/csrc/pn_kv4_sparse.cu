@@ -140,36 +140,39 @@ struct SelectRow {
 };
 
 // A block scores some pages for up to `tile` rows of one kv head.  Four lanes share a page's
-// mean, held as fp64 for all rows of a sequence in turn; the group's queries are summed
-// once per block.
+// mean, held as fp64 for all rows of a sequence; the group's queries are summed once per
+// block.  Rows are taken four at a time: one by one the kernel waits for their loads from
+// shared memory (502 rows x 8 heads of 250 pages 63 us, 79 one by one; the fp64 units are busy for a
+// ninth of it).
 template <int D>
 __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4SelectArgs a) {
     constexpr int E = D / 4;  // dims per lane: chunks of 8, four lanes in turn
     __shared__ double q[kScoreTile][D];
     __shared__ int seq[kScoreTile], from[kScoreTile], to[kScoreTile];
+    __shared__ int64_t base[kScoreTile];
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row0 = (int64_t)blockIdx.x * a.tile;
     const int head = blockIdx.y;
-    for (int r = 0; r < a.tile; ++r) {
-        const SelectRow at(a, row0 + r);
-        const int n = max(at.free_end - a.first, 0);
-        if (tid == 0) {
-            seq[r] = n > a.top ? (int)at.b : -1;  // (with fewer pages all are taken)
-            from[r] = a.first, to[r] = at.free_end;
+    if (tid < a.tile) {
+        const SelectRow at(a, row0 + tid);
+        seq[tid] = max(at.free_end - a.first, 0) > a.top ? (int)at.b : -1;  // (with fewer pages all are taken)
+        from[tid] = a.first, to[tid] = at.free_end;
+        base[tid] = a.s.cu ? (row0 + tid) * a.q_sl : at.b * a.q_sb + at.i * a.q_sl;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int k = tid; k < a.tile * D; k += kScoreThreads) {
+        const int r = k / D, d = k % D;
+        if (seq[r] < 0) continue;
+        double sum = 0.0;
+        for (int g = 0; g < a.G; ++g) {
+            const int64_t p = base[r] + (int64_t)(head * a.G + g) * a.q_sh + d;
+            sum += (double)(a.q_f32 ? static_cast<const float*>(a.q)[p]
+                                    : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[p]));
         }
-        if (n <= a.top) continue;
-        const int64_t base = a.s.cu ? (row0 + r) * a.q_sl : at.b * a.q_sb + at.i * a.q_sl;
-        for (int d = tid; d < D; d += kScoreThreads) {
-            double sum = 0.0;
-            for (int g = 0; g < a.G; ++g) {
-                const int64_t p = base + (int64_t)(head * a.G + g) * a.q_sh + d;
-                sum += (double)(a.q_f32 ? static_cast<const float*>(a.q)[p]
-                                        : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[p]));
-            }
-            q[r][d] = sum;
-        }
+        q[r][d] = sum;
     }
     __syncthreads();
     const int part = lane & 3, sub = warp * 8 + (lane >> 2);
@@ -182,8 +185,8 @@ __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4Selec
         for (; r1 < a.tile && seq[r1] == seq[r0]; ++r1) hi = max(hi, to[r1]);
         const int64_t b = seq[r0];
         // the pages [lo, hi) in runs of 32 to a block
-        for (int base = lo + blockIdx.z * 32; base < hi; base += a.splits * 32) {
-            const int i = base + sub;
+        for (int run = lo + blockIdx.z * 32; run < hi; run += a.splits * 32) {
+            const int i = run + sub;
             const int p = i < hi ? __ldg(a.s.table + b * a.s.table_ld + i) : -1;
             const bool there = p >= 0 && p < a.s.n_pages;
             double m[E];
@@ -198,7 +201,7 @@ __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4Selec
                     m[c * 8 + 2 * j + 1] = (double)__uint_as_float(w[j] & 0xFFFF0000u);
                 }
             }
-            for (int r = r0; r < r1; ++r) {
+            auto part_of = [&](int r) {  // this lane's part of the score of row r
                 double sum = 0.0, sum2 = 0.0;
 #pragma unroll
                 for (int c = 0; c < E / 8; ++c)
@@ -208,11 +211,28 @@ __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4Selec
                         sum = fma(x.x, m[c * 8 + j], sum);
                         sum2 = fma(x.y, m[c * 8 + j + 1], sum2);
                     }
-                sum += sum2;
+                return sum + sum2;
+            };
+            auto put = [&](int r, double sum) {
+                if (i < to[r]) a.keys[((row0 + r) * a.s.Hk + head) * a.s.table_w + i] = there ? score_key(sum) : 0;
+            };
+            if (r1 - r0 == 1) {
+                double sum = part_of(r0);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (part == 0 && i < to[r])
-                    a.keys[((row0 + r) * a.s.Hk + head) * a.s.table_w + i] = there ? score_key(sum) : 0;
+                if (part == 0) put(r0, sum);
+                continue;
+            }
+            // four rows at once: their loads and sums do not wait for one another, and each lane ends with one row
+            for (int r = r0; r < r1; r += 4) {
+                double s[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[k] = part_of(min(r + k, r1 - 1));
+                const bool odd = part & 1, high = part & 2;
+                const double two[2] = {(odd ? s[1] : s[0]) + __shfl_xor_sync(0xffffffffu, odd ? s[0] : s[1], 1),
+                                       (odd ? s[3] : s[2]) + __shfl_xor_sync(0xffffffffu, odd ? s[2] : s[3], 1)};
+                const double sum = (high ? two[1] : two[0]) + __shfl_xor_sync(0xffffffffu, high ? two[0] : two[1], 2);
+                if (r + part < r1) put(r + part, sum);
             }
         }
         r0 = r1;
