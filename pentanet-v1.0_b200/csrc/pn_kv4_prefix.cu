@@ -169,6 +169,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const Kv4Me
 
 // The kernel for the rows over the prefixes, which walk long sequences together; the host knows no
 // more of the lengths than the table's width.
+// Not attn_kind's rule: the tiles are few, but their walks long.  A call in us, chunk and long kernel: 64 rows
+// of 8 heads over 131071 tokens 184 and 188, 128 rows over 8192 tokens 64 and 61; 32 rows there 53 and 52.
 static AttnKind prefix_kind(int64_t P, int64_t T, int64_t Hk, int64_t G) {
     const int64_t rows = (T + P - 1) / P * G;
     if (rows <= 16) return rows <= 8 ? kAttn8 : kAttn16;
