@@ -16,6 +16,20 @@
 // relative to the largest s_v that the row has seen; sums, the softmax's maximum
 // and total, and the z term are fp32.
 //
+// Long walks.  sum p s_v c grows with the tokens while the result is its small
+// difference from sum p z_v, and the tensor core cuts off what its products lose
+// against a large sum: all one way, as codes and weights are not negative.  Left
+// to grow over 131072 tokens the sums put the result off by 6 (decode kernel) to
+// 25 % (tcgen05) of its norm, normal random data.  So the sums are kept near zero.
+// The tcgen05 kernel, which rewrites each code anyway, takes the middle code out
+// of it: 7 of even tokens, 8 of odd ones (7.5 is no multiple of the subnormals'
+// unit), and z_v + 7 s_v or z_v + 8 s_v is the z term.  The others, where that would be
+// an instruction per register of codes, take out of a row's sums every kCentre
+// steps what one of them has reached, and add it, with the z term of these
+// steps, to a base that stays small (its two parts cancel in one fma).
+// Over any length to 131072 tokens the error is now that of the rounded weights alone,
+// 3e-4 of the result's norm in the tcgen05 kernel and 6e-4 to 8e-4 in the others.
+//
 // Shape of the decode kernel.  Keys are the 16-row operand of m16n8k16 (16
 // tokens), the query rows of one kv head (group x new tokens) its 8 columns,
 // so one product serves a whole group and wastes no more than 8 - rows
@@ -79,6 +93,9 @@ struct Kv4AttnArgs {
     int n_grp;
 };
 
+// Minus the middle codes of an even token (7) and of the odd one beside it (8), as a pair of masked
+// codes, and 2^4 of them.
+constexpr uint32_t kMiddle = 0x80088007u, kMiddle16 = 0x80808070u;
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 
@@ -109,6 +126,10 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t add_f16(uint32_t a, uint32_t b) {
+    const __half2 h = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 // 2^e for e in [-126, 127].
@@ -402,6 +423,8 @@ struct AttnCfg {
     static constexpr int W = D / 32;             // words per thread and token
     static constexpr int kRows = 8 * NT;         // query rows of a row tile
     static constexpr int kTokens = 128;          // tokens of a unit: 32 per warp
+    // Runs between two centrings.  64 sequences of 4096 tokens, 8 heads of 8 rows: 71.7 us with 4, 71.3 with 8, 69.0 with none.
+    static constexpr int kCentre = 4;
     static constexpr int kThreads = kAttnThreads;
     static constexpr int kStages = 6;
     static constexpr int kCodes = 16 * (D / 2);  // bytes of one 16-token piece of keys or values
@@ -522,6 +545,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
         }
 
         float o[NT][D / 16][4];
+        float2 base[NT];  // what was taken out of o, and the z term with it
         float2 neg_r[NT], limit[NT], l[NT], zs[NT];  // the rows' references; totals of p and of p z (this lane's tokens)
         float loud = kFirstLoud;  // the least of the rows'
 #pragma unroll
@@ -532,6 +556,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
             for (int j = 0; j < D / 16; ++j)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) o[n][j][k] = 0.0f;
+            base[n] = make_float2(0.0f, 0.0f);
         }
 
         // The two pieces of run i.  kMask: some token of them is not seen by some row.
@@ -631,6 +656,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
                     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) o[n][j][k] *= f[k & 1];
+                    base[n] = mul2(base[n], make_float2(f[0], f[1]));
                 }
             }
             // ---- weights, then dims x rows of the output
@@ -677,9 +703,32 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
                     }
             }
         };
+        // Back to about zero: of a row's sums, what this lane's first has reached (all its dims share the base).
+        auto centre = [&]() {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float2 r = make_float2(o[n][0][0], o[n][0][1]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) {
+                    zs[n].x += __shfl_xor_sync(0xffffffffu, zs[n].x, d);
+                    zs[n].y += __shfl_xor_sync(0xffffffffu, zs[n].y, d);
+                }
+                base[n] = add2(base[n], fma2(r, make_float2(16777216.0f, 16777216.0f), zs[n]));
+                zs[n] = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; k += 2) {
+                        const float up = k ? -16.0f : -1.0f;
+                        const float2 y = fma2(r, make_float2(up, up), make_float2(o[n][j][k], o[n][j][k + 1]));
+                        o[n][j][k] = y.x, o[n][j][k + 1] = y.y;
+                    }
+            }
+        };
         uint32_t slot = 0, fill = (ST - 2) * C::kStage;  // stages of runs i and i + ST / 2 - 1
         for (int i = 0; i < count; ++i) {
             issue(i + ST / 2 - 1, fill);
+            if (i % C::kCentre == 0 && i > 0) centre();
             cp_wait<ST / 2 - 1>();
             __syncwarp();
             const bool mask = (dead >> (2 * (i & 15)) & 3u) || tok_base + i * C::kTokens + 31 > sg.lim_min;
@@ -692,6 +741,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
             slot = slot == (ST - 2) * C::kStage ? 0 : slot + 2 * C::kStage;
         }
 
+        centre();  // (what is left of the z term joins the base)
+
         // ---- join the four warps
         float* mine = reinterpret_cast<float*>(ring);  // nothing is in flight
         const float up = 16777216.0f;                  // the codes' 2^-24
@@ -701,13 +752,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
             for (int d = 4; d < 32; d <<= 1) {
                 l[n].x += __shfl_xor_sync(0xffffffffu, l[n].x, d);
                 l[n].y += __shfl_xor_sync(0xffffffffu, l[n].y, d);
-                zs[n].x += __shfl_xor_sync(0xffffffffu, zs[n].x, d);
-                zs[n].y += __shfl_xor_sync(0xffffffffu, zs[n].y, d);
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const int r = n * 8 + 2 * t + k;
-                const float z = k ? zs[n].y : zs[n].x;
+                const float z = k ? base[n].y : base[n].x;
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j)
                     *reinterpret_cast<float2*>(mine + r * C::kPitch + 4 * (g * W + j / 2) + 2 * (j & 1)) =
@@ -772,6 +821,7 @@ struct ChunkCfg {
     static constexpr bool kMore = M;
     static constexpr int W = D / 32;
     static constexpr int kRows = 64, kTokens = 64, kThreads = kAttnThreads;
+    static constexpr int kCentre = 4;  // tiles between two centrings (8: the same time)
     static constexpr int kStages = 3;
     static constexpr int kCodes = 16 * (D / 2);
     static constexpr int kPiece = 2 * kCodes + 128;  // 16 tokens, as in AttnCfg
@@ -860,6 +910,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D, M>::kBlocks) kv4_chu
             for (int k = 0; k < 4; ++k) o[j][k] = 0.0f;
         l[0] = l[1] = zs[0] = zs[1] = make_float2(0.0f, 0.0f);
 
+        float base[2] = {};  // what was taken out of o, and the z term with it
         // 32 tokens from tok on, pieces `st` and the next.
         auto half = [&](const uint8_t* st, int tok, bool dead0, bool dead1, auto mask) {
             constexpr bool kMask = decltype(mask)::value;
@@ -941,6 +992,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D, M>::kBlocks) kv4_chu
                     zs[k] = mul2(zs[k], make_float2(f, f));
 #pragma unroll
                     for (int j = 0; j < D / 8; ++j) o[j][2 * k] *= f, o[j][2 * k + 1] *= f;
+                    base[k] *= f;
                 }
             }
             // ---- weights, in place as the first operand of the output's products
@@ -984,8 +1036,26 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D, M>::kBlocks) kv4_chu
                     }
             }
         };
+        auto centre = [&]() {  // as in the decode kernel
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const float r = o[0][2 * k];
+                float z = zs[k].x + zs[k].y;
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
+                base[k] += fmaf(r, 16777216.0f, z);
+                zs[k] = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < D / 8; ++j) {
+                    const float up = j & 1 ? -16.0f : -1.0f;
+                    const float2 y = fma2(make_float2(r, r), make_float2(up, up), make_float2(o[j][2 * k], o[j][2 * k + 1]));
+                    o[j][2 * k] = y.x, o[j][2 * k + 1] = y.y;
+                }
+            }
+        };
         int stage = 0;
         for (int i = 0; i < count; ++i) {
+            if (i % C::kCentre == 0 && i > 0) centre();
             cp_wait<ST - 2>();
             __syncthreads();  // tile i is there for all; all are done with the stage that is filled next
             issue(i + ST - 1, stage == 0 ? ST - 1 : stage - 1);
@@ -1003,18 +1073,17 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D, M>::kBlocks) kv4_chu
             stage = stage == ST - 1 ? 0 : stage + 1;
         }
 
+        centre();
+
         // ---- results: row g's columns 2t and 2t + 1 are 4 W dims each
         const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
         const float up = 16777216.0f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            float sum = l[k].x + l[k].y, z = zs[k].x + zs[k].y;
+            float sum = l[k].x + l[k].y, z = base[k];
 #pragma unroll
-            for (int d = 1; d < 4; d <<= 1) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                z += __shfl_xor_sync(0xffffffffu, z, d);
-            }
+            for (int d = 1; d < 4; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             const int r = warp * 16 + k * 8 + g;
             if (r >= sg.rows) continue;
             const uint32_t rr = (uint32_t)sg.r0 + r, i = rr / a.G;
@@ -1277,7 +1346,8 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 const bool none = dead[stage][tok >> 4] || tok_base + i * C::kTokens + tok >= sg.kv_end;
                 to[0] = none ? 0.0f : pair_lo(p);  // whatever lies behind the sequence
                 // (a dead piece's tokens are told by a zero of +inf: their logits are dropped)
-                to[C::kTokens] = !none ? pair_hi(p) : !kv && dead[stage][tok >> 4] ? INFINITY : 0.0f;
+                const float zero = kv ? fmaf(7 + (tok & 1), pair_lo(p), pair_hi(p)) : pair_hi(p);  // of centred value codes
+                to[C::kTokens] = !none ? zero : !kv && dead[stage][tok >> 4] ? INFINITY : 0.0f;
                 if (kv) {
                     const float top = none ? 0.0f : fmaxf(pair_lo(p), 0.0f);  // (a NaN does not count)
                     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
@@ -1296,10 +1366,11 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int n = (k + (j >> 1)) & 3;  // the dims in turn, so that eight lanes meet different banks
-                    const uint32_t sh = (n & 2) * 4, mask = n & 1 ? 0x00F000F0u : 0x000F000Fu;
+                    const uint32_t sh = (n & 2) * 4, mask = n & 1 ? 0x00F000F0u : 0x000F000Fu, mid = n & 1 ? kMiddle16 : kMiddle;
                     const int r = 4 * j + n;
                     *reinterpret_cast<uint4*>(vop + r * 128 + ((q ^ (r & 7)) * 16)) =
-                        make_uint4(w[0] >> sh & mask, w[1] >> sh & mask, w[2] >> sh & mask, w[3] >> sh & mask);
+                        make_uint4(add_f16(w[0] >> sh & mask, mid), add_f16(w[1] >> sh & mask, mid),
+                                   add_f16(w[2] >> sh & mask, mid), add_f16(w[3] >> sh & mask, mid));
                 }
             }
         };
