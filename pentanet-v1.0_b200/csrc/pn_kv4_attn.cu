@@ -20,15 +20,16 @@
 // difference from sum p z_v, and the tensor core cuts off what its products lose
 // against a large sum: all one way, as codes and weights are not negative.  Left
 // to grow over 131072 tokens the sums put the result off by 6 (decode kernel) to
-// 25 % (tcgen05) of its norm, normal random data.  So the sums are kept near zero.
-// The tcgen05 kernel, which rewrites each code anyway, takes the middle code out
-// of it: 7 of even tokens, 8 of odd ones (7.5 is no multiple of the subnormals'
-// unit), and z_v + 7 s_v or z_v + 8 s_v is the z term.  The others, where that would be
-// an instruction per register of codes, take out of a row's sums every kCentre
-// steps what one of them has reached, and add it, with the z term of these
-// steps, to a base that stays small (its two parts cancel in one fma).
-// Over any length to 131072 tokens the error is now that of the rounded weights alone,
-// 3e-4 of the result's norm in the tcgen05 kernel and 6e-4 to 8e-4 in the others.
+// 25 % (tcgen05) of its norm, normal random data.  So the sums are kept near zero:
+// every kCentre steps what they have reached (the middle one of three dims, so that
+// a loud dim does not lead the others away) is taken out of a row's sums and joins,
+// with the z term of these steps, a base that stays small, as its two parts cancel
+// in one fma.  In tensor memory that is dear, and done seldom; the tcgen05 kernel, which
+// rewrites each code anyway, also takes a middle code out of it: 7 of even tokens, 8
+// of odd ones (7.5 is no multiple of the subnormals' unit), with z_v + 7 s_v or
+// z_v + 8 s_v in the z term.  Over any length to 131072 tokens the error is now that of
+// the rounded weights alone, 2e-4 of the result's norm in the tcgen05 kernel (7e-4
+// where the mean code is far from 7.5) and 5e-4 to 8e-4 in the others.
 //
 // Shape of the decode kernel.  Keys are the 16-row operand of m16n8k16 (16
 // tokens), the query rows of one kv head (group x new tokens) its 8 columns,
@@ -132,6 +133,7 @@ __device__ __forceinline__ uint32_t add_f16(uint32_t a, uint32_t b) {
     const __half2 h = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ float middle3(float a, float b, float c) { return fmaxf(fminf(a, b), fminf(fmaxf(a, b), c)); }
 // 2^e for e in [-126, 127].
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -703,11 +705,11 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
                     }
             }
         };
-        // Back to about zero: of a row's sums, what this lane's first has reached (all its dims share the base).
+        // A row's sums back to about zero (all dims of a lane share the base).
         auto centre = [&]() {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float2 r = make_float2(o[n][0][0], o[n][0][1]);
+                const float2 r = make_float2(middle3(o[n][0][0], o[n][1][0], o[n][2][0]), middle3(o[n][0][1], o[n][1][1], o[n][2][1]));
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
                     zs[n].x += __shfl_xor_sync(0xffffffffu, zs[n].x, d);
@@ -1039,7 +1041,7 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D, M>::kBlocks) kv4_chu
         auto centre = [&]() {  // as in the decode kernel
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float r = o[0][2 * k];
+                const float r = middle3(o[0][2 * k], o[2][2 * k], o[4][2 * k]);
                 float z = zs[k].x + zs[k].y;
 #pragma unroll
                 for (int d = 1; d < 4; d <<= 1) z += __shfl_xor_sync(0xffffffffu, z, d);
@@ -1136,6 +1138,7 @@ template <int D, bool M>
 struct TcCfg {
     static constexpr bool kMore = M;
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
+    static constexpr int kCentre = 16;  // tiles between two centrings, at most (16 x 512 rows: 119.2 us, 119.0 with none)
     static constexpr int kStages = 3;
     static constexpr int kRawK = kTokens * (D / 2);      // codes of a tile's keys (or values)
     static constexpr int kRaw = 2 * kRawK + 8 * kTokens; // and the pairs: the keys', then the values'
@@ -1203,7 +1206,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
     __shared__ int s_abort;
     __shared__ uint8_t dead[ST][4];     // pieces that are not there
     __shared__ uint32_t v_top[2][2];    // largest value scale of a tile's halves (bits)
-    __shared__ float ex[2][2][128];     // exchange between a row's two threads
+    __shared__ float ex[3][2][128];     // exchange between a row's two threads
     uint8_t* qop = smem_base + (1024 - smem_u32(smem_base) % 1024) % 1024;
     uint8_t* kop = qop + C::kQ;
     uint8_t* vop = kop + C::kK;
@@ -1382,6 +1385,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
 
         float neg_r = INFINITY, limit = kFirstLimit, loud = kFirstLoud;  // the row's reference
         float2 l2 = make_float2(0.0f, 0.0f), z2 = make_float2(0.0f, 0.0f);  // sums over this thread's tokens
+        float base = 0.0f;  // what was taken out of its dims' sums, and the z term with it
         float2 x[16];
         // weights of tile i into tensor memory; kMask: some token is not seen by some row
         auto weights = [&](const float* pk, auto mask) {
@@ -1471,7 +1475,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
             for (int k = 0; k < 16; ++k) top = fmaxf(top, fmaxf(x[k].x, x[k].y));
             top *= ca;
             cp_wait<1>();  // tile i + 1 (visible to all behind the barrier)
-            if (__syncthreads_or(top + neg_r > limit || vt >= loud)) {  // seldom
+            if (__syncthreads_or(top + neg_r > limit || vt >= loud || (i > 0 && i % C::kCentre == 0))) {  // seldom
                 if (mask) {  // the scales of the tokens that the row sees
                     vt = 0.0f;
 #pragma unroll
@@ -1483,21 +1487,27 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 }
                 ex[0][tq][row] = top;
                 ex[1][tq][row] = vt;
+                ex[2][tq][row] = z2.x + z2.y;
                 __syncthreads();
                 top = fmaxf(ex[0][0][row], ex[0][1][row]);
                 vt = fmaxf(ex[1][0][row], ex[1][1][row]);
                 const float f = raise_reference(top, vt, neg_r, limit);
                 loud = loud_of(limit);
                 l2 = mul2(l2, make_float2(f, f));
-                z2 = mul2(z2, make_float2(f, f));
-                if (i > 0) {  // the output so far
+                z2 = make_float2(0.0f, 0.0f);
+                if (i > 0) {  // the output so far, and back to about zero
+                    float r = 0.0f;
 #pragma unroll 1
                     for (int h = 0; h < kDims / 16; ++h) {
                         uint32_t u[16];
                         tmem_ld16(tl + C::kColO + tq * kDims + h * 16, u);
                         tmem_wait_ld();
+                        if (h == 0) {
+                            r = f * middle3(__uint_as_float(u[0]), __uint_as_float(u[2]), __uint_as_float(u[4]));
+                            base = fmaf(base, f, fmaf(r, 16777216.0f, f * (ex[2][0][row] + ex[2][1][row])));
+                        }
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__uint_as_float(u[k]) * f);
+                        for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(fmaf(__uint_as_float(u[k]), f, k & 1 ? -16.0f * r : -r));
                         tmem_st16(tl + C::kColO + tq * kDims + h * 16, u);
                     }
                     tmem_wait_st();
@@ -1533,7 +1543,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
         ex[0][tq][row] = l2.x + l2.y;
         ex[1][tq][row] = z2.x + z2.y;
         __syncthreads();
-        const float l = ex[0][0][row] + ex[0][1][row], zs = ex[1][0][row] + ex[1][1][row];
+        const float l = ex[0][0][row] + ex[0][1][row], zs = base + (ex[1][0][row] + ex[1][1][row]);
         const bool whole = sg.t0 == 0 && sg.t1 == sg.nt;
         float* part = a.part + ((int64_t)blockIdx.x * 2 + (unit == run.begin ? 0 : 1)) * C::kPart;
         const float up = 16777216.0f, inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;

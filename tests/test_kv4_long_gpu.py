@@ -19,9 +19,10 @@ def attend64(q, k, v):
 
 
 class Long:
-    """One sequence of n tokens, random keys and values, that any number of table rows share."""
+    """One sequence of n tokens, random keys and values, that any number of table rows share.
+    values "skewed": of mean zero but mostly below it, as codes are then; "loud": a few dims are far above the others."""
 
-    def __init__(self, n, hk, d, device, page=64):
+    def __init__(self, n, hk, d, device, page=64, values="normal"):
         g = torch.Generator(device=device).manual_seed(n + d)
         W = -(-n // page)
         self.n, self.hk, self.d, self.device = n, hk, d, device
@@ -29,6 +30,13 @@ class Long:
         self.table = torch.arange(W, dtype=torch.int32, device=device)[None]
         self.lens = torch.tensor([n], dtype=torch.int32, device=device)
         k, v = (torch.randn(n, hk, d, generator=g, device=device) for _ in range(2))
+        if values == "skewed":
+            v = v.abs().square() - 1
+        elif values == "loud":
+            v[..., :d // 2:d // 8] += 40
+        self.quiet = torch.ones(d, dtype=torch.bool, device=device)
+        if values == "loud":
+            self.quiet[:d // 2:d // 8] = False
         pc.kv4_append(k, v, self.cache, self.table, self.lens)
         self.k, self.v = pc.kv4_gather(self.cache, d, self.table, self.lens, (n,), dtype=torch.float32)
 
@@ -42,12 +50,13 @@ class Long:
         from token to token, and meets a code: the error of a sum over the tokens is to the sum as that times
         the codes' root mean square, in the values' units v - z, is to the values'.  (Its own root mean square is
         at most 1 / sqrt 3 of this limit, and it is taken over thousands of dims.)  No length in it."""
-        code = self.v - self.v.amin(-1, keepdim=True)
-        return 2.0 ** -11 * float(code.square().mean().sqrt() / self.v.square().mean().sqrt())
+        code, v = (self.v - self.v.amin(-1, keepdim=True))[..., self.quiet], self.v[..., self.quiet]
+        return 2.0 ** -11 * float(code.square().mean().sqrt() / (v - v.mean((0, 1))).square().mean().sqrt())
 
     def check(self, q, y, rows):
         want = attend64(torch.stack([q[b, l] for b, l in rows]), self.k, self.v)
-        got = torch.stack([y[b, l] for b, l in rows]).double()
+        want = want[..., self.quiet]
+        got = torch.stack([y[b, l] for b, l in rows]).double()[..., self.quiet]
         err = float((got - want).norm() / want.norm())
         assert err <= self.limit(), (err, self.limit())
         assert nat.device_status() == 0
@@ -85,3 +94,14 @@ def test_a_million_tokens(cuda_device):
     q = s.queries(600, 1, 4)
     y = pc.kv4_attention(q, s.cache, s.table.expand(600, -1).contiguous(), s.lens.expand(600).contiguous())
     s.check(q, y, [(0, 0), (300, 0), (599, 0)])
+
+
+@pytest.mark.parametrize("values", ["skewed", "loud"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("B,L,H", SHAPES)
+def test_values_to_one_side(cuda_device, B, L, H, d, values):
+    """Codes whose mean is not the middle one; of the loud dims' neighbours, whose results are small beside theirs."""
+    s = Long(131072, 8, d, cuda_device, values=values)
+    q = s.queries(B, L, H)
+    y = pc.kv4_attention(q, s.cache, s.table.expand(B, -1).contiguous(), s.lens.expand(B).contiguous())
+    s.check(q, y, [(0, L - 1), (B // 2, L - 1), (B - 1, L - 1)])
