@@ -24,12 +24,11 @@
 // every kCentre steps what they have reached (the middle one of three dims, so that
 // a loud dim does not lead the others away) is taken out of a row's sums and joins,
 // with the z term of these steps, a base that stays small, as its two parts cancel
-// in one fma.  In tensor memory that is dear, and done seldom; the tcgen05 kernel, which
-// rewrites each code anyway, also takes a middle code out of it: 7 of even tokens, 8
-// of odd ones (7.5 is no multiple of the subnormals' unit), with z_v + 7 s_v or
-// z_v + 8 s_v in the z term.  Over any length to 131072 tokens the error is now that of
-// the rounded weights alone, 2e-4 of the result's norm in the tcgen05 kernel (7e-4
-// where the mean code is far from 7.5) and 5e-4 to 8e-4 in the others.
+// in one fma.  Over any length to 131072 tokens the error is now that of the rounded
+// weights alone, 5e-4 to 8e-4 of the result's norm in every kernel.  (With the middle
+// code, 7.5, taken out of each value instead, which the tcgen05 kernel could do as
+// it spreads them, that is 3e-4, but dims of low codes are less exact than now, and
+// values to one side drift as before.)
 //
 // Shape of the decode kernel.  Keys are the 16-row operand of m16n8k16 (16
 // tokens), the query rows of one kv head (group x new tokens) its 8 columns,
@@ -94,9 +93,6 @@ struct Kv4AttnArgs {
     int n_grp;
 };
 
-// Minus the middle codes of an even token (7) and of the odd one beside it (8), as a pair of masked
-// codes, and 2^4 of them.
-constexpr uint32_t kMiddle = 0x80088007u, kMiddle16 = 0x80808070u;
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 
@@ -127,10 +123,6 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-__device__ __forceinline__ uint32_t add_f16(uint32_t a, uint32_t b) {
-    const __half2 h = __hadd2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float middle3(float a, float b, float c) { return fmaxf(fminf(a, b), fminf(fmaxf(a, b), c)); }
@@ -1138,7 +1130,7 @@ template <int D, bool M>
 struct TcCfg {
     static constexpr bool kMore = M;
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
-    static constexpr int kCentre = 16;  // tiles between two centrings, at most (16 x 512 rows: 119.2 us, 119.0 with none)
+    static constexpr int kCentre = 8;  // tiles between two centrings, at most (16 x 512 rows: 119.6 us, 117.0 with none, 121.5 with 4)
     static constexpr int kStages = 3;
     static constexpr int kRawK = kTokens * (D / 2);      // codes of a tile's keys (or values)
     static constexpr int kRaw = 2 * kRawK + 8 * kTokens; // and the pairs: the keys', then the values'
@@ -1349,8 +1341,7 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
                 const bool none = dead[stage][tok >> 4] || tok_base + i * C::kTokens + tok >= sg.kv_end;
                 to[0] = none ? 0.0f : pair_lo(p);  // whatever lies behind the sequence
                 // (a dead piece's tokens are told by a zero of +inf: their logits are dropped)
-                const float zero = kv ? fmaf(7 + (tok & 1), pair_lo(p), pair_hi(p)) : pair_hi(p);  // of centred value codes
-                to[C::kTokens] = !none ? zero : !kv && dead[stage][tok >> 4] ? INFINITY : 0.0f;
+                to[C::kTokens] = !none ? pair_hi(p) : !kv && dead[stage][tok >> 4] ? INFINITY : 0.0f;
                 if (kv) {
                     const float top = none ? 0.0f : fmaxf(pair_lo(p), 0.0f);  // (a NaN does not count)
                     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
@@ -1369,11 +1360,10 @@ __global__ void __launch_bounds__(256, 2) kv4_long_kernel(const Kv4AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int n = (k + (j >> 1)) & 3;  // the dims in turn, so that eight lanes meet different banks
-                    const uint32_t sh = (n & 2) * 4, mask = n & 1 ? 0x00F000F0u : 0x000F000Fu, mid = n & 1 ? kMiddle16 : kMiddle;
+                    const uint32_t sh = (n & 2) * 4, mask = n & 1 ? 0x00F000F0u : 0x000F000Fu;
                     const int r = 4 * j + n;
                     *reinterpret_cast<uint4*>(vop + r * 128 + ((q ^ (r & 7)) * 16)) =
-                        make_uint4(add_f16(w[0] >> sh & mask, mid), add_f16(w[1] >> sh & mask, mid),
-                                   add_f16(w[2] >> sh & mask, mid), add_f16(w[3] >> sh & mask, mid));
+                        make_uint4(w[0] >> sh & mask, w[1] >> sh & mask, w[2] >> sh & mask, w[3] >> sh & mask);
                 }
             }
         };
