@@ -45,9 +45,21 @@ struct Kv4Seq {
     const int32_t* grp;  // (B + 1)
 };
 
+// An entry of a table or a length.  kMore: they may be what the kernel before wrote, and this one may have
+// begun while it did (a dependent launch): memory that changes under a grid is not for __ldg, whose loads
+// need not stay behind the grid's wait.
+template <bool kMore>
+__device__ __forceinline__ int kv4_load(const int32_t* p) {
+    if constexpr (kMore)
+        return *p;
+    else
+        return __ldg(p);
+}
 // The length of sequence b, and how much of it its table has room for.
-__device__ __forceinline__ int kv4_len(const Kv4Seq& s, int64_t b) { return min(max(__ldg(s.lens + b), 0), 1 << 30); }
-__device__ __forceinline__ int kv4_held(const Kv4Seq& s, int64_t b) { return min(kv4_len(s, b), s.table_w * s.page); }
+template <bool kMore = false>
+__device__ __forceinline__ int kv4_len(const Kv4Seq& s, int64_t b) { return min(max(kv4_load<kMore>(s.lens + b), 0), 1 << 30); }
+template <bool kMore = false>
+__device__ __forceinline__ int kv4_held(const Kv4Seq& s, int64_t b) { return min(kv4_len<kMore>(s, b), s.table_w * s.page); }
 
 // First row and number of rows of sequence b (kMore: which may be a prefix).
 template <bool kMore = false>

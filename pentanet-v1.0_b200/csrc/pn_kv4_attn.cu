@@ -161,8 +161,8 @@ template <typename C>
 __device__ __forceinline__ uint32_t attn_units(const Kv4AttnArgs& a, int64_t b, uint32_t& nt) {
     int64_t first, n;
     kv4_rows<C::kMore>(a.s, b, first, n);
-    if (C::kMore && a.s.table_hd && __ldg(a.s.lens + b) < 0) n = 0;  // (of chosen pages: a row that is no sequence's)
-    nt = max((kv4_held(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
+    if (C::kMore && a.s.table_hd && kv4_load<true>(a.s.lens + b) < 0) n = 0;  // (of chosen pages: a row that is no sequence's)
+    nt = max((kv4_held<C::kMore>(a.s, b) + C::kTokens - 1) / C::kTokens, 1);
     return ((uint32_t)n * a.G + C::kRows - 1) / C::kRows * nt * a.s.Hk;
 }
 
@@ -262,9 +262,9 @@ struct AttnSeg {
         t0 = in_seq - tile * nt;
         t1 = min(nt, t0 + left);
         const bool all = C::kMore && a.s.grouped;
-        pos0 = kv4_len(a.s, b) - (int)n_rows;
-        kv_end = all ? kv4_held(a.s, b) : min(max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0), kv4_held(a.s, b));
-        if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && pos0 + (int)n_rows > kv4_held(a.s, b)) record_status(PN_ERR_ARG);
+        pos0 = kv4_len<C::kMore>(a.s, b) - (int)n_rows;
+        kv_end = all ? kv4_held<C::kMore>(a.s, b) : min(max(pos0 + (int)(((uint32_t)r0 + rows - 1) / a.G) + 1, 0), kv4_held<C::kMore>(a.s, b));
+        if (t0 == 0 && threadIdx.x == 0 && a.s.table_w > 0 && pos0 + (int)n_rows > kv4_held<C::kMore>(a.s, b)) record_status(PN_ERR_ARG);
         lim_min = all ? kv_end - 1 : min(pos0 + (int)((uint32_t)r0 / a.G), kv_end - 1);
     }
     // Where query row r of the tile (r < rows) lies in q, in elements.
@@ -315,7 +315,7 @@ struct AttnPages {
         off = 0;
         if (!want) return;
         const uint32_t i = (uint32_t)tok / (uint32_t)a.s.page;
-        const int p = __ldg(a.s.table + b * a.s.table_ld + (C::kMore ? head * a.s.table_hd : 0) + i);
+        const int p = kv4_load<C::kMore>(a.s.table + b * a.s.table_ld + (C::kMore ? head * a.s.table_hd : 0) + i);
         off = tok - (int)i * a.s.page;
         if (p >= 0 && p < a.s.n_pages)
             addr = (uint64_t)(a.cache + ((int64_t)p * a.s.Hk + head) * 2 * block);
