@@ -42,3 +42,66 @@ def test_sparse_calls_one_behind_the_other(cuda_device, B, rows, hk, G):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for x, y in zip(held, want) for a, b in zip(x, y))
     assert nat.device_status() == 0
+
+
+def sparse_rows(s, q, cu, G, top, some, first=1, last=1):
+    """One call over all rows; the rows `some`, (row, sequence, position), against the definition."""
+    means = pc.kv4_means(s.cache, s.d)
+    pc.kv4_page_means(s.cache, means, s.table, s.lens, (sum(s.lengths),), cu_q=cu_of(s.lengths, s.device))
+    out = torch.full_like(q, 7.0)
+    y, pages = pc.kv4_sparse_attention(q, s.cache, means, s.table, s.lens, top, first_pages=first, last_pages=last, cu_q=cu,
+                                       out=out, return_pages=True)
+    end = int(cu[-1])
+    assert (y[end:] == 7).all() and (pages[end:] == -1).all()
+    for row, i, pos in some:
+        if pos < 0:
+            assert not y[row].any() and (pages[row] == -1).all()
+            continue
+        want = more.choose(q[row].cpu(), more.means(s.k[i], s.page), pos, s.page, top, first, last)
+        for h, chosen in enumerate(want):
+            assert pages[row, h].tolist() == chosen + [-1] * (top + first + last - len(chosen)), (row, h)
+            tok = torch.cat([torch.arange(p * s.page, min((p + 1) * s.page, pos + 1)) for p in chosen])
+            part = slice(h * G, (h + 1) * G)
+            ref, bound = oracle.attention(q[row][None, part].cpu(), s.k[i][tok][:, h:h + 1], s.v[i][tok][:, h:h + 1], None)
+            bound = bound + 2.0 ** -8 * (ref.abs() + bound)
+            err = (y[row, part].double().cpu() - ref[0]).abs()
+            assert (err <= bound[0] + 1e-30).all(), (row, h, err.max())
+    assert nat.device_status() == 0
+
+
+# per sequence and kv head, G rows to a tile; tiles of 16 rows above four times the SMs take the kernel for 64 rows, and
+# more than 64 of them per head and eight times the SMs the one for 128: 300 x 2 x 2 and x 3 tiles, 600 x 2 x 5
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("G,n_rows", [(20, 300), (40, 300), (70, 600)])
+def test_sparse_wide_groups_and_many_rows(cuda_device, d, G, n_rows):
+    """Tables per kv head in the kernels for many rows, rows before the sequence's start, rows of no sequence."""
+    hk, page = 2, 16
+    s = Batch([700, 5, 333], hk, d, page, cuda_device, seed=G + d)
+    rows = [n_rows - 150, 9, 141]
+    q = torch.randn(n_rows + 25, G * hk, d, generator=torch.Generator().manual_seed(G)).to(torch.bfloat16).to(cuda_device)
+    at = [0, rows[0], rows[0] + 9]
+    some = [(at[i] + r, i, s.lengths[i] - rows[i] + r) for i, some in
+            enumerate(([0, 1, 77, rows[0] - 1], [0, 3, 4, 8], [0, 64, 140])) for r in some]
+    sparse_rows(s, q, cu_of(rows, cuda_device), G, 4, some)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prefix_own_rows_on_the_chunk_kernel(cuda_device, d):
+    """40 sequences x 12 rows of 4 query heads each: their own tokens in the kernel for 64 rows, causal, ragged
+    lengths, some rows before their sequence's start and some sequences without a prefix."""
+    B, G, hk = 42, 4, 8
+    own = [(53 * i) % 120 + 1 for i in range(B)]
+    rows = [12 if i % 5 else 17 for i in range(B)]
+    assert any(n < r for n, r in zip(own, rows))
+    s = Shared(own, [200, 33, 0], [25, 10, 5], hk, d, 16, cuda_device, seed=d)
+    q = torch.randn(sum(rows), G * hk, d, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    y = s.call(q.to(cuda_device), rows)
+    some = [0, 1, 7, 24, 25, 34, 35, 39, 40, 41] + [i for i in range(B) if own[i] < rows[i]][:3]
+    part, x = y.split(rows), q.split(rows)
+    whole = s.own, s.of, s.b.k, s.b.v
+    for i in some:  # (all of them would take minutes)
+        s.own, s.of = [whole[0][i]], [whole[1][i]]
+        s.b.k, s.b.v = ([t[i]] + t[B:] for t in whole[2:])
+        s.check([part[i]], [x[i]])
+        s.own, s.of, s.b.k, s.b.v = whole
+    assert nat.device_status() == 0
