@@ -30,7 +30,9 @@ constexpr int kMeansRows = 64;  // per block, at most
 
 // A block looks at a few rows: one that is its sequence's last, or whose successor starts a
 // page, stands for its page.  The block's warps share the tokens of each such page, lane
-// (token parity, word of eight dims), in fp64 (a code times its scale is exact in fp32).
+// (token parity, word of eight dims), in fp64.  A code times its scale is exact in fp32, where a sixteenth of
+// the largest scales keeps it below the largest number.  (Products in fp64, whose conversions from integers are
+// slow: a page of 256 tokens 11.7 us, 7.7 so.)
 template <int D>
 __global__ void __launch_bounds__(kMeansThreads) kv4_means_kernel(const Kv4MeansArgs a) {
     constexpr int WORDS = D / 8, TP = 32 / WORDS, WARPS = kMeansThreads / 32;  // words of a key, tokens per warp and step
@@ -74,8 +76,11 @@ __global__ void __launch_bounds__(kMeansThreads) kv4_means_kernel(const Kv4Means
             const uint32_t c = *reinterpret_cast<const uint32_t*>(p + t * (D / 2) + word * 4);
             const uint32_t pair = *reinterpret_cast<const uint32_t*>(p + a.s.page * (D / 2) + t * 4);
             const float s = __uint_as_float(pair << 16), z = __uint_as_float(pair & 0xFFFF0000u);
+            const bool large = s >= 0x1p123f;
+            const float less = large ? s * 0.0625f : s;
+            const double up = large ? 16.0 : 1.0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[j] += (double)(s * (float)(c >> (4 * j) & 15));
+            for (int j = 0; j < 8; ++j) acc[j] = fma((double)(less * (float)(c >> (4 * j) & 15)), up, acc[j]);
             zeros += (double)z;
         }
         __syncthreads();  // the sums of the page before are read

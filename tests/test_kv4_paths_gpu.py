@@ -105,3 +105,21 @@ def test_prefix_own_rows_on_the_chunk_kernel(cuda_device, d):
         s.check([part[i]], [x[i]])
         s.own, s.of, s.b.k, s.b.v = whole
     assert nat.device_status() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_page_means_of_the_largest_keys(cuda_device, d):
+    """Keys whose range is nearly fp32's: fifteen times the scale, which is rounded up, is no fp32 number, the keys
+    read back and their mean are."""
+    page, n = 16, 37
+    low, top = -2.0 ** 127, 2.0 ** 127 * (1 - 2.0 ** -8)  # (apart by less than the largest fp32 number)
+    s = Batch([n], 2, d, page, cuda_device, seed=d)
+    for i in range(n):
+        s.k[0][i, :, i % d], s.k[0][i, :, (i + 7) % d] = low, top
+    s.store([n])
+    k, _ = pc.kv4_gather(s.cache, d, s.table, s.lens, (n,), dtype=torch.float32)
+    assert k.isfinite().all()
+    assert (oracle.quantise(s.k[0])[1] * 15).isinf().all()
+    means = pc.kv4_means(s.cache, d)
+    pc.kv4_page_means(s.cache, means, s.table, s.lens, (n,))
+    assert torch.equal(means[s.table[0].long()].cpu(), more.means(s.k[0], page))
