@@ -20,7 +20,8 @@ def attend64(q, k, v):
 
 class Long:
     """One sequence of n tokens, random keys and values, that any number of table rows share.
-    values "skewed": of mean zero but mostly below it, as codes are then; "loud": a few dims are far above the others."""
+    values "skewed": of mean zero but mostly below it, as codes are then; "loud": a few dims are far above the others;
+    "largest", "least": near the ends of the range that kv4_attention states."""
 
     def __init__(self, n, hk, d, device, page=64, values="normal"):
         g = torch.Generator(device=device).manual_seed(n + d)
@@ -34,6 +35,8 @@ class Long:
             v = v.abs().square() - 1
         elif values == "loud":
             v[..., :d // 2:d // 8] += 40
+        elif values in ("largest", "least"):
+            v = v * 2.0 ** (104 if values == "largest" else -48)
         self.quiet = torch.ones(d, dtype=torch.bool, device=device)
         if values == "loud":
             self.quiet[:d // 2:d // 8] = False
@@ -105,3 +108,15 @@ def test_values_to_one_side(cuda_device, B, L, H, d, values):
     q = s.queries(B, L, H)
     y = pc.kv4_attention(q, s.cache, s.table.expand(B, -1).contiguous(), s.lens.expand(B).contiguous())
     s.check(q, y, [(0, L - 1), (B // 2, L - 1), (B - 1, L - 1)])
+
+
+@pytest.mark.parametrize("values", ["largest", "least"])
+@pytest.mark.parametrize("B,L,H", SHAPES)
+def test_values_of_any_size(cuda_device, B, L, H, values):
+    """No sum on the way leaves fp32's range where the values are in theirs."""
+    s = Long(3000, 8, 64, cuda_device, values=values)
+    q = s.queries(B, L, H)
+    y = pc.kv4_attention(q, s.cache, s.table.expand(B, -1).contiguous(), s.lens.expand(B).contiguous())
+    up = 2.0 ** (-104 if values == "largest" else 48)
+    s.v = s.v * up  # (the check squares)
+    s.check(q, y * up, [(0, L - 1), (B // 2, L - 1), (B - 1, L - 1)])
