@@ -109,14 +109,16 @@ __device__ __forceinline__ uint64_t score_key(double v) {
 struct Kv4SelectArgs {
     Kv4Seq s;
     const void* q;
-    int q_f32, q_vec;
+    int q_f32;
     int64_t q_sb, q_sl, q_sh;
     int G;
     const __nv_bfloat16* means;
     int first, last, top;
-    int width;            // first + last + top: pages of a row's table
-    uint64_t* keys;       // workspace (T, Hk, table_w): scores
-    int32_t* pages;       // workspace (T, Hk, width): the chosen pages, as entries of the block table
+    int width;            // first + last + top
+    int list;             // pages of a row's table: as many, or all that the block table has
+    int64_t row0, row1;   // the rows of this launch
+    uint64_t* keys;       // workspace (row1 - row0, Hk, table_w): scores
+    int32_t* pages;       // workspace (T, Hk, list): the chosen pages, as entries of the block table
     int32_t* lens;        // workspace (T): tokens of them; -1: no row
     int32_t* chosen;      // (T, Hk, width): their numbers in the sequence, or null
     int tile;             // rows of a block of the score kernel
@@ -133,7 +135,7 @@ struct SelectRow {
     bool over;                // the table has no room for all of them
     __device__ __forceinline__ SelectRow(const Kv4SelectArgs& a, int64_t row)
         : b(0), i(0), seen(0), free_end(0), len(-1), over(false) {
-        if (row >= a.s.T || !kv4_find(a.s, row, b, i)) return;
+        if (row >= a.row1 || !kv4_find(a.s, row, b, i)) return;
         int64_t at, n;
         kv4_rows(a.s, b, at, n);
         const int64_t pos = (int64_t)kv4_len(a.s, b) - n + i;
@@ -153,17 +155,17 @@ template <int D>
 __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4SelectArgs a) {
     constexpr int E = D / 4;  // dims per lane: chunks of 8, four lanes in turn
     __shared__ double q[kScoreTile][D];
-    __shared__ int seq[kScoreTile], from[kScoreTile], to[kScoreTile];
+    __shared__ int seq[kScoreTile], to[kScoreTile];
     __shared__ int64_t base[kScoreTile];
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row0 = (int64_t)blockIdx.x * a.tile;
+    const int64_t row0 = a.row0 + (int64_t)blockIdx.x * a.tile;
     const int head = blockIdx.y;
     if (tid < a.tile) {
         const SelectRow at(a, row0 + tid);
         seq[tid] = max(at.free_end - a.first, 0) > a.top ? (int)at.b : -1;  // (with fewer pages all are taken)
-        from[tid] = a.first, to[tid] = at.free_end;
+        to[tid] = at.free_end;
         base[tid] = a.s.cu ? (row0 + tid) * a.q_sl : at.b * a.q_sb + at.i * a.q_sl;
     }
     __syncthreads();
@@ -186,11 +188,11 @@ __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4Selec
             ++r0;
             continue;
         }
-        int r1 = r0 + 1, lo = from[r0], hi = to[r0];
+        int r1 = r0 + 1, hi = to[r0];
         for (; r1 < a.tile && seq[r1] == seq[r0]; ++r1) hi = max(hi, to[r1]);
         const int64_t b = seq[r0];
-        // the pages [lo, hi) in runs of 32 to a block
-        for (int run = lo + blockIdx.z * 32; run < hi; run += a.splits * 32) {
+        // the pages [first, hi) in runs of 32 to a block
+        for (int run = a.first + blockIdx.z * 32; run < hi; run += a.splits * 32) {
             const int i = run + sub;
             const int p = i < hi ? __ldg(a.s.table + b * a.s.table_ld + i) : -1;
             const bool there = p >= 0 && p < a.s.n_pages;
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4Selec
                 return sum + sum2;
             };
             auto put = [&](int r, double sum) {
-                if (i < to[r]) a.keys[((row0 + r) * a.s.Hk + head) * a.s.table_w + i] = there ? score_key(sum) : 0;
+                if (i < to[r]) a.keys[((row0 - a.row0 + r) * a.s.Hk + head) * a.s.table_w + i] = there ? score_key(sum) : 0;
             };
             if (r1 - r0 == 1) {
                 double sum = part_of(r0);
@@ -296,35 +298,33 @@ __device__ __forceinline__ void select_border(const int* bins, int need, int* wa
 // A row's list in one kv head, and what of it does not depend on the scores.
 struct SelectList {
     SelectRow at;
-    int64_t row, list;
+    int64_t row, unit;
     int head, n;   // n: pages that may be chosen
     bool choose;   // not all of them are
     const uint64_t* keys;
     const int32_t* table;
-    __device__ __forceinline__ SelectList(const Kv4SelectArgs& a, int64_t unit)
-        : at(a, unit / a.s.Hk), row(unit / a.s.Hk), list(unit * a.width), head((int)(unit - row * a.s.Hk)) {}
+    __device__ __forceinline__ SelectList(const Kv4SelectArgs& a, int64_t u)  // u: of this launch's rows
+        : at(a, a.row0 + u / a.s.Hk), row(a.row0 + u / a.s.Hk), unit(a.row0 * a.s.Hk + u), head((int)(unit - row * a.s.Hk)) {}
     // falls: so do row starts, and nothing is computed
     __device__ __forceinline__ void settle(const Kv4SelectArgs& a, bool falls, bool speaks) {
         if (falls) at.len = -1, at.seen = at.free_end = 0, at.over = true;
         if (at.over && head == 0 && speaks) record_status(PN_ERR_ARG);
         n = max(at.free_end - a.first, 0);
         choose = n > a.top;
-        keys = a.keys + (row * a.s.Hk + head) * a.s.table_w + a.first;
+        keys = a.keys + (unit - a.row0 * a.s.Hk) * a.s.table_w + a.first;
         table = a.s.table + at.b * a.s.table_ld;
     }
     __device__ __forceinline__ void put(const Kv4SelectArgs& a, int slot, int i) const {
-        a.pages[list + slot] = i < a.s.table_w ? __ldg(table + i) : -1;
-        if (a.chosen) a.chosen[list + slot] = i;
+        a.pages[unit * a.list + slot] = i < a.s.table_w ? __ldg(table + i) : -1;
+        if (a.chosen) a.chosen[unit * a.width + slot] = i;
     }
     // The first and the last pages (or all), the rest of the list, and the row's length; by thread `me` of `of`.
     __device__ __forceinline__ void frame(const Kv4SelectArgs& a, int me, int of) const {
         const int taken = choose ? a.first + a.top : at.seen, last = choose ? at.free_end : at.seen, kept = taken + at.seen - last;
         for (int i = me; i < (choose ? a.first : taken); i += of) put(a, i, i);
         for (int i = me; i < at.seen - last; i += of) put(a, taken + i, last + i);
-        for (int i = kept + me; i < a.width; i += of) {
-            a.pages[list + i] = -1;
-            if (a.chosen) a.chosen[list + i] = -1;
-        }
+        for (int i = kept + me; i < a.list; i += of) a.pages[unit * a.list + i] = -1;
+        for (int i = kept + me; i < a.width && a.chosen; i += of) a.chosen[unit * a.width + i] = -1;
         if (head == 0 && me == 0)  // all pages but the last are whole
             a.lens[row] = at.len <= 0 ? at.len : (kept - 1) * a.s.page + at.len - (at.seen - 1) * a.s.page;
     }
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(kWarpSelects * 32) kv4_select_warp_kernel(cons
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * kWarpSelects + (threadIdx.x >> 5);
-    if (unit >= a.s.T * a.s.Hk) return;
+    if (unit >= (a.row1 - a.row0) * a.s.Hk) return;
     SelectList to(a, unit);
     bool falls = false;
     if (a.s.cu)
@@ -567,17 +567,24 @@ __global__ void __launch_bounds__(kWarpSelects * 32) kv4_select_warp_kernel(cons
     }
 }
 
+// The scores' share of the workspace: calls that need more take their rows in turn.
+constexpr size_t kKeyBytes = (size_t)256 << 20;
+
 struct SparseLayout {  // of the workspace
-    size_t keys, pages, lens, total;
-    SparseLayout(int64_t T, int64_t Hk, int64_t G, int64_t D, int64_t table_w, int64_t width) {
+    bool scored;   // else every page is taken, of any row
+    int list;      // pages of a row's table
+    int64_t rows;  // whose scores are held at once
+    size_t keys, pages, lens, attn, total;
+    SparseLayout(int64_t T, int64_t Hk, int64_t G, int64_t D, int64_t table_w, int64_t width)
+        : scored(table_w > width), list((int)std::max<int64_t>(std::min(table_w, width), 1)), rows(T) {
         keys = 0;
-        pages = keys + round256((size_t)T * Hk * table_w * 8);
-        lens = pages + round256((size_t)T * Hk * width * 4);
-        total = lens + round256((size_t)T * 4);
-        attn = total;
-        total += attn_workspace(T, T, Hk, G, D);
+        const size_t row = (size_t)Hk * table_w * 8;
+        if (scored && T * row > kKeyBytes) rows = std::max<int64_t>(kKeyBytes / row / kScoreTile * kScoreTile, 1);
+        pages = keys + (scored ? round256(std::min(rows, T) * row) : 0);
+        lens = pages + round256((size_t)T * Hk * list * 4);
+        attn = lens + round256((size_t)T * 4);
+        total = attn + attn_workspace(T, T, Hk, G, D);
     }
-    size_t attn;
 };
 
 template <typename... Args>
@@ -649,11 +656,11 @@ int pn_kv4_sparse_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q
     if (!aligned(means, 16)) return fail(PN_ERR_ALIGN, "%s: means needs 16-byte alignment", name);
     if (!aligned(chosen, 4)) return fail(PN_ERR_ALIGN, "%s: misaligned pointer", name);
     if (kv_heads > 65535 || (double)T * kv_heads > 2e9) return fail(PN_ERR_SHAPE, "%s: %lld rows of %lld kv heads", name, (long long)T, (long long)kv_heads);
-    if ((double)T * kv_heads * ((double)table_w + width) * 8 > 6e10)
+    if ((double)T * kv_heads * std::min(width, table_w) * 4 > 3e10 || (double)kv_heads * table_w * 8 > 3e10)
         return fail(PN_ERR_SHAPE, "%s: %lld rows over tables of %lld pages are too much for one call", name, (long long)T, (long long)table_w);
-    pn::Kv4Seq rows = a.s;  // (every row a sequence of its own)
-    rows.B = T;
-    if (int st = check_attn_units(name, rows, a.G, std::min(width, table_w) * page)) return st;
+    pn::Kv4Seq each = a.s;  // (every row a sequence of its own)
+    each.B = T;
+    if (int st = check_attn_units(name, each, a.G, std::min(width, table_w) * page)) return st;
     if (int st = check_device()) return st;
     if (T == 0 || B == 0) return ok();
     const pn::SparseLayout lay(T, kv_heads, a.G, head_dim, a.s.table_w, width);
@@ -662,40 +669,44 @@ int pn_kv4_sparse_attention(const void* q, int64_t q_sb, int64_t q_sl, int64_t q
     char* ws = static_cast<char*>(workspace);
     pn::Kv4SelectArgs c{};
     c.s = a.s;
-    c.q = q, c.q_f32 = a.q_f32, c.q_vec = a.q_vec, c.q_sb = q_sb, c.q_sl = q_sl, c.q_sh = q_sh, c.G = a.G;
+    c.q = q, c.q_f32 = a.q_f32, c.q_sb = q_sb, c.q_sl = q_sl, c.q_sh = q_sh, c.G = a.G;
     c.means = static_cast<const __nv_bfloat16*>(means);
-    c.first = (int)first_pages, c.last = (int)last_pages, c.top = (int)top_pages, c.width = (int)width;
+    c.first = (int)first_pages, c.last = (int)last_pages, c.top = (int)top_pages, c.width = (int)width, c.list = lay.list;
     c.keys = reinterpret_cast<uint64_t*>(ws + lay.keys);
     c.pages = reinterpret_cast<int32_t*>(ws + lay.pages);
     c.lens = reinterpret_cast<int32_t*>(ws + lay.lens);
     c.chosen = chosen;
     const cudaStream_t s = (cudaStream_t)stream;
     cudaError_t err = cudaSuccess;
-    if (top_pages > 0 && a.s.table_w > width) {  // (else every page is taken)
-        c.tile = 1;
-        while (c.tile < pn::kScoreTile && 2 * c.tile <= T / B) c.tile *= 2;
-        const int64_t tiles = (T + c.tile - 1) / c.tile, runs = (a.s.table_w + 31) / 32;
-        c.splits = (int)std::min<int64_t>(std::max<int64_t>(8 * pn::sm_count() / (tiles * kv_heads), 1), std::min<int64_t>(runs, 65535));
-        const dim3 grid((unsigned)tiles, (unsigned)kv_heads, (unsigned)c.splits);
-        err = head_dim == 64 ? pn::launch_dependent(pn::kv4_score_kernel<64>, grid, pn::kScoreThreads, s, c)
-                             : pn::launch_dependent(pn::kv4_score_kernel<128>, grid, pn::kScoreThreads, s, c);
+    const bool scored = lay.scored && top_pages > 0;
+    c.tile = 1;
+    while (c.tile < pn::kScoreTile && 2 * c.tile <= T / B) c.tile *= 2;
+    for (c.row0 = 0; c.row0 < T; c.row0 = c.row1) {
+        c.row1 = scored ? std::min(c.row0 + lay.rows, T) : T;
+        const int64_t rows = c.row1 - c.row0, units = rows * kv_heads;
+        if (scored) {
+            const int64_t tiles = (rows + c.tile - 1) / c.tile, runs = (a.s.table_w + 31) / 32;
+            c.splits = (int)std::min<int64_t>(std::max<int64_t>(8 * pn::sm_count() / (tiles * kv_heads), 1), std::min<int64_t>(runs, 65535));
+            const dim3 grid((unsigned)tiles, (unsigned)kv_heads, (unsigned)c.splits);
+            err = head_dim == 64 ? pn::launch_dependent(pn::kv4_score_kernel<64>, grid, pn::kScoreThreads, s, c)
+                                 : pn::launch_dependent(pn::kv4_score_kernel<128>, grid, pn::kScoreThreads, s, c);
+            if (err != cudaSuccess) return cuda_fail(err, name);
+        }
+        const dim3 blocks((unsigned)units);
+        // (for few rows the passes of each are what takes the time)
+        if (a.s.table_w > pn::kSmallPages)
+            err = units <= pn::sm_count() ? pn::launch_dependent(pn::kv4_select_kernel<1024, 8>, blocks, 1024, s, c)
+                                          : pn::launch_dependent(pn::kv4_select_kernel<256, 8>, blocks, 256, s, c);
+        else if (units <= 8 * pn::sm_count())
+            err = pn::launch_dependent(pn::kv4_select_kernel<256, 2>, blocks, 256, s, c);
+        else
+            err = pn::launch_dependent(pn::kv4_select_warp_kernel, dim3((unsigned)((units + pn::kWarpSelects - 1) / pn::kWarpSelects)),
+                                       pn::kWarpSelects * 32, s, c);
         if (err != cudaSuccess) return cuda_fail(err, name);
     }
-    const int64_t units = T * kv_heads;
-    const dim3 blocks((unsigned)units);
-    // (for few rows the passes of each are what takes the time)
-    if (a.s.table_w > pn::kSmallPages)
-        err = units <= pn::sm_count() ? pn::launch_dependent(pn::kv4_select_kernel<1024, 8>, blocks, 1024, s, c)
-                                      : pn::launch_dependent(pn::kv4_select_kernel<256, 8>, blocks, 256, s, c);
-    else if (units <= 8 * pn::sm_count())
-        err = pn::launch_dependent(pn::kv4_select_kernel<256, 2>, blocks, 256, s, c);
-    else
-        err = pn::launch_dependent(pn::kv4_select_warp_kernel, dim3((unsigned)((units + pn::kWarpSelects - 1) / pn::kWarpSelects)),
-                                   pn::kWarpSelects * 32, s, c);
-    if (err != cudaSuccess) return cuda_fail(err, name);
     // every row a sequence of its own
     a.q_l = cu_q ? T : a.s.L;  // (with cu_q rows lie one after another)
-    a.s.table = c.pages, a.s.table_hd = width, a.s.table_ld = kv_heads * width, a.s.table_w = n_pages > 0 ? (int)width : 0;
+    a.s.table = c.pages, a.s.table_hd = lay.list, a.s.table_ld = kv_heads * lay.list, a.s.table_w = n_pages > 0 ? lay.list : 0;
     a.s.lens = c.lens, a.s.cu = nullptr, a.s.B = T, a.s.L = 1;
     err = pn::attn_pass<true>(a, pn::attn_kind(T, T, kv_heads, a.G), head_dim, ws + lay.attn, s);
     return err == cudaSuccess ? ok() : cuda_fail(err, name);

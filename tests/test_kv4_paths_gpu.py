@@ -123,3 +123,49 @@ def test_page_means_of_the_largest_keys(cuda_device, d):
     means = pc.kv4_means(s.cache, d)
     pc.kv4_page_means(s.cache, means, s.table, s.lens, (n,))
     assert torch.equal(means[s.table[0].long()].cpu(), more.means(s.k[0], page))
+
+
+def test_sparse_workspace(cuda_device):
+    """What a call holds for its scores has a limit, is nothing where none are made, and a list holds no more pages
+    than there are, however many are asked for."""
+    size = lambda T, W, width: pc._sparse_workspace(T, 32, 8, 128, W, width, cuda_device.index or 0)
+    some = size(4096, 64, 64)  # no scores
+    assert size(4096, 64, 1 << 20) == some and some < size(4096, 65, 64)
+    assert size(4096, 8192, 64) - some < 300 << 20  # (2 GB of scores)
+    assert size(1, 64, 1 << 20) < 64 << 20
+    s = Batch([300, 170], 2, 64, 16, cuda_device, seed=2)
+    means = pc.kv4_means(s.cache, 64)
+    pc.kv4_page_means(s.cache, means, s.table, s.lens, (470,), cu_q=cu_of(s.lengths, cuda_device))
+    q = torch.randn(2, 8, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(cuda_device)
+    want = pc.kv4_sparse_attention(q, s.cache, means, s.table, s.lens, 19)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    assert torch.equal(pc.kv4_sparse_attention(q, s.cache, means, s.table, s.lens, 50_000_000), want)
+    assert torch.cuda.max_memory_allocated() - before < 64 << 20
+    assert nat.device_status() == 0
+
+
+@pytest.mark.parametrize("rows,hk,pages", [([2000, 1100], 4, 3000), ([1] * 70, 2, 300000)])
+def test_sparse_rows_in_turn(cuda_device, rows, hk, pages):
+    """Rows whose scores together are beyond the workspace's share of them: they are chosen for in turn."""
+    G, d, page = 1, 64, 16
+    assert sum(rows) * hk * pages * 8 > 256 << 20
+    B, held = len(rows), 200
+    s = Batch([held * page] * 2, hk, d, page, cuda_device, seed=hk)
+    table = torch.zeros(B, pages, dtype=torch.int32, device=cuda_device)  # wide tables, of which little is used
+    table[:, :held] = s.table[torch.arange(B) % 2]
+    lens = ints([held * page - (7 * i) % 50 for i in range(B)], cuda_device)
+    means = pc.kv4_means(s.cache, d)
+    pc.kv4_page_means(s.cache, means, s.table, s.lens, (2 * held * page,), cu_q=cu_of(s.lengths, cuda_device))
+    q = torch.randn(sum(rows), hk, d, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda_device)
+    cu = cu_of(rows, cuda_device)
+    y, chosen = pc.kv4_sparse_attention(q, s.cache, means, table, lens, 4, cu_q=cu, return_pages=True)
+    narrow = table[:, :held].contiguous()  # in one
+    z, again = pc.kv4_sparse_attention(q, s.cache, means, narrow, lens, 4, cu_q=cu, return_pages=True)
+    assert torch.equal(chosen, again) and torch.equal(y, z)
+    assert nat.device_status() == 0
+    mean = [more.means(k, page) for k in s.k]
+    for row in range(0, sum(rows), 97):
+        b = int((cu <= row).sum()) - 1
+        pos = int(lens[b]) - rows[b] + row - int(cu[b])
+        assert chosen[row].tolist() == [c + [-1] * (7 - len(c)) for c in more.choose(q[row].cpu(), mean[b % 2], pos, page, 4, 1, 2)]
