@@ -394,11 +394,15 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4Gather
         const bool kv = at.hv >= a.s.Hk;
         const int tok = rows[at.r].tok;
         const uint8_t* blk = a.cache + rows[at.r].dst + (int64_t)(kv ? 2 * (at.hv - a.s.Hk) + 1 : 2 * at.hv) * a.step.block;
-        pair = *reinterpret_cast<const uint32_t*>(blk + a.s.page * (D / 2) + tok * 4);
+        // (written out: the compiler puts its loads where they are used, 17.6 us for 15.2)
+        asm volatile("ld.global.u32 %0, [%1];" : "=r"(pair) : "l"(blk + a.s.page * (D / 2) + tok * 4));
         if (!kv) {
-            w = *reinterpret_cast<const uint2*>(blk + tok * (D / 2) + l * 8);
+            asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(w.x), "=r"(w.y) : "l"(blk + tok * (D / 2) + l * 8));
         } else {
-            const uint4 two = *reinterpret_cast<const uint4*>(blk + (tok >> 1) * D + l * 16);
+            uint4 two;
+            asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(two.x), "=r"(two.y), "=r"(two.z), "=r"(two.w)
+                         : "l"(blk + (tok >> 1) * D + l * 16));
             const uint32_t which = tok & 1 ? 0x7632 : 0x5410;
             w = make_uint2(__byte_perm(two.x, two.y, which), __byte_perm(two.z, two.w, which));
         }

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const Kv4Me
     }
     for (int base = 0; base < n_own + n_pre; base += 32) {
         const int n = min(n_own + n_pre - base, 32), j = base + lane;
-        const float* from = nullptr;
+        const float* from = a.y[0];  // (somewhere, for lanes without one)
         float m = -INFINITY, l = 0.0f;
         if (lane < n) {
             const int which = j < n_own ? 0 : 1, k = which ? j - n_own : j;
@@ -131,31 +131,37 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const Kv4Me
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] *= f;
         const uint32_t some = __ballot_sync(0xffffffffu, l != 0.0f);
-        // Loads in flight.  512 rows of 55 partial results: 24 us (38 with each load behind a branch, 17 with eight
-        // at once, which cost the cases of two or three results 3 us more).
-        constexpr int AT_ONCE = 4;
+        // Results are read so many at once, no load behind a branch or behind another's use: 512 rows of 55, the longest
+        // lists, 23 us (37 where the compiler orders them, four at a time), 768 rows of two to four 27 (33 with eight for all).
+        auto add = [&](auto at_once) {
+            constexpr int N = decltype(at_once)::value;
 #pragma unroll 1
-        for (int k = 0; k < n; k += AT_ONCE) {
-            float u[AT_ONCE][E];
+            for (int k = 0; k < n; k += N) {
+                float u[N][E];
 #pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
-                const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), k + j));
-                const bool on = some >> (k + j) & 1;  // (what weighs nothing is not read: it may be no number)
-                if constexpr (E == 4) {
-                    const float4 v = on ? reinterpret_cast<const float4*>(src)[lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    u[j][0] = v.x, u[j][1] = v.y, u[j][2] = v.z, u[j][3] = v.w;
-                } else {
-                    const float2 v = on ? reinterpret_cast<const float2*>(src)[lane] : make_float2(0.0f, 0.0f);
-                    u[j][0] = v.x, u[j][1] = v.y;
+                for (int j = 0; j < N; ++j) {
+                    const float* src = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), k + j));
+                    if constexpr (E == 4)
+                        asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(u[j][0]), "=f"(u[j][1]), "=f"(u[j][2]), "=f"(u[j][3]) : "l"(src + lane * 4));
+                    else
+                        asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(u[j][0]), "=f"(u[j][1]) : "l"(src + lane * 2));
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const bool on = some >> (k + j) & 1;  // (what weighs nothing may be no number)
+                    const float wk = __shfl_sync(0xffffffffu, w, k + j);
+#pragma unroll
+                    for (int e = 0; e < E; ++e) y[e] = on ? fmaf(wk, u[j][e], y[e]) : y[e];
                 }
             }
-#pragma unroll
-            for (int j = 0; j < AT_ONCE; ++j) {
-                const float wk = __shfl_sync(0xffffffffu, w, k + j);
-#pragma unroll
-                for (int e = 0; e < E; ++e) y[e] = fmaf(wk, u[j][e], y[e]);
-            }
-        }
+        };
+        if (n <= 2)
+            add(std::integral_constant<int, 2>{});
+        else if (n <= 4)
+            add(std::integral_constant<int, 4>{});
+        else
+            add(std::integral_constant<int, 8>{});
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
