@@ -342,7 +342,7 @@ int pn_kv4_gather(const void *cache, int64_t n_pages, int64_t kv_heads, int64_t 
  * exactly down to 2^-28 of it; magnitudes from 2^116 on overflow), a token's weight
  * times its value scale s as fp16: 11 bits down to 2^-20 of the largest s among the tokens
  * that the row sees (counted as 2^-54 at least; s from 2^107 on overflows), fewer below, none
- * below 2^-31.  Sums and the softmax are fp32.
+ * below 2^-31.  Sums and the softmax are fp32; the error does not grow with the length.
  * Workspace: pn_kv4_attention_workspace_size bytes, 256-byte aligned, no
  * initialisation needed; calls that may overlap need one each. */
 size_t pn_kv4_attention_workspace_size(int64_t B, int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim);
@@ -360,7 +360,7 @@ int pn_kv4_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, in
  * rotated / 2) fp32, rows table_stride apart; a row at position p of sequence b takes
  * entry p + offsets[b] (int32; p where offsets is NULL).  The rotated queries go to
  * q_out (T, q_heads, head_dim), contiguous, 16-byte aligned, rounded once (q_out may be
- * q itself, where q is contiguous; other overlaps of the two are not allowed).  Keys
+ * q itself, where q is contiguous; it overlaps neither q otherwise nor k or v).  Keys
  * are quantised from fp32, values as pn_kv4_append does.  Rows behind cu_q[B] are left as
  * they were in q_out (zero_rest != 0: become zeros); a row at a negative position gives zeros there, and one whose
  * entry is outside the tables zeros, nothing stored and PN_ERR_ARG in the device
@@ -405,7 +405,8 @@ int pn_kv4_page_means(const void *cache, int64_t n_pages, int64_t kv_heads, int6
  * an entry that is no page of the cache, come last.  Of page j it sees the tokens up to
  * its own.  chosen: NULL, or (T, kv_heads, width) int32 with width = first_pages +
  * last_pages + top_pages: the pages' numbers in the sequence, ascending, then -1 (all -1 for
- * rows that are no sequence's). */
+ * rows that are no sequence's).  Workspace as above; scores of more than 256 MiB are formed and
+ * used for some rows at a time. */
 size_t pn_kv4_sparse_attention_workspace_size(int64_t T, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t table_w,
                                               int64_t width);
 int pn_kv4_sparse_attention(const void *q, int64_t q_sb, int64_t q_sl, int64_t q_sh, int q_dtype, int64_t q_heads,

@@ -374,7 +374,7 @@ struct Kv4GatherArgs {
 // The reverse, zeros for rows that are not there: a code is masked into the low
 // bits of 2^23, one fma per value.  Bound by latency: the rows' look-up, a barrier and the
 // codes' loads stand before a block's first store (43 % of the issue slots used); the same
-// rows 15.3 us, 3.4 TB/s.
+// rows 15.2 us, 3.4 TB/s.
 template <int D>
 __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4GatherArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");

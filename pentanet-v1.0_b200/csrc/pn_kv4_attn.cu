@@ -405,19 +405,20 @@ __device__ __forceinline__ void load_query(const Kv4AttnArgs& a, const char* row
 // piece of 16 tokens takes a warp about 260 instructions (d = 128, up to 8 rows: 64 masks
 // and shifts, 32 products, the softmax of 16 x 8 logits), each waiting for the one
 // before, and the registers leave room for twelve warps to an SM: they issue 1.9
-// instructions of four possible per cycle, the ALU pipe is 45 % and the tensor
-// pipe 24 % busy.
-// 32 sequences of up to 8191 tokens, 8 heads: 49 us, 3.3 TB/s; one of 131072: 41 us,
+// instructions of four possible per cycle, the ALU pipe is 44 % and the tensor
+// pipe 23 % busy.
+// 32 sequences of up to 8191 tokens, 8 heads: 50 us, 3.3 TB/s; one of 131072: 42 us,
 // 3.4 TB/s (half of the copy's rate).  Three blocks of six stages per SM: two, four or
 // five blocks, and more stages in two, are all slower.  With 16 rows at d = 128 the
-// registers do not suffice (372 bytes spilled per thread).
+// registers do not suffice (404 bytes spilled per thread).
 template <int D, int NT, bool M>
 struct AttnCfg {
     static constexpr bool kMore = M;
     static constexpr int W = D / 32;             // words per thread and token
     static constexpr int kRows = 8 * NT;         // query rows of a row tile
     static constexpr int kTokens = 128;          // tokens of a unit: 32 per warp
-    // Runs between two centrings.  64 sequences of 4096 tokens, 8 heads of 8 rows: 71.7 us with 4, 71.3 with 8, 69.0 with none.
+    // Runs between two centrings.  64 sequences of 4096 tokens, 8 heads of 8 rows: 71.7 us with 4, 71.3 with 8, 69.0
+    // with none.
     static constexpr int kCentre = 4;
     static constexpr int kThreads = kAttnThreads;
     static constexpr int kStages = 6;
@@ -806,10 +807,10 @@ __global__ void __launch_bounds__(kAttnThreads, AttnCfg<D, NT, M>::kBlocks) kv4_
 //
 // What bounds it: m16n8k16 runs at one per ten cycles on each quarter of an SM
 // (measured; 460 TFLOP/s over the device), 128 of them to a warp's 64 tokens at
-// d = 128, and 320 mask and shift instructions; but the tensor pipe is only 34 % busy
+// d = 128, and 320 mask and shift instructions; but the tensor pipe is only 33 % busy
 // and 41 % of the issue slots are used: as in the decode kernel the warps (twelve to
 // an SM) wait for their own last instruction.  64 sequences x 64 rows x 4 heads over 1024
-// tokens: 72 us (two blocks to an SM: 2 % slower than three); 148 bytes spilled per thread.
+// tokens: 70 us (two blocks to an SM: 2 % slower than three); 180 bytes spilled per thread.
 template <int D, bool M>
 struct ChunkCfg {
     static constexpr bool kMore = M;
@@ -1125,12 +1126,12 @@ __global__ void __launch_bounds__(kAttnThreads, ChunkCfg<D, M>::kBlocks) kv4_chu
 // 500 per thread and step, which all warps do in turn between the block's barriers (3500 to
 // 4500 cycles for an SM's two blocks, 47 % of the issue slots used); the products take
 // 512 cycles of a step at the tensor core's rate.  16 sequences x 512 rows x 8
-// heads over 1024 tokens: 115 us (the chunk kernel 146).
+// heads over 1024 tokens: 114 us (the chunk kernel 144).
 template <int D, bool M>
 struct TcCfg {
     static constexpr bool kMore = M;
     static constexpr int kRows = 128, kTokens = 64, kThreads = 256;
-    static constexpr int kCentre = 8;  // tiles between two centrings, at most (16 x 512 rows: 119.6 us, 117.0 with none, 121.5 with 4)
+    static constexpr int kCentre = 8;  // tiles between two centrings, at most (2 % slower than with none; 4: 4 %)
     static constexpr int kStages = 3;
     static constexpr int kRawK = kTokens * (D / 2);      // codes of a tile's keys (or values)
     static constexpr int kRaw = 2 * kRawK + 8 * kTokens; // and the pairs: the keys', then the values'
@@ -1658,15 +1659,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const Kv4Attn
 // cache more often, but gives the SMs more to share: up to four tiles of 16 rows
 // per SM the 16-row kernel wins whatever the number of rows, from eight per SM
 // on the larger one of the others.  In us for d = 128 (16 rows / chunk / tcgen05):
-//   4 sequences x 128 rows x 8 heads of 2048 tokens (256 tiles)      46 /  61 /  94
-//   one prompt of 500 tokens, 8 heads (256 tiles)                    29 /  44 /  37
-//   8 x 144 x 8 heads of 2048 tokens (576 tiles)                     74 /  78 /  80
-//   one prompt of 768 tokens, 12 heads (576 tiles)                   40 /  40 /  73
-//   64 x 96 x 2 heads of 1024 tokens (768 tiles)                     65 /  63 /  67
-//   32 prompts of 24 tokens, 12 heads (768 tiles)                    24 /  13 /  20
-//   64 x 64 x 4 heads of 1024 tokens (1024 tiles)                    83 /  72 /  77
-//   64 x 96 x 4 heads of 1024 tokens (1536 tiles)                   110 /  93 /  82
-//   16 x 512 x 8 heads of 1024 tokens (4096 tiles)                  227 / 146 / 115
+//   4 sequences x 128 rows x 8 heads of 2048 tokens (256 tiles)      46 /  61 /  93
+//   one prompt of 500 tokens, 8 heads (256 tiles)                    28 /  43 /  36
+//   8 x 144 x 8 heads of 2048 tokens (576 tiles)                     75 /  78 /  80
+//   one prompt of 768 tokens, 12 heads (576 tiles)                   40 /  40 /  71
+//   64 x 96 x 2 heads of 1024 tokens (768 tiles)                     65 /  63 /  66
+//   32 prompts of 24 tokens, 12 heads (768 tiles)                    23 /  12 /  20
+//   64 x 64 x 4 heads of 1024 tokens (1024 tiles)                    84 /  70 /  76
+//   64 x 96 x 4 heads of 1024 tokens (1536 tiles)                   111 /  91 /  80
+//   16 x 512 x 8 heads of 1024 tokens (4096 tiles)                  233 / 144 / 114
 // and at 8 rows 23 against 34 (64 heads of 4096 tokens: the 8-row kernel, the 16-row
 // one).  Where the rule is wrong: few tiles over very long sequences (290
 // tokens x 4 behind 8192, 584 tiles: 196 / 179 / 152), many prompts of 128 to 512

@@ -12,13 +12,14 @@
 // were split over blocks in parts.  The third kernel (here) joins whatever either left, so
 // that no pass needs a joining kernel of its own.
 //
-// What bounds it: over the prefix, the exponentials and the unpacking of codes for every tile of
-// 128 rows.  64 sequences x 8 heads of 128 dims x 8 rows a head over 8192 tokens: 63 us of the
-// call's 113 (510 TFLOP/s from one length to the next; cuBLAS reaches 1667), the rows'
-// own 1000 tokens 40, the joining 13.  A kernel for the prefix alone was built too (256 rows to a tile,
+// What bounds it: over the prefix, that a step's softmax and the spreading of its codes stand between
+// the block's barriers (issue slots 40 %, tensor pipe 16 %), and that the passes run one behind the
+// other.  64 sequences x 8 heads of 128 dims x 8 rows a head over 8192 tokens: 65 us over the prefix,
+// the rows' own 1000 tokens 39, the joining 13, together 107 as each begins before the one in front has
+// ended.  A kernel for the prefix alone was built too (256 rows to a tile,
 // warps by task, the logits of a step formed while the softmax of the one before ran): 75 us
 // there and 186 over one prefix of 131071 tokens for 64 rows a head, where the chunk kernel
-// takes 148; its five kinds of warps did not fit the instruction cache, and it was given up.
+// took 148; its five kinds of warps did not fit the instruction cache, and it was given up.
 #include "pn_common.cuh"
 #include "pn_internal.h"
 
@@ -175,8 +176,14 @@ __global__ void __launch_bounds__(kMergeWarps * 32) kv4_merge_kernel(const Kv4Me
 
 // The kernel for the rows over the prefixes, which walk long sequences together; the host knows no
 // more of the lengths than the table's width.
-// Not attn_kind's rule: the tiles are few, but their walks long.  A call in us, chunk and long kernel: 64 rows
-// of 8 heads over 131071 tokens 184 and 188, 128 rows over 8192 tokens 64 and 61; 32 rows there 53 and 52.
+// Not attn_kind's rule: the tiles are few, but their walks long.  A call in us with the kernels for 8, 16, 64 and
+// 128 rows, 8 heads of 128 dims:
+//   64 rows a head over 131071 tokens      - / 202 / 185 / 174
+//   128 rows over 8192 tokens              - /  58 /  59 /  58
+//   32, 16, 8 rows there                  36 /  47 /  52 /  48,  34 / 41 / 50 / 46,  33 / 40 / 46 / 45
+// Where the rule is wrong: few rows over a prefix of some thousand tokens (the 8-row kernel leads up to 32), 64
+// rows over very long ones (the tcgen05 kernel does), and shares that are not alike, as it knows their mean: of eight
+// prefixes of 8192 tokens with 500 rows behind one the chunk kernel is taken, 154 (tcgen05 124).
 static AttnKind prefix_kind(int64_t P, int64_t T, int64_t Hk, int64_t G) {
     const int64_t rows = (T + P - 1) / P * G;
     if (rows <= 16) return rows <= 8 ? kAttn8 : kAttn16;

@@ -109,8 +109,8 @@ __device__ __forceinline__ void rotary_scale(const float (&v)[16], float& s, flo
 // two that meet, so that no value crosses lanes and a lane needs eight angles, which it
 // keeps for all heads of its row.  A warp takes a row (or one of `parts` shares of its
 // vectors, where there are few rows), no block-wide step anywhere.  Its loads of the next step are in
-// flight during this one; six blocks to an SM spill 40 bytes, but have more of them: 7 ragged prompts of up to 2047
-// rows, 32 + 2 x 8 heads of 128 dims: 55 us (five blocks, no spills: 58; eight: 64), reading and writing once 31.
+// flight during this one; six blocks to an SM spill 4 to 32 bytes, but have more of them: 7 ragged prompts of up to 2047
+// rows, 32 + 2 x 8 heads of 128 dims: 53 us (five blocks, no spills: 58; eight: 64), reading and writing once 31.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRotaryThreads, 6) kv4_rotary_kernel(const Kv4RotaryArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");

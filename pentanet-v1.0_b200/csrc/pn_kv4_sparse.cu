@@ -149,8 +149,8 @@ struct SelectRow {
 // A block scores some pages for up to `tile` rows of one kv head.  Four lanes share a page's
 // mean, held as fp64 for all rows of a sequence; the group's queries are summed once per
 // block.  Rows are taken four at a time: one by one the kernel waits for their loads from
-// shared memory (502 rows x 8 heads of 250 pages 63 us, 79 one by one; the fp64 units are busy for a
-// ninth of it).
+// shared memory (251 rows of 250 pages and 157 of 138, 8 heads: 65 us, 79 one by one; the fp64 units
+// are busy for a fourteenth of it).
 template <int D>
 __global__ void __launch_bounds__(kScoreThreads) kv4_score_kernel(const Kv4SelectArgs a) {
     constexpr int E = D / 4;  // dims per lane: chunks of 8, four lanes in turn
@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(THREADS) kv4_select_kernel(const Kv4SelectArgs
 
 // The same for tables of up to kSmallPages pages and many rows: a warp per row and kv head, its keys
 // in registers, the threshold found bit by bit from the highest in which two keys differ, until exactly
-// `top` are at or above it or the bits are out.  502 rows x 8 heads of 250 pages: 16 us, 35 with a
+// `top` are at or above it or the bits are out.  251 rows of 250 pages and 157 of 138, 8 heads: 16 us, 35 with a
 // block for each; few rows wait for its steps, though (32 x 8 of up to 512: 12 us, 9 with blocks).
 constexpr int kWarpHeld = 16, kSmallPages = 32 * kWarpHeld, kWarpSelects = 4;
 __global__ void __launch_bounds__(kWarpSelects * 32) kv4_select_warp_kernel(const Kv4SelectArgs a) {

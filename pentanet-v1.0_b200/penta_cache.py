@@ -168,8 +168,8 @@ def kv4_append_rotary(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: to
     whose entry the tables do not have is not stored, gives zeros, and shows in
     penta_native.device_status().  Keys are quantised without a rounding to bf16 in between.
 
-    out: a contiguous tensor for the queries, which may be q itself but not overlap it
-    otherwise; rows of it behind cu_q[B] are left as they were (zeros where no out is
+    out: a contiguous tensor for the queries, which may be q itself but overlaps neither q
+    otherwise nor k or v; rows of it behind cu_q[B] are left as they were (zeros where no out is
     given)."""
     assert q.is_cuda, "kv4_append_rotary requires CUDA tensors"
     dev, dtype, D = q.get_device(), q.dtype, q.shape[-1]
@@ -282,7 +282,8 @@ def kv4_prefix_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torc
     [cu_prefix[g], cu_prefix[g + 1]) share prefix g (cu_prefix (P + 1) int32, never falling;
     without it B / P sequences each); sequences outside have none.  A row sees all of its
     prefix and then its sequence's own tokens up to its position, which block_table and
-    seq_lens count from 0.  The rest is as in kv4_attention."""
+    seq_lens count from 0.  The rest is as in kv4_attention, its precision over either
+    part included; the two parts are joined in fp32."""
     assert q.is_cuda and q.dtype in _FLOATS, "kv4_prefix_attention takes bfloat16 or float32 CUDA queries"
     D = q.shape[-1]
     dev = q.get_device()
@@ -358,8 +359,8 @@ def kv4_sparse_attention(q: torch.Tensor, cache: torch.Tensor, means: torch.Tens
     A row whose position is in page j of its sequence attends to the first first_pages
     pages, to the last last_pages (at least one: page j itself, up to its position) and to
     the top_pages of the others with the largest scores (sum of the kv head's queries) .
-    mean key (means, kept by kv4_page_means), in 64 bits, ties by the lowest page; all pages
-    where there are no more.  With return_pages also the choice: int32 (*rows, kv heads,
+    mean key (means, kept by kv4_page_means), in 64 bits, ties by the lowest page, a NaN score
+    and an entry that is no page last; all pages where there are no more.  With return_pages also the choice: int32 (*rows, kv heads,
     first_pages + top_pages + last_pages), the pages' numbers in the sequence, ascending,
     then -1.
 
