@@ -24,8 +24,11 @@
 // every kCentre steps what they have reached (the middle one of three dims, so that
 // a loud dim does not lead the others away) is taken out of a row's sums and joins,
 // with the z term of these steps, a base that stays small, as its two parts cancel
-// in one fma.  Over any length to 131072 tokens the error is now that of the rounded
-// weights alone, 5e-4 to 8e-4 of the result's norm in every kernel.  (With the middle
+// in one fma.  To 262144 tokens the error is now that of the rounded weights alone,
+// 5e-4 to 8e-4 of the result's norm in every kernel.  What a product of 16 tokens
+// loses against the sums that are left is up to 2^-24 of the result: over a million
+// tokens that one block walks the error is 6e-4 to 9e-4 (decode), 17e-4 (chunk) and
+// 27e-4 (tcgen05).  (With the middle
 // code, 7.5, taken out of each value instead, which the tcgen05 kernel could do as
 // it spreads them, that is 3e-4, but dims of low codes are less exact than now, and
 // values to one side drift as before.)

@@ -240,9 +240,10 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
 
     The products take 11 bits of fp32 queries (all of bf16 ones) and 11 of a token's
     weight times its value scale, relative to the largest such scale that the row
-    sees; sums and the softmax are fp32, and the error does not grow with the length.
-    A value vector's range (largest less smallest) is taken from 2^-50 to 2^110: smaller
-    ones lose some of these 11 bits, larger ones may give infinities."""
+    sees; sums and the softmax are fp32, and 16 tokens' products cost a sum no more than
+    2^-24 of the result, however far its terms cancel.  A value vector's range
+    (largest less smallest) is taken from 2^-50 to 2^110: smaller ones lose some of
+    these 11 bits, larger ones may give infinities."""
     assert q.is_cuda and q.dtype in _FLOATS, "kv4_attention takes bfloat16 or float32 CUDA queries"
     D = q.shape[-1]
     dev = q.get_device()

@@ -56,12 +56,12 @@ class Long:
         code, v = (self.v - self.v.amin(-1, keepdim=True))[..., self.quiet], self.v[..., self.quiet]
         return 2.0 ** -11 * float(code.square().mean().sqrt() / (v - v.mean((0, 1))).square().mean().sqrt())
 
-    def check(self, q, y, rows):
+    def check(self, q, y, rows, more=0.0):
         want = attend64(torch.stack([q[b, l] for b, l in rows]), self.k, self.v)
         want = want[..., self.quiet]
         got = torch.stack([y[b, l] for b, l in rows]).double()[..., self.quiet]
         err = float((got - want).norm() / want.norm())
-        assert err <= self.limit(), (err, self.limit())
+        assert err <= self.limit() + more, (err, self.limit())
         assert nat.device_status() == 0
 
 
@@ -120,3 +120,12 @@ def test_values_of_any_size(cuda_device, B, L, H, values):
     up = 2.0 ** (-104 if values == "largest" else 48)
     s.v = s.v * up  # (the check squares)
     s.check(q, y * up, [(0, L - 1), (B // 2, L - 1), (B - 1, L - 1)])
+
+
+@pytest.mark.parametrize("B,L,H", [(450, 1, 16), (450, 64, 1), (300, 128, 1)])
+def test_a_million_tokens_in_every_kernel(cuda_device, B, L, H):
+    """A block walks all of them.  Each product of 16 tokens may cut 2^-24 of the sum so far, which is the result's."""
+    s = Long(1 << 20, 1, 64, cuda_device)
+    q = s.queries(B, L, H)
+    y = pc.kv4_attention(q, s.cache, s.table.expand(B, -1).contiguous(), s.lens.expand(B).contiguous())
+    s.check(q, y, [(0, L - 1), (B // 2, L - 1), (B - 1, L - 1)], more=s.n / 16 * 2.0 ** -24)
